@@ -30,7 +30,9 @@ INCLUDE = REPO_ROOT / "include"
 
 CORE_SOURCES = ["capi.cu", "assign_tc.cu", "norm_ext.cu", "assign_simt.cu", "update.cu",
                 "update_det.cu",
-                "finalize.cu", "lloyd_graph.cu", "assign_noalloc.cu", "selftest.cu"]
+                "finalize.cu", "lloyd_graph.cu", "assign_noalloc.cu", "selftest.cu",
+                "cluster_group.cu", "cluster_lookup.cu", "cluster_select.cu",
+                "cluster_attention.cu", "cluster_attention_grad.cu", "cluster_capi.cu"]
 CORE_LIB = OUT_DIR / "libfkc_b200.so"
 TORCH_API_LIB = OUT_DIR / "libflash_kmeans_cuda.so"
 
@@ -132,9 +134,9 @@ def build_py_module(force: bool = False) -> Path | None:
         from torch.utils import cpp_extension
     except Exception:  # pragma: no cover - torch is part of the image
         return None
-    src = CSRC / "py_C.cpp"
+    srcs = [CSRC / "py_C.cpp", CSRC / "py_clusters.cpp"]
     out = OUT_DIR / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
-    if not (force or _newer(out, [src, INCLUDE / "fkc_capi.h", CORE_LIB])):
+    if not (force or _newer(out, [*srcs, CSRC / "py_common.h", INCLUDE / "fkc_capi.h", CORE_LIB])):
         return out
     libdir = Path(torch.__file__).parent / "lib"
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -144,7 +146,7 @@ def build_py_module(force: bool = False) -> Path | None:
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         *[f"-I{p}" for p in cpp_extension.include_paths()],
         f"-I{sysconfig.get_paths()['include']}", "-I/usr/local/cuda/include", f"-I{INCLUDE}",
-        str(src), "-o", str(out),
+        *map(str, srcs), "-o", str(out),
         f"-L{libdir}", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
         "-ltorch_cuda", f"-L{OUT_DIR}", "-lfkc_b200",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libdir}",

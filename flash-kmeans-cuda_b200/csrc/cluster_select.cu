@@ -1,0 +1,574 @@
+// Selection of clusters for a query by a cheap score:
+//
+//   score[r, i, c] = scale * max over the heads h of the group of q[b, h, i] . centroid[r, c]
+//                    + bias[r, c]
+//
+// Clusters without positions, and (with q_pos) those whose first position lies
+// behind the query, cannot be selected, nor can one whose score is NaN or -inf. The
+// top best of the rest, ties to the lowest index, are written in ascending order; -1
+// fills what is left.
+//
+//   score  (score_kernel)  128 clusters x 16 or 64 queries per CTA; the heads are
+//          walked one by one and the running maximum stays in the accumulator layout,
+//          so any group size fills the instruction (m16n8k16, fp32 accumulation). Also
+//          the largest norms of a query's heads and of a tile's centroids.
+//   choose (choose_warp_kernel, one warp per query up to 1024 clusters, and
+//          choose_cta_kernel)  the top-th largest fp32 score t by bisection over its
+//          bits. What lies above t by more than the scores can be off is in, what lies
+//          below by more is out; where that leaves more candidates than places, theirs
+//          are computed again in 64 bits and ranked. So the selection is that of exact
+//          arithmetic, whatever order the products were added in.
+//
+// How far an fp32 score can be off: a product of two 16-bit values is exact in fp32;
+// adding D of them with truncation to 2^-22 of the largest magnitude so far, none of
+// which exceeds |q||c|, is off by at most D * 2^-22 |q||c|; the two roundings of scale
+// and the rounding of the sum with bias add 2^-22 (scale |q||c| + |score|) at most.
+//
+// The scores go through memory (4 bytes a score, L2 at the usual sizes): for 4096
+// queries x 256 clusters x 8 rows 34 MB against 17 GFLOP of products.
+#include <algorithm>
+#include <cmath>
+
+#include "cluster_attention.cuh"
+#include "fkc_common.cuh"
+
+namespace fkc {
+namespace attn {
+namespace {
+
+constexpr int kClusters = 128;  // clusters per tile
+constexpr uint32_t kNever = 0xFFC0DEADu;  // score bits of a cluster that cannot be selected
+
+struct SelectArgs {
+  const void *q, *centroids;
+  Strides qs;
+  const int32_t* offsets;
+  const int32_t* order;  // with q_pos
+  const int32_t* q_pos;
+  const float* bias;  // (R, K) or null
+  int Hkv, G, Nq, N, K, top, D;
+  double scale;
+};
+
+__device__ __forceinline__ float fold_max(float a, float b) {
+  return (isnan(a) || isnan(b)) ? INFINITY : fmaxf(a, b);  // a NaN norm counts as unbounded
+}
+
+// QW warps along the queries, 4 / QW along the clusters.
+template <typename T, int DP, int QW>
+__global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restrict__ scores,
+                                                    float* __restrict__ q_norm,
+                                                    float* __restrict__ c_norm, int ctiles,
+                                                    int qtiles) {
+  constexpr int CW = 4 / QW, KS = DP / 16, CH = DP / 8;
+  constexpr int NW = kClusters / CW / 8;  // 8-cluster groups per warp
+  constexpr int MQ = 16 * QW;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_bias[kClusters];
+  __shared__ int s_first[kClusters];  // first position; INT_MAX: never selected
+  __shared__ float s_red[4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  const uint32_t ct = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  const uint32_t qt0 = ct + kClusters * DP * 2;
+  pdl_wait();
+  const int tile = blockIdx.x % ctiles, rest = blockIdx.x / ctiles;
+  const int qtile = rest % qtiles, r = rest / qtiles;
+  const int b = r / a.Hkv, hk = r - b * a.Hkv;
+  const int c0 = tile * kClusters, i0 = qtile * MQ;
+  const T* cen = static_cast<const T*>(a.centroids) + (static_cast<int64_t>(r) * a.K + c0) * a.D;
+  const T* q = static_cast<const T*>(a.q) + b * a.qs.b + static_cast<int64_t>(hk) * a.G * a.qs.h;
+  const int dchunks = a.D / 8;
+  for (int e = tid; e < kClusters * CH; e += 128) {
+    const int row = e / CH, c = e % CH;
+    const bool ok = c0 + row < a.K && c < dchunks;
+    mma::cp_async16(ct + tile_at<DP>(row, c), cen + (ok ? static_cast<int64_t>(row) * a.D + c * 8 : 0),
+                    ok);
+  }
+  auto load_q = [&](int h, int buf) {
+    const uint32_t qt = qt0 + buf * (MQ * DP * 2);
+    for (int e = tid; e < MQ * CH; e += 128) {
+      const int row = e / CH, c = e % CH;
+      const bool ok = i0 + row < a.Nq && c < dchunks;
+      mma::cp_async16(qt + tile_at<DP>(row, c),
+                      q + (ok ? h * a.qs.h + (i0 + row) * a.qs.n + c * 8 : 0), ok);
+    }
+  };
+  load_q(0, 0);
+  mma::cp_async_commit();
+  {
+    const int c = c0 + tid;
+    int first = INT_MAX;
+    float bias = 0.f;
+    if (c < a.K) {
+      const int32_t* of = a.offsets + static_cast<int64_t>(r) * (a.K + 1) + c;
+      const int s = of[0], e = of[1];
+      if (e > s && s >= 0 && s < a.N)
+        first = a.q_pos != nullptr ? a.order[static_cast<int64_t>(r) * a.N + s] : 0;
+      if (first < 0) first = INT_MAX;
+      if (a.bias != nullptr) bias = a.bias[static_cast<int64_t>(r) * a.K + c];
+      if (isnan(bias) || bias == -INFINITY) first = INT_MAX;
+    }
+    s_first[tid] = first;
+    s_bias[tid] = bias;
+  }
+  const int wq = warp % QW, wc = warp / QW;
+  float best[NW][4];
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) best[n][e] = -INFINITY;
+  float qn = 0.f;  // largest norm^2 of the heads, thread tid < MQ: query i0 + tid
+  for (int h = 0; h < a.G; ++h) {
+    mma::cp_async_wait<0>();
+    __syncthreads();
+    if (h + 1 < a.G) load_q(h + 1, (h + 1) & 1);
+    mma::cp_async_commit();
+    const uint32_t qt = qt0 + (h & 1) * (MQ * DP * 2);
+    if (tile == 0 && tid < MQ) {
+      float s = 0.f;
+      const uint8_t* base = smem + (qt - ct);
+      for (int c = 0; c < CH; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(base + tile_at<DP>(tid, c));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = mma::unpack2<T>(w[k]);
+          s += f.x * f.x + f.y * f.y;
+        }
+      }
+      qn = fold_max(qn, s);
+    }
+    float acc[NW][4];
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      uint32_t fa[4];
+      load_a<DP>(fa, qt, wq * 16, kk);
+#pragma unroll
+      for (int n = 0; n < NW; n += 2) {
+        uint32_t fb[4];
+        load_b<DP>(fb, ct, (wc * NW + n) * 8, kk);
+        mma::m16n8k16<T>(acc[n], fa, fb[0], fb[1]);
+        mma::m16n8k16<T>(acc[n + 1], fa, fb[2], fb[3]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) best[n][e] = fmaxf(best[n][e], acc[n][e]);
+  }
+  if (tile == 0 && tid < MQ && i0 + tid < a.Nq)
+    q_norm[static_cast<int64_t>(r) * a.Nq + i0 + tid] = sqrtf(qn);
+  if (qtile == 0) {  // the tile's largest centroid norm, of the clusters that can be selected
+    float s = 0.f;
+    for (int c = 0; c < CH; ++c) {
+      const uint4 u = *reinterpret_cast<const uint4*>(smem + tile_at<DP>(tid, c));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = mma::unpack2<T>(w[k]);
+        s += f.x * f.x + f.y * f.y;
+      }
+    }
+    if (s_first[tid] == INT_MAX) s = 0.f;
+    s = fold_max(s, 0.f);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xFFFFFFFFu, s, o));
+    if (lane == 0) s_red[warp] = s;
+    __syncthreads();
+    if (tid == 0)
+      c_norm[static_cast<int64_t>(r) * ctiles + tile] =
+          sqrtf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
+  }
+  const float scale = static_cast<float>(a.scale);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int i = i0 + wq * 16 + half * 8 + g;
+    if (i >= a.Nq) continue;
+    const int pos = a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : INT_MAX - 1;
+    float* row = scores + (static_cast<int64_t>(r) * a.Nq + i) * a.K;
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int cl = (wc * NW + n) * 8 + t4 * 2 + e;
+        if (c0 + cl >= a.K) continue;
+        const float s = best[n][half * 2 + e] * scale + s_bias[cl];
+        row[c0 + cl] = s_first[cl] > pos ? __uint_as_float(kNever) : s;
+      }
+  }
+}
+
+// fp32 scores as integers that compare the same way; 0: cannot be selected.
+__device__ __forceinline__ uint32_t sort_key(float s) {
+  const uint32_t u = __float_as_uint(s);
+  if (u == kNever) return 0u;
+  if (isnan(s)) return 1u;  // undecided: only 64 bits can tell
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+// The score of cluster c for query i in 64 bits, over the warp.
+template <typename T>
+__device__ double exact_score(const SelectArgs& a, int r, int i, int c) {
+  const int lane = threadIdx.x & 31;
+  const int b = r / a.Hkv, hk = r - b * a.Hkv;
+  const T* cen = static_cast<const T*>(a.centroids) + (static_cast<int64_t>(r) * a.K + c) * a.D;
+  const T* q = static_cast<const T*>(a.q) + b * a.qs.b + static_cast<int64_t>(hk) * a.G * a.qs.h +
+               i * a.qs.n;
+  double best = -INFINITY;
+  bool nan = false;
+  for (int h = 0; h < a.G; ++h) {
+    double s = 0.0;
+    for (int d = lane; d < a.D; d += 32)
+      s += static_cast<double>(to_f32<T>(q[h * a.qs.h + d])) * static_cast<double>(to_f32<T>(cen[d]));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    nan |= isnan(s);
+    best = fmax(best, s);
+  }
+  double s = best * a.scale;
+  if (a.bias != nullptr) s += static_cast<double>(a.bias[static_cast<int64_t>(r) * a.K + c]);
+  return nan || isnan(s) ? -INFINITY : s;
+}
+
+// The band around the top-th score t in which fp32 cannot tell; infinite where a
+// norm or the score is not finite.
+__device__ __forceinline__ float band_of(const SelectArgs& a, float t, float qn, float cn) {
+  const float mag = static_cast<float>(fabs(a.scale)) * qn * cn;
+  const float eps = mag * (static_cast<float>(a.D) * 0x1p-22f + 0x1p-21f) + fabsf(t) * 0x1p-22f;
+  return eps < INFINITY ? 2.f * eps : INFINITY;
+}
+
+__device__ __forceinline__ float largest_norm(const float* c_norm, int64_t r, int ctiles) {
+  float m = 0.f;
+  for (int i = threadIdx.x & 31; i < ctiles; i += 32) m = fmaxf(m, c_norm[r * ctiles + i]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  return m;
+}
+
+// One warp per query; KPL scores a lane, cluster j * 32 + lane.
+template <typename T, int KPL>
+__global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
+                                                          const float* __restrict__ scores,
+                                                          const float* __restrict__ q_norm,
+                                                          const float* __restrict__ c_norm,
+                                                          int ctiles, int32_t* __restrict__ sel,
+                                                          int64_t queries) {
+  __shared__ double s_exact[4][KPL * 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  const int64_t qi = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (qi >= queries) return;
+  const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
+  const float* row = scores + qi * a.K;
+  uint32_t key[KPL];
+  int have = 0;
+#pragma unroll
+  for (int j = 0; j < KPL; ++j) {
+    key[j] = j * 32 + lane < a.K ? sort_key(row[j * 32 + lane]) : 0u;
+    have += key[j] != 0u;
+  }
+  have = __reduce_add_sync(0xFFFFFFFFu, have);
+  const uint32_t below = (1u << lane) - 1u;
+  uint32_t t = 0;
+  const int want = min(a.top, have);
+  if (have > 0) {
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = t | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < KPL; ++j) n += key[j] >= cand;
+      if (__reduce_add_sync(0xFFFFFFFFu, n) >= want) t = cand;
+    }
+  }
+  const float cn = largest_norm(c_norm, r, ctiles);
+  const float ts = key_score(t);
+  const float band = t <= 1u ? INFINITY : band_of(a, ts, q_norm[qi], cn);
+  const bool open = !(band < INFINITY) || isinf(ts);  // fp32 says nothing: all in 64 bits
+  // in: above the band; undecided: inside
+  uint32_t in = 0, mid = 0;
+  int sure = 0, undecided = 0;
+#pragma unroll
+  for (int j = 0; j < KPL; ++j) {
+    if (key[j] == 0u) continue;
+    const float s = key_score(key[j]);
+    if (!open && s > ts + band)
+      in |= 1u << j, ++sure;
+    else if (open || s >= ts - band)
+      mid |= 1u << j, ++undecided;
+  }
+  sure = __reduce_add_sync(0xFFFFFFFFu, sure);
+  undecided = __reduce_add_sync(0xFFFFFFFFu, undecided);
+  const int places = want - sure;
+  if (undecided == places && !open) {
+    in |= mid;  // no choice to make
+  } else if (undecided > 0) {
+    double* ex = s_exact[warp];
+#pragma unroll 1
+    for (int j = 0; j < KPL; ++j) {
+      uint32_t todo = __ballot_sync(0xFFFFFFFFu, mid >> j & 1u);
+      while (todo != 0) {
+        const int who = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const double s = exact_score<T>(a, r, i, j * 32 + who);
+        if (lane == who) ex[j * 32 + lane] = s;
+      }
+    }
+    __syncwarp();
+    // the places best of them: largest score, then lowest index
+    for (int n = 0; n < places; ++n) {
+      double best = -INFINITY;
+      int at = INT_MAX;
+#pragma unroll 1
+      for (int j = 0; j < KPL; ++j)
+        if (mid >> j & 1u) {
+          const double s = ex[j * 32 + lane];
+          if (s > best) best = s, at = j * 32 + lane;
+        }
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        const double s = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+        const int x = __shfl_xor_sync(0xFFFFFFFFu, at, o);
+        if (s > best || (s == best && x < at)) best = s, at = x;
+      }
+      if (at == INT_MAX) break;  // nothing above -inf is left
+      if ((at & 31) == lane) {
+        mid &= ~(1u << (at >> 5));
+        in |= 1u << (at >> 5);
+      }
+    }
+  }
+  int32_t* out = sel + qi * a.top;
+  int done = 0;
+#pragma unroll
+  for (int j = 0; j < KPL; ++j) {
+    const bool on = in >> j & 1u;
+    const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
+    const int at = done + __popc(who & below);
+    if (on && at < a.top) out[at] = j * 32 + lane;
+    done += __popc(who);
+  }
+  for (int j = done + lane; j < a.top; j += 32) out[j] = -1;
+}
+
+constexpr int kCtaThreads = 512;
+
+// Sum over the CTA (every thread gets it).
+__device__ __forceinline__ int cta_sum(int v, int* red) {
+  v = __reduce_add_sync(0xFFFFFFFFu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < kCtaThreads / 32; ++w) s += red[w];
+  return s;
+}
+
+// One CTA per query, up to 16384 clusters: keys, states and 64-bit scores in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
+    SelectArgs a, const float* __restrict__ scores, const float* __restrict__ q_norm,
+    const float* __restrict__ c_norm, int ctiles, int32_t* __restrict__ sel) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int red[kCtaThreads / 32];
+  __shared__ double s_best[kCtaThreads / 32];
+  __shared__ int s_at[kCtaThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  double* ex = reinterpret_cast<double*>(smem);
+  uint32_t* key = reinterpret_cast<uint32_t*>(smem + static_cast<size_t>(a.K) * 8);
+  uint8_t* state = smem + static_cast<size_t>(a.K) * 12;  // 0 out, 1 in, 2 undecided
+  pdl_wait();
+  const int64_t qi = blockIdx.x;
+  const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
+  const float* row = scores + qi * a.K;
+  int have = 0;
+  for (int c = tid; c < a.K; c += kCtaThreads) {
+    key[c] = sort_key(row[c]);
+    have += key[c] != 0u;
+  }
+  have = cta_sum(have, red);
+  const int want = min(a.top, have);
+  uint32_t t = 0;
+  if (have > 0)
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = t | (1u << bit);
+      int n = 0;
+      for (int c = tid; c < a.K; c += kCtaThreads) n += key[c] >= cand;
+      if (cta_sum(n, red) >= want) t = cand;
+    }
+  const float cn = largest_norm(c_norm, r, ctiles);
+  const float ts = key_score(t);
+  const float band = t <= 1u ? INFINITY : band_of(a, ts, q_norm[qi], cn);
+  const bool open = !(band < INFINITY) || isinf(ts);
+  int sure = 0, undecided = 0;
+  for (int c = tid; c < a.K; c += kCtaThreads) {
+    uint8_t st = 0;
+    if (key[c] != 0u) {
+      const float s = key_score(key[c]);
+      if (!open && s > ts + band)
+        st = 1, ++sure;
+      else if (open || s >= ts - band)
+        st = 2, ++undecided;
+    }
+    state[c] = st;
+  }
+  sure = cta_sum(sure, red);
+  undecided = cta_sum(undecided, red);
+  const int places = want - sure;
+  const bool all = undecided == places && !open;
+  if (!all && undecided > 0) {
+    __syncthreads();
+    for (int c = warp; c < a.K; c += kCtaThreads / 32)
+      if (state[c] == 2) {
+        const double s = exact_score<T>(a, r, i, c);
+        if (lane == 0) ex[c] = s;
+      }
+    __syncthreads();
+    for (int n = 0; n < places; ++n) {
+      double best = -INFINITY;
+      int at = INT_MAX;
+      for (int c = tid; c < a.K; c += kCtaThreads)
+        if (state[c] == 2 && ex[c] > best) best = ex[c], at = c;
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        const double s = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+        const int x = __shfl_xor_sync(0xFFFFFFFFu, at, o);
+        if (s > best || (s == best && x < at)) best = s, at = x;
+      }
+      if (lane == 0) s_best[warp] = best, s_at[warp] = at;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kCtaThreads / 32; ++w)
+        if (s_best[w] > best || (s_best[w] == best && s_at[w] < at)) best = s_best[w], at = s_at[w];
+      if (at == INT_MAX) break;  // the same in every thread
+      if (tid == 0) state[at] = 1;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  int32_t* out = sel + qi * a.top;
+  int done = 0;
+  for (int c0 = 0; c0 < a.K; c0 += kCtaThreads) {
+    const int c = c0 + tid;
+    const bool on = c < a.K && (state[c] == 1 || (all && state[c] == 2));
+    const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
+    __syncthreads();
+    if (lane == 0) red[warp] = __popc(who);
+    __syncthreads();
+    int before = done, total = 0;
+#pragma unroll
+    for (int w = 0; w < kCtaThreads / 32; ++w) {
+      if (w < warp) before += red[w];
+      total += red[w];
+    }
+    const int at = before + __popc(who & ((1u << lane) - 1u));
+    if (on && at < a.top) out[at] = c;
+    done += total;
+  }
+  for (int j = done + tid; j < a.top; j += kCtaThreads) out[j] = -1;
+}
+
+size_t cta_smem(int K) { return align_up(static_cast<size_t>(K) * 13, 16); }
+
+struct SelectLayout {
+  size_t scores, q_norm, c_norm, total;
+  int ctiles;
+};
+
+SelectLayout select_layout(int64_t R, int64_t Nq, int64_t K) {
+  SelectLayout l{};
+  l.ctiles = static_cast<int>((K + kClusters - 1) / kClusters);
+  l.scores = 0;
+  l.q_norm = align_up(static_cast<size_t>(R * Nq * K) * 4, 256);
+  l.c_norm = l.q_norm + align_up(static_cast<size_t>(R * Nq) * 4, 256);
+  l.total = l.c_norm + align_up(static_cast<size_t>(R * l.ctiles) * 4, 256);
+  return l;
+}
+
+template <typename T, int DP, int QW>
+int score_typed(const SelectArgs& a, int64_t R, float* scores, float* qn, float* cn, int ctiles,
+                cudaStream_t stream) {
+  const int qtiles = (a.Nq + 16 * QW - 1) / (16 * QW);
+  const int smem = (kClusters + 2 * 16 * QW) * DP * 2;
+  auto kern = score_kernel<T, DP, QW>;
+  FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t blocks = R * qtiles * ctiles;
+  FKC_REQUIRE(blocks <= 2147483647ll, "select: too many tiles");
+  return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(128), smem, stream, a, scores,
+                    qn, cn, ctiles, qtiles);
+}
+
+template <typename T>
+int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cudaStream_t stream) {
+  const SelectLayout l = select_layout(R, a.Nq, a.K);
+  float* scores = reinterpret_cast<float*>(ws + l.scores);
+  float* qn = reinterpret_cast<float*>(ws + l.q_norm);
+  float* cn = reinterpret_cast<float*>(ws + l.c_norm);
+  // a few queries: one warp's rows, the other warps take clusters
+  const bool few = a.Nq <= 16;
+  if (a.D <= 64)
+    FKC_TRY((few ? score_typed<T, 64, 1> : score_typed<T, 64, 4>)(a, R, scores, qn, cn, l.ctiles,
+                                                                  stream));
+  else
+    FKC_TRY((few ? score_typed<T, 128, 1> : score_typed<T, 128, 4>)(a, R, scores, qn, cn, l.ctiles,
+                                                                    stream));
+  const int64_t queries = R * a.Nq;
+  if (a.K <= 1024) {
+    auto kern = a.K <= 128   ? choose_warp_kernel<T, 4>
+                : a.K <= 256 ? choose_warp_kernel<T, 8>
+                : a.K <= 512 ? choose_warp_kernel<T, 16>
+                             : choose_warp_kernel<T, 32>;
+    return launch_pdl(kern, dim3(static_cast<unsigned>((queries + 3) / 4)), dim3(128), 0, stream, a,
+                      static_cast<const float*>(scores), static_cast<const float*>(qn),
+                      static_cast<const float*>(cn), l.ctiles, sel, queries);
+  }
+  const size_t smem = cta_smem(a.K);
+  FKC_CUDA_TRY(cudaFuncSetAttribute(choose_cta_kernel<T>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(smem)));
+  return launch_pdl(choose_cta_kernel<T>, dim3(static_cast<unsigned>(queries)), dim3(kCtaThreads),
+                    smem, stream, a, static_cast<const float*>(scores),
+                    static_cast<const float*>(qn), static_cast<const float*>(cn), l.ctiles, sel);
+}
+
+}  // namespace
+
+size_t select_workspace_bytes(int64_t R, int64_t Nq, int64_t K) {
+  return select_layout(R, Nq, K).total;
+}
+
+int launch_select(const Args& f, const void* centroids, const float* bias, double scale, int dtype,
+                  int32_t* sel, void* ws, cudaStream_t stream) {
+  SelectArgs a{};
+  a.q = f.q;
+  a.centroids = centroids;
+  a.qs = f.qs;
+  a.offsets = f.offsets;
+  a.order = f.order;
+  a.q_pos = f.q_pos;
+  a.bias = bias;
+  a.Hkv = f.Hkv;
+  a.G = f.G;
+  a.Nq = f.Nq;
+  a.N = f.N;
+  a.K = f.K;
+  a.top = f.top;
+  a.D = f.D;
+  a.scale = scale;
+  const int64_t R = static_cast<int64_t>(f.batch) * f.Hkv;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  return dtype == FKC_DTYPE_F16 ? select_dtype<__half>(a, R, w, sel, stream)
+                                : select_dtype<__nv_bfloat16>(a, R, w, sel, stream);
+}
+
+}  // namespace attn
+}  // namespace fkc

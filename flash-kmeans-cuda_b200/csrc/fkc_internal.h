@@ -240,4 +240,19 @@ int launch_finalize(const float* sums, const int32_t* counts, const void* old_c,
                     float* c_sq_out, void* cext_out, float* shift_out, int64_t B, int64_t K,
                     int64_t D, int dtype, cudaStream_t stream, bool shift_zeroed = false);
 
+// Grouping of positions by id (cluster_group.cu): order (B, N), offsets (B, K + 1).
+// ids are int32 or int64; ids outside [0, K) come last, as -1. B * N and B * (K + 1)
+// below 2^31, ws of group_workspace_bytes.
+size_t group_workspace_bytes(int64_t B, int64_t N, int64_t K);
+int launch_group(const void* ids, bool ids_64, int32_t* order, int32_t* offsets, int64_t B,
+                 int64_t N, int64_t K, void* ws, cudaStream_t stream);
+
+// y = scale * table[ids], and the gradient of the table (cluster_lookup.cu).
+int launch_lookup(const void* table, const void* ids, bool ids_64, void* y, int64_t B, int64_t N,
+                  int64_t K, int64_t D, int dtype, float scale, cudaStream_t stream);
+size_t lookup_grad_workspace_bytes(int64_t B, int64_t N, int64_t K, int64_t D);
+int launch_lookup_grad(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B,
+                       int64_t N, int64_t K, int64_t D, int dtype, float scale, void* ws,
+                       cudaStream_t stream);
+
 }  // namespace fkc

@@ -16,45 +16,13 @@
 // Every call runs on the current PyTorch stream of the inputs' device; argument
 // errors and C-ABI failures raise RuntimeError (the reference's TORCH_CHECK).
 // Scratch memory comes from PyTorch's caching allocator.
-#include <torch/extension.h>
-
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-
 #include <optional>
-#include <stdexcept>
-#include <string>
 
-#include "fkc_capi.h"
+#include "py_common.h"
+
+using namespace fkc_py;
 
 namespace {
-
-void require(bool ok, const char* msg) {
-  if (!ok) throw std::runtime_error(msg);
-}
-
-void check_status(int status, const char* what) {
-  if (status != FKC_OK)
-    throw std::runtime_error(std::string(what) + ": " + fkc_status_string(status) + ": " +
-                             fkc_last_error());
-}
-
-int dtype_code(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kHalf: return FKC_DTYPE_F16;
-    case at::kBFloat16: return FKC_DTYPE_BF16;
-    case at::kFloat: return FKC_DTYPE_F32;
-    default:
-      throw std::runtime_error(std::string("unsupported dtype ") +
-                               c10::toString(t.scalar_type()) +
-                               " (expected float16, bfloat16 or float32)");
-  }
-}
-
-fkc_stream_t stream_of(const at::Tensor& t) {
-  return reinterpret_cast<fkc_stream_t>(
-      at::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
 
 at::Tensor euclid_assign(const at::Tensor& x, const at::Tensor& centroids,
                          const at::Tensor& x_sq, const at::Tensor& c_sq,
@@ -189,4 +157,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("centroid_finalize", &centroid_finalize, py::arg("centroid_sums"),
         py::arg("centroid_counts"), py::arg("old_centroids"), py::arg("out") = py::none(),
         "new = counts > 0 ? sums / counts : old, in old's dtype");
+  fkc_py::bind_clusters(m);
 }

@@ -73,7 +73,36 @@ _SIGNATURES = {
     "fkc_multimem_step_wait": (c_int, [c_vp, ctypes.c_uint32, c_int, c_vp]),
     "fkc_lloyd_run": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, ctypes.c_float,
                               c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_size, c_vp]),
+    "fkc_cluster_order_workspace_size": (c_size, [c_i64, c_i64, c_i64]),
+    "fkc_cluster_order": (c_int, [c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_size,
+                                  c_vp]),
+    "fkc_cluster_lookup": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_int,
+                                   ctypes.c_float, c_vp]),
+    "fkc_cluster_lookup_grad_workspace_size": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "fkc_cluster_lookup_grad": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                        c_int, ctypes.c_float, c_vp, c_size, c_vp]),
+    # c_vp: a fkc_attention_desc (AttentionDesc below)
+    "fkc_cluster_select_workspace_size": (c_size, [c_vp]),
+    "fkc_cluster_select": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "fkc_cluster_attention_workspace_size": (c_size, [c_vp]),
+    "fkc_cluster_attention": (c_int, [c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "fkc_cluster_attention_grad_workspace_size": (c_size, [c_vp]),
+    "fkc_cluster_attention_grad": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                           c_size, c_vp]),
 }
+
+
+class AttentionDesc(ctypes.Structure):
+    """fkc_attention_desc of ``include/fkc_capi.h``."""
+
+    _fields_ = (
+        [(n, c_vp) for n in ("q", "k", "v")]
+        + [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+        + [(n, c_vp) for n in ("sel", "order", "offsets", "q_pos")]
+        + [(n, c_i64) for n in ("batch", "q_heads", "kv_heads", "n_queries", "n_keys",
+                                "n_clusters", "top_k", "head_dim")]
+        + [("dtype", c_int), ("scale", ctypes.c_double)]
+    )
 
 EXPORTED = tuple(_SIGNATURES)
 

@@ -313,6 +313,89 @@ FKC_CAPI_EXPORT int fkc_lloyd_run(const void* x, void* centroids, int32_t* ids, 
                                   int dtype, void* workspace, size_t workspace_bytes,
                                   fkc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Operators on clustered rows (no counterpart in the reference): what a model
+ * does with the labels and centroids of a clustering.
+ *
+ * Grouping: order (B,N) lists the positions of every cluster in ascending
+ *   order, cluster after cluster; offsets (B,K+1): first slot of each cluster.
+ *   ids (B,N) int32, or int64 with ids_64 != 0. An id outside [0,K) belongs to
+ *   no cluster: the slots from offsets[b,K] on hold -1. Deterministic.
+ * ---------------------------------------------------------------------- */
+FKC_CAPI_EXPORT size_t fkc_cluster_order_workspace_size(int64_t B, int64_t N, int64_t K);
+FKC_CAPI_EXPORT int fkc_cluster_order(const void* ids, int ids_64, int32_t* order,
+                                      int32_t* offsets, int64_t B, int64_t N, int64_t K,
+                                      void* workspace, size_t workspace_bytes,
+                                      fkc_stream_t stream);
+
+/* Lookup: y[b,n,:] = scale * table[b,ids[b,n],:], zeros for an id outside [0,K).
+ *   table (B,K,D) and y (B,N,D) of `dtype`, computed in fp32.
+ * Gradient: dtable[b,k,:] = scale * sum of dy[b,n,:] over the n with
+ *   ids[b,n] = k, summed in fp32 in an order fixed by the ids (deterministic);
+ *   every row of dtable is written. */
+FKC_CAPI_EXPORT int fkc_cluster_lookup(const void* table, const void* ids, int ids_64, void* y,
+                                       int64_t B, int64_t N, int64_t K, int64_t D, int dtype,
+                                       float scale, fkc_stream_t stream);
+FKC_CAPI_EXPORT size_t fkc_cluster_lookup_grad_workspace_size(int64_t B, int64_t N, int64_t K,
+                                                              int64_t D);
+FKC_CAPI_EXPORT int fkc_cluster_lookup_grad(const void* dy, const void* ids, int ids_64,
+                                            void* dtable, int64_t B, int64_t N, int64_t K,
+                                            int64_t D, int dtype, float scale, void* workspace,
+                                            size_t workspace_bytes, fkc_stream_t stream);
+
+/* Selection of clusters and attention over their keys. Rows of clusters are
+ * r = b * kv_heads + h, as a clustering of keys laid out (batch * kv_heads,
+ * n_keys, head_dim) numbers them; query head h reads kv head h / (q_heads /
+ * kv_heads). Strides are in elements, {batch, head, position}; head_dim is
+ * dense, a multiple of 8, at most 128. Rows are 16-byte aligned. */
+typedef struct {
+  const void* q; /* (batch, q_heads, n_queries, head_dim) */
+  const void* k; /* (batch, kv_heads, n_keys, head_dim); attention only, as v */
+  const void* v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int32_t* sel;     /* (batch * kv_heads, n_queries, top_k); attention only. Entries outside
+                             [0, n_clusters) select nothing; a cluster listed twice counts twice. */
+  const int32_t* order;   /* (batch * kv_heads, n_keys), of fkc_cluster_order; every position at
+                             most once. Selection reads it with q_pos only. */
+  const int32_t* offsets; /* (batch * kv_heads, n_clusters + 1) */
+  const int32_t* q_pos;   /* (batch, n_queries) or NULL: the last position a query sees (-1: none);
+                             NULL: every position */
+  int64_t batch, q_heads, kv_heads, n_queries, n_keys, n_clusters, top_k, head_dim;
+  int dtype;    /* FKC_DTYPE_F16 or FKC_DTYPE_BF16 */
+  double scale; /* of q . k and of q . centroid */
+} fkc_attention_desc;
+
+/* sel (batch * kv_heads, n_queries, top_k) int32: the top_k clusters of largest
+ *   score = scale * max over the group's heads of q . centroid + bias,
+ * ascending, -1 behind them. Ties go to the lowest index; the choice is that of
+ * exact arithmetic. Never selected: a cluster without positions, one whose
+ * first position lies behind q_pos, a score of -inf or NaN. centroids
+ * (batch * kv_heads, n_clusters, head_dim) of dtype; bias (batch * kv_heads,
+ * n_clusters) fp32 or NULL (+inf forces a cluster in). n_clusters <= 16384,
+ * top_k <= 1024. */
+FKC_CAPI_EXPORT size_t fkc_cluster_select_workspace_size(const fkc_attention_desc* desc);
+FKC_CAPI_EXPORT int fkc_cluster_select(const fkc_attention_desc* desc, const void* centroids,
+                                       const float* bias, int32_t* sel, void* workspace,
+                                       size_t workspace_bytes, fkc_stream_t stream);
+
+/* out (batch, q_heads, n_queries, head_dim) of dtype, lse (batch, q_heads,
+ * n_queries) fp32: attention over the visible keys of the selected clusters;
+ * zeros and -inf for a query without any. A key that a query does not see has
+ * no influence on it, whatever it holds. top_k <= 1024, top_k * n_keys <= 2^30. */
+FKC_CAPI_EXPORT size_t fkc_cluster_attention_workspace_size(const fkc_attention_desc* desc);
+FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* out, float* lse,
+                                          void* workspace, size_t workspace_bytes,
+                                          fkc_stream_t stream);
+
+/* Gradients of out for dout (contiguous like out), from the forward's out and
+ * lse. dq like out; dk, dv (batch, kv_heads, n_keys, head_dim), zeros where no
+ * query reads. dq may be NULL, and so may dk and dv together. Deterministic. */
+FKC_CAPI_EXPORT size_t fkc_cluster_attention_grad_workspace_size(const fkc_attention_desc* desc);
+FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, const void* out,
+                                               const float* lse, const void* dout, void* dq,
+                                               void* dk, void* dv, void* workspace,
+                                               size_t workspace_bytes, fkc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
