@@ -331,6 +331,7 @@ int fwd_dtype(const Args& a, void* out, float* lse, float* ws, cudaStream_t stre
 }  // namespace
 
 size_t forward_workspace_bytes(const Args& a) {
+  if (use_tiles(a)) return tiles_forward_workspace_bytes(a);
   const int nsplit = split_count(a);
   if (nsplit == 1) return 0;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.Hq * a.Nq;
@@ -339,6 +340,7 @@ size_t forward_workspace_bytes(const Args& a) {
 
 int launch_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                    cudaStream_t stream) {
+  if (use_tiles(a)) return launch_tiles_forward(a, dtype, out, lse, ws, stream);
   return dtype == FKC_DTYPE_F16
              ? fwd_dtype<__half>(a, out, lse, static_cast<float*>(ws), stream)
              : fwd_dtype<__nv_bfloat16>(a, out, lse, static_cast<float*>(ws), stream);

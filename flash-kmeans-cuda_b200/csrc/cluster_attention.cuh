@@ -128,6 +128,11 @@ int launch_select(const Args& a, const void* centroids, const float* bias, doubl
                   int32_t* sel, void* ws, cudaStream_t stream);
 size_t forward_workspace_bytes(const Args& a);
 int launch_forward(const Args& a, int dtype, void* out, float* lse, void* ws, cudaStream_t stream);
+// The form by clusters (cluster_attention_tiles.cu), taken where use_tiles says so.
+bool use_tiles(const Args& a);
+size_t tiles_forward_workspace_bytes(const Args& a);
+int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
+                         cudaStream_t stream);
 size_t backward_workspace_bytes(const Args& a);
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);

@@ -547,8 +547,8 @@ int grad_typed(const Args& a, const T* out, const float* lse, const T* dout, T* 
       FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, delta, dq, stream)));
   }
   if (dk == nullptr) return FKC_OK;
-  FKC_TRY(launch_group(a.sel, false, inv_order, inv_offsets, R, static_cast<int64_t>(a.Nq) * a.top,
-                       a.K, ws + l.group, stream));
+  FKC_TRY(launch_group(a.sel, false, static_cast<int64_t>(a.Nq) * a.top, inv_order, inv_offsets, R,
+                       static_cast<int64_t>(a.Nq) * a.top, a.K, ws + l.group, stream));
   FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
                      tile_off));
   const size_t kv_bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);

@@ -134,7 +134,7 @@ FKC_CAPI_EXPORT int fkc_cluster_order(const void* ids, int ids_64, int32_t* orde
   FKC_REQUIRE(ids_aligned(ids, ids_64), "ids must be aligned to their type");
   FKC_TRY(check_workspace("order", workspace, workspace_bytes, group_workspace_bytes(B, N, K)));
   FKC_TRY(check_device());
-  return launch_group(ids, ids_64 != 0, order, offsets, B, N, K, workspace, as_stream(stream));
+  return launch_group(ids, ids_64 != 0, N, order, offsets, B, N, K, workspace, as_stream(stream));
 }
 
 FKC_CAPI_EXPORT int fkc_cluster_lookup(const void* table, const void* ids, int ids_64, void* y,

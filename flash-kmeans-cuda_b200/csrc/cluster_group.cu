@@ -61,16 +61,17 @@ __device__ __forceinline__ int key_of(Id v, int K) {
 }
 
 template <typename Id>
-__global__ void __launch_bounds__(kThreads) group_hist_kernel(const Id* __restrict__ ids, int N,
-                                                              int K, int R, int C, int shift,
-                                                              int bits, int32_t* __restrict__ hist) {
+__global__ void __launch_bounds__(kThreads) group_hist_kernel(const Id* __restrict__ ids,
+                                                              int64_t stride, int N, int K, int R,
+                                                              int C, int shift, int bits,
+                                                              int32_t* __restrict__ hist) {
   extern __shared__ int32_t cnt32[];
   const int bins = 1 << bits;
   for (int i = threadIdx.x; i < bins; i += kThreads) cnt32[i] = 0;
   __syncthreads();
   pdl_wait();
   const int b = blockIdx.x / C, c = blockIdx.x - b * C;
-  const int64_t rb = static_cast<int64_t>(b) * N;
+  const int64_t rb = static_cast<int64_t>(b) * stride;
   const int r1 = static_cast<int>(min(static_cast<int64_t>(c + 1) * R, static_cast<int64_t>(N)));
   for (int r = c * R + threadIdx.x; r < r1; r += kThreads)
     atomicAdd(&cnt32[(key_of<Id>(ids[rb + r], K) >> shift) & (bins - 1)], 1);
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(1024) group_prefix_kernel(int32_t* __restrict_
 // sorts): the first slot of every cluster.
 template <typename Id>
 __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
-    const Id* __restrict__ keys_in, const int32_t* __restrict__ vals_in,
+    const Id* __restrict__ keys_in, int64_t stride, const int32_t* __restrict__ vals_in,
     const int32_t* __restrict__ hist, const int32_t* __restrict__ total,
     int32_t* __restrict__ keys_out, int32_t* __restrict__ vals_out,
     int32_t* __restrict__ offsets, bool last, int N, int K, int R, int C, int shift, int bits) {
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
   pdl_wait();
   const int b = blockIdx.x / C, c = blockIdx.x - b * C;
   const int64_t rb = static_cast<int64_t>(b) * N;
+  const Id* keys = keys_in + b * stride;
   const int RW = R / kWarps;
   // 64-bit: the last chunk may end past 2^31
   const int64_t q0 = static_cast<int64_t>(c) * R + warp * RW;
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
       int key[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        key[u] = at + u * 32 + lane < r1 ? key_of<Id>(keys_in[rb + at + u * 32 + lane], K) : -1;
+        key[u] = at + u * 32 + lane < r1 ? key_of<Id>(keys[at + u * 32 + lane], K) : -1;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (at + u * 32 >= r1) break;  // warp-uniform
@@ -256,15 +258,15 @@ size_t carve_group(const GroupGeom& g, int64_t B, int64_t N, void* ws, GroupBuff
 
 // One pass: src keys (and values) -> dst.
 template <typename Id>
-int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in,
+int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in, int64_t stride,
                const int32_t* vals_in, int32_t* keys_out, int32_t* vals_out, int32_t* offsets,
                int pass, int64_t B, int64_t N, int64_t K, cudaStream_t stream) {
   const int bins = 1 << g.bits, shift = pass * g.bits;
   const int n = static_cast<int>(N), k = static_cast<int>(K);
   const dim3 grid(static_cast<unsigned>(B * g.C));
   if (g.C > 1) {
-    FKC_TRY(launch_pdl(group_hist_kernel<Id>, grid, dim3(kThreads), bins * 4, stream, keys_in, n, k,
-                       g.R, g.C, shift, g.bits, w.hist));
+    FKC_TRY(launch_pdl(group_hist_kernel<Id>, grid, dim3(kThreads), bins * 4, stream, keys_in,
+                       stride, n, k, g.R, g.C, shift, g.bits, w.hist));
     const int per_row = (bins + 31) / 32;
     FKC_TRY(launch_pdl(group_prefix_kernel, dim3(static_cast<unsigned>(B * per_row)), dim3(1024), 0,
                        stream, w.hist, w.total, bins, g.C, per_row));
@@ -274,25 +276,25 @@ int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in,
     FKC_CUDA_TRY(cudaFuncSetAttribute(group_scatter_kernel<Id>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       static_cast<int>(smem)));
-  return launch_pdl(group_scatter_kernel<Id>, grid, dim3(kThreads), smem, stream, keys_in, vals_in,
+  return launch_pdl(group_scatter_kernel<Id>, grid, dim3(kThreads), smem, stream, keys_in, stride, vals_in,
                     static_cast<const int32_t*>(w.hist), static_cast<const int32_t*>(w.total),
                     keys_out, vals_out, offsets, pass == g.passes - 1, n, k, g.R, g.C, shift,
                     g.bits);
 }
 
 template <typename Id>
-int launch_group_typed(const Id* ids, int32_t* order, int32_t* offsets, int64_t B, int64_t N,
+int launch_group_typed(const Id* ids, int64_t stride, int32_t* order, int32_t* offsets, int64_t B, int64_t N,
                        int64_t K, void* ws, cudaStream_t stream) {
   const GroupGeom g = group_geom(B, N, K);
   GroupBuffers w;
   carve_group(g, B, N, ws, &w);
   if (g.passes == 1)
-    return group_pass<Id>(g, w, ids, nullptr, nullptr, order, offsets, 0, B, N, K, stream);
-  FKC_TRY(group_pass<Id>(g, w, ids, nullptr, w.keys[0], w.vals[0], nullptr, 0, B, N, K, stream));
+    return group_pass<Id>(g, w, ids, stride, nullptr, nullptr, order, offsets, 0, B, N, K, stream);
+  FKC_TRY(group_pass<Id>(g, w, ids, stride, nullptr, w.keys[0], w.vals[0], nullptr, 0, B, N, K, stream));
   int cur = 0;
   for (int p = 1; p < g.passes; ++p, cur ^= 1) {
     const bool last = p == g.passes - 1;
-    FKC_TRY(group_pass<int32_t>(g, w, w.keys[cur], w.vals[cur], w.keys[cur ^ 1],
+    FKC_TRY(group_pass<int32_t>(g, w, w.keys[cur], N, w.vals[cur], w.keys[cur ^ 1],
                                 last ? order : w.vals[cur ^ 1], nullptr, p, B, N, K, stream));
   }
   const int64_t count = B * (K + 1);
@@ -308,12 +310,13 @@ size_t group_workspace_bytes(int64_t B, int64_t N, int64_t K) {
   return carve_group(group_geom(B, N, K), B, N, nullptr, nullptr);
 }
 
-int launch_group(const void* ids, bool ids_64, int32_t* order, int32_t* offsets, int64_t B,
-                 int64_t N, int64_t K, void* ws, cudaStream_t stream) {
+int launch_group(const void* ids, bool ids_64, int64_t stride, int32_t* order, int32_t* offsets,
+                 int64_t B, int64_t N, int64_t K, void* ws, cudaStream_t stream) {
   if (ids_64)
-    return launch_group_typed(static_cast<const int64_t*>(ids), order, offsets, B, N, K, ws,
+    return launch_group_typed(static_cast<const int64_t*>(ids), stride, order, offsets, B, N, K, ws,
                               stream);
-  return launch_group_typed(static_cast<const int32_t*>(ids), order, offsets, B, N, K, ws, stream);
+  return launch_group_typed(static_cast<const int32_t*>(ids), stride, order, offsets, B, N, K, ws,
+                            stream);
 }
 
 }  // namespace fkc

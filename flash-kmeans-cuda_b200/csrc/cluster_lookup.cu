@@ -276,7 +276,7 @@ int grad_typed(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B
   int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + l.offsets);
   float* part = reinterpret_cast<float*>(ws + l.part);
-  FKC_TRY(launch_group(ids, ids_64, order, offsets, B, N, K, ws + l.group, stream));
+  FKC_TRY(launch_group(ids, ids_64, N, order, offsets, B, N, K, ws + l.group, stream));
   const int nvec = static_cast<int>(D / VEC);
   const int log_l = lanes_log2(nvec);
   const bool large = N > 2 * l.Lb;

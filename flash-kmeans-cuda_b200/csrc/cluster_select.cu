@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
   for (int half = 0; half < 2; ++half) {
     const int i = i0 + wq * 16 + half * 8 + g;
     if (i >= a.Nq) continue;
-    const int pos = a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : INT_MAX - 1;
+    const int pos =
+        a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.Nq + i], a.N) : a.N;
     float* row = scores + (static_cast<int64_t>(r) * a.Nq + i) * a.K;
 #pragma unroll
     for (int n = 0; n < NW; ++n)

@@ -241,11 +241,11 @@ int launch_finalize(const float* sums, const int32_t* counts, const void* old_c,
                     int64_t D, int dtype, cudaStream_t stream, bool shift_zeroed = false);
 
 // Grouping of positions by id (cluster_group.cu): order (B, N), offsets (B, K + 1).
-// ids are int32 or int64; ids outside [0, K) come last, as -1. B * N and B * (K + 1)
-// below 2^31, ws of group_workspace_bytes.
+// ids are int32 or int64, their rows `stride` elements apart; ids outside [0, K) come last,
+// as -1. ws of group_workspace_bytes.
 size_t group_workspace_bytes(int64_t B, int64_t N, int64_t K);
-int launch_group(const void* ids, bool ids_64, int32_t* order, int32_t* offsets, int64_t B,
-                 int64_t N, int64_t K, void* ws, cudaStream_t stream);
+int launch_group(const void* ids, bool ids_64, int64_t stride, int32_t* order, int32_t* offsets,
+                 int64_t B, int64_t N, int64_t K, void* ws, cudaStream_t stream);
 
 // y = scale * table[ids], and the gradient of the table (cluster_lookup.cu).
 int launch_lookup(const void* table, const void* ids, bool ids_64, void* y, int64_t B, int64_t N,

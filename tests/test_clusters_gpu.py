@@ -278,6 +278,40 @@ def test_attention(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
     attention_check(clusters, *attention_case(B, Hkv, G, Nq, N, K, D, top, dtype, seed=Nq + D, causal=causal))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("B,Hkv,G,Nq,N,K,D,top", [(1, 2, 4, 700, 1500, 23, 128, 7), (2, 1, 3, 1001, 1300, 17, 72, 5),
+                                                  (1, 1, 16, 400, 2500, 30, 64, 9), (2, 2, 1, 3000, 3001, 100, 32, 4),
+                                                  (1, 1, 24, 300, 1500, 9, 128, 9)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_many_queries(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
+    attention_check(clusters, *attention_case(B, Hkv, G, Nq, N, K, D, top, dtype, seed=Nq + D, causal=causal))
+
+
+def test_attention_rounds(clusters):
+    """So many parts that the queries are taken in rounds."""
+    q, k, v, sel, order, offsets, pos = attention_case(1, 4, 32, 300, 17500, 128, 128, 128, BF)
+    out, lse = clusters.cluster_attention(q, k, v, sel, order, offsets, q_pos=pos, return_lse=True)
+    for h in range(4):
+        heads, row = slice(32 * h, 32 * h + 32), slice(h, h + 1)
+        val, tol = attention_ref(q[:, heads], k[:, row], v[:, row], sel[row], order[row], offsets[row], pos)
+        close(out[:, heads], val["out"], tol["out"], "out")
+        close(lse[:, heads], val["lse"], tol["lse"], "lse")
+
+
+def test_positions_of_any_size(clusters):
+    """q_pos far behind the last key, and below zero."""
+    for args in (attention_case(1, 1, 2, 40, 100, 6, 64, 4, BF), attention_case(1, 1, 4, 900, 900, 12, 64, 6, BF)):
+        q, k, v, sel, order, offsets, pos = args
+        pos[:, ::3] = (1 << 31) - 1
+        pos[:, 1::3] = -(1 << 31)
+        attention_check(clusters, q, k, v, sel, order, offsets, pos)
+        K = offsets.shape[1] - 1
+        cen = randn(1, K, 64, seed=8).to(BF)
+        offsets[:, 3:] = offsets[:, 3:4]  # empty clusters behind the third
+        got = clusters.cluster_select(q, cen, offsets, 5, order=order, q_pos=pos)
+        assert torch.equal(got, select_ref(q, cen, offsets, 5, order, pos))
+
+
 def test_attention_large_clusters(clusters):
     """Clusters of many key tiles, one of them selected by every query."""
     q, k, v, sel, order, offsets, pos = attention_case(1, 1, 4, 400, 3000, 4, 64, 2, BF, drop=0.0)
