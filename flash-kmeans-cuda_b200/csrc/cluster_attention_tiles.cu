@@ -9,37 +9,45 @@
 // joins a query's top parts. So the traffic is D * (2 + 4 + 4) bytes per (query, slot,
 // head) instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster a sixth.
 //
-// A tile's CTA: four warps of 32 rows; Q gathered once; keys and values in tiles of 64,
-// gathered into a double buffer; online softmax over the cluster's tiles in registers
-// (m16n8k16: S = Q K^T, then P straight from the score registers as the A operand).
-// P is rounded to the 16-bit input type for the second product, as its operand type
-// demands.
+// tiles_fwd_kernel is persistent, one CTA per SM, over units of 256 rows (two MMAs of 128)
+// of one cluster: four warps gather Q, and the cluster's keys and values in steps of 128,
+// with 16-byte asynchronous copies (the rows lie anywhere; TMA tiles could not); one
+// thread issues S = Q K^T (tcgen05, both operands in shared memory) and O += P V (P from
+// TMEM, V as MN-major operand) into TMEM; two warpgroups turn S into P in place, a thread a
+// row, with the running maximum and sum in fp32, and write O out. P is rounded to the 16-bit
+// input type for the second product, as its operand type demands.
 #include <algorithm>
 
 #include "cluster_attention.cuh"
+#include "cluster_tiles.cuh"
 
 namespace fkc {
 namespace attn {
 namespace {
 
-constexpr int kRows = 128;  // rows (query, head) per tile
-constexpr int kKeys = 64;   // keys per step
+constexpr int kRows = 2 * kSub;  // rows of a unit
 
-// units[r, j] = (cluster, first row of the tile among the cluster's rows); count[r] of them.
-__global__ void __launch_bounds__(1024) tile_units_kernel(const int32_t* __restrict__ inv_offsets,
-                                                          int2* __restrict__ units,
-                                                          int32_t* __restrict__ count, int K, int G,
+// Appends the units of row r. Which place they get is up to the order of the rows' claims;
+// what a unit computes and writes does not depend on it.
+__global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
+                                                          const int32_t* __restrict__ inv_offsets,
+                                                          Unit* __restrict__ units, int32_t* count,
                                                           int rows, int units_max) {
   __shared__ int warp_total[32];
+  __shared__ int first;
   pdl_wait();
   const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int32_t* of = inv_offsets + static_cast<int64_t>(r) * (K + 1);
-  int2* out = units + static_cast<int64_t>(r) * units_max;
-  int carry = 0;
-  for (int c0 = 0; c0 < K; c0 += 1024) {
+  const int32_t* of = inv_offsets + static_cast<int64_t>(r) * (a.K + 1);
+  for (int c0 = 0; c0 < a.K; c0 += 1024) {
     const int c = c0 + threadIdx.x;
-    int n = 0;
-    if (c < K) n = static_cast<int>((static_cast<int64_t>(of[c + 1] - of[c]) * G + rows - 1) / rows);
+    int s0 = 0, s1 = 0, e0 = 0;
+    int64_t all = 0;
+    if (c < a.K) {
+      cluster_span(a, r, c, s0, s1);
+      e0 = of[c];
+      if (s1 > s0) all = static_cast<int64_t>(of[c + 1] - e0) * a.G;
+    }
+    const int n = static_cast<int>((all + rows - 1) / rows);
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -49,263 +57,391 @@ __global__ void __launch_bounds__(1024) tile_units_kernel(const int32_t* __restr
     __syncthreads();
     if (lane == 31) warp_total[warp] = inc;
     __syncthreads();
-    int at = carry + inc - n;
+    int at = inc - n, sum = 0;
     for (int w = 0; w < 32; ++w) {
       if (w < warp) at += warp_total[w];
-      carry += warp_total[w];
+      sum += warp_total[w];
     }
+    if (threadIdx.x == 0) first = atomicAdd(count, sum);
+    __syncthreads();
+    at += first;
     for (int t = 0; t < n; ++t)
-      if (at + t < units_max) out[at + t] = make_int2(c, t * rows);
+      if (at + t < units_max)  // always, with the workspace of carve_units
+        units[at + t] = Unit{c, t * rows, s0, s1, e0, static_cast<int>(min(static_cast<int64_t>(rows), all - static_cast<int64_t>(t) * rows)), r, 0};
   }
-  if (threadIdx.x == 0) count[r] = min(carry, units_max);
 }
 
-// What a tile of `kRows` rows knows about them.
-struct RowData {
-  int64_t q[kRows];   // element offset of the query row
-  int32_t slot[kRows];  // (query, slot, head) of its part; -1: no row
-  int32_t pos[kRows];   // last position it sees; -1: none
-};
-
+// Shared memory of the forward kernel: operand tiles (1024-byte aligned), then the rest.
 template <int DP>
 struct FwdSmem {
-  static constexpr int kQ = 0;
-  static constexpr int kTile = kKeys * DP * 2;
-  static constexpr int kK = kRows * DP * 2;      // two buffers
-  static constexpr int kV = kK + 2 * kTile;      // two buffers
-  static constexpr int kBytes = kV + 2 * kTile;
+  static constexpr uint32_t kTile = tc_tile_bytes<DP>();
+  static constexpr uint32_t kQ = 0;              // one tile per 128 rows
+  static constexpr uint32_t kK = 2 * kTile;      // two stages
+  static constexpr uint32_t kV = 4 * kTile;      // two stages
+  static constexpr uint32_t kMeta = 6 * kTile;
+  struct Meta {
+    int64_t q[2][kSub];       // element offsets of a sub-tile's query rows
+    int32_t slot[2][2][kSub];  // [sub][parity]: (pair, head) of a row; -1: no row
+    int32_t pos[2][2][kSub];   // last position that it sees; -1: none
+    int32_t key[2][kKeysStep]; // positions of a stage's keys; INT_MAX behind the last
+    int32_t high[2][4];
+    uint64_t kv_full[2], kv_free[2], q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], o_free[2];
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+  };
+  static constexpr uint32_t kBytes = kMeta + sizeof(Meta) + 1024;
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(128, 2) tiles_fwd_kernel(
-    Args a, int i0, int nq, const int32_t* __restrict__ inv_order,
-    const int32_t* __restrict__ inv_offsets, const int2* __restrict__ units,
-    const int32_t* __restrict__ count, float* __restrict__ part_o, float* __restrict__ part_lse,
-    int units_max) {
-  constexpr int KS = DP / 16, CH = DP / 8;
-  using S = FwdSmem<DP>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ RowData rows;
-  __shared__ int s_key[2][kKeys];  // positions of a step's keys; INT_MAX behind the last
-  __shared__ int s_high;           // the largest of the rows' positions
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t4 = lane & 3;
-  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  if (a.D < DP)
-    for (int o = tid * 16; o < S::kBytes; o += 2048)
-      *reinterpret_cast<uint4*>(smem + o) = make_uint4(0, 0, 0, 0);
-  if (tid == 0) s_high = -1;
-  __syncthreads();
-  pdl_wait();
-  const int r = blockIdx.x / units_max, unit = blockIdx.x - r * units_max;
-  if (unit >= count[r]) return;
-  const int2 un = units[static_cast<int64_t>(r) * units_max + unit];
-  const int c = un.x, b = r / a.Hkv, hk = r - b * a.Hkv;
-  const int32_t* iof = inv_offsets + static_cast<int64_t>(r) * (a.K + 1);
-  const int e0 = iof[c];
-  const int64_t rows_all = static_cast<int64_t>(iof[c + 1] - e0) * a.G;
-  int s0, s1;
-  cluster_span(a, r, c, s0, s1);
-  const int steps = (s1 - s0 + kKeys - 1) / kKeys;
-  const int32_t* order = a.order + static_cast<int64_t>(r) * a.N;
-  {
-    const int64_t row = un.y + static_cast<int64_t>(tid);
-    int64_t q = 0;
-    int slot = -1, pos = -1;
-    if (row < rows_all) {
-      const int e = static_cast<int>(row / a.G), h = static_cast<int>(row - static_cast<int64_t>(e) * a.G);
-      const int p = inv_order[static_cast<int64_t>(r) * nq * a.top + e0 + e];
-      const int i = i0 + p / a.top;
-      slot = p * a.G + h;
-      pos = min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N);
-      q = b * a.qs.b + (static_cast<int64_t>(hk) * a.G + h) * a.qs.h + i * a.qs.n;
-      atomicMax(&s_high, pos);
-    }
-    rows.q[tid] = q;
-    rows.slot[tid] = slot;
-    rows.pos[tid] = pos;
-  }
-  auto key_at = [&](int step) {  // threads 0 .. kKeys - 1
-    const int s = s0 + step * kKeys + tid;
-    if (s >= s1) return INT_MAX;
-    const int row = order[s];
-    return row >= 0 && row < a.N ? row : INT_MAX;
-  };
-  if (tid < kKeys) {
-    s_key[0][tid] = steps > 0 ? key_at(0) : INT_MAX;
-    s_key[1][tid] = steps > 1 ? key_at(1) : INT_MAX;
-  }
-  __syncthreads();
-  const int high = s_high;
-  const T* q = static_cast<const T*>(a.q);
-  const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
-  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-  const int dchunks = a.D / 8;
-  auto copy_keys = [&](int step) {
-    const int u = step & 1;
-#pragma unroll
-    for (int it = 0; it < kKeys * CH / 128; ++it) {
-      const int e = it * 128 + tid, key = e / CH, ch = e % CH;
-      if (ch >= dchunks) continue;
-      const int row = s_key[u][key];
-      const bool on = row <= high;  // a key that no row sees is not read
-      const int64_t at = on ? row : 0;
-      mma::cp_async16(base + S::kK + u * S::kTile + tile_at<DP>(key, ch), kb + at * a.ks.n + ch * 8, on);
-      mma::cp_async16(base + S::kV + u * S::kTile + tile_at<DP>(key, ch), vb + at * a.vs.n + ch * 8, on);
-    }
-  };
-#pragma unroll
-  for (int it = 0; it < kRows * CH / 128; ++it) {
-    const int e = it * 128 + tid, row = e / CH, ch = e % CH;
-    if (ch >= dchunks) continue;
-    const bool on = rows.pos[row] >= 0;
-    mma::cp_async16(base + S::kQ + tile_at<DP>(row, ch), q + (on ? rows.q[row] + ch * 8 : 0), on);
-  }
-  if (steps > 0) copy_keys(0);
-  mma::cp_async_commit();
+enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 
-  const int row0 = warp * 32;
-  int pos[2][2];
-  float m[2][2], l[2][2];
-  float o[2][DP / 8][4];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      pos[x][y] = rows.pos[row0 + x * 16 + y * 8 + g];
-      m[x][y] = -INFINITY;
-      l[x][y] = 0.f;
-    }
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
+// Warps 0-3 and 4-7: softmax and output of rows 0-127 and 128-255 of a unit (a thread a
+// row); warp 8: the MMAs; warps 9-12: gathers.
+constexpr int kFwdThreads = 32 * 13;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
+    Args a, int i0, int nq, const int32_t* __restrict__ inv_order, const Unit* __restrict__ units,
+    const int32_t* __restrict__ count, float* __restrict__ part_o, float* __restrict__ part_lse,
+    int* err) {
+  using namespace ptx;
+  using S = FwdSmem<DP>;
+  constexpr int CH = DP / 8;
+  constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t sb = smem_u32(smem);
+  typename S::Meta& mt = *reinterpret_cast<typename S::Meta*>(smem + S::kMeta);
+  volatile int* abort = &mt.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.D < DP) {  // columns past D are never copied: they stay zero
+    for (uint32_t o = threadIdx.x * 16; o < S::kMeta; o += kFwdThreads * 16)
+      *reinterpret_cast<uint4*>(smem + o) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
-  const bool idle = un.y + row0 >= rows_all;  // no row for this warp
-  const float sc = a.scale * kLog2e;
-  for (int step = 0; step < steps; ++step) {
-    mma::cp_async_wait<0>();
-    __syncthreads();  // this step's tiles; the other buffers are free
-    if (step + 1 < steps) copy_keys(step + 1);
-    mma::cp_async_commit();
-    int later = INT_MAX;
-    if (tid < kKeys && step + 2 < steps) later = key_at(step + 2);
-    const int u = step & 1;
-    const int keys = min(kKeys, s1 - s0 - step * kKeys);
-    if (!idle) {
-      const uint32_t kt = base + S::kK + u * S::kTile, vt = base + S::kV + u * S::kTile;
-      float s[2][kKeys / 8][4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[x][n][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        uint32_t fa[2][4];
-        load_a<DP>(fa[0], base + S::kQ, row0, kk);
-        load_a<DP>(fa[1], base + S::kQ, row0 + 16, kk);
-#pragma unroll
-        for (int n = 0; n < kKeys / 8; n += 2) {
-          if (n * 8 >= keys) break;
-          uint32_t f[4];
-          load_b<DP>(f, kt, n * 8, kk);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            mma::m16n8k16<T>(s[x][n], fa[x], f[0], f[1]);
-            mma::m16n8k16<T>(s[x][n + 1], fa[x], f[2], f[3]);
-          }
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(smem_u32(&mt.kv_full[x]), 256);  // each gather thread: its stores, its copies
+      mbar_init(smem_u32(&mt.q_full[x]), 256);
+      mbar_init(smem_u32(&mt.kv_free[x]), 1);
+      mbar_init(smem_u32(&mt.q_free[x]), 1);
+      mbar_init(smem_u32(&mt.s_full[x]), 1);
+      mbar_init(smem_u32(&mt.p_full[x]), 128);
+      mbar_init(smem_u32(&mt.o_full[x]), 1);
+      mbar_init(smem_u32(&mt.o_free[x]), 128);
+    }
+    mbar_init(smem_u32(&mt.drain), 1);
+    mt.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&mt.tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = mt.tmem;  // sub-tile x: S (then P) at 256 x, O at 256 x + 128
+  pdl_wait();
+  const int total = *count;
+  const int stride = gridDim.x;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax, output
+    const int sub = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + sub * 256, t_o = t_s + 128;
+    const float sc = a.scale * kLog2e;
+    uint32_t item = 0, uses = 0, s_uses = 0;
+    bool ok = true;
+    for (int n = blockIdx.x; ok && n < total; n += stride) {
+      const Unit un = load_unit(units + n);
+      const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+      if (un.nrows <= sub * kSub) {
+        item += steps;
+        continue;
+      }
+      ok = warp_mbar_wait(&mt.q_full[sub], uses & 1, abort);
+      if (!ok) {
+        give_up(abort, err, kErrSoftmax);
+        break;
+      }
+      const int slot = mt.slot[sub][uses & 1][row], pos = mt.pos[sub][uses & 1][row];
+      const int pos_min = __reduce_min_sync(0xFFFFFFFFu, slot < 0 ? INT_MAX : pos);
+      float m = -INFINITY, l = 0.f;
+      for (int step = 0; step < steps; ++step, ++item, ++s_uses) {
+        const int st = item & 1;
+        ok = warp_mbar_wait(&mt.kv_full[st], (item >> 1) & 1, abort) &&
+             warp_mbar_wait(&mt.s_full[sub], s_uses & 1, abort);
+        if (!ok) {
+          give_up(abort, err, kErrSoftmax);
+          break;
         }
-      }
-      float top[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
+        tc_fence_after();
+        const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
+        const int32_t* key = mt.key[st];
+        float top = -INFINITY;
+        uint32_t open = 0;  // 32-key chunks that every row of the warp sees whole
 #pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n) {
-        const int2 key = *reinterpret_cast<const int2*>(&s_key[u][n * 8 + t4 * 2]);
+        for (int c = 0; c < kKeysStep / 32; ++c) {
+          if (c * 32 >= keys) break;
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(t_s + c * 32, s);
+          const bool whole = __reduce_max_sync(0xFFFFFFFFu, key[c * 32 + lane]) <= pos_min;
+          tmem_wait_ld();
+          if (whole) {
+            open |= 1u << c;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
+          } else {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            float& a0 = s[x][n][y * 2];
-            float& a1 = s[x][n][y * 2 + 1];
-            a0 = key.x <= pos[x][y] ? a0 * sc : -INFINITY;
-            a1 = key.y <= pos[x][y] ? a1 * sc : -INFINITY;
-            top[x][y] = fmaxf(top[x][y], fmaxf(a0, a1));
-          }
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float v = top[x][y];
-          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
-          const float mn = fmaxf(m[x][y], v);
-          const float from = mn == -INFINITY ? 0.f : mn;
-          const float alpha = exp2f(m[x][y] - from);
-          m[x][y] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              s[x][n][y * 2 + e] = exp2f(s[x][n][y * 2 + e] - from);
-              sum += s[x][n][y * 2 + e];
+            for (int j = 0; j < 32; j += 4) {
+              const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
+              top = fmaxf(top, k4.x <= pos ? __uint_as_float(s[j]) : -INFINITY);
+              top = fmaxf(top, k4.y <= pos ? __uint_as_float(s[j + 1]) : -INFINITY);
+              top = fmaxf(top, k4.z <= pos ? __uint_as_float(s[j + 2]) : -INFINITY);
+              top = fmaxf(top, k4.w <= pos ? __uint_as_float(s[j + 3]) : -INFINITY);
             }
-          l[x][y] = l[x][y] * alpha + sum;
-          if (step > 0)
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) o[x][n][y * 2] *= alpha, o[x][n][y * 2 + 1] *= alpha;
+          }
         }
+        const float mn = fmaxf(m, top * sc);  // the scale is positive
+        const float from = mn == -INFINITY ? 0.f : mn;
+        const float alpha = ex2(m - from);
+        m = mn;
+        if (step > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
+          // the product of the step before has ended: its commit came before this S's
 #pragma unroll
-      for (int j = 0; j < kKeys / 16; ++j) {
-        if (j * 16 >= keys) break;
-        uint32_t p[2][4];
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st_32x32b_x32(t_o + c * 32, o);
+          }
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kKeysStep / 32; ++c) {
+          if (c * 32 >= keys) break;
+          uint32_t s[32], p[16];
+          tmem_ld_32x32b_x32(t_s + c * 32, s);
+          tmem_wait_ld();
+          if (open >> c & 1u) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              s[j] = __float_as_uint(ex2(fmaf(__uint_as_float(s[j]), sc, -from)));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
+              const int k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[j + e] = __float_as_uint(
+                    ex2(k[e] <= pos ? fmaf(__uint_as_float(s[j + e]), sc, -from) : -INFINITY));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float p0 = __uint_as_float(s[2 * j]), p1 = __uint_as_float(s[2 * j + 1]);
+            sum[0] += p0;
+            sum[1] += p1;
+            p[j] = mma::pack2<T>(p0, p1);
+          }
+          tmem_st_32x32b_x16(t_s + c * 16, p);  // over scores that are read already
+        }
+        l = l * alpha + (sum[0] + sum[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&mt.p_full[sub]));
+      }
+      if (!ok) break;
+      ok = warp_mbar_wait(&mt.o_full[sub], uses & 1, abort);
+      if (!ok) {
+        give_up(abort, err, kErrSoftmax);
+        break;
+      }
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = static_cast<int64_t>(un.r) * nq * a.top * a.G + slot;
+      float* out = part_o + at * a.D;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_o + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[j + e]) * inv;
+          if (slot >= 0 && c * 32 + j < a.D) st_global_v8(out + c * 32 + j, v);
+        }
+        __syncwarp();
+      }
+      if (slot >= 0) part_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+      tc_fence_before();
+      mbar_arrive(smem_u32(&mt.o_free[sub]));
+      ++uses;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMAs (one thread)
+    if (lane == 0) {
+      const int dsteps = (a.D + 15) / 16;
+      constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, kSub, DP) | kIdescMnB;
+      uint32_t item = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+      struct Pending {
+        bool has, first, last;
+        int stage, ksteps;
+      } pend[2] = {};
+      bool ok = true;
+      auto product = [&](int sub) {  // O (+)= P V of the pending step
+        Pending& p = pend[sub];
+        if (!p.has) return;
+        p.has = false;
+        ok = ok && mbar_wait(smem_u32(&mt.p_full[sub]), p_uses[sub] & 1, abort);
+        ++p_uses[sub];
+        // the output of the use before: q_uses counts the S of this one already
+        if (ok && p.first) ok = mbar_wait(smem_u32(&mt.o_free[sub]), q_uses[sub] & 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        mma_tmem_rows(tmem + sub * 256 + 128, tmem + sub * 256, sb + S::kV + p.stage * S::kTile,
+                      idesc_o, p.ksteps, p.first);
+        if (p.last) umma_commit(smem_u32(&mt.o_full[sub]));
+      };
+      for (int n = blockIdx.x; ok && n < total; n += stride) {
+        const Unit un = load_unit(units + n);
+        const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+        for (int step = 0; ok && step < steps; ++step, ++item) {
+          const int st = item & 1;
+          const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
+          const int k16 = (keys + 15) / 16;
+          const uint32_t idesc_s = umma_idesc_f16(kBf16, kSub, 16 * k16);
+          for (int sub = 0; sub < 2; ++sub) {
+            product(sub);
+            if (!ok || un.nrows <= sub * kSub) continue;
+            ok = mbar_wait(smem_u32(&mt.kv_full[st]), (item >> 1) & 1, abort);
+            if (ok && step == 0) {
+              ok = mbar_wait(smem_u32(&mt.q_full[sub]), q_uses[sub] & 1, abort);
+              ++q_uses[sub];
+            }
+            if (!ok) break;
+            fence_proxy_async_smem();  // the gathered rows, written by generic copies
+            mma_kmajor<DP>(tmem + sub * 256, sb + S::kQ + sub * S::kTile, sb + S::kK + st * S::kTile,
+                           idesc_s, dsteps);
+            umma_commit(smem_u32(&mt.s_full[sub]));
+            if (step == steps - 1) umma_commit(smem_u32(&mt.q_free[sub]));
+            pend[sub] = {true, step == 0, step == steps - 1, st, k16};
+          }
+          if (ok && item > 0) umma_commit(smem_u32(&mt.kv_free[st ^ 1]));
+        }
+      }
+      for (int sub = 0; sub < 2; ++sub)
+        if (ok) product(sub);
+      if (!ok) give_up(abort, err, kErrMma);
+      umma_commit(smem_u32(&mt.drain));  // nothing is in flight when TMEM is freed
+      const int never = 0;
+      mbar_wait(smem_u32(&mt.drain), 0, &never);
+    }
+  } else {
+    // ------------------------------------------------------------ gathers
+    const int t = threadIdx.x - 9 * 32, w = warp - 9;
+    const T* q = static_cast<const T*>(a.q);
+    const int dchunks = a.D / 8;
+    uint32_t item = 0, uses[2] = {0, 0}, seq = 0;
+    bool ok = true;
+    for (int n = blockIdx.x; ok && n < total; n += stride, ++seq) {
+      const Unit un = load_unit(units + n);
+      const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
+      const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+      const int32_t* order = a.order + static_cast<int64_t>(un.r) * a.N;
+      const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+      const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+      auto key_at = [&](int step) {
+        const int s = un.s0 + step * kKeysStep + t;
+        if (s >= un.s1) return INT_MAX;
+        const int row = order[s];
+        return row >= 0 && row < a.N ? row : INT_MAX;
+      };
+      int key = key_at(0);
+      int64_t qoff[2] = {0, 0};
+      int slot[2] = {-1, -1}, pos[2] = {-1, -1};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int rr = x * kSub + t;
+        if (rr < un.nrows) {
+          const int row = un.row0 + rr, e = row / a.G, h = row - e * a.G;
+          const int p = inv_order[static_cast<int64_t>(un.r) * nq * a.top + un.e0 + e];
+          const int i = i0 + p / a.top;
+          slot[x] = p * a.G + h;
+          pos[x] = min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N);
+          qoff[x] = b * a.qs.b + (static_cast<int64_t>(hk) * a.G + h) * a.qs.h + i * a.qs.n;
+        }
+      }
+      const int hi = __reduce_max_sync(0xFFFFFFFFu, max(pos[0], pos[1]));
+      if (lane == 0) mt.high[seq & 1][w] = hi;
+      named_barrier(1, 128);
+      const int high = max(max(mt.high[seq & 1][0], mt.high[seq & 1][1]),
+                           max(mt.high[seq & 1][2], mt.high[seq & 1][3]));
+      for (int step = 0; ok && step < steps; ++step, ++item) {
+        const int st = item & 1;
+        if (step > 0) key = key_at(step);
+        ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
+        if (!ok) give_up(abort, err, kErrLoad);
+        mt.key[st][t] = key;
+        ok = !named_barrier_any(1, 128, !ok);  // the gather warps leave together
+        if (!ok) break;
+        const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
+        const int its = ((keys + 15) / 16) * 16 * CH / 128;
+        const uint32_t kt = sb + S::kK + st * S::kTile, vt = sb + S::kV + st * S::kTile;
+#pragma unroll 4
+        for (int it = 0; it < its; ++it) {
+          const int e = it * 128 + t, r = e / CH, ch = e % CH;
+          if (ch >= dchunks) continue;
+          const int row = mt.key[st][r];
+          const bool on = row <= high;  // a key that no row sees is not read
+          const int64_t at = on ? row : 0;
+          mma::cp_async16(kt + tc_at(r, ch), kb + at * a.ks.n + ch * 8, on);
+          mma::cp_async16(vt + tc_at(r, ch), vb + at * a.vs.n + ch * 8, on);
+        }
+        cp_async_mbar_arrive(smem_u32(&mt.kv_full[st]));
+        mbar_arrive(smem_u32(&mt.kv_full[st]));
+        if (step > 0) continue;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          p[x][0] = mma::pack2<T>(s[x][2 * j][0], s[x][2 * j][1]);
-          p[x][1] = mma::pack2<T>(s[x][2 * j][2], s[x][2 * j][3]);
-          p[x][2] = mma::pack2<T>(s[x][2 * j + 1][0], s[x][2 * j + 1][1]);
-          p[x][3] = mma::pack2<T>(s[x][2 * j + 1][2], s[x][2 * j + 1][3]);
-        }
-#pragma unroll
-        for (int nd = 0; nd < KS; ++nd) {
-          uint32_t f[4];
-          load_b_trans<DP>(f, vt, j * 16, nd);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            mma::m16n8k16<T>(o[x][2 * nd], p[x], f[0], f[1]);
-            mma::m16n8k16<T>(o[x][2 * nd + 1], p[x], f[2], f[3]);
+          if (un.nrows <= x * kSub) break;
+          ok = warp_mbar_wait(&mt.q_free[x], (uses[x] & 1) ^ 1, abort);
+          if (!ok) give_up(abort, err, kErrLoad);
+          mt.q[x][t] = qoff[x];
+          mt.slot[x][uses[x] & 1][t] = slot[x];
+          mt.pos[x][uses[x] & 1][t] = pos[x];
+          ok = !named_barrier_any(1, 128, !ok);
+          if (!ok) break;
+          const uint32_t qt = sb + S::kQ + x * S::kTile;
+#pragma unroll 4
+          for (int it = 0; it < CH; ++it) {
+            const int e = it * 128 + t, r = e / CH, ch = e % CH;
+            if (ch >= dchunks) continue;
+            const bool on = mt.pos[x][uses[x] & 1][r] >= 0;
+            mma::cp_async16(qt + tc_at(r, ch), q + (on ? mt.q[x][r] + ch * 8 : 0), on);
           }
+          cp_async_mbar_arrive(smem_u32(&mt.q_full[x]));
+          mbar_arrive(smem_u32(&mt.q_full[x]));
+          ++uses[x];
         }
       }
     }
-    __syncthreads();  // all reads of this step's tiles and positions
-    if (tid < kKeys) s_key[u][tid] = later;
+    mma::cp_async_commit();
+    mma::cp_async_wait<0>();
   }
-  mma::cp_async_wait<0>();
-  if (idle) return;
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      float sum = l[x][y];
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      const int slot = rows.slot[row0 + x * 16 + y * 8 + g];
-      if (slot < 0) continue;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = static_cast<int64_t>(r) * nq * a.top * a.G + slot;
-      if (t4 == 0) part_lse[at] = sum == 0.f ? -INFINITY : m[x][y] + log2f(sum);
-      float* row = part_o + at * a.D;
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        const int d = n * 8 + t4 * 2;
-        if (d < a.D)
-          *reinterpret_cast<float2*>(row + d) =
-              make_float2(o[x][n][y * 2] * inv, o[x][n][y * 2 + 1] * inv);
-      }
-    }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 // One warp per (query, head): joins the parts of its clusters, whose log-sum-exps are to base 2.
@@ -327,8 +463,16 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
   const float* pl = part_lse + qi * a.top * a.G + h;  // slot s: + s * G
   const float* po = part_o + (qi * a.top * a.G + h) * a.D;
   float top = -INFINITY;
-  for (int s = lane; s < a.top; s += 32)
-    if (sel[s] >= 0 && sel[s] < a.K) top = fmaxf(top, pl[static_cast<int64_t>(s) * a.G]);
+  uint32_t has = 0;  // bit s of lane l: slot 32 s + l has a part
+  for (int s0 = 0; s0 < a.top; s0 += 32) {
+    const int s = s0 + lane;
+    int from = 0, to = 0;
+    if (s < a.top) cluster_span(a, r, sel[s], from, to);
+    if (to > from) {
+      has |= 1u << (s0 >> 5);
+      top = fmaxf(top, pl[static_cast<int64_t>(s) * a.G]);
+    }
+  }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const float from = top == -INFINITY ? 0.f : top;
@@ -336,8 +480,8 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
   const bool on = lane * 4 < a.D;
 #pragma unroll 4
   for (int s = 0; s < a.top; ++s) {
-    const bool has = sel[s] >= 0 && sel[s] < a.K;
-    const float ls = has ? pl[static_cast<int64_t>(s) * a.G] : -INFINITY;
+    const bool part = __shfl_sync(0xFFFFFFFFu, has, s & 31) >> (s >> 5) & 1u;
+    const float ls = part ? pl[static_cast<int64_t>(s) * a.G] : -INFINITY;
     const float w = ls == -INFINITY ? 0.f : exp2f(ls - from);
     if (ls == -INFINITY) continue;
     sum += w;
@@ -371,58 +515,45 @@ int64_t queries_per_round(const Args& a) {
 }
 
 struct Layout {
-  size_t inv_order, inv_offsets, units, count, part_lse, part_o, group, total;
-  int64_t nq, units_max;
+  UnitPlan plan;
+  size_t part_lse, part_o, total;
+  int64_t nq;
 };
 
-Layout fwd_layout(const Args& a) {
+Layout fwd_layout(const Args& a, uint8_t* ws) {
   Layout l{};
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   l.nq = queries_per_round(a);
-  const int64_t entries = l.nq * a.top;
-  l.units_max = entries * a.G / kRows + std::min<int64_t>(a.K, entries);
-  size_t at = 0;
+  size_t at = carve_units(a, l.nq, kRows, ws, &l.plan);
   auto take = [&](int64_t bytes) {
     const size_t p = at;
     at += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  l.inv_order = take(R * entries * 4);
-  l.inv_offsets = take(R * (a.K + 1) * 4);
-  l.units = take(R * l.units_max * 8);
-  l.count = take(R * 4);
-  l.part_lse = take(R * entries * a.G * 4);
-  l.part_o = take(R * entries * a.G * a.D * 4);
-  l.group = take(static_cast<int64_t>(group_workspace_bytes(R, entries, a.K)));
+  l.part_lse = take(R * l.nq * a.top * a.G * 4);
+  l.part_o = take(R * l.nq * a.top * a.G * a.D * 4);
   l.total = at;
   return l;
 }
 
 template <typename T, int DP>
 int fwd_typed(const Args& a, T* out, float* lse, uint8_t* ws, cudaStream_t stream) {
-  const Layout l = fwd_layout(a);
+  const Layout l = fwd_layout(a, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  int32_t* inv_order = reinterpret_cast<int32_t*>(ws + l.inv_order);
-  int32_t* inv_offsets = reinterpret_cast<int32_t*>(ws + l.inv_offsets);
-  int2* units = reinterpret_cast<int2*>(ws + l.units);
-  int32_t* count = reinterpret_cast<int32_t*>(ws + l.count);
   float* part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   float* part_o = reinterpret_cast<float*>(ws + l.part_o);
   auto kern = tiles_fwd_kernel<T, DP>;
-  const int smem = FwdSmem<DP>::kBytes;
+  const int smem = static_cast<int>(FwdSmem<DP>::kBytes);
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
-    FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, inv_order,
-                         inv_offsets, R, static_cast<int64_t>(nq) * a.top, a.K, ws + l.group, stream));
-    FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream,
-                       static_cast<const int32_t*>(inv_offsets), units, count, a.K, a.G, kRows,
-                       static_cast<int>(l.units_max)));
-    FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(R * l.units_max)), dim3(128), smem, stream, a,
-                       static_cast<int>(i0), nq, static_cast<const int32_t*>(inv_order),
-                       static_cast<const int32_t*>(inv_offsets), static_cast<const int2*>(units),
-                       static_cast<const int32_t*>(count), part_o, part_lse,
-                       static_cast<int>(l.units_max)));
+    FKC_TRY(launch_units(a, i0, nq, kRows, l.plan, stream));
+    const int64_t grid = std::min<int64_t>(sm_count(), l.plan.units_max);
+    FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), smem, stream, a,
+                       static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.inv_order),
+                       static_cast<const Unit*>(l.plan.units),
+                       static_cast<const int32_t*>(l.plan.count), part_o, part_lse,
+                       device_error_word()));
     const int64_t rows = R * nq * a.G;
     FKC_TRY(launch_pdl(tiles_join_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
                        stream, a, static_cast<int>(i0), nq, static_cast<const float*>(part_o),
@@ -440,16 +571,56 @@ int fwd_dtype(const Args& a, void* out, float* lse, void* ws, cudaStream_t strea
 
 }  // namespace
 
+int sm_count() {
+  const DeviceInfo* di = nullptr;
+  return current_device_info(&di) == FKC_OK ? di->sm_count : 148;
+}
+
+size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, UnitPlan* out) {
+  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
+  const int64_t pairs = nq * a.top;
+  UnitPlan p{};
+  // every cluster with pairs may end in a unit that is not full
+  p.units_max = R * (pairs * a.G / rows_per_unit + std::min<int64_t>(a.K, pairs));
+  size_t at = 0;
+  auto take = [&](int64_t bytes) -> void* {
+    void* q = ws != nullptr ? ws + at : nullptr;
+    at += align_up(static_cast<size_t>(bytes), 256);
+    return q;
+  };
+  p.inv_order = static_cast<int32_t*>(take(R * pairs * 4));
+  p.inv_offsets = static_cast<int32_t*>(take(R * (a.K + 1) * 4));
+  p.units = static_cast<Unit*>(take(p.units_max * static_cast<int64_t>(sizeof(Unit))));
+  p.count = static_cast<int32_t*>(take(4));
+  p.group_ws = take(static_cast<int64_t>(group_workspace_bytes(R, pairs, a.K)));
+  if (out != nullptr) *out = p;
+  return at;
+}
+
+int launch_units(const Args& a, int64_t i0, int64_t nq, int rows_per_unit, const UnitPlan& p,
+                 cudaStream_t stream) {
+  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
+  FKC_REQUIRE(p.units_max <= 2147483647ll, "attention: too many tiles");
+  FKC_TRY(launch_zero_fill(p.count, 4, stream));
+  FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
+                       p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
+  return launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
+                    static_cast<const int32_t*>(p.inv_offsets), p.units, p.count, rows_per_unit,
+                    static_cast<int>(p.units_max));
+}
+
 bool use_tiles(const Args& a) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t per_round = queries_per_round(a) * a.top;
   // rows of a cluster fill half a tile, keys of a cluster repay its parts, and there are
   // enough tiles for the GPU
-  return per_round * a.G >= 64ll * a.K && a.N / a.K >= 4 * a.G + 8 &&
-         R * a.Nq * a.top * a.G >= 148ll * kRows;
+  // 32-bit numbers of a row's (pair, head)
+  if (queries_per_round(a) * a.top * a.G > (1ll << 30)) return false;
+  return a.scale > 0.f && per_round * a.G >= 64ll * a.K && a.N / a.K >= 4 * a.G + 8 &&
+         R * a.Nq * a.top * a.G >= 148ll * kSub;
 }
 
-size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a).total; }
+size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a, nullptr).total; }
 
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream) {

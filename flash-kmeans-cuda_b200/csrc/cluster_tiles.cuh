@@ -1,0 +1,127 @@
+// Tiles of attention by clusters (cluster_attention_tiles.cu and its backward): the units
+// of work, and operand tiles gathered row by row into the layout that tcgen05.mma reads.
+//
+// A pair is one entry of sel: query i's slot s, number p = (i - i0) * top + s of its row r.
+// Grouping sel by cluster (cluster_group.cu) brings the pairs of a cluster together; the
+// G heads of its pairs, one after another, are the cluster's rows. A unit is up to 256 of them.
+#pragma once
+
+#include <algorithm>
+
+#include "cluster_attention.cuh"
+#include "fkc_ptx.cuh"
+
+namespace fkc {
+namespace attn {
+
+constexpr int kSub = 128;        // rows of one MMA
+constexpr int kKeysStep = 128;   // keys per step
+
+// One unit: cluster c of row r, whose slots are [s0, s1) and whose pairs start at e0; rows
+// [row0, row0 + nrows) of the cluster.
+struct __align__(16) Unit {
+  int c, row0, s0, s1;
+  int e0, nrows, r, pad;
+};
+
+__device__ __forceinline__ Unit load_unit(const Unit* u) {
+  Unit x;
+  const int4 lo = __ldg(reinterpret_cast<const int4*>(u));
+  const int4 hi = __ldg(reinterpret_cast<const int4*>(u) + 1);
+  x.c = lo.x, x.row0 = lo.y, x.s0 = lo.z, x.s1 = lo.w;
+  x.e0 = hi.x, x.nrows = hi.y, x.r = hi.z, x.pad = 0;
+  return x;
+}
+
+// Operand tile of 128 rows x DP 16-bit elements: column blocks of 64 elements (128 rows x
+// 128 bytes each, 128-byte swizzle). As K-major operand a row is a row; as MN-major
+// operand a row is a k. Byte offset of 16-byte chunk ch of a row:
+__device__ __forceinline__ uint32_t tc_at(int row, int ch) {
+  return static_cast<uint32_t>((ch >> 3) * (128 * kSub) + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+}
+template <int DP>
+constexpr uint32_t tc_tile_bytes() {
+  return kSub * DP * 2;
+}
+
+// D (+)= A B^T over the first `depth` elements (a multiple of 16) of K-major tiles.
+template <int DP>
+__device__ __forceinline__ void mma_kmajor(uint32_t d, uint32_t a_tile, uint32_t b_tile,
+                                           uint32_t idesc, int ksteps) {
+  constexpr uint32_t hi = ptx::umma_desc_hi(1024, ptx::kLayoutSwizzle128B);
+  const uint32_t a = ptx::umma_desc_lo(a_tile), b = ptx::umma_desc_lo(b_tile);
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    if (k >= ksteps) break;
+    const uint32_t o = ((k >> 2) * (128 * kSub) + (k & 3) * 32) >> 4;
+    ptx::umma_f16(d, ptx::umma_desc(a + o, hi), ptx::umma_desc(b + o, hi), idesc, k > 0);
+  }
+}
+
+// D (+)= A B, A [lanes x 16 * ksteps] in TMEM, B the first 16 * ksteps rows of a tile (MN-major).
+__device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a_tmem, uint32_t b_tile,
+                                              uint32_t idesc, int ksteps, bool fresh) {
+  for (int k = 0; k < ksteps; ++k)
+    ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc_mn(b_tile + k * 2048, 128 * kSub), idesc,
+                     !(fresh && k == 0));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Eight floats to a 32-byte aligned address.
+__device__ __forceinline__ void st_global_v8(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// The same; true in all of the threads when `any` is in one.
+__device__ __forceinline__ bool named_barrier_any(int id, int threads, bool any) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(any ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
+
+// Bounded wait of a whole warp; the same answer in every lane.
+__device__ __forceinline__ bool warp_mbar_wait(const uint64_t* bar, uint32_t parity,
+                                               const volatile int* abort) {
+  return __all_sync(0xFFFFFFFFu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort));
+}
+
+// A bounded wait gave up: every role leaves, the host reads the code (fkc_device_status).
+__device__ __forceinline__ void give_up(volatile int* abort, int* err, int code) {
+  *abort = 1;
+  if (err != nullptr) atomicCAS(err, 0, code);
+}
+
+// The grouping and units of a range of queries, in the caller's workspace.
+struct UnitPlan {
+  int32_t* inv_order;    // (R, nq * top) pairs by cluster
+  int32_t* inv_offsets;  // (R, K + 1)
+  Unit* units;
+  int32_t* count;        // of units
+  void* group_ws;
+  int64_t units_max;
+};
+size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, UnitPlan* out);
+// Groups sel of the queries [i0, i0 + nq) and lists the units.
+int launch_units(const Args& a, int64_t i0, int64_t nq, int rows_per_unit, const UnitPlan& p,
+                 cudaStream_t stream);
+int sm_count();
+
+}  // namespace attn
+}  // namespace fkc
