@@ -111,9 +111,8 @@ int* device_error_word() {
   return g_err_word[dev];
 }
 
-int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t dim0,
-                   uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes, uint64_t stride2_bytes,
-                   uint32_t box0, uint32_t box1, CUtensorMapSwizzle swizzle) {
+namespace {
+int need_encode() {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -125,6 +124,14 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
   });
   if (g_encode == nullptr)
     return set_error(FKC_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  return FKC_OK;
+}
+}  // namespace
+
+int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t dim0,
+                   uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes, uint64_t stride2_bytes,
+                   uint32_t box0, uint32_t box1, CUtensorMapSwizzle swizzle) {
+  FKC_TRY(need_encode());
   const cuuint64_t dims[3] = {dim0, dim1, dim2};
   const cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
   const cuuint32_t box[3] = {box0, box1, 1};
@@ -139,6 +146,25 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
                      static_cast<int>(r), static_cast<unsigned long long>(dim0),
                      static_cast<unsigned long long>(dim1), static_cast<unsigned long long>(dim2),
                      box0, box1);
+  return FKC_OK;
+}
+
+int encode_tmap_rows(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t elems,
+                     uint64_t rows, uint64_t stride_bytes) {
+  FKC_TRY(need_encode());
+  const cuuint64_t dims[2] = {elems, rows};
+  const cuuint64_t strides[1] = {stride_bytes};
+  const cuuint32_t box[2] = {64, 1};
+  const cuuint32_t elem_strides[2] = {1, 1};
+  const CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box,
+                              elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FKC_ECUDA, "cuTensorMapEncodeTiled failed (%d): rows {%llu,%llu} of %llu bytes",
+                     static_cast<int>(r), static_cast<unsigned long long>(elems),
+                     static_cast<unsigned long long>(rows),
+                     static_cast<unsigned long long>(stride_bytes));
   return FKC_OK;
 }
 

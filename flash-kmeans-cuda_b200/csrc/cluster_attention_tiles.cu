@@ -10,13 +10,14 @@
 // head) instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster a sixth.
 //
 // tiles_fwd_kernel is persistent, one CTA per SM, over units of 256 rows (two MMAs of 128)
-// of one cluster: four warps gather Q, and the cluster's keys and values in steps of 128,
-// with 16-byte asynchronous copies (the rows lie anywhere; TMA tiles could not); one
+// of one cluster: TMA row gathers (four rows an instruction) fetch Q, and the cluster's keys and
+// values in steps of 128; one
 // thread issues S = Q K^T (tcgen05, both operands in shared memory) and O += P V (P from
 // TMEM, V as MN-major operand) into TMEM; two warpgroups turn S into P in place, a thread a
 // row, with the running maximum and sum in fp32, and write O out. P is rounded to the 16-bit
 // input type for the second product, as its operand type demands.
 #include <algorithm>
+#include <numeric>
 
 #include "cluster_attention.cuh"
 #include "cluster_tiles.cuh"
@@ -80,12 +81,11 @@ struct FwdSmem {
   static constexpr uint32_t kV = 4 * kTile;      // two stages
   static constexpr uint32_t kMeta = 6 * kTile;
   struct Meta {
-    int64_t q[2][kSub];       // element offsets of a sub-tile's query rows
     int32_t slot[2][2][kSub];  // [sub][parity]: (pair, head) of a row; -1: no row
     int32_t pos[2][2][kSub];   // last position that it sees; -1: none
     int32_t key[2][kKeysStep]; // positions of a stage's keys; INT_MAX behind the last
-    int32_t high[2][4];
     uint64_t kv_full[2], kv_free[2], q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], o_free[2];
+    uint64_t m_full[2][2];     // slot and pos of [sub][parity]: the rows of Q run ahead by one use
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -96,17 +96,23 @@ struct FwdSmem {
 enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 
 // Warps 0-3 and 4-7: softmax and output of rows 0-127 and 128-255 of a unit (a thread a
-// row); warp 8: the MMAs; warps 9-12: gathers.
-constexpr int kFwdThreads = 32 * 13;
+// row); warp 8: the MMAs; warp 9 gathers keys and values, warps 10 and 11 the rows of Q.
+constexpr int kFwdThreads = 32 * 12;
+
+// Pair number e of a row's list, and the last position its query sees.
+__device__ __forceinline__ int pair_pos(const Args& a, int b, int i) {
+  return min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N);
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
-    Args a, int i0, int nq, const int32_t* __restrict__ inv_order, const Unit* __restrict__ units,
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+    const __grid_constant__ CUtensorMap tm_v, RowMap rq, RowMap rk, RowMap rv, Args a, int i0, int nq,
+    const int32_t* __restrict__ inv_order, const Unit* __restrict__ units,
     const int32_t* __restrict__ count, float* __restrict__ part_o, float* __restrict__ part_lse,
     int* err) {
   using namespace ptx;
   using S = FwdSmem<DP>;
-  constexpr int CH = DP / 8;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -114,15 +120,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   typename S::Meta& mt = *reinterpret_cast<typename S::Meta*>(smem + S::kMeta);
   volatile int* abort = &mt.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (a.D < DP) {  // columns past D are never copied: they stay zero
-    for (uint32_t o = threadIdx.x * 16; o < S::kMeta; o += kFwdThreads * 16)
-      *reinterpret_cast<uint4*>(smem + o) = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
-  }
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
-      mbar_init(smem_u32(&mt.kv_full[x]), 256);  // each gather thread: its stores, its copies
-      mbar_init(smem_u32(&mt.q_full[x]), 256);
+      mbar_init(smem_u32(&mt.kv_full[x]), 32);  // the lanes of the gathering warp, and the bytes
+      mbar_init(smem_u32(&mt.q_full[x]), 1);
+      mbar_init(smem_u32(&mt.m_full[x][0]), 32);
+      mbar_init(smem_u32(&mt.m_full[x][1]), 32);
       mbar_init(smem_u32(&mt.kv_free[x]), 1);
       mbar_init(smem_u32(&mt.q_free[x]), 1);
       mbar_init(smem_u32(&mt.s_full[x]), 1);
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         item += steps;
         continue;
       }
-      ok = warp_mbar_wait(&mt.q_full[sub], uses & 1, abort);
+      ok = warp_mbar_wait(&mt.m_full[sub][uses & 1], (uses >> 1) & 1, abort);
       if (!ok) {
         give_up(abort, err, kErrSoftmax);
         break;
@@ -327,7 +330,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
               ++q_uses[sub];
             }
             if (!ok) break;
-            fence_proxy_async_smem();  // the gathered rows, written by generic copies
             mma_kmajor<DP>(tmem + sub * 256, sb + S::kQ + sub * S::kTile, sb + S::kK + st * S::kTile,
                            idesc_s, dsteps);
             umma_commit(smem_u32(&mt.s_full[sub]));
@@ -346,94 +348,108 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     }
   } else {
     // ------------------------------------------------------------ gathers
-    const int t = threadIdx.x - 9 * 32, w = warp - 9;
-    const T* q = static_cast<const T*>(a.q);
-    const int dchunks = a.D / 8;
-    uint32_t item = 0, uses[2] = {0, 0}, seq = 0;
+    // What the next unit needs from memory is fetched while this one's copies run.
+    const bool kv = warp == 9;
+    const int sub = warp - 10;
+    const int64_t row_pairs = static_cast<int64_t>(nq) * a.top;
+    uint32_t item = 0, uses = 0;
     bool ok = true;
-    for (int n = blockIdx.x; ok && n < total; n += stride, ++seq) {
-      const Unit un = load_unit(units + n);
-      const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
-      const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
-      const int32_t* order = a.order + static_cast<int64_t>(un.r) * a.N;
-      const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
-      const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-      auto key_at = [&](int step) {
-        const int s = un.s0 + step * kKeysStep + t;
-        if (s >= un.s1) return INT_MAX;
-        const int row = order[s];
-        return row >= 0 && row < a.N ? row : INT_MAX;
-      };
-      int key = key_at(0);
-      int64_t qoff[2] = {0, 0};
-      int slot[2] = {-1, -1}, pos[2] = {-1, -1};
+    Unit un{}, nx{};
+    int idx[4], slot[4], pos[4], high = -1;
+    auto key4 = [&](const Unit& u, int step) {  // keys 4 lane .. of a step
+      const int32_t* order = a.order + static_cast<int64_t>(u.r) * a.N;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int rr = x * kSub + t;
-        if (rr < un.nrows) {
-          const int row = un.row0 + rr, e = row / a.G, h = row - e * a.G;
-          const int p = inv_order[static_cast<int64_t>(un.r) * nq * a.top + un.e0 + e];
-          const int i = i0 + p / a.top;
-          slot[x] = p * a.G + h;
-          pos[x] = min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N);
-          qoff[x] = b * a.qs.b + (static_cast<int64_t>(hk) * a.G + h) * a.qs.h + i * a.qs.n;
+      for (int j = 0; j < 4; ++j) {
+        const int s = u.s0 + step * kKeysStep + lane * 4 + j;
+        const int row = s < u.s1 ? order[s] : -1;
+        idx[j] = row >= 0 && row < a.N ? row : INT_MAX;
+      }
+    };
+    auto prepare = [&](const Unit& u) {
+      const int b = u.r / a.Hkv, hk = u.r - b * a.Hkv;
+      const int32_t* list = inv_order + u.r * row_pairs + u.e0;
+      if (kv) {
+        key4(u, 0);
+        high = -1;  // the last position that a row of the unit sees
+        const int first = u.row0 / a.G, last = (u.row0 + u.nrows - 1) / a.G;
+        for (int e = first + lane; e <= last; e += 32)
+          high = max(high, pair_pos(a, b, i0 + list[e] / a.top));
+        high = __reduce_max_sync(0xFFFFFFFFu, high);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int rr = sub * kSub + lane * 4 + j;
+          slot[j] = -1, pos[j] = -1, idx[j] = rq.rows;
+          if (rr < u.nrows) {
+            const int row = u.row0 + rr, e = row / a.G, h = row - e * a.G;
+            const int p = list[e], i = i0 + p / a.top;
+            slot[j] = p * a.G + h;
+            pos[j] = pair_pos(a, b, i);
+            if (pos[j] >= 0) idx[j] = rq.at(b, hk * a.G + h, i);
+          }
         }
       }
-      const int hi = __reduce_max_sync(0xFFFFFFFFu, max(pos[0], pos[1]));
-      if (lane == 0) mt.high[seq & 1][w] = hi;
-      named_barrier(1, 128);
-      const int high = max(max(mt.high[seq & 1][0], mt.high[seq & 1][1]),
-                           max(mt.high[seq & 1][2], mt.high[seq & 1][3]));
-      for (int step = 0; ok && step < steps; ++step, ++item) {
-        const int st = item & 1;
-        if (step > 0) key = key_at(step);
-        ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
-        if (!ok) give_up(abort, err, kErrLoad);
-        mt.key[st][t] = key;
-        ok = !named_barrier_any(1, 128, !ok);  // the gather warps leave together
-        if (!ok) break;
-        const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
-        const int its = ((keys + 15) / 16) * 16 * CH / 128;
-        const uint32_t kt = sb + S::kK + st * S::kTile, vt = sb + S::kV + st * S::kTile;
-#pragma unroll 4
-        for (int it = 0; it < its; ++it) {
-          const int e = it * 128 + t, r = e / CH, ch = e % CH;
-          if (ch >= dchunks) continue;
-          const int row = mt.key[st][r];
-          const bool on = row <= high;  // a key that no row sees is not read
-          const int64_t at = on ? row : 0;
-          mma::cp_async16(kt + tc_at(r, ch), kb + at * a.ks.n + ch * 8, on);
-          mma::cp_async16(vt + tc_at(r, ch), vb + at * a.vs.n + ch * 8, on);
-        }
-        cp_async_mbar_arrive(smem_u32(&mt.kv_full[st]));
-        mbar_arrive(smem_u32(&mt.kv_full[st]));
-        if (step > 0) continue;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (un.nrows <= x * kSub) break;
-          ok = warp_mbar_wait(&mt.q_free[x], (uses[x] & 1) ^ 1, abort);
-          if (!ok) give_up(abort, err, kErrLoad);
-          mt.q[x][t] = qoff[x];
-          mt.slot[x][uses[x] & 1][t] = slot[x];
-          mt.pos[x][uses[x] & 1][t] = pos[x];
-          ok = !named_barrier_any(1, 128, !ok);
+    };
+    if (blockIdx.x < total) {
+      un = load_unit(units + blockIdx.x);
+      prepare(un);
+    }
+    for (int n = blockIdx.x; ok && n < total; n += stride) {
+      if (n + stride < total) nx = load_unit(units + n + stride);
+      if (kv) {
+        const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
+        const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+        for (int step = 0; step < steps; ++step, ++item) {
+          const int st = item & 1;
+          if (step > 0) key4(un, step);
+          ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
           if (!ok) break;
-          const uint32_t qt = sb + S::kQ + x * S::kTile;
-#pragma unroll 4
-          for (int it = 0; it < CH; ++it) {
-            const int e = it * 128 + t, r = e / CH, ch = e % CH;
-            if (ch >= dchunks) continue;
-            const bool on = mt.pos[x][uses[x] & 1][r] >= 0;
-            mma::cp_async16(qt + tc_at(r, ch), q + (on ? mt.q[x][r] + ch * 8 : 0), on);
+          const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
+          const int quads = ((keys + 15) / 16) * 4;
+          *reinterpret_cast<int4*>(&mt.key[st][lane * 4]) = make_int4(idx[0], idx[1], idx[2], idx[3]);
+          if (lane == 0)
+            mbar_arrive_expect_tx(smem_u32(&mt.kv_full[st]), quads * 4 * 2 * DP * 2);
+          else
+            mbar_arrive(smem_u32(&mt.kv_full[st]));
+          if (lane < quads) {
+            int r[4], v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // a key that no row sees is not read
+              r[j] = idx[j] <= high ? rk.at(b, hk, idx[j]) : rk.rows;
+              v[j] = idx[j] <= high ? rv.at(b, hk, idx[j]) : rv.rows;
+            }
+            gather_rows4<DP>(sb + S::kK + st * S::kTile, &tm_k, &mt.kv_full[st], lane * 4, r[0], r[1],
+                             r[2], r[3]);
+            gather_rows4<DP>(sb + S::kV + st * S::kTile, &tm_v, &mt.kv_full[st], lane * 4, v[0], v[1],
+                             v[2], v[3]);
           }
-          cp_async_mbar_arrive(smem_u32(&mt.q_full[x]));
-          mbar_arrive(smem_u32(&mt.q_full[x]));
-          ++uses[x];
+          __syncwarp();
         }
+      } else if (un.nrows > sub * kSub) {
+        ok = warp_mbar_wait(&mt.q_free[sub], (uses & 1) ^ 1, abort);
+        if (!ok) break;
+        *reinterpret_cast<int4*>(&mt.slot[sub][uses & 1][lane * 4]) =
+            make_int4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<int4*>(&mt.pos[sub][uses & 1][lane * 4]) =
+            make_int4(pos[0], pos[1], pos[2], pos[3]);
+        mbar_arrive(smem_u32(&mt.m_full[sub][uses & 1]));
+        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.q_full[sub]), S::kTile);
+        gather_rows4<DP>(sb + S::kQ + sub * S::kTile, &tm_q, &mt.q_full[sub], lane * 4, idx[0], idx[1],
+                         idx[2], idx[3]);
+        __syncwarp();
+        ++uses;
+      }
+      un = nx;
+      if (n + stride < total) prepare(un);
+    }
+    if (!ok) give_up(abort, err, kErrLoad);
+    // copies in flight end before the CTA does: the MMA warp waits for all of them, and
+    // after a wait that gave up they are waited for here
+    if (!ok || *abort) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {
       }
     }
-    mma::cp_async_commit();
-    mma::cp_async_wait<0>();
   }
   __syncwarp();
   tc_fence_before();
@@ -537,11 +553,16 @@ Layout fwd_layout(const Args& a, uint8_t* ws) {
 }
 
 template <typename T, int DP>
-int fwd_typed(const Args& a, T* out, float* lse, uint8_t* ws, cudaStream_t stream) {
+int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStream_t stream) {
   const Layout l = fwd_layout(a, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   float* part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   float* part_o = reinterpret_cast<float*>(ws + l.part_o);
+  CUtensorMap tm_q, tm_k, tm_v;
+  RowMap rq, rk, rv;
+  FKC_TRY(encode_rows(a.q, a.qs, a.batch, a.Hq, a.Nq, a.D, dtype, &tm_q, &rq));
+  FKC_TRY(encode_rows(a.k, a.ks, a.batch, a.Hkv, a.N, a.D, dtype, &tm_k, &rk));
+  FKC_TRY(encode_rows(a.v, a.vs, a.batch, a.Hkv, a.N, a.D, dtype, &tm_v, &rv));
   auto kern = tiles_fwd_kernel<T, DP>;
   const int smem = static_cast<int>(FwdSmem<DP>::kBytes);
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -549,8 +570,8 @@ int fwd_typed(const Args& a, T* out, float* lse, uint8_t* ws, cudaStream_t strea
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
     FKC_TRY(launch_units(a, i0, nq, kRows, l.plan, stream));
     const int64_t grid = std::min<int64_t>(sm_count(), l.plan.units_max);
-    FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), smem, stream, a,
-                       static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.inv_order),
+    FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), smem, stream, tm_q,
+                       tm_k, tm_v, rq, rk, rv, a, static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.inv_order),
                        static_cast<const Unit*>(l.plan.units),
                        static_cast<const int32_t*>(l.plan.count), part_o, part_lse,
                        device_error_word()));
@@ -563,10 +584,11 @@ int fwd_typed(const Args& a, T* out, float* lse, uint8_t* ws, cudaStream_t strea
 }
 
 template <typename T>
-int fwd_dtype(const Args& a, void* out, float* lse, void* ws, cudaStream_t stream) {
+int fwd_dtype(const Args& a, int dtype, void* out, float* lse, void* ws, cudaStream_t stream) {
   T* o = static_cast<T*>(out);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  return a.D <= 64 ? fwd_typed<T, 64>(a, o, lse, w, stream) : fwd_typed<T, 128>(a, o, lse, w, stream);
+  return a.D <= 64 ? fwd_typed<T, 64>(a, dtype, o, lse, w, stream)
+                   : fwd_typed<T, 128>(a, dtype, o, lse, w, stream);
 }
 
 }  // namespace
@@ -574,6 +596,27 @@ int fwd_dtype(const Args& a, void* out, float* lse, void* ws, cudaStream_t strea
 int sm_count() {
   const DeviceInfo* di = nullptr;
   return current_device_info(&di) == FKC_OK ? di->sm_count : 148;
+}
+
+bool row_map(const Strides& s, int64_t nb, int64_t nh, int64_t nn, int64_t D, RowMap* map,
+             int64_t* unit) {
+  const int64_t u0 = std::gcd(std::gcd(s.b, s.h), s.n);
+  const int64_t u = u0 == 0 ? D : u0;
+  const int64_t last = ((nb - 1) * s.b + (nh - 1) * s.h + (nn - 1) * s.n) / u;
+  if (u < D || last >= 2147483647ll - 1) return false;
+  if (map != nullptr) *map = {s.b / u, s.h / u, s.n / u, static_cast<int>(last + 1)};
+  if (unit != nullptr) *unit = u;
+  return true;
+}
+
+int encode_rows(const void* base, const Strides& s, int64_t nb, int64_t nh, int64_t nn, int64_t D,
+                int dtype, CUtensorMap* tm, RowMap* map) {
+  int64_t unit = 0;
+  FKC_REQUIRE(row_map(s, nb, nh, nn, D, map, &unit), "attention: strides without a common unit");
+  return encode_tmap_rows(
+      tm, dtype == FKC_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+      base, static_cast<uint64_t>(D), static_cast<uint64_t>(map->rows),
+      static_cast<uint64_t>(unit) * 2);
 }
 
 size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, UnitPlan* out) {
@@ -614,6 +657,11 @@ bool use_tiles(const Args& a) {
   const int64_t per_round = queries_per_round(a) * a.top;
   // rows of a cluster fill half a tile, keys of a cluster repay its parts, and there are
   // enough tiles for the GPU
+  // the gathers' maps
+  if (!row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
+      !row_map(a.ks, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr) ||
+      !row_map(a.vs, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr))
+    return false;
   // 32-bit numbers of a row's (pair, head)
   if (queries_per_round(a) * a.top * a.G > (1ll << 30)) return false;
   return a.scale > 0.f && per_round * a.G >= 64ll * a.K && a.N / a.K >= 4 * a.G + 8 &&
@@ -624,8 +672,8 @@ size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a, nullp
 
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream) {
-  return dtype == FKC_DTYPE_F16 ? fwd_dtype<__half>(a, out, lse, ws, stream)
-                                : fwd_dtype<__nv_bfloat16>(a, out, lse, ws, stream);
+  return dtype == FKC_DTYPE_F16 ? fwd_dtype<__half>(a, dtype, out, lse, ws, stream)
+                                : fwd_dtype<__nv_bfloat16>(a, dtype, out, lse, ws, stream);
 }
 
 }  // namespace attn

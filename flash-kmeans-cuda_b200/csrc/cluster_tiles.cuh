@@ -34,11 +34,8 @@ __device__ __forceinline__ Unit load_unit(const Unit* u) {
 }
 
 // Operand tile of 128 rows x DP 16-bit elements: column blocks of 64 elements (128 rows x
-// 128 bytes each, 128-byte swizzle). As K-major operand a row is a row; as MN-major
-// operand a row is a k. Byte offset of 16-byte chunk ch of a row:
-__device__ __forceinline__ uint32_t tc_at(int row, int ch) {
-  return static_cast<uint32_t>((ch >> 3) * (128 * kSub) + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-}
+// 128 bytes each, 128-byte swizzle). As K-major operand a row is a row; as MN-major operand a
+// row is a k. Elements past D are filled with zeros by the copy.
 template <int DP>
 constexpr uint32_t tc_tile_bytes() {
   return kSub * DP * 2;
@@ -106,6 +103,31 @@ __device__ __forceinline__ bool warp_mbar_wait(const uint64_t* bar, uint32_t par
 __device__ __forceinline__ void give_up(volatile int* abort, int* err, int code) {
   *abort = 1;
   if (err != nullptr) atomicCAS(err, 0, code);
+}
+
+// A strided (batch, heads, positions) tensor as rows of a 2-D map: row b * b_ + h * h_ + n * n_,
+// `rows` of them; row number `rows` reads as zeros.
+struct RowMap {
+  int64_t b, h, n;
+  int rows;
+  __device__ __forceinline__ int at(int ib, int ih, int in) const {
+    return static_cast<int>(ib * b + ih * h + in * n);
+  }
+};
+// False where the strides have no common unit of a row's length, or there are 2^31 rows.
+bool row_map(const Strides& s, int64_t nb, int64_t nh, int64_t nn, int64_t D, RowMap* map,
+             int64_t* unit);
+int encode_rows(const void* base, const Strides& s, int64_t nb, int64_t nh, int64_t nn, int64_t D,
+                int dtype, CUtensorMap* tm, RowMap* map);
+
+// Four rows of an operand tile, the rows' 16 * CH bytes in blocks of 64 elements.
+template <int DP>
+__device__ __forceinline__ void gather_rows4(uint32_t tile, const CUtensorMap* tm, const uint64_t* bar,
+                                             int row, int r0, int r1, int r2, int r3) {
+#pragma unroll
+  for (int blk = 0; blk < DP / 64; ++blk)
+    ptx::tma_gather4(tile + blk * (128 * kSub) + row * 128, tm, ptx::smem_u32(bar), blk * 64, r0, r1,
+                     r2, r3);
 }
 
 // The grouping and units of a range of queries, in the caller's workspace.

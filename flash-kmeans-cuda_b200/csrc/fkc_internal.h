@@ -55,6 +55,9 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
                    uint64_t dim0, uint64_t dim1, uint64_t dim2, uint64_t stride1_bytes,
                    uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                    CUtensorMapSwizzle swizzle);
+// 2-D map for gathers of single rows (16-bit elements, boxes of 64 x 1, 128-byte swizzle).
+int encode_tmap_rows(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t elems,
+                     uint64_t rows, uint64_t stride_bytes);
 
 inline size_t dtype_size(int dtype) { return dtype == FKC_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_valid(int dtype) {

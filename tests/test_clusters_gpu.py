@@ -21,6 +21,15 @@ def clusters(cuda_device):
     return clusters
 
 
+@pytest.fixture(autouse=True)
+def no_wait_expired():
+    """No kernel of a test gave up a wait."""
+    yield
+    from flash_kmeans_cuda import _lib
+
+    _lib.device_status()
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
