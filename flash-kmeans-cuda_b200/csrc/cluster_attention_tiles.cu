@@ -26,14 +26,13 @@ namespace fkc {
 namespace attn {
 namespace {
 
-constexpr int kRows = 2 * kSub;  // rows of a unit
-
 // Appends the units of row r. Which place they get is up to the order of the rows' claims;
 // what a unit computes and writes does not depend on it.
 __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
                                                           const int32_t* __restrict__ inv_offsets,
                                                           Unit* __restrict__ units, int32_t* count,
-                                                          int rows, int units_max) {
+                                                          int units_max) {
+  constexpr int rows = kUnitRows;
   __shared__ int warp_total[32];
   __shared__ int first;
   pdl_wait();
@@ -72,6 +71,40 @@ __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
   }
 }
 
+// The rows of the units, one warp a unit: a lane takes rows lane + 32 j.
+__global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, RowMap rq,
+                                                        const int32_t* __restrict__ inv_order,
+                                                        Unit* __restrict__ units,
+                                                        const int32_t* __restrict__ count,
+                                                        int32_t* __restrict__ q_row,
+                                                        int2* __restrict__ slot_pos) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (u >= *count) return;
+  const Unit un = units[u];
+  const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
+  const int32_t* list = inv_order + static_cast<int64_t>(un.r) * nq * a.top + un.e0;
+  int high = -1;
+#pragma unroll
+  for (int j = 0; j < kUnitRows / 32; ++j) {
+    const int rr = j * 32 + lane;
+    int slot = -1, pos = -1, row = rq.rows;
+    if (rr < un.nrows) {
+      const int at = un.row0 + rr, e = at / a.G, h = at - e * a.G;
+      const int p = list[e], i = i0 + p / a.top;
+      slot = p * a.G + h;
+      pos = max(-1, min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N));
+      if (pos >= 0) row = rq.at(b, hk * a.G + h, i);
+    }
+    q_row[u * kUnitRows + rr] = row;
+    slot_pos[u * kUnitRows + rr] = make_int2(slot, pos);
+    high = max(high, pos);
+  }
+  high = __reduce_max_sync(0xFFFFFFFFu, high);
+  if (lane == 0) units[u].high = high;
+}
+
 // Shared memory of the forward kernel: operand tiles (1024-byte aligned), then the rest.
 template <int DP>
 struct FwdSmem {
@@ -81,11 +114,9 @@ struct FwdSmem {
   static constexpr uint32_t kV = 4 * kTile;      // two stages
   static constexpr uint32_t kMeta = 6 * kTile;
   struct Meta {
-    int32_t slot[2][2][kSub];  // [sub][parity]: (pair, head) of a row; -1: no row
-    int32_t pos[2][2][kSub];   // last position that it sees; -1: none
     int32_t key[2][kKeysStep]; // positions of a stage's keys; INT_MAX behind the last
-    uint64_t kv_full[2], kv_free[2], q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], o_free[2];
-    uint64_t m_full[2][2];     // slot and pos of [sub][parity]: the rows of Q run ahead by one use
+    uint64_t k_full[2], v_full[2], kv_free[2], q_full[2], q_free[2];
+    uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -96,21 +127,39 @@ struct FwdSmem {
 enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 
 // Warps 0-3 and 4-7: softmax and output of rows 0-127 and 128-255 of a unit (a thread a
-// row); warp 8: the MMAs; warp 9 gathers keys and values, warps 10 and 11 the rows of Q.
-constexpr int kFwdThreads = 32 * 12;
+// row); warp 8: the MMAs; warps 9, 10: gathers of keys and of values; 11, 12: of Q.
+constexpr int kFwdThreads = 32 * 13;
 
-// Pair number e of a row's list, and the last position its query sees.
-__device__ __forceinline__ int pair_pos(const Args& a, int b, int i) {
-  return min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N);
-}
+// The steps of a CTA's units in turn, the next unit always fetched ahead.
+struct StepIter {
+  const Unit* units;
+  int n, total, stride, step;
+  Unit un, next;
+  __device__ __forceinline__ StepIter(const Unit* u, int first, int count, int str)
+      : units(u), n(first), total(count), stride(str), step(0) {
+    if (n < total) un = load_unit(units + n);
+    if (n + stride < total) next = load_unit(units + n + stride);
+  }
+  __device__ __forceinline__ bool valid() const { return n < total; }
+  __device__ __forceinline__ void advance() {
+    if (++step < un.steps()) return;
+    next_unit();
+  }
+  __device__ __forceinline__ void next_unit() {
+    step = 0;
+    n += stride;
+    un = next;
+    if (n + stride < total) next = load_unit(units + n + stride);
+  }
+};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
     const __grid_constant__ CUtensorMap tm_v, RowMap rq, RowMap rk, RowMap rv, Args a, int i0, int nq,
-    const int32_t* __restrict__ inv_order, const Unit* __restrict__ units,
-    const int32_t* __restrict__ count, float* __restrict__ part_o, float* __restrict__ part_lse,
-    int* err) {
+    const int32_t* __restrict__ q_row, const int2* __restrict__ slot_pos,
+    const Unit* __restrict__ units, const int32_t* __restrict__ count, float* __restrict__ part_o,
+    float* __restrict__ part_lse, int* err) {
   using namespace ptx;
   using S = FwdSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -122,10 +171,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
-      mbar_init(smem_u32(&mt.kv_full[x]), 32);  // the lanes of the gathering warp, and the bytes
+      mbar_init(smem_u32(&mt.k_full[x]), 32);  // the gathering lanes (their keys), and the bytes
+      mbar_init(smem_u32(&mt.v_full[x]), 1);
       mbar_init(smem_u32(&mt.q_full[x]), 1);
-      mbar_init(smem_u32(&mt.m_full[x][0]), 32);
-      mbar_init(smem_u32(&mt.m_full[x][1]), 32);
       mbar_init(smem_u32(&mt.kv_free[x]), 1);
       mbar_init(smem_u32(&mt.q_free[x]), 1);
       mbar_init(smem_u32(&mt.s_full[x]), 1);
@@ -157,33 +205,32 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const float sc = a.scale * kLog2e;
     uint32_t item = 0, uses = 0, s_uses = 0;
     bool ok = true;
-    for (int n = blockIdx.x; ok && n < total; n += stride) {
-      const Unit un = load_unit(units + n);
-      const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+    StepIter it(units, blockIdx.x, total, stride);
+    const int2* meta = slot_pos + sub * kSub + row;
+    int2 ahead = it.valid() ? __ldg(meta + static_cast<int64_t>(it.n) * kUnitRows) : make_int2(-1, -1);
+    for (; ok && it.valid(); it.next_unit()) {
+      const Unit& un = it.un;
+      const int steps = un.steps();
+      const int slot = ahead.x, pos = ahead.y;
+      if (it.n + stride < total) ahead = __ldg(meta + static_cast<int64_t>(it.n + stride) * kUnitRows);
       if (un.nrows <= sub * kSub) {
         item += steps;
         continue;
       }
-      ok = warp_mbar_wait(&mt.m_full[sub][uses & 1], (uses >> 1) & 1, abort);
-      if (!ok) {
-        give_up(abort, err, kErrSoftmax);
-        break;
-      }
-      const int slot = mt.slot[sub][uses & 1][row], pos = mt.pos[sub][uses & 1][row];
       const int pos_min = __reduce_min_sync(0xFFFFFFFFu, slot < 0 ? INT_MAX : pos);
       float m = -INFINITY, l = 0.f;
       for (int step = 0; step < steps; ++step, ++item, ++s_uses) {
         const int st = item & 1;
-        ok = warp_mbar_wait(&mt.kv_full[st], (item >> 1) & 1, abort) &&
+        ok = warp_mbar_wait(&mt.k_full[st], (item >> 1) & 1, abort) &&
              warp_mbar_wait(&mt.s_full[sub], s_uses & 1, abort);
         if (!ok) {
           give_up(abort, err, kErrSoftmax);
           break;
         }
         tc_fence_after();
-        const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
+        const int keys = un.keys(step);
         const int32_t* key = mt.key[st];
-        float top = -INFINITY;
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         uint32_t open = 0;  // 32-key chunks that every row of the warp sees whole
 #pragma unroll
         for (int c = 0; c < kKeysStep / 32; ++c) {
@@ -195,18 +242,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
           if (whole) {
             open |= 1u << c;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
+            for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(s[j]));
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
-              top = fmaxf(top, k4.x <= pos ? __uint_as_float(s[j]) : -INFINITY);
-              top = fmaxf(top, k4.y <= pos ? __uint_as_float(s[j + 1]) : -INFINITY);
-              top = fmaxf(top, k4.z <= pos ? __uint_as_float(s[j + 2]) : -INFINITY);
-              top = fmaxf(top, k4.w <= pos ? __uint_as_float(s[j + 3]) : -INFINITY);
+              tops[0] = fmaxf(tops[0], k4.x <= pos ? __uint_as_float(s[j]) : -INFINITY);
+              tops[1] = fmaxf(tops[1], k4.y <= pos ? __uint_as_float(s[j + 1]) : -INFINITY);
+              tops[2] = fmaxf(tops[2], k4.z <= pos ? __uint_as_float(s[j + 2]) : -INFINITY);
+              tops[3] = fmaxf(tops[3], k4.w <= pos ? __uint_as_float(s[j + 3]) : -INFINITY);
             }
           }
         }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float mn = fmaxf(m, top * sc);  // the scale is positive
         const float from = mn == -INFINITY ? 0.f : mn;
         const float alpha = ex2(m - from);
@@ -223,7 +271,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
             tmem_st_32x32b_x32(t_o + c * 32, o);
           }
         }
-        float sum[2] = {0.f, 0.f};
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kKeysStep / 32; ++c) {
           if (c * 32 >= keys) break;
@@ -248,13 +296,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float p0 = __uint_as_float(s[2 * j]), p1 = __uint_as_float(s[2 * j + 1]);
-            sum[0] += p0;
-            sum[1] += p1;
+            sum[(2 * j) & 3] += p0;
+            sum[(2 * j + 1) & 3] += p1;
             p[j] = mma::pack2<T>(p0, p1);
           }
           tmem_st_32x32b_x16(t_s + c * 16, p);  // over scores that are read already
         }
-        l = l * alpha + (sum[0] + sum[1]);
+        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(smem_u32(&mt.p_full[sub]));
@@ -297,6 +345,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       struct Pending {
         bool has, first, last;
         int stage, ksteps;
+        uint32_t parity;  // of the stage's values
       } pend[2] = {};
       bool ok = true;
       auto product = [&](int sub) {  // O (+)= P V of the pending step
@@ -307,24 +356,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         ++p_uses[sub];
         // the output of the use before: q_uses counts the S of this one already
         if (ok && p.first) ok = mbar_wait(smem_u32(&mt.o_free[sub]), q_uses[sub] & 1, abort);
+        ok = ok && mbar_wait(smem_u32(&mt.v_full[p.stage]), p.parity, abort);
         if (!ok) return;
         tc_fence_after();
         mma_tmem_rows(tmem + sub * 256 + 128, tmem + sub * 256, sb + S::kV + p.stage * S::kTile,
                       idesc_o, p.ksteps, p.first);
         if (p.last) umma_commit(smem_u32(&mt.o_full[sub]));
       };
-      for (int n = blockIdx.x; ok && n < total; n += stride) {
-        const Unit un = load_unit(units + n);
-        const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
+      for (StepIter it(units, blockIdx.x, total, stride); ok && it.valid(); it.next_unit()) {
+        const Unit& un = it.un;
+        const int steps = un.steps();
         for (int step = 0; ok && step < steps; ++step, ++item) {
           const int st = item & 1;
-          const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
-          const int k16 = (keys + 15) / 16;
+          const int k16 = (un.keys(step) + 15) / 16;
           const uint32_t idesc_s = umma_idesc_f16(kBf16, kSub, 16 * k16);
           for (int sub = 0; sub < 2; ++sub) {
             product(sub);
             if (!ok || un.nrows <= sub * kSub) continue;
-            ok = mbar_wait(smem_u32(&mt.kv_full[st]), (item >> 1) & 1, abort);
+            ok = mbar_wait(smem_u32(&mt.k_full[st]), (item >> 1) & 1, abort);
             if (ok && step == 0) {
               ok = mbar_wait(smem_u32(&mt.q_full[sub]), q_uses[sub] & 1, abort);
               ++q_uses[sub];
@@ -334,7 +383,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
                            idesc_s, dsteps);
             umma_commit(smem_u32(&mt.s_full[sub]));
             if (step == steps - 1) umma_commit(smem_u32(&mt.q_free[sub]));
-            pend[sub] = {true, step == 0, step == steps - 1, st, k16};
+            pend[sub] = {true, step == 0, step == steps - 1, st, k16, (item >> 1) & 1};
           }
           if (ok && item > 0) umma_commit(smem_u32(&mt.kv_free[st ^ 1]));
         }
@@ -348,99 +397,66 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     }
   } else {
     // ------------------------------------------------------------ gathers
-    // What the next unit needs from memory is fetched while this one's copies run.
-    const bool kv = warp == 9;
-    const int sub = warp - 10;
-    const int64_t row_pairs = static_cast<int64_t>(nq) * a.top;
-    uint32_t item = 0, uses = 0;
+    // The next step's (or unit's) row numbers are fetched while this one's copies run.
     bool ok = true;
-    Unit un{}, nx{};
-    int idx[4], slot[4], pos[4], high = -1;
-    auto key4 = [&](const Unit& u, int step) {  // keys 4 lane .. of a step
-      const int32_t* order = a.order + static_cast<int64_t>(u.r) * a.N;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int s = u.s0 + step * kKeysStep + lane * 4 + j;
-        const int row = s < u.s1 ? order[s] : -1;
-        idx[j] = row >= 0 && row < a.N ? row : INT_MAX;
-      }
-    };
-    auto prepare = [&](const Unit& u) {
-      const int b = u.r / a.Hkv, hk = u.r - b * a.Hkv;
-      const int32_t* list = inv_order + u.r * row_pairs + u.e0;
-      if (kv) {
-        key4(u, 0);
-        high = -1;  // the last position that a row of the unit sees
-        const int first = u.row0 / a.G, last = (u.row0 + u.nrows - 1) / a.G;
-        for (int e = first + lane; e <= last; e += 32)
-          high = max(high, pair_pos(a, b, i0 + list[e] / a.top));
-        high = __reduce_max_sync(0xFFFFFFFFu, high);
-      } else {
+    if (warp <= 10) {
+      const bool values = warp == 10;
+      const CUtensorMap* tm = values ? &tm_v : &tm_k;
+      const RowMap rm = values ? rv : rk;
+      const uint32_t tiles = sb + (values ? S::kV : S::kK);
+      StepIter it(units, blockIdx.x, total, stride);
+      auto fetch = [&](int (&idx)[4]) {  // positions of keys 4 lane .. of the step
+        const int32_t* order = a.order + static_cast<int64_t>(it.un.r) * a.N;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int rr = sub * kSub + lane * 4 + j;
-          slot[j] = -1, pos[j] = -1, idx[j] = rq.rows;
-          if (rr < u.nrows) {
-            const int row = u.row0 + rr, e = row / a.G, h = row - e * a.G;
-            const int p = list[e], i = i0 + p / a.top;
-            slot[j] = p * a.G + h;
-            pos[j] = pair_pos(a, b, i);
-            if (pos[j] >= 0) idx[j] = rq.at(b, hk * a.G + h, i);
-          }
+          const int s = it.un.s0 + it.step * kKeysStep + lane * 4 + j;
+          const int row = s < it.un.s1 ? __ldg(order + s) : -1;
+          idx[j] = row >= 0 && row < a.N ? row : INT_MAX;
         }
-      }
-    };
-    if (blockIdx.x < total) {
-      un = load_unit(units + blockIdx.x);
-      prepare(un);
-    }
-    for (int n = blockIdx.x; ok && n < total; n += stride) {
-      if (n + stride < total) nx = load_unit(units + n + stride);
-      if (kv) {
-        const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
-        const int steps = (un.s1 - un.s0 + kKeysStep - 1) / kKeysStep;
-        for (int step = 0; step < steps; ++step, ++item) {
-          const int st = item & 1;
-          if (step > 0) key4(un, step);
-          ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
-          if (!ok) break;
-          const int keys = min(kKeysStep, un.s1 - un.s0 - step * kKeysStep);
-          const int quads = ((keys + 15) / 16) * 4;
-          *reinterpret_cast<int4*>(&mt.key[st][lane * 4]) = make_int4(idx[0], idx[1], idx[2], idx[3]);
-          if (lane == 0)
-            mbar_arrive_expect_tx(smem_u32(&mt.kv_full[st]), quads * 4 * 2 * DP * 2);
-          else
-            mbar_arrive(smem_u32(&mt.kv_full[st]));
-          if (lane < quads) {
-            int r[4], v[4];
+      };
+      int idx[4];
+      if (it.valid()) fetch(idx);
+      for (uint32_t item = 0; it.valid(); ++item) {
+        const int st = item & 1;
+        const int b = it.un.r / a.Hkv, hk = it.un.r - b * a.Hkv;
+        const int quads = (it.un.keys(it.step) + 15) / 16 * 4;
+        int rows[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // a key that no row sees is not read
-              r[j] = idx[j] <= high ? rk.at(b, hk, idx[j]) : rk.rows;
-              v[j] = idx[j] <= high ? rv.at(b, hk, idx[j]) : rv.rows;
-            }
-            gather_rows4<DP>(sb + S::kK + st * S::kTile, &tm_k, &mt.kv_full[st], lane * 4, r[0], r[1],
-                             r[2], r[3]);
-            gather_rows4<DP>(sb + S::kV + st * S::kTile, &tm_v, &mt.kv_full[st], lane * 4, v[0], v[1],
-                             v[2], v[3]);
-          }
-          __syncwarp();
-        }
-      } else if (un.nrows > sub * kSub) {
+        for (int j = 0; j < 4; ++j)  // a key that no row sees is not read
+          rows[j] = idx[j] <= it.un.high ? rm.at(b, hk, idx[j]) : rm.rows;
+        const int4 key = make_int4(idx[0], idx[1], idx[2], idx[3]);
+        it.advance();
+        if (it.valid()) fetch(idx);
+        ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
+        if (!ok) break;
+        uint64_t* full = values ? &mt.v_full[st] : &mt.k_full[st];
+        if (!values) *reinterpret_cast<int4*>(&mt.key[st][lane * 4]) = key;
+        if (lane == 0)
+          mbar_arrive_expect_tx(smem_u32(full), quads * 4 * DP * 2);
+        else if (!values)
+          mbar_arrive(smem_u32(full));
+        if (lane < quads)
+          gather_rows4<DP>(tiles + st * S::kTile, tm, full, lane * 4, rows[0], rows[1], rows[2], rows[3]);
+        __syncwarp();
+      }
+    } else {
+      const int sub = warp - 11;
+      const int4* src = reinterpret_cast<const int4*>(q_row) + sub * (kSub / 4) + lane;
+      StepIter it(units, blockIdx.x, total, stride);
+      int4 ahead = it.valid() ? __ldg(src + static_cast<int64_t>(it.n) * (kUnitRows / 4)) : make_int4(0, 0, 0, 0);
+      uint32_t uses = 0;
+      for (; it.valid(); it.next_unit()) {
+        const int4 rows = ahead;
+        if (it.n + stride < total) ahead = __ldg(src + static_cast<int64_t>(it.n + stride) * (kUnitRows / 4));
+        if (it.un.nrows <= sub * kSub) continue;
         ok = warp_mbar_wait(&mt.q_free[sub], (uses & 1) ^ 1, abort);
         if (!ok) break;
-        *reinterpret_cast<int4*>(&mt.slot[sub][uses & 1][lane * 4]) =
-            make_int4(slot[0], slot[1], slot[2], slot[3]);
-        *reinterpret_cast<int4*>(&mt.pos[sub][uses & 1][lane * 4]) =
-            make_int4(pos[0], pos[1], pos[2], pos[3]);
-        mbar_arrive(smem_u32(&mt.m_full[sub][uses & 1]));
         if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.q_full[sub]), S::kTile);
-        gather_rows4<DP>(sb + S::kQ + sub * S::kTile, &tm_q, &mt.q_full[sub], lane * 4, idx[0], idx[1],
-                         idx[2], idx[3]);
+        gather_rows4<DP>(sb + S::kQ + sub * S::kTile, &tm_q, &mt.q_full[sub], lane * 4, rows.x, rows.y,
+                         rows.z, rows.w);
         __syncwarp();
         ++uses;
       }
-      un = nx;
-      if (n + stride < total) prepare(un);
     }
     if (!ok) give_up(abort, err, kErrLoad);
     // copies in flight end before the CTA does: the MMA warp waits for all of them, and
@@ -494,19 +510,28 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
   const float from = top == -INFINITY ? 0.f : top;
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
   const bool on = lane * 4 < a.D;
-#pragma unroll 4
-  for (int s = 0; s < a.top; ++s) {
-    const bool part = __shfl_sync(0xFFFFFFFFu, has, s & 31) >> (s >> 5) & 1u;
-    const float ls = part ? pl[static_cast<int64_t>(s) * a.G] : -INFINITY;
-    const float w = ls == -INFINITY ? 0.f : exp2f(ls - from);
-    if (ls == -INFINITY) continue;
-    sum += w;
-    if (on) {
-      const float4 v = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * a.G * a.D + lane * 4);
-      acc[0] += w * v.x;
-      acc[1] += w * v.y;
-      acc[2] += w * v.z;
-      acc[3] += w * v.w;
+  constexpr int kAhead = 8;  // parts in flight
+  for (int s0 = 0; s0 < a.top; s0 += kAhead) {
+    float4 v[kAhead];
+    float w[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int s = s0 + u;
+      const bool part = s < a.top && (__shfl_sync(0xFFFFFFFFu, has, s & 31) >> (s >> 5) & 1u);
+      w[u] = part ? pl[static_cast<int64_t>(s) * a.G] : -INFINITY;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (part && on)
+        v[u] = __ldcs(reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * a.G * a.D + lane * 4));
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (w[u] == -INFINITY) continue;  // sees nothing of this cluster
+      const float e = exp2f(w[u] - from);
+      sum += e;
+      acc[0] += e * v[u].x;
+      acc[1] += e * v[u].y;
+      acc[2] += e * v[u].z;
+      acc[3] += e * v[u].w;
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -540,7 +565,7 @@ Layout fwd_layout(const Args& a, uint8_t* ws) {
   Layout l{};
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   l.nq = queries_per_round(a);
-  size_t at = carve_units(a, l.nq, kRows, ws, &l.plan);
+  size_t at = carve_units(a, l.nq, ws, &l.plan);
   auto take = [&](int64_t bytes) {
     const size_t p = at;
     at += align_up(static_cast<size_t>(bytes), 256);
@@ -568,10 +593,11 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
-    FKC_TRY(launch_units(a, i0, nq, kRows, l.plan, stream));
+    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, stream));
     const int64_t grid = std::min<int64_t>(sm_count(), l.plan.units_max);
     FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), smem, stream, tm_q,
-                       tm_k, tm_v, rq, rk, rv, a, static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.inv_order),
+                       tm_k, tm_v, rq, rk, rv, a, static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.q_row),
+                       static_cast<const int2*>(l.plan.slot_pos),
                        static_cast<const Unit*>(l.plan.units),
                        static_cast<const int32_t*>(l.plan.count), part_o, part_lse,
                        device_error_word()));
@@ -619,12 +645,12 @@ int encode_rows(const void* base, const Strides& s, int64_t nb, int64_t nh, int6
       static_cast<uint64_t>(unit) * 2);
 }
 
-size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, UnitPlan* out) {
+size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t pairs = nq * a.top;
   UnitPlan p{};
   // every cluster with pairs may end in a unit that is not full
-  p.units_max = R * (pairs * a.G / rows_per_unit + std::min<int64_t>(a.K, pairs));
+  p.units_max = R * (pairs * a.G / kUnitRows + std::min<int64_t>(a.K, pairs));
   size_t at = 0;
   auto take = [&](int64_t bytes) -> void* {
     void* q = ws != nullptr ? ws + at : nullptr;
@@ -635,21 +661,27 @@ size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, Un
   p.inv_offsets = static_cast<int32_t*>(take(R * (a.K + 1) * 4));
   p.units = static_cast<Unit*>(take(p.units_max * static_cast<int64_t>(sizeof(Unit))));
   p.count = static_cast<int32_t*>(take(4));
+  p.q_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
+  p.slot_pos = static_cast<int2*>(take(p.units_max * kUnitRows * 8));
   p.group_ws = take(static_cast<int64_t>(group_workspace_bytes(R, pairs, a.K)));
   if (out != nullptr) *out = p;
   return at;
 }
 
-int launch_units(const Args& a, int64_t i0, int64_t nq, int rows_per_unit, const UnitPlan& p,
+int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p,
                  cudaStream_t stream) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   FKC_REQUIRE(p.units_max <= 2147483647ll, "attention: too many tiles");
   FKC_TRY(launch_zero_fill(p.count, 4, stream));
   FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
                        p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
-  return launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
-                    static_cast<const int32_t*>(p.inv_offsets), p.units, p.count, rows_per_unit,
-                    static_cast<int>(p.units_max));
+  FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
+                     static_cast<const int32_t*>(p.inv_offsets), p.units, p.count,
+                     static_cast<int>(p.units_max)));
+  return launch_pdl(tile_rows_kernel, dim3(static_cast<unsigned>((p.units_max + 7) / 8)), dim3(256), 0,
+                    stream, a, static_cast<int>(i0), static_cast<int>(nq), rq,
+                    static_cast<const int32_t*>(p.inv_order), p.units,
+                    static_cast<const int32_t*>(p.count), p.q_row, p.slot_pos);
 }
 
 bool use_tiles(const Args& a) {

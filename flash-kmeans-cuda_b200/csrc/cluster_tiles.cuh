@@ -18,10 +18,15 @@ constexpr int kSub = 128;        // rows of one MMA
 constexpr int kKeysStep = 128;   // keys per step
 
 // One unit: cluster c of row r, whose slots are [s0, s1) and whose pairs start at e0; rows
-// [row0, row0 + nrows) of the cluster.
+// [row0, row0 + nrows) of the cluster; high: the last position that one of them sees.
 struct __align__(16) Unit {
   int c, row0, s0, s1;
-  int e0, nrows, r, pad;
+  int e0, nrows, r, high;
+
+  __device__ __forceinline__ int steps() const { return (s1 - s0 + kKeysStep - 1) / kKeysStep; }
+  __device__ __forceinline__ int keys(int step) const {
+    return min(kKeysStep, s1 - s0 - step * kKeysStep);
+  }
 };
 
 __device__ __forceinline__ Unit load_unit(const Unit* u) {
@@ -29,7 +34,7 @@ __device__ __forceinline__ Unit load_unit(const Unit* u) {
   const int4 lo = __ldg(reinterpret_cast<const int4*>(u));
   const int4 hi = __ldg(reinterpret_cast<const int4*>(u) + 1);
   x.c = lo.x, x.row0 = lo.y, x.s0 = lo.z, x.s1 = lo.w;
-  x.e0 = hi.x, x.nrows = hi.y, x.r = hi.z, x.pad = 0;
+  x.e0 = hi.x, x.nrows = hi.y, x.r = hi.z, x.high = hi.w;
   return x;
 }
 
@@ -130,18 +135,23 @@ __device__ __forceinline__ void gather_rows4(uint32_t tile, const CUtensorMap* t
                      r2, r3);
 }
 
-// The grouping and units of a range of queries, in the caller's workspace.
+// The grouping, units and rows of a range of queries, in the caller's workspace. Unit u's row
+// j is entry kUnitRows * u + j of the rows' arrays.
+constexpr int kUnitRows = 2 * kSub;
 struct UnitPlan {
   int32_t* inv_order;    // (R, nq * top) pairs by cluster
   int32_t* inv_offsets;  // (R, K + 1)
   Unit* units;
   int32_t* count;        // of units
+  int32_t* q_row;        // row of Q's map; the one past its last for a row that sees nothing
+  int2* slot_pos;        // (pair, head) number within r, or -1 past the unit's last row; last
+                         // position that the row sees
   void* group_ws;
   int64_t units_max;
 };
-size_t carve_units(const Args& a, int64_t nq, int rows_per_unit, uint8_t* ws, UnitPlan* out);
-// Groups sel of the queries [i0, i0 + nq) and lists the units.
-int launch_units(const Args& a, int64_t i0, int64_t nq, int rows_per_unit, const UnitPlan& p,
+size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out);
+// Groups sel of the queries [i0, i0 + nq), lists the units and fills the rows.
+int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p,
                  cudaStream_t stream);
 int sm_count();
 
