@@ -126,11 +126,11 @@ __device__ __forceinline__ void load_b_trans(uint32_t (&f)[4], uint32_t tile, in
 size_t select_workspace_bytes(int64_t R, int64_t Nq, int64_t K);
 int launch_select(const Args& a, const void* centroids, const float* bias, double scale, int dtype,
                   int32_t* sel, void* ws, cudaStream_t stream);
-size_t forward_workspace_bytes(const Args& a);
+size_t forward_workspace_bytes(const Args& a, int dtype);
 int launch_forward(const Args& a, int dtype, void* out, float* lse, void* ws, cudaStream_t stream);
 // The form by clusters (cluster_attention_tiles.cu), taken where use_tiles says so.
 bool use_tiles(const Args& a);
-size_t tiles_forward_workspace_bytes(const Args& a);
+size_t tiles_forward_workspace_bytes(const Args& a, int dtype);
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream);
 size_t backward_workspace_bytes(const Args& a);

@@ -26,18 +26,37 @@ namespace fkc {
 namespace attn {
 namespace {
 
+__global__ void __launch_bounds__(256) tile_init_kernel(int64_t* count, int32_t* __restrict__ pair_row,
+                                                        int64_t pairs) {
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i == 0) *count = 0;
+  for (int64_t p = i; p < pairs; p += static_cast<int64_t>(gridDim.x) * 256) pair_row[p] = -1;
+}
+
 // Appends the units of row r. Which place they get is up to the order of the rows' claims;
 // what a unit computes and writes does not depend on it.
 __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
                                                           const int32_t* __restrict__ inv_offsets,
-                                                          Unit* __restrict__ units, int32_t* count,
+                                                          Unit* __restrict__ units, int64_t* count,
+                                                          int32_t* __restrict__ cum, int i0, int nq,
                                                           int units_max) {
   constexpr int rows = kUnitRows;
   __shared__ int warp_total[32];
-  __shared__ int first;
+  __shared__ unsigned long long warp_sum[32];
+  __shared__ unsigned long long first;
   pdl_wait();
   const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t* of = inv_offsets + static_cast<int64_t>(r) * (a.K + 1);
+  int high = a.q_pos != nullptr ? -1 : a.N;
+  if (a.q_pos != nullptr) {
+    const int32_t* pos = a.q_pos + static_cast<int64_t>(r / a.Hkv) * a.Nq + i0;
+    for (int i = threadIdx.x; i < nq; i += 1024) high = max(high, min(pos[i], a.N));
+    high = __reduce_max_sync(0xFFFFFFFFu, high);
+    if (lane == 0) warp_total[warp] = high;
+    __syncthreads();
+    for (int w = 0; w < 32; ++w) high = max(high, warp_total[w]);
+  }
   for (int c0 = 0; c0 < a.K; c0 += 1024) {
     const int c = c0 + threadIdx.x;
     int s0 = 0, s1 = 0, e0 = 0;
@@ -47,62 +66,83 @@ __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
       e0 = of[c];
       if (s1 > s0) all = static_cast<int64_t>(of[c + 1] - e0) * a.G;
     }
+    // units, and their cost above 2^32
     const int n = static_cast<int>((all + rows - 1) / rows);
-    int inc = n;
+    Unit un{c, 0, s0, s1, e0, 0, r, high};
+    const unsigned long long own =
+        (static_cast<unsigned long long>(n) * un.cost() << 32) | static_cast<unsigned>(n);
+    unsigned long long inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
       if (lane >= o) inc += u;
     }
     __syncthreads();
-    if (lane == 31) warp_total[warp] = inc;
+    if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
-    int at = inc - n, sum = 0;
+    unsigned long long at = inc - own, sum = 0;
     for (int w = 0; w < 32; ++w) {
-      if (w < warp) at += warp_total[w];
-      sum += warp_total[w];
+      if (w < warp) at += warp_sum[w];
+      sum += warp_sum[w];
     }
-    if (threadIdx.x == 0) first = atomicAdd(count, sum);
+    if (threadIdx.x == 0) first = atomicAdd(reinterpret_cast<unsigned long long*>(count), sum);
     __syncthreads();
     at += first;
-    for (int t = 0; t < n; ++t)
-      if (at + t < units_max)  // always, with the workspace of carve_units
-        units[at + t] = Unit{c, t * rows, s0, s1, e0, static_cast<int>(min(static_cast<int64_t>(rows), all - static_cast<int64_t>(t) * rows)), r, 0};
+    for (int t = 0; t < n; ++t) {
+      const int64_t u = static_cast<int64_t>(at & 0xFFFFFFFFu) + t;
+      un.row0 = t * rows;
+      un.nrows = static_cast<int>(min(static_cast<int64_t>(rows), all - static_cast<int64_t>(t) * rows));
+      if (u < units_max) {  // always, with the workspace of carve_units
+        units[u] = un;
+        cum[u] = static_cast<int32_t>((at >> 32) + static_cast<unsigned long long>(t) * un.cost());
+      }
+    }
   }
 }
 
 // The rows of the units, one warp a unit: a lane takes rows lane + 32 j.
 __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, RowMap rq,
                                                         const int32_t* __restrict__ inv_order,
-                                                        Unit* __restrict__ units,
-                                                        const int32_t* __restrict__ count,
+                                                        const Unit* __restrict__ units,
+                                                        const int64_t* __restrict__ count,
+                                                        const int32_t* __restrict__ cum,
+                                                        int32_t* __restrict__ start, int ctas,
                                                         int32_t* __restrict__ q_row,
-                                                        int2* __restrict__ slot_pos) {
+                                                        int32_t* __restrict__ row_pos,
+                                                        int32_t* __restrict__ pair_row) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (u >= *count) return;
+  const int64_t total = *count & 0xFFFFFFFFll, cost = *count >> 32;
+  if (u == 0 && total == 0)
+    for (int j = lane; j <= ctas; j += 32) start[j] = 0;
+  if (u >= total) return;
   const Unit un = units[u];
+  {
+    // CTA j starts at the first unit whose cost begins at j / ctas of the whole or later
+    const int64_t to = cum[u], from = u == 0 ? -1 : cum[u - 1];
+    const int64_t j0 = u == 0 ? 0 : from * ctas / cost + 1;
+    for (int64_t j = j0 + lane; j <= ctas && j * cost <= to * ctas; j += 32) start[j] = static_cast<int32_t>(u);
+    if (u == total - 1)
+      for (int64_t j = to * ctas / cost + 1 + lane; j <= ctas; j += 32) start[j] = static_cast<int32_t>(total);
+  }
   const int b = un.r / a.Hkv, hk = un.r - b * a.Hkv;
-  const int32_t* list = inv_order + static_cast<int64_t>(un.r) * nq * a.top + un.e0;
-  int high = -1;
+  const int64_t pairs0 = static_cast<int64_t>(un.r) * nq * a.top;
+  const int32_t* list = inv_order + pairs0 + un.e0;
 #pragma unroll
   for (int j = 0; j < kUnitRows / 32; ++j) {
     const int rr = j * 32 + lane;
-    int slot = -1, pos = -1, row = rq.rows;
+    int pos = -1, row = rq.rows;
     if (rr < un.nrows) {
       const int at = un.row0 + rr, e = at / a.G, h = at - e * a.G;
       const int p = list[e], i = i0 + p / a.top;
-      slot = p * a.G + h;
+      if (h == 0) pair_row[pairs0 + p] = static_cast<int32_t>(u * kUnitRows + rr);
       pos = max(-1, min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N));
       if (pos >= 0) row = rq.at(b, hk * a.G + h, i);
     }
     q_row[u * kUnitRows + rr] = row;
-    slot_pos[u * kUnitRows + rr] = make_int2(slot, pos);
-    high = max(high, pos);
+    row_pos[u * kUnitRows + rr] = pos;
   }
-  high = __reduce_max_sync(0xFFFFFFFFu, high);
-  if (lane == 0) units[u].high = high;
 }
 
 // Shared memory of the forward kernel: operand tiles (1024-byte aligned), then the rest.
@@ -112,7 +152,8 @@ struct FwdSmem {
   static constexpr uint32_t kQ = 0;              // one tile per 128 rows
   static constexpr uint32_t kK = 2 * kTile;      // two stages
   static constexpr uint32_t kV = 4 * kTile;      // two stages
-  static constexpr uint32_t kMeta = 6 * kTile;
+  static constexpr uint32_t kOut = 6 * kTile;    // 4 KB per output warp
+  static constexpr uint32_t kMeta = kOut + 8 * 4096;
   struct Meta {
     int32_t key[2][kKeysStep]; // positions of a stage's keys; INT_MAX behind the last
     uint64_t k_full[2], v_full[2], kv_free[2], q_full[2], q_free[2];
@@ -127,39 +168,58 @@ struct FwdSmem {
 enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 
 // Warps 0-3 and 4-7: softmax and output of rows 0-127 and 128-255 of a unit (a thread a
-// row); warp 8: the MMAs; warps 9, 10: gathers of keys and of values; 11, 12: of Q.
-constexpr int kFwdThreads = 32 * 13;
+// row); warp 8: the MMAs; warps 9, 10: gathers of keys and of values; 11-14: of Q, 64 rows
+// each (a gather takes its warp some 70 cycles to issue, so they are spread over warps).
+constexpr int kFwdThreads = 32 * 15;
 
-// The steps of a CTA's units in turn, the next unit always fetched ahead.
-struct StepIter {
+// A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn, the next one always
+// fetched ahead. Keys and values are loaded into two stages, load number `load` into
+// stage load & 1; a unit of the same cluster as the one before it, whose steps both
+// stages hold, uses them again.
+struct UnitIter {
   const Unit* units;
-  int n, total, stride, step;
+  int n, total;
+  uint32_t load;        // number of the unit's first step among the loads
+  bool again, keep;     // the unit uses the loads of the one before; the next one will use its
   Unit un, next;
-  __device__ __forceinline__ StepIter(const Unit* u, int first, int count, int str)
-      : units(u), n(first), total(count), stride(str), step(0) {
+
+  __device__ __forceinline__ UnitIter(const Unit* u, const int32_t* start)
+      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), load(0), again(false) {
     if (n < total) un = load_unit(units + n);
-    if (n + stride < total) next = load_unit(units + n + stride);
+    look();
+  }
+  __device__ __forceinline__ void look() {
+    keep = false;
+    if (n + 1 >= total) return;
+    next = load_unit(units + n + 1);
+    keep = next.c == un.c && next.r == un.r && un.steps() <= 2;
   }
   __device__ __forceinline__ bool valid() const { return n < total; }
   __device__ __forceinline__ void advance() {
-    if (++step < un.steps()) return;
-    next_unit();
-  }
-  __device__ __forceinline__ void next_unit() {
-    step = 0;
-    n += stride;
+    if (!keep) load += un.steps();
+    again = keep;
+    ++n;
     un = next;
-    if (n + stride < total) next = load_unit(units + n + stride);
+    if (n < total) look();
   }
+};
+
+// A part's output over one cluster as stored: fp32, or for bf16 inputs fp16 values under a
+// power of two of the row's own. Two of its roundings of 2^-11 stay far below the 2^-8
+// of out, and the parts are most of what the two kernels move.
+template <typename T>
+struct Part {
+  static constexpr bool kHalf = !std::is_same<T, __half>::value;
+  static constexpr int kBytes = kHalf ? 2 : 4;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-    const __grid_constant__ CUtensorMap tm_v, RowMap rq, RowMap rk, RowMap rv, Args a, int i0, int nq,
-    const int32_t* __restrict__ q_row, const int2* __restrict__ slot_pos,
-    const Unit* __restrict__ units, const int32_t* __restrict__ count, float* __restrict__ part_o,
-    float* __restrict__ part_lse, int* err) {
+    const __grid_constant__ CUtensorMap tm_v, RowMap rk, RowMap rv, Args a,
+    const int32_t* __restrict__ q_row, const int32_t* __restrict__ row_pos,
+    const Unit* __restrict__ units, const int32_t* __restrict__ start, uint8_t* __restrict__ part_o,
+    float2* __restrict__ part_lse, int* err) {
   using namespace ptx;
   using S = FwdSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -173,7 +233,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&mt.k_full[x]), 32);  // the gathering lanes (their keys), and the bytes
       mbar_init(smem_u32(&mt.v_full[x]), 1);
-      mbar_init(smem_u32(&mt.q_full[x]), 1);
+      mbar_init(smem_u32(&mt.q_full[x]), 2);
       mbar_init(smem_u32(&mt.kv_free[x]), 1);
       mbar_init(smem_u32(&mt.q_free[x]), 1);
       mbar_init(smem_u32(&mt.s_full[x]), 1);
@@ -194,8 +254,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   tc_fence_after();
   const uint32_t tmem = mt.tmem;  // sub-tile x: S (then P) at 256 x, O at 256 x + 128
   pdl_wait();
-  const int total = *count;
-  const int stride = gridDim.x;
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax, output
@@ -203,25 +261,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + sub * 256, t_o = t_s + 128;
     const float sc = a.scale * kLog2e;
-    uint32_t item = 0, uses = 0, s_uses = 0;
+    uint32_t uses = 0, s_uses = 0;
     bool ok = true;
-    StepIter it(units, blockIdx.x, total, stride);
-    const int2* meta = slot_pos + sub * kSub + row;
-    int2 ahead = it.valid() ? __ldg(meta + static_cast<int64_t>(it.n) * kUnitRows) : make_int2(-1, -1);
-    for (; ok && it.valid(); it.next_unit()) {
+    UnitIter it(units, start);
+    const int32_t* meta = row_pos + sub * kSub + row;
+    int ahead = it.valid() ? __ldg(meta + static_cast<int64_t>(it.n) * kUnitRows) : -1;
+    for (; ok && it.valid(); it.advance()) {
       const Unit& un = it.un;
       const int steps = un.steps();
-      const int slot = ahead.x, pos = ahead.y;
-      if (it.n + stride < total) ahead = __ldg(meta + static_cast<int64_t>(it.n + stride) * kUnitRows);
-      if (un.nrows <= sub * kSub) {
-        item += steps;
-        continue;
-      }
-      const int pos_min = __reduce_min_sync(0xFFFFFFFFu, slot < 0 ? INT_MAX : pos);
+      const int pos = ahead;
+      if (it.n + 1 < it.total) ahead = __ldg(meta + static_cast<int64_t>(it.n + 1) * kUnitRows);
+      if (un.nrows <= sub * kSub) continue;
+      const int pos_min =
+          __reduce_min_sync(0xFFFFFFFFu, sub * kSub + row < un.nrows ? pos : INT_MAX);
       float m = -INFINITY, l = 0.f;
-      for (int step = 0; step < steps; ++step, ++item, ++s_uses) {
-        const int st = item & 1;
-        ok = warp_mbar_wait(&mt.k_full[st], (item >> 1) & 1, abort) &&
+      for (int step = 0; step < steps; ++step, ++s_uses) {
+        const uint32_t load = it.load + step;
+        const int st = load & 1;
+        ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
              warp_mbar_wait(&mt.s_full[sub], s_uses & 1, abort);
         if (!ok) {
           give_up(abort, err, kErrSoftmax);
@@ -315,38 +372,73 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       }
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = static_cast<int64_t>(un.r) * nq * a.top * a.G + slot;
-      float* out = part_o + at * a.D;
+      const int64_t urow = static_cast<int64_t>(it.n) * kUnitRows + sub * kSub + row;
+      const float ls = l == 0.f ? -INFINITY : m + log2f(l);
+      const uint32_t buf = sb + S::kOut + warp * 4096;
+      constexpr int kBytes = Part<T>::kBytes, kCols = 128 / kBytes;  // columns in 128 bytes
+      uint8_t* dst = part_o + (urow - lane) * (DP * kBytes);
+      float scale = inv, back = 1.f;
+      if constexpr (Part<T>::kHalf) {
+        float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_o + c * 32, o);
-        tmem_wait_ld();
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + c * 32, o);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[j + e]) * inv;
-          if (slot >= 0 && c * 32 + j < a.D) st_global_v8(out + c * 32 + j, v);
+          for (int j = 0; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], fabsf(__uint_as_float(o[j])));
         }
-        __syncwarp();
+        // the row's largest value to [2^14, 2^15); a row that is not finite stays as it is
+        const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * inv;
+        const int e =
+            top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -112) : 0;
+        scale = inv * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
       }
-      if (slot >= 0) part_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+      part_lse[urow] = make_float2(ls, back);
+#pragma unroll
+      for (int c = 0; c < DP / kCols; ++c) {
+        uint4 piece[8];
+#pragma unroll
+        for (int x = 0; x < kCols / 32; ++x) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + c * kCols + x * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * scale);
+#pragma unroll
+          for (int j = 0; j < 8 * 32 / kCols; ++j) {
+            if constexpr (Part<T>::kHalf) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                y[e] = mma::pack2<__half>(__uint_as_float(o[8 * j + 2 * e]),
+                                          __uint_as_float(o[8 * j + 2 * e + 1]));
+              piece[x * 4 + j] = make_uint4(y[0], y[1], y[2], y[3]);
+            } else {
+              piece[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+          }
+        }
+        store_segment(buf, piece, dst + c * 4096);
+      }
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.o_free[sub]));
       ++uses;
     }
+    if (lane == 0) bulk_wait_all();
   } else if (warp == 8) {
     // ------------------------------------------------------------ MMAs (one thread)
     if (lane == 0) {
       const int dsteps = (a.D + 15) / 16;
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, kSub, DP) | kIdescMnB;
-      uint32_t item = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+      uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
       struct Pending {
         bool has, first, last;
         int stage, ksteps;
         uint32_t parity;  // of the stage's values
       } pend[2] = {};
+      int to_free = -1;  // the stage of the step before, if nothing uses it again
       bool ok = true;
       auto product = [&](int sub) {  // O (+)= P V of the pending step
         Pending& p = pend[sub];
@@ -363,17 +455,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
                       idesc_o, p.ksteps, p.first);
         if (p.last) umma_commit(smem_u32(&mt.o_full[sub]));
       };
-      for (StepIter it(units, blockIdx.x, total, stride); ok && it.valid(); it.next_unit()) {
+      for (UnitIter it(units, start); ok && it.valid(); it.advance()) {
         const Unit& un = it.un;
         const int steps = un.steps();
-        for (int step = 0; ok && step < steps; ++step, ++item) {
-          const int st = item & 1;
+        for (int step = 0; ok && step < steps; ++step) {
+          const uint32_t load = it.load + step;
+          const int st = load & 1;
           const int k16 = (un.keys(step) + 15) / 16;
           const uint32_t idesc_s = umma_idesc_f16(kBf16, kSub, 16 * k16);
           for (int sub = 0; sub < 2; ++sub) {
             product(sub);
             if (!ok || un.nrows <= sub * kSub) continue;
-            ok = mbar_wait(smem_u32(&mt.k_full[st]), (item >> 1) & 1, abort);
+            ok = mbar_wait(smem_u32(&mt.k_full[st]), (load >> 1) & 1, abort);
             if (ok && step == 0) {
               ok = mbar_wait(smem_u32(&mt.q_full[sub]), q_uses[sub] & 1, abort);
               ++q_uses[sub];
@@ -383,9 +476,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
                            idesc_s, dsteps);
             umma_commit(smem_u32(&mt.s_full[sub]));
             if (step == steps - 1) umma_commit(smem_u32(&mt.q_free[sub]));
-            pend[sub] = {true, step == 0, step == steps - 1, st, k16, (item >> 1) & 1};
+            pend[sub] = {true, step == 0, step == steps - 1, st, k16, (load >> 1) & 1};
           }
-          if (ok && item > 0) umma_commit(smem_u32(&mt.kv_free[st ^ 1]));
+          if (ok && to_free >= 0) umma_commit(smem_u32(&mt.kv_free[to_free]));
+          to_free = it.keep ? -1 : st;
         }
       }
       for (int sub = 0; sub < 2; ++sub)
@@ -404,30 +498,36 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       const CUtensorMap* tm = values ? &tm_v : &tm_k;
       const RowMap rm = values ? rv : rk;
       const uint32_t tiles = sb + (values ? S::kV : S::kK);
-      StepIter it(units, blockIdx.x, total, stride);
-      auto fetch = [&](int (&idx)[4]) {  // positions of keys 4 lane .. of the step
+      UnitIter it(units, start);
+      int step = 0, idx[4];
+      auto fetch = [&] {  // positions of keys 4 lane .. of the step
         const int32_t* order = a.order + static_cast<int64_t>(it.un.r) * a.N;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int s = it.un.s0 + it.step * kKeysStep + lane * 4 + j;
+          const int s = it.un.s0 + step * kKeysStep + lane * 4 + j;
           const int row = s < it.un.s1 ? __ldg(order + s) : -1;
           idx[j] = row >= 0 && row < a.N ? row : INT_MAX;
         }
       };
-      int idx[4];
-      if (it.valid()) fetch(idx);
-      for (uint32_t item = 0; it.valid(); ++item) {
-        const int st = item & 1;
+      if (it.valid()) fetch();
+      while (it.valid()) {
+        const uint32_t load = it.load + step;
+        const int st = load & 1;
         const int b = it.un.r / a.Hkv, hk = it.un.r - b * a.Hkv;
-        const int quads = (it.un.keys(it.step) + 15) / 16 * 4;
+        const int quads = (it.un.keys(step) + 15) / 16 * 4;
         int rows[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)  // a key that no row sees is not read
+        for (int j = 0; j < 4; ++j)  // a key that no query sees is not read
           rows[j] = idx[j] <= it.un.high ? rm.at(b, hk, idx[j]) : rm.rows;
         const int4 key = make_int4(idx[0], idx[1], idx[2], idx[3]);
-        it.advance();
-        if (it.valid()) fetch(idx);
-        ok = warp_mbar_wait(&mt.kv_free[st], ((item >> 1) & 1) ^ 1, abort);
+        if (++step == it.un.steps()) {
+          step = 0;
+          do {
+            it.advance();
+          } while (it.valid() && it.again);
+        }
+        if (it.valid()) fetch();
+        ok = warp_mbar_wait(&mt.kv_free[st], ((load >> 1) & 1) ^ 1, abort);
         if (!ok) break;
         uint64_t* full = values ? &mt.v_full[st] : &mt.k_full[st];
         if (!values) *reinterpret_cast<int4*>(&mt.key[st][lane * 4]) = key;
@@ -440,20 +540,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         __syncwarp();
       }
     } else {
-      const int sub = warp - 11;
-      const int4* src = reinterpret_cast<const int4*>(q_row) + sub * (kSub / 4) + lane;
-      StepIter it(units, blockIdx.x, total, stride);
+      const int x = (warp - 11) >> 1, row0 = ((warp - 11) & 1) * 64 + (lane & 15) * 4;
+      const int4* src = reinterpret_cast<const int4*>(q_row) + (x * kSub + row0) / 4;
+      UnitIter it(units, start);
       int4 ahead = it.valid() ? __ldg(src + static_cast<int64_t>(it.n) * (kUnitRows / 4)) : make_int4(0, 0, 0, 0);
       uint32_t uses = 0;
-      for (; it.valid(); it.next_unit()) {
+      for (; it.valid(); it.advance()) {
         const int4 rows = ahead;
-        if (it.n + stride < total) ahead = __ldg(src + static_cast<int64_t>(it.n + stride) * (kUnitRows / 4));
-        if (it.un.nrows <= sub * kSub) continue;
-        ok = warp_mbar_wait(&mt.q_free[sub], (uses & 1) ^ 1, abort);
+        if (it.n + 1 < it.total) ahead = __ldg(src + static_cast<int64_t>(it.n + 1) * (kUnitRows / 4));
+        if (it.un.nrows <= x * kSub) continue;
+        ok = warp_mbar_wait(&mt.q_free[x], (uses & 1) ^ 1, abort);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.q_full[sub]), S::kTile);
-        gather_rows4<DP>(sb + S::kQ + sub * S::kTile, &tm_q, &mt.q_full[sub], lane * 4, rows.x, rows.y,
-                         rows.z, rows.w);
+        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.q_full[x]), S::kTile / 2);
+        // a block of 64 elements by each half of the warp
+        const int blk = lane >> 4;
+        if (blk < DP / 64)
+          tma_gather4(sb + S::kQ + x * S::kTile + blk * (128 * kSub) + row0 * 128, &tm_q,
+                      smem_u32(&mt.q_full[x]), blk * 64, rows.x, rows.y, rows.z, rows.w);
         __syncwarp();
         ++uses;
       }
@@ -476,80 +579,95 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   }
 }
 
-// One warp per (query, head): joins the parts of its clusters, whose log-sum-exps are to base 2.
-template <typename T>
+// One warp per (query, head): joins the parts of its clusters, whose log-sum-exps are to base
+// 2. A part's row takes L lanes of 16 bytes.
+template <typename T, int DP>
 __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
-                                                         const float* __restrict__ part_o,
-                                                         const float* __restrict__ part_lse,
+                                                         const int32_t* __restrict__ pair_row,
+                                                         const uint8_t* __restrict__ part_o,
+                                                         const float2* __restrict__ part_lse,
                                                          T* __restrict__ out,
                                                          float* __restrict__ lse, int64_t rows) {
+  constexpr int E = 16 / Part<T>::kBytes, L = DP / E, P = 32 / L;
+  constexpr int kAhead = 8;  // loads in flight: 8 * P parts
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, grp = lane / L, d = lane % L * E;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i - i0, h)
   if (row >= rows) return;
   const int h = static_cast<int>(row % a.G);
   const int64_t qi = row / a.G;
   const int r = static_cast<int>(qi / nq), i = i0 + static_cast<int>(qi % nq);
   const int b = r / a.Hkv, hq = (r - b * a.Hkv) * a.G + h;
-  const int32_t* sel = a.sel + (static_cast<int64_t>(r) * a.Nq + i) * a.top;
-  const float* pl = part_lse + qi * a.top * a.G + h;  // slot s: + s * G
-  const float* po = part_o + (qi * a.top * a.G + h) * a.D;
-  float top = -INFINITY;
-  uint32_t has = 0;  // bit s of lane l: slot 32 s + l has a part
-  for (int s0 = 0; s0 < a.top; s0 += 32) {
-    const int s = s0 + lane;
-    int from = 0, to = 0;
-    if (s < a.top) cluster_span(a, r, sel[s], from, to);
-    if (to > from) {
-      has |= 1u << (s0 >> 5);
-      top = fmaxf(top, pl[static_cast<int64_t>(s) * a.G]);
+  const int32_t* pairs = pair_row + qi * a.top;
+  float top = -INFINITY, sum = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s0 = 0; s0 < a.top; s0 += kAhead * P) {
+    uint4 v[kAhead];
+    float2 w[kAhead];
+    float big = top;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int s = s0 + u * P + grp;
+      const int64_t n = s < a.top ? pairs[s] : -1;
+      w[u] = n >= 0 ? part_lse[n + h] : make_float2(-INFINITY, 0.f);
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (n >= 0)
+        v[u] = __ldcs(reinterpret_cast<const uint4*>(
+            part_o + part_at(n + h, lane % L, DP * Part<T>::kBytes)));
+      big = fmaxf(big, w[u].x);
+    }
+#pragma unroll
+    for (int o = 16; o >= L; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+    const float from = big == -INFINITY ? 0.f : big, alpha = exp2f(top - from);
+    top = big;
+    sum *= alpha;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= alpha;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (w[u].x == -INFINITY) continue;  // no part, or it sees nothing of its cluster
+      const float p = exp2f(w[u].x - from), f = p * w[u].y;
+      sum += p;
+      const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      if constexpr (Part<T>::kHalf) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = mma::unpack2<__half>(x[e]);
+          acc[2 * e] += f * y.x;
+          acc[2 * e + 1] += f * y.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f * __uint_as_float(x[e]);
+      }
     }
   }
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  const float from = top == -INFINITY ? 0.f : top;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  const bool on = lane * 4 < a.D;
-  constexpr int kAhead = 8;  // parts in flight
-  for (int s0 = 0; s0 < a.top; s0 += kAhead) {
-    float4 v[kAhead];
-    float w[kAhead];
+  for (int o = 16; o >= L; o >>= 1) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int s = s0 + u;
-      const bool part = s < a.top && (__shfl_sync(0xFFFFFFFFu, has, s & 31) >> (s >> 5) & 1u);
-      w[u] = part ? pl[static_cast<int64_t>(s) * a.G] : -INFINITY;
-      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (part && on)
-        v[u] = __ldcs(reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * a.G * a.D + lane * 4));
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (w[u] == -INFINITY) continue;  // sees nothing of this cluster
-      const float e = exp2f(w[u] - from);
-      sum += e;
-      acc[0] += e * v[u].x;
-      acc[1] += e * v[u].y;
-      acc[2] += e * v[u].z;
-      acc[3] += e * v[u].w;
-    }
+    for (int e = 0; e < E; ++e) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], o);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t at = (static_cast<int64_t>(b) * a.Hq + hq) * a.Nq + i;
-  if (on) {
-    uint2 v;
-    v.x = mma::pack2<T>(acc[0] * inv, acc[1] * inv);
-    v.y = mma::pack2<T>(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2*>(out + at * a.D + lane * 4) = v;
+  if (grp == 0 && d < a.D) {
+    uint32_t y[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    if constexpr (E == 8)
+      *reinterpret_cast<uint4*>(out + at * a.D + d) = make_uint4(y[0], y[1], y[2], y[3]);
+    else
+      *reinterpret_cast<uint2*>(out + at * a.D + d) = make_uint2(y[0], y[1]);
   }
-  if (lane == 0) lse[at] = sum == 0.f ? -INFINITY : (from + log2f(sum)) * kLn2;
+  if (lane == 0) lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// Queries that one round takes: rounds of equal size whose parts stay below 2^31 bytes (a
-// round has its own grouping, so short ones cost launches), 64 queries at least.
+// Queries that one round takes: rounds of equal size whose parts stay below some 2^31 bytes
+// (a round has its own grouping, so short ones cost launches), 64 queries at least.
 int64_t queries_per_round(const Args& a) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t per = R * a.top * a.G * (a.D + 1) * 4;
+  const int64_t per = R * a.top * a.G * ((a.D <= 64 ? 64 : 128) * 4 + 8);
   const int64_t most = std::max<int64_t>(64, (1ll << 31) / per);
   const int64_t rounds = (a.Nq + most - 1) / most;
   return (a.Nq + rounds - 1) / rounds;
@@ -561,9 +679,8 @@ struct Layout {
   int64_t nq;
 };
 
-Layout fwd_layout(const Args& a, uint8_t* ws) {
+Layout fwd_layout(const Args& a, int part_bytes, uint8_t* ws) {
   Layout l{};
-  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   l.nq = queries_per_round(a);
   size_t at = carve_units(a, l.nq, ws, &l.plan);
   auto take = [&](int64_t bytes) {
@@ -571,18 +688,18 @@ Layout fwd_layout(const Args& a, uint8_t* ws) {
     at += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  l.part_lse = take(R * l.nq * a.top * a.G * 4);
-  l.part_o = take(R * l.nq * a.top * a.G * a.D * 4);
+  l.part_lse = take(l.plan.units_max * kUnitRows * 8);
+  l.part_o = take(l.plan.units_max * kUnitRows * (a.D <= 64 ? 64 : 128) * part_bytes);
   l.total = at;
   return l;
 }
 
 template <typename T, int DP>
 int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStream_t stream) {
-  const Layout l = fwd_layout(a, ws);
+  const Layout l = fwd_layout(a, Part<T>::kBytes, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  float* part_lse = reinterpret_cast<float*>(ws + l.part_lse);
-  float* part_o = reinterpret_cast<float*>(ws + l.part_o);
+  float2* part_lse = reinterpret_cast<float2*>(ws + l.part_lse);
+  uint8_t* part_o = ws + l.part_o;
   CUtensorMap tm_q, tm_k, tm_v;
   RowMap rq, rk, rv;
   FKC_TRY(encode_rows(a.q, a.qs, a.batch, a.Hq, a.Nq, a.D, dtype, &tm_q, &rq));
@@ -593,18 +710,20 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
-    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, stream));
-    const int64_t grid = std::min<int64_t>(sm_count(), l.plan.units_max);
-    FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), smem, stream, tm_q,
-                       tm_k, tm_v, rq, rk, rv, a, static_cast<int>(i0), nq, static_cast<const int32_t*>(l.plan.q_row),
-                       static_cast<const int2*>(l.plan.slot_pos),
+    const int ctas = static_cast<int>(std::min<int64_t>(std::min(sm_count(), kMaxCtas), l.plan.units_max));
+    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, ctas, stream));
+    FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kFwdThreads), smem, stream, tm_q, tm_k, tm_v, rk, rv, a,
+                       static_cast<const int32_t*>(l.plan.q_row),
+                       static_cast<const int32_t*>(l.plan.row_pos),
                        static_cast<const Unit*>(l.plan.units),
-                       static_cast<const int32_t*>(l.plan.count), part_o, part_lse,
+                       static_cast<const int32_t*>(l.plan.start), part_o, part_lse,
                        device_error_word()));
     const int64_t rows = R * nq * a.G;
-    FKC_TRY(launch_pdl(tiles_join_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
-                       stream, a, static_cast<int>(i0), nq, static_cast<const float*>(part_o),
-                       static_cast<const float*>(part_lse), out, lse, rows));
+    FKC_TRY(launch_pdl(tiles_join_kernel<T, DP>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256),
+                       0, stream, a, static_cast<int>(i0), nq,
+                       static_cast<const int32_t*>(l.plan.pair_row),
+                       static_cast<const uint8_t*>(part_o),
+                       static_cast<const float2*>(part_lse), out, lse, rows));
   }
   return FKC_OK;
 }
@@ -660,47 +779,57 @@ size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out) {
   p.inv_order = static_cast<int32_t*>(take(R * pairs * 4));
   p.inv_offsets = static_cast<int32_t*>(take(R * (a.K + 1) * 4));
   p.units = static_cast<Unit*>(take(p.units_max * static_cast<int64_t>(sizeof(Unit))));
-  p.count = static_cast<int32_t*>(take(4));
+  p.count = static_cast<int64_t*>(take(8));
+  p.start = static_cast<int32_t*>(take((kMaxCtas + 1) * 4));
+  p.cum = static_cast<int32_t*>(take(p.units_max * 4));
   p.q_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
-  p.slot_pos = static_cast<int2*>(take(p.units_max * kUnitRows * 8));
+  p.row_pos = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
+  p.pair_row = static_cast<int32_t*>(take(R * pairs * 4));
   p.group_ws = take(static_cast<int64_t>(group_workspace_bytes(R, pairs, a.K)));
   if (out != nullptr) *out = p;
   return at;
 }
 
-int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p,
+int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
                  cudaStream_t stream) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  FKC_REQUIRE(p.units_max <= 2147483647ll, "attention: too many tiles");
-  FKC_TRY(launch_zero_fill(p.count, 4, stream));
+  FKC_REQUIRE(p.units_max * kUnitRows <= 2147483647ll, "attention: too many tiles");
+  const int64_t blocks = std::min<int64_t>((R * nq * a.top + 255) / 256, sm_count() * 8ll);
+  FKC_TRY(launch_pdl(tile_init_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p.count,
+                     p.pair_row, R * nq * a.top));
   FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
                        p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
   FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
-                     static_cast<const int32_t*>(p.inv_offsets), p.units, p.count,
-                     static_cast<int>(p.units_max)));
+                     static_cast<const int32_t*>(p.inv_offsets), p.units, p.count, p.cum,
+                     static_cast<int>(i0), static_cast<int>(nq), static_cast<int>(p.units_max)));
   return launch_pdl(tile_rows_kernel, dim3(static_cast<unsigned>((p.units_max + 7) / 8)), dim3(256), 0,
                     stream, a, static_cast<int>(i0), static_cast<int>(nq), rq,
-                    static_cast<const int32_t*>(p.inv_order), p.units,
-                    static_cast<const int32_t*>(p.count), p.q_row, p.slot_pos);
+                    static_cast<const int32_t*>(p.inv_order),
+                    static_cast<const Unit*>(p.units),
+                    static_cast<const int64_t*>(p.count), static_cast<const int32_t*>(p.cum),
+                    p.start, ctas, p.q_row, p.row_pos, p.pair_row);
 }
 
 bool use_tiles(const Args& a) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t per_round = queries_per_round(a) * a.top;
-  // rows of a cluster fill half a tile, keys of a cluster repay its parts, and there are
-  // enough tiles for the GPU
-  // the gathers' maps
-  if (!row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
+  const int64_t rows = queries_per_round(a) * a.top * a.G;  // of a row's clusters together
+  // 32-bit row numbers; a running maximum of unscaled scores; the gathers' maps
+  if (rows > (1ll << 30) || !(a.scale > 0.f) ||
+      !row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
       !row_map(a.ks, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr) ||
       !row_map(a.vs, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr))
     return false;
-  // 32-bit numbers of a row's (pair, head)
-  if (queries_per_round(a) * a.top * a.G > (1ll << 30)) return false;
-  return a.scale > 0.f && per_round * a.G >= 64ll * a.K && a.N / a.K >= 4 * a.G + 8 &&
+  // the rows of a cluster fill an MMA, its keys repay its parts, and there are enough tiles
+  // for the GPU
+  return rows >= kSub * static_cast<int64_t>(a.K) && a.N / a.K >= 4 * a.G + 8 &&
          R * a.Nq * a.top * a.G >= 148ll * kSub;
 }
 
-size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a, nullptr).total; }
+size_t tiles_forward_workspace_bytes(const Args& a, int dtype) {
+  return fwd_layout(a, dtype == FKC_DTYPE_F16 ? Part<__half>::kBytes : Part<__nv_bfloat16>::kBytes,
+                    nullptr)
+      .total;
+}
 
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream) {

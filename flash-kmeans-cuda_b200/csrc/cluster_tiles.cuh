@@ -18,12 +18,19 @@ constexpr int kSub = 128;        // rows of one MMA
 constexpr int kKeysStep = 128;   // keys per step
 
 // One unit: cluster c of row r, whose slots are [s0, s1) and whose pairs start at e0; rows
-// [row0, row0 + nrows) of the cluster; high: the last position that one of them sees.
+// [row0, row0 + nrows) of the cluster; high: the last position that a query of the range
+// sees. Units of one cluster follow one another.
 struct __align__(16) Unit {
   int c, row0, s0, s1;
   int e0, nrows, r, high;
 
   __device__ __forceinline__ int steps() const { return (s1 - s0 + kKeysStep - 1) / kKeysStep; }
+  // in about 550 cycles: rows in and out (8), each of the one or two steps whose keys stay in
+  // shared memory from unit to unit (9), or each step of more, which every unit loads
+  // again (18); capped, so that sums stay below 2^31
+  __device__ __forceinline__ int cost() const {
+    return min(8 + (steps() <= 2 ? 9 : 18) * steps(), 1020);
+  }
   __device__ __forceinline__ int keys(int step) const {
     return min(kKeysStep, s1 - s0 - step * kKeysStep);
   }
@@ -74,11 +81,35 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Eight floats to a 32-byte aligned address.
-__device__ __forceinline__ void st_global_v8(float* p, const float (&v)[8]) {
-  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]),
-               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+__device__ __forceinline__ void st_shared_v4(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
                : "memory");
+}
+
+// What the units' rows leave for the join, one row of `bytes` per (unit, row), is stored as the
+// warps write it: per 32 rows, segments of 128 bytes of each row (4 KB), whose 16-byte pieces
+// are xored with the row's low bits as in the operand tiles. Byte offset of piece j (16 bytes)
+// of row n of all units' rows:
+__device__ __forceinline__ int64_t part_at(int64_t n, int j, int bytes) {
+  const int r = static_cast<int>(n & 31);
+  return (n >> 5) * (32 * bytes) + (j >> 3) * 4096 + r * 128 + (((j & 7) ^ (r & 7)) << 4);
+}
+// One segment: lane l's 128 bytes of row l, to 4 KB at dst, through the warp's buffer; the copy
+// goes on while the warp does other things (the stores themselves, 16 bytes a lane to
+// rows or to whole lines alike, held the warps for some 170 cycles each).
+__device__ __forceinline__ void store_segment(uint32_t buf, const uint4 (&piece)[8], uint8_t* dst) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) ptx::bulk_wait_read();  // the buffer's last copy
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) st_shared_v4(buf + lane * 128 + ((j ^ (lane & 7)) << 4), piece[j]);
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    ptx::bulk_store(dst, buf, 4096);
+    ptx::bulk_commit();
+  }
 }
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
@@ -142,17 +173,21 @@ struct UnitPlan {
   int32_t* inv_order;    // (R, nq * top) pairs by cluster
   int32_t* inv_offsets;  // (R, K + 1)
   Unit* units;
-  int32_t* count;        // of units
+  int64_t* count;        // units; their cost above 2^32
+  int32_t* cum;          // cost of the units before each
+  int32_t* start;        // first unit of each CTA, and their number
   int32_t* q_row;        // row of Q's map; the one past its last for a row that sees nothing
-  int2* slot_pos;        // (pair, head) number within r, or -1 past the unit's last row; last
-                         // position that the row sees
+  int32_t* row_pos;      // last position that the row sees; -1: none, or no row
+  int32_t* pair_row;     // (R, nq * top) unit row of a pair's first head; -1: no key
   void* group_ws;
   int64_t units_max;
 };
 size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out);
-// Groups sel of the queries [i0, i0 + nq), lists the units and fills the rows.
-int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p,
+// Groups sel of the queries [i0, i0 + nq), lists the units, fills the rows and shares the
+// units among `ctas` CTAs.
+int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
                  cudaStream_t stream);
+constexpr int kMaxCtas = 1024;
 int sm_count();
 
 }  // namespace attn

@@ -72,7 +72,10 @@ def attention_ref(q, k, v, sel, order, offsets, q_pos=None, scale=None, dout=Non
     rel = 4 * ds_                                   # ... and the sum, with room for the square
     n_add = min(N, int(m.sum(-1).max().item()) if m.numel() else 1) + 8
     acc = n_add * 2.0 ** -22
-    tol_out = (u + rel + acc) * (p @ vd.abs()) * (1 + u) + u * out.abs()
+    # the parts of a row over single clusters, which add up to p @ |v| at most in magnitude, may be
+    # held with 11 bits (fp16 under a power of two) when out has 8: another 2**-11 of them
+    held = 2.0 ** -11 if q.dtype == torch.bfloat16 else 0.0
+    tol_out = (u + held + rel + acc) * (p @ vd.abs()) * (1 + u) + u * out.abs()
     val = {"out": out.reshape(q.shape), "lse": lse.reshape(B, Hq, Nq)}
     tol = {"out": tol_out.reshape(q.shape),
            "lse": (rel.squeeze(-1) + acc + 2.0 ** -22 * lse.abs().masked_fill(lse.isinf(), 0.0)).reshape(B, Hq, Nq)}

@@ -289,7 +289,7 @@ def test_attention(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("B,Hkv,G,Nq,N,K,D,top", [(1, 2, 4, 700, 1500, 23, 128, 7), (2, 1, 3, 1001, 1300, 17, 72, 5),
-                                                  (1, 1, 16, 400, 2500, 30, 64, 9), (2, 2, 1, 3000, 3001, 100, 32, 4),
+                                                  (1, 1, 16, 400, 2500, 30, 64, 9), (2, 2, 1, 3000, 3001, 100, 32, 5),
                                                   (1, 1, 24, 300, 1500, 9, 128, 9)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_many_queries(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
