@@ -33,7 +33,8 @@ CORE_SOURCES = ["capi.cu", "assign_tc.cu", "norm_ext.cu", "assign_simt.cu", "upd
                 "finalize.cu", "lloyd_graph.cu", "assign_noalloc.cu", "selftest.cu",
                 "cluster_group.cu", "cluster_lookup.cu", "cluster_select.cu",
                 "cluster_attention.cu", "cluster_attention_tiles.cu",
-                "cluster_attention_grad.cu", "cluster_capi.cu"]
+                "cluster_attention_grad.cu", "cluster_attention_tiles_grad.cu",
+                "cluster_capi.cu"]
 CORE_LIB = OUT_DIR / "libfkc_b200.so"
 TORCH_API_LIB = OUT_DIR / "libflash_kmeans_cuda.so"
 

@@ -133,7 +133,11 @@ bool use_tiles(const Args& a);
 size_t tiles_forward_workspace_bytes(const Args& a, int dtype);
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream);
-size_t backward_workspace_bytes(const Args& a);
+bool use_tiles_grad(const Args& a);
+size_t tiles_backward_workspace_bytes(const Args& a, int dtype);
+int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
+                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
+size_t backward_workspace_bytes(const Args& a, int dtype);
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
 

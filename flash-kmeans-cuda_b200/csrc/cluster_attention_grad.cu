@@ -494,10 +494,10 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
 }
 
 struct GradLayout {
-  size_t delta, inv_order, inv_offsets, tile_off, group, total;
+  size_t delta, inv_order, inv_offsets, tile_off, group, tiles, total;
 };
 
-GradLayout grad_layout(const Args& a) {
+GradLayout grad_layout(const Args& a, int dtype) {
   GradLayout l{};
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   size_t at = 0;
@@ -507,6 +507,11 @@ GradLayout grad_layout(const Args& a) {
     return p;
   };
   l.delta = take(static_cast<size_t>(a.batch) * a.Hq * a.Nq * 4);
+  if (use_tiles_grad(a)) {
+    l.tiles = take(tiles_backward_workspace_bytes(a, dtype));
+    l.total = at;
+    return l;
+  }
   l.inv_order = take(static_cast<size_t>(R) * a.Nq * a.top * 4);
   l.inv_offsets = take(static_cast<size_t>(R) * (a.K + 1) * 4);
   l.tile_off = take(static_cast<size_t>(R) * (a.K + 1) * 4);
@@ -529,9 +534,9 @@ int dq_typed(const Args& a, const T* dout, const float* lse, const float* delta,
 }
 
 template <typename T, int DP>
-int grad_typed(const Args& a, const T* out, const float* lse, const T* dout, T* dq, T* dk, T* dv,
+int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T* dout, T* dq, T* dk, T* dv,
                uint8_t* ws, cudaStream_t stream) {
-  const GradLayout l = grad_layout(a);
+  const GradLayout l = grad_layout(a, dtype);
   float* delta = reinterpret_cast<float*>(ws + l.delta);
   int32_t* inv_order = reinterpret_cast<int32_t*>(ws + l.inv_order);
   int32_t* inv_offsets = reinterpret_cast<int32_t*>(ws + l.inv_offsets);
@@ -540,6 +545,8 @@ int grad_typed(const Args& a, const T* out, const float* lse, const T* dout, T* 
   const int64_t rows = static_cast<int64_t>(a.batch) * a.Hq * a.Nq;
   FKC_TRY(launch_pdl(attn_delta_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
                      stream, out, dout, delta, a.D, rows));
+  if (use_tiles_grad(a))
+    return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, ws + l.tiles, stream);
   if (dq != nullptr) {
     if (a.G <= 8)
       FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, stream)));
@@ -567,24 +574,24 @@ int grad_typed(const Args& a, const T* out, const float* lse, const T* dout, T* 
 }
 
 template <typename T>
-int grad_dtype(const Args& a, const void* out, const float* lse, const void* dout, void* dq,
+int grad_dtype(const Args& a, int dtype, const void* out, const float* lse, const void* dout, void* dq,
                void* dk, void* dv, void* ws, cudaStream_t stream) {
   const T *o = static_cast<const T*>(out), *d = static_cast<const T*>(dout);
   T *q = static_cast<T*>(dq), *k = static_cast<T*>(dk), *v = static_cast<T*>(dv);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  return a.D <= 64 ? grad_typed<T, 64>(a, o, lse, d, q, k, v, w, stream)
-                   : grad_typed<T, 128>(a, o, lse, d, q, k, v, w, stream);
+  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, o, lse, d, q, k, v, w, stream)
+                   : grad_typed<T, 128>(a, dtype, o, lse, d, q, k, v, w, stream);
 }
 
 }  // namespace
 
-size_t backward_workspace_bytes(const Args& a) { return grad_layout(a).total; }
+size_t backward_workspace_bytes(const Args& a, int dtype) { return grad_layout(a, dtype).total; }
 
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {
   return dtype == FKC_DTYPE_F16
-             ? grad_dtype<__half>(a, out, lse, dout, dq, dk, dv, ws, stream)
-             : grad_dtype<__nv_bfloat16>(a, out, lse, dout, dq, dk, dv, ws, stream);
+             ? grad_dtype<__half>(a, dtype, out, lse, dout, dq, dk, dv, ws, stream)
+             : grad_dtype<__nv_bfloat16>(a, dtype, out, lse, dout, dq, dk, dv, ws, stream);
 }
 
 }  // namespace attn

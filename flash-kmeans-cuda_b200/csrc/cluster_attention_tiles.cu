@@ -39,8 +39,9 @@ __global__ void __launch_bounds__(256) tile_init_kernel(int64_t* count, int32_t*
 __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
                                                           const int32_t* __restrict__ inv_offsets,
                                                           Unit* __restrict__ units, int64_t* count,
-                                                          int32_t* __restrict__ cum, int i0, int nq,
-                                                          int units_max) {
+                                                          int32_t* __restrict__ cum,
+                                                          int32_t* __restrict__ first_unit, int i0,
+                                                          int nq, int units_max) {
   constexpr int rows = kUnitRows;
   __shared__ int warp_total[32];
   __shared__ unsigned long long warp_sum[32];
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
     if (threadIdx.x == 0) first = atomicAdd(reinterpret_cast<unsigned long long*>(count), sum);
     __syncthreads();
     at += first;
+    if (n > 0) first_unit[static_cast<int64_t>(r) * a.K + c] = static_cast<int32_t>(at & 0xFFFFFFFFu);
     for (int t = 0; t < n; ++t) {
       const int64_t u = static_cast<int64_t>(at & 0xFFFFFFFFu) + t;
       un.row0 = t * rows;
@@ -109,7 +111,12 @@ __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, 
                                                         int32_t* __restrict__ start, int ctas,
                                                         int32_t* __restrict__ q_row,
                                                         int32_t* __restrict__ row_pos,
-                                                        int32_t* __restrict__ pair_row) {
+                                                        int32_t* __restrict__ pair_row,
+                                                        const float* __restrict__ lse,
+                                                        const float* __restrict__ delta,
+                                                        int32_t* __restrict__ do_row,
+                                                        float* __restrict__ row_lse,
+                                                        float* __restrict__ row_delta) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -133,12 +140,21 @@ __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, 
   for (int j = 0; j < kUnitRows / 32; ++j) {
     const int rr = j * 32 + lane;
     int pos = -1, row = rq.rows;
+    int64_t flat = -1;  // row of (batch, Hq, Nq)
     if (rr < un.nrows) {
       const int at = un.row0 + rr, e = at / a.G, h = at - e * a.G;
       const int p = list[e], i = i0 + p / a.top;
       if (h == 0) pair_row[pairs0 + p] = static_cast<int32_t>(u * kUnitRows + rr);
       pos = max(-1, min(a.q_pos != nullptr ? a.q_pos[static_cast<int64_t>(b) * a.Nq + i] : a.N, a.N));
-      if (pos >= 0) row = rq.at(b, hk * a.G + h, i);
+      if (pos >= 0) {
+        row = rq.at(b, hk * a.G + h, i);
+        flat = (static_cast<int64_t>(b) * a.Hq + hk * a.G + h) * a.Nq + i;
+      }
+    }
+    if (lse != nullptr) {
+      do_row[u * kUnitRows + rr] = static_cast<int32_t>(flat >= 0 ? flat : static_cast<int64_t>(a.batch) * a.Hq * a.Nq);
+      row_lse[u * kUnitRows + rr] = flat >= 0 ? lse[flat] * kLog2e : 0.f;
+      row_delta[u * kUnitRows + rr] = flat >= 0 ? delta[flat] : 0.f;
     }
     q_row[u * kUnitRows + rr] = row;
     row_pos[u * kUnitRows + rr] = pos;
@@ -171,47 +187,6 @@ enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 // row); warp 8: the MMAs; warps 9, 10: gathers of keys and of values; 11-14: of Q, 64 rows
 // each (a gather takes its warp some 70 cycles to issue, so they are spread over warps).
 constexpr int kFwdThreads = 32 * 15;
-
-// A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn, the next one always
-// fetched ahead. Keys and values are loaded into two stages, load number `load` into
-// stage load & 1; a unit of the same cluster as the one before it, whose steps both
-// stages hold, uses them again.
-struct UnitIter {
-  const Unit* units;
-  int n, total;
-  uint32_t load;        // number of the unit's first step among the loads
-  bool again, keep;     // the unit uses the loads of the one before; the next one will use its
-  Unit un, next;
-
-  __device__ __forceinline__ UnitIter(const Unit* u, const int32_t* start)
-      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), load(0), again(false) {
-    if (n < total) un = load_unit(units + n);
-    look();
-  }
-  __device__ __forceinline__ void look() {
-    keep = false;
-    if (n + 1 >= total) return;
-    next = load_unit(units + n + 1);
-    keep = next.c == un.c && next.r == un.r && un.steps() <= 2;
-  }
-  __device__ __forceinline__ bool valid() const { return n < total; }
-  __device__ __forceinline__ void advance() {
-    if (!keep) load += un.steps();
-    again = keep;
-    ++n;
-    un = next;
-    if (n < total) look();
-  }
-};
-
-// A part's output over one cluster as stored: fp32, or for bf16 inputs fp16 values under a
-// power of two of the row's own. Two of its roundings of 2^-11 stay far below the 2^-8
-// of out, and the parts are most of what the two kernels move.
-template <typename T>
-struct Part {
-  static constexpr bool kHalf = !std::is_same<T, __half>::value;
-  static constexpr int kBytes = kHalf ? 2 : 4;
-};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
@@ -682,7 +657,7 @@ struct Layout {
 Layout fwd_layout(const Args& a, int part_bytes, uint8_t* ws) {
   Layout l{};
   l.nq = queries_per_round(a);
-  size_t at = carve_units(a, l.nq, ws, &l.plan);
+  size_t at = carve_units(a, l.nq, false, ws, &l.plan);
   auto take = [&](int64_t bytes) {
     const size_t p = at;
     at += align_up(static_cast<size_t>(bytes), 256);
@@ -711,7 +686,7 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
     const int ctas = static_cast<int>(std::min<int64_t>(std::min(sm_count(), kMaxCtas), l.plan.units_max));
-    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, ctas, stream));
+    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, ctas, nullptr, nullptr, stream));
     FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kFwdThreads), smem, stream, tm_q, tm_k, tm_v, rk, rv, a,
                        static_cast<const int32_t*>(l.plan.q_row),
                        static_cast<const int32_t*>(l.plan.row_pos),
@@ -764,7 +739,7 @@ int encode_rows(const void* base, const Strides& s, int64_t nb, int64_t nh, int6
       static_cast<uint64_t>(unit) * 2);
 }
 
-size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out) {
+size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* out) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t pairs = nq * a.top;
   UnitPlan p{};
@@ -785,13 +760,19 @@ size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out) {
   p.q_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
   p.row_pos = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
   p.pair_row = static_cast<int32_t*>(take(R * pairs * 4));
+  p.first_unit = static_cast<int32_t*>(take(R * a.K * 4));
+  if (grad) {
+    p.do_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
+    p.row_lse = static_cast<float*>(take(p.units_max * kUnitRows * 4));
+    p.row_delta = static_cast<float*>(take(p.units_max * kUnitRows * 4));
+  }
   p.group_ws = take(static_cast<int64_t>(group_workspace_bytes(R, pairs, a.K)));
   if (out != nullptr) *out = p;
   return at;
 }
 
 int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
-                 cudaStream_t stream) {
+                 const float* lse, const float* delta, cudaStream_t stream) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   FKC_REQUIRE(p.units_max * kUnitRows <= 2147483647ll, "attention: too many tiles");
   const int64_t blocks = std::min<int64_t>((R * nq * a.top + 255) / 256, sm_count() * 8ll);
@@ -800,14 +781,15 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
   FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
                        p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
   FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
-                     static_cast<const int32_t*>(p.inv_offsets), p.units, p.count, p.cum,
+                     static_cast<const int32_t*>(p.inv_offsets), p.units, p.count, p.cum, p.first_unit,
                      static_cast<int>(i0), static_cast<int>(nq), static_cast<int>(p.units_max)));
   return launch_pdl(tile_rows_kernel, dim3(static_cast<unsigned>((p.units_max + 7) / 8)), dim3(256), 0,
                     stream, a, static_cast<int>(i0), static_cast<int>(nq), rq,
                     static_cast<const int32_t*>(p.inv_order),
                     static_cast<const Unit*>(p.units),
                     static_cast<const int64_t*>(p.count), static_cast<const int32_t*>(p.cum),
-                    p.start, ctas, p.q_row, p.row_pos, p.pair_row);
+                    p.start, ctas, p.q_row, p.row_pos, p.pair_row, lse, delta, p.do_row,
+                    p.row_lse, p.row_delta);
 }
 
 bool use_tiles(const Args& a) {

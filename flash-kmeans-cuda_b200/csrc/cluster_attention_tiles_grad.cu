@@ -1,0 +1,1095 @@
+// Gradients of attention over selected clusters, cluster by cluster (see
+// cluster_attention_tiles.cu for units and rows, cluster_attention_grad.cu for the formulas).
+//
+//   dQ      (tiles_dq_kernel)   a unit's 128 rows against the cluster's keys in steps of 128:
+//           S = Q K^T and dP = dO V^T into TMEM, dS in place, dQ += dS K. A row leaves its
+//           gradient over that cluster as the forward leaves its output (Part), and
+//           tiles_dq_join_kernel adds a query's top parts.
+//   dK, dV  (tiles_dkv_kernel)  128 keys of a cluster against the cluster's rows in steps of
+//           128: S^T = K Q^T and dP^T = V dO^T, P^T and dS^T in place, dV += P^T dO and
+//           dK += dS^T Q. All steps of all key tiles are one sequence, cut into equal shares, so
+//           that a cluster that many queries read occupies many CTAs; a key tile cut by a
+//           border leaves fp32 sums of each side, and tiles_dkv_join_kernel adds them in order.
+//           The sequence is fixed by the inputs, so two runs give the same bits.
+//
+// Both run 128 columns as two halves of 64, a warpgroup each (a thread a row of TMEM): while
+// one turns its scores into dS the other's products run on the tensor cores. P and dS are
+// rounded to the 16-bit input type, as the operand type demands, dS of dQ into two terms
+// (see cluster_attention_grad.cu).
+#include <algorithm>
+
+#include "cluster_tiles.cuh"
+#include "fkc_common.cuh"
+
+namespace fkc {
+namespace attn {
+namespace {
+
+enum : int { kErrDqLoad = 161, kErrDqMma = 162, kErrDq = 163, kErrDkvLoad = 171, kErrDkvMma = 172, kErrDkv = 173 };
+
+// ---------------------------------------------------------------------------- dQ
+// The 128-row halves of a CTA's units in turn, as UnitIter.
+struct SubIter {
+  const Unit* units;
+  int n, total, x;
+  uint32_t load;
+  bool again, keep;
+  Unit un, next;
+
+  __device__ __forceinline__ SubIter(const Unit* u, const int32_t* start)
+      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), x(0), load(0), again(false) {
+    if (n < total) un = load_unit(units + n);
+    if (n + 1 < total) next = load_unit(units + n + 1);
+    look();
+  }
+  __device__ __forceinline__ void look() {
+    keep = false;
+    if (n >= total || un.steps() > 2) return;
+    keep = more() || (n + 1 < total && next.c == un.c && next.r == un.r);
+  }
+  __device__ __forceinline__ bool more() const { return x == 0 && un.nrows > kSub; }
+  __device__ __forceinline__ bool valid() const { return n < total; }
+  // unit row of the half's first row, and of the next half's (-1: none)
+  __device__ __forceinline__ int64_t row() const { return static_cast<int64_t>(n) * kUnitRows + x * kSub; }
+  __device__ __forceinline__ int64_t next_row() const {
+    return more() ? row() + kSub : n + 1 < total ? static_cast<int64_t>(n + 1) * kUnitRows : -1;
+  }
+  __device__ __forceinline__ void advance() {
+    if (!keep) load += un.steps();
+    again = keep;
+    if (more()) {
+      x = 1;
+    } else {
+      x = 0;
+      ++n;
+      un = next;
+      if (n + 1 < total) next = load_unit(units + n + 1);
+    }
+    look();
+  }
+};
+
+template <int DP>
+struct DqSmem {
+  static constexpr uint32_t kTile = tc_tile_bytes<DP>();
+  static constexpr uint32_t kQ = 0, kDo = kTile;
+  static constexpr uint32_t kK = 2 * kTile;  // two stages
+  static constexpr uint32_t kV = 4 * kTile;  // two stages
+  static constexpr uint32_t kOut = 6 * kTile;
+  static constexpr uint32_t kMeta = kOut + 8 * 4096;
+  struct Meta {
+    int32_t key[2][kKeysStep];
+    uint64_t k_full[2], v_full[2], kv_free[2], q_full, q_free, sp_full[2], ds_full[2], dq_full, dq_free;
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+  };
+  static constexpr uint32_t kBytes = kMeta + sizeof(Meta) + 1024;
+};
+
+// Warps 0-3, 4-7: keys 0-63 and 64-127 of a step; 8: the MMAs; 9, 10: gathers of keys and
+// values; 11, 12: of Q; 13, 14: of dout.
+constexpr int kGradThreads = 32 * 15;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do, RowMap rk,
+    RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
+    const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
+    const float* __restrict__ row_delta, const Unit* __restrict__ units,
+    const int32_t* __restrict__ start, uint8_t* __restrict__ part, float* __restrict__ part_scale,
+    int* err) {
+  using namespace ptx;
+  using S = DqSmem<DP>;
+  constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr int kBytes = Part<T>::kBytes, kCols = 128 / kBytes;  // columns in a segment
+  constexpr int kSegs = DP / kCols;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t sb = smem_u32(smem);
+  typename S::Meta& mt = *reinterpret_cast<typename S::Meta*>(smem + S::kMeta);
+  volatile int* abort = &mt.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(smem_u32(&mt.k_full[x]), 32);  // the gathering lanes (their keys), and the bytes
+      mbar_init(smem_u32(&mt.v_full[x]), 1);
+      mbar_init(smem_u32(&mt.kv_free[x]), 1);
+      mbar_init(smem_u32(&mt.sp_full[x]), 1);
+      mbar_init(smem_u32(&mt.ds_full[x]), 128);
+    }
+    mbar_init(smem_u32(&mt.q_full), 4);
+    mbar_init(smem_u32(&mt.q_free), 1);
+    mbar_init(smem_u32(&mt.dq_full), 1);
+    mbar_init(smem_u32(&mt.dq_free), 256);
+    mbar_init(smem_u32(&mt.drain), 1);
+    mt.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&mt.tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = mt.tmem;  // S at 0, dP at 128, dQ at 256
+  pdl_wait();
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ dS, output
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + half * 64, t_p = t_s + 128, t_q = tmem + lanes + 256;
+    const float sc = a.scale * kLog2e;
+    uint32_t uses = 0, s_uses = 0;
+    bool ok = true;
+    SubIter it(units, start);
+    int pos_next = -1;
+    float lse_next = 0.f, delta_next = 0.f;
+    auto fetch = [&](int64_t first) {
+      if (first < 0) return;
+      pos_next = __ldg(row_pos + first + row);
+      lse_next = __ldg(row_lse + first + row);
+      delta_next = __ldg(row_delta + first + row);
+    };
+    if (it.valid()) fetch(it.row());
+    for (; ok && it.valid(); it.advance(), ++uses) {
+      const int pos = pos_next;
+      const float lse = lse_next, delta = delta_next;
+      fetch(it.next_row());
+      const int steps = it.un.steps();
+      for (int step = 0; step < steps; ++step) {
+        const int keys = it.un.keys(step) - half * 64;
+        if (keys <= 0) continue;
+        const uint32_t load = it.load + step;
+        const int st = load & 1;
+        ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
+             warp_mbar_wait(&mt.sp_full[half], s_uses & 1, abort);
+        if (!ok) break;
+        ++s_uses;
+        tc_fence_after();
+        const int32_t* key = mt.key[st] + half * 64;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c * 32 >= keys) break;
+          float s[32], dp[32];
+          tmem_ld_f32_x32(t_s + c * 32, s);
+          tmem_ld_f32_x32(t_p + c * 32, dp);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
+            const int k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float p = ex2(fmaf(s[j + e], sc, -lse)) * (dp[j + e] - delta);
+              s[j + e] = k[e] <= pos ? p : 0.f;
+            }
+          }
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            hi[j] = mma::pack2<T>(s[2 * j], s[2 * j + 1]);
+            const float2 f = mma::unpack2<T>(hi[j]);
+            lo[j] = mma::pack2<T>(s[2 * j] - f.x, s[2 * j + 1] - f.y);
+          }
+          tmem_st_32x32b_x16(t_s + c * 16, hi);  // over values that are read already
+          tmem_st_32x32b_x16(t_p + c * 16, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&mt.ds_full[half]));
+      }
+      if (ok) ok = warp_mbar_wait(&mt.dq_full, uses & 1, abort);
+      if (!ok) break;
+      tc_fence_after();
+      const int64_t urow = it.row() + row;
+      const uint32_t buf = sb + S::kOut + warp * 4096;
+      uint8_t* dst = part + (urow - lane) * (DP * kBytes);
+#pragma unroll
+      for (int c = 0; c < kSegs; ++c) {  // the segments are shared out
+        if ((kSegs == 1 ? 0 : c * 2 / kSegs) != half) continue;
+        uint4 piece[8];
+        float scale = a.scale, back = 1.f;
+        if constexpr (Part<T>::kHalf) {
+          float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < kCols / 32; ++x) {
+            float o[32];
+            tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], fabsf(o[j]));
+          }
+          // the segment's largest value to [2^14, 2^15); one that is not finite stays as it is
+          const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * fabsf(a.scale);
+          const int e =
+              top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -112) : 0;
+          scale *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          part_scale[urow * 2 + c] = back;
+        }
+#pragma unroll
+        for (int x = 0; x < kCols / 32; ++x) {
+          float o[32];
+          tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] *= scale;
+#pragma unroll
+          for (int j = 0; j < 8 * 32 / kCols; ++j) {
+            if constexpr (Part<T>::kHalf)
+              piece[x * 4 + j] =
+                  make_uint4(mma::pack2<__half>(o[8 * j], o[8 * j + 1]), mma::pack2<__half>(o[8 * j + 2], o[8 * j + 3]),
+                             mma::pack2<__half>(o[8 * j + 4], o[8 * j + 5]), mma::pack2<__half>(o[8 * j + 6], o[8 * j + 7]));
+            else
+              piece[j] = make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                    __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3]));
+          }
+        }
+        store_segment(buf, piece, dst + c * 4096);
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&mt.dq_free));
+    }
+    if (!ok) give_up(abort, err, kErrDq);
+    if (lane == 0) bulk_wait_all();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMAs (one thread)
+    if (lane == 0) {
+      const int dsteps = (a.D + 15) / 16;
+      constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, kSub, DP) | kIdescMnB;
+      uint32_t uses = 0, ds_uses[2] = {0, 0};
+      struct Pending {
+        bool has, first, last;
+        int stage, ksteps;
+        uint32_t use;
+      } pend[2] = {};
+      int to_free = -1;
+      bool ok = true;
+      auto product = [&](int half) {  // dQ (+)= dS K over the half's keys
+        Pending& p = pend[half];
+        if (!p.has) return;
+        p.has = false;
+        ok = ok && mbar_wait(smem_u32(&mt.ds_full[half]), ds_uses[half] & 1, abort);
+        ++ds_uses[half];
+        if (ok && p.first) ok = mbar_wait(smem_u32(&mt.dq_free), (p.use & 1) ^ 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t kt = sb + S::kK + p.stage * S::kTile + half * 64 * 128;
+        mma_tmem_rows(tmem + 256, tmem + half * 64, kt, idesc_o, p.ksteps, p.first);
+        mma_tmem_rows(tmem + 256, tmem + 128 + half * 64, kt, idesc_o, p.ksteps, false);
+        if (p.last) umma_commit(smem_u32(&mt.dq_full));
+      };
+      for (SubIter it(units, start); ok && it.valid(); it.advance(), ++uses) {
+        const int steps = it.un.steps();
+        for (int step = 0; ok && step < steps; ++step) {
+          const uint32_t load = it.load + step;
+          const int st = load & 1;
+          const int keys = it.un.keys(step);
+          for (int half = 0; half < 2; ++half) {
+            product(half);
+            const int mine = min(64, keys - half * 64);
+            if (!ok || mine <= 0) continue;
+            ok = mbar_wait(smem_u32(&mt.k_full[st]), (load >> 1) & 1, abort) &&
+                 mbar_wait(smem_u32(&mt.v_full[st]), (load >> 1) & 1, abort) &&
+                 mbar_wait(smem_u32(&mt.q_full), uses & 1, abort);
+            if (!ok) break;
+            const int k16 = (mine + 15) / 16;
+            const uint32_t idesc = umma_idesc_f16(kBf16, kSub, 16 * k16);
+            mma_kmajor<DP>(tmem + half * 64, sb + S::kQ, sb + S::kK + st * S::kTile + half * 64 * 128,
+                           idesc, dsteps);
+            mma_kmajor<DP>(tmem + 128 + half * 64, sb + S::kDo,
+                           sb + S::kV + st * S::kTile + half * 64 * 128, idesc, dsteps);
+            umma_commit(smem_u32(&mt.sp_full[half]));
+            const bool last = step == steps - 1 && (half == 1 || keys <= 64);
+            if (last) umma_commit(smem_u32(&mt.q_free));
+            pend[half] = {true, step == 0 && half == 0, last, st, k16, uses};
+          }
+          if (ok && to_free >= 0) umma_commit(smem_u32(&mt.kv_free[to_free]));
+          to_free = it.keep ? -1 : st;
+        }
+      }
+      for (int half = 0; half < 2; ++half)
+        if (ok) product(half);
+      if (!ok) give_up(abort, err, kErrDqMma);
+      umma_commit(smem_u32(&mt.drain));  // nothing is in flight when TMEM is freed
+      const int never = 0;
+      mbar_wait(smem_u32(&mt.drain), 0, &never);
+    }
+  } else {
+    // ------------------------------------------------------------ gathers
+    bool ok = true;
+    SubIter it(units, start);
+    if (warp <= 10) {
+      const bool values = warp == 10;
+      const CUtensorMap* tm = values ? &tm_v : &tm_k;
+      const RowMap rm = values ? rv : rk;
+      const uint32_t tiles = sb + (values ? S::kV : S::kK);
+      int step = 0, idx[4];
+      auto fetch = [&] {  // positions of keys 4 lane .. of the step
+        const int32_t* order = a.order + static_cast<int64_t>(it.un.r) * a.N;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int s = it.un.s0 + step * kKeysStep + lane * 4 + j;
+          const int row = s < it.un.s1 ? __ldg(order + s) : -1;
+          idx[j] = row >= 0 && row < a.N ? row : INT_MAX;
+        }
+      };
+      if (it.valid()) fetch();
+      while (it.valid()) {
+        const uint32_t load = it.load + step;
+        const int st = load & 1;
+        const int b = it.un.r / a.Hkv, hk = it.un.r - b * a.Hkv;
+        const int quads = (it.un.keys(step) + 15) / 16 * 4;
+        int rows[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // a key that no query sees is not read
+          rows[j] = idx[j] <= it.un.high ? rm.at(b, hk, idx[j]) : rm.rows;
+        const int4 key = make_int4(idx[0], idx[1], idx[2], idx[3]);
+        if (++step == it.un.steps()) {
+          step = 0;
+          do {
+            it.advance();
+          } while (it.valid() && it.again);
+        }
+        if (it.valid()) fetch();
+        ok = warp_mbar_wait(&mt.kv_free[st], ((load >> 1) & 1) ^ 1, abort);
+        if (!ok) break;
+        uint64_t* full = values ? &mt.v_full[st] : &mt.k_full[st];
+        if (!values) *reinterpret_cast<int4*>(&mt.key[st][lane * 4]) = key;
+        if (lane == 0)
+          mbar_arrive_expect_tx(smem_u32(full), quads * 4 * DP * 2);
+        else if (!values)
+          mbar_arrive(smem_u32(full));
+        if (lane < quads)
+          gather_rows4<DP>(tiles + st * S::kTile, tm, full, lane * 4, rows[0], rows[1], rows[2], rows[3]);
+        __syncwarp();
+      }
+    } else {
+      const bool grads = warp >= 13;
+      const CUtensorMap* tm = grads ? &tm_do : &tm_q;
+      const int row0 = ((warp - 11) & 1) * 64 + (lane & 15) * 4, blk = lane >> 4;
+      const int32_t* src = (grads ? do_row : q_row) + row0;
+      const uint32_t dst = sb + (grads ? S::kDo : S::kQ) + blk * (128 * kSub) + row0 * 128;
+      auto fetch = [&](int64_t first) {
+        return first < 0 ? make_int4(0, 0, 0, 0) : __ldg(reinterpret_cast<const int4*>(src + first));
+      };
+      int4 ahead = it.valid() ? fetch(it.row()) : make_int4(0, 0, 0, 0);
+      for (uint32_t uses = 0; it.valid(); it.advance(), ++uses) {
+        const int4 rows = ahead;
+        ahead = fetch(it.next_row());
+        ok = warp_mbar_wait(&mt.q_free, (uses & 1) ^ 1, abort);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.q_full), S::kTile / 2);
+        if (blk < DP / 64)  // a block of 64 elements by each half of the warp
+          tma_gather4(dst, tm, smem_u32(&mt.q_full), blk * 64, rows.x, rows.y, rows.z, rows.w);
+        __syncwarp();
+      }
+    }
+    if (!ok) give_up(abort, err, kErrDqLoad);
+    if (!ok || *abort) {  // copies in flight end before the CTA does
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// One warp per (query, head): dq = the sum of its clusters' parts. A part's row takes L
+// lanes of 16 bytes.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, const int32_t* __restrict__ pair_row,
+                                                            const uint8_t* __restrict__ part,
+                                                            const float* __restrict__ part_scale,
+                                                            T* __restrict__ dq, int64_t rows) {
+  constexpr int E = 16 / Part<T>::kBytes, L = DP / E, P = 32 / L;
+  constexpr int kAhead = 8;  // loads in flight: 8 * P parts
+  pdl_wait();
+  const int lane = threadIdx.x & 31, grp = lane / L, d = lane % L * E;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i, h)
+  if (row >= rows) return;
+  const int h = static_cast<int>(row % a.G);
+  const int64_t qi = row / a.G;
+  const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
+  const int b = r / a.Hkv, hq = (r - b * a.Hkv) * a.G + h;
+  const int32_t* pairs = pair_row + qi * a.top;
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s0 = 0; s0 < a.top; s0 += kAhead * P) {
+    uint4 v[kAhead];
+    float f[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int s = s0 + u * P + grp;
+      const int64_t n = s < a.top ? pairs[s] : -1;
+      v[u] = make_uint4(0, 0, 0, 0);
+      f[u] = 0.f;
+      if (n >= 0) {
+        v[u] = __ldcs(reinterpret_cast<const uint4*>(part + part_at(n + h, lane % L, DP * Part<T>::kBytes)));
+        f[u] = Part<T>::kHalf ? part_scale[(n + h) * 2 + (lane % L) / 8] : 1.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      if constexpr (Part<T>::kHalf) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = mma::unpack2<__half>(x[e]);
+          acc[2 * e] += f[u] * y.x;
+          acc[2 * e + 1] += f[u] * y.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __uint_as_float(x[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= L; o >>= 1)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], o);
+  if (grp != 0 || d >= a.D) return;
+  T* out = dq + ((static_cast<int64_t>(b) * a.Hq + hq) * a.Nq + i) * a.D + d;
+  uint32_t y[E / 2];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(acc[2 * e], acc[2 * e + 1]);
+  if constexpr (E == 8)
+    *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
+  else
+    *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[1]);
+}
+
+// ---------------------------------------------------------------------------- dK, dV
+// 128 keys of a cluster: slots [s0, s0 + keys) of row r, and the cluster's `nrows` rows from unit
+// row row0 on, in steps of 128; base: steps of the tiles before.
+struct __align__(16) KeyTile {
+  int r, s0, keys, high;
+  int row0, nrows;
+  int64_t base;
+  __device__ __forceinline__ int steps() const { return (nrows + kSub - 1) / kSub; }
+};
+__device__ __forceinline__ KeyTile load_tile(const KeyTile* t) {
+  KeyTile x;
+  const int4 lo = __ldg(reinterpret_cast<const int4*>(t)), hi = __ldg(reinterpret_cast<const int4*>(t) + 1);
+  x.r = lo.x, x.s0 = lo.y, x.keys = lo.z, x.high = lo.w;
+  x.row0 = hi.x, x.nrows = hi.y;
+  x.base = (static_cast<int64_t>(hi.w) << 32) | static_cast<uint32_t>(hi.z);
+  return x;
+}
+
+// Key tiles and steps of every row r: first[2 r], first[2 r + 1] before the scan over rows.
+__device__ __forceinline__ void tiles_of(const Args& a, const int32_t* inv_offsets, int r, int c, int& s0,
+                                         int& s1, int& nrows) {
+  nrows = 0;
+  s0 = s1 = 0;
+  if (c >= a.K) return;
+  const int32_t* of = inv_offsets + static_cast<int64_t>(r) * (a.K + 1) + c;
+  cluster_span(a, r, c, s0, s1);
+  nrows = (of[1] - of[0]) * a.G;
+}
+
+__global__ void __launch_bounds__(1024) key_count_kernel(Args a, const int32_t* __restrict__ inv_offsets,
+                                                         int64_t* __restrict__ first) {
+  __shared__ int64_t sums[2][32];
+  pdl_wait();
+  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t tiles = 0, steps = 0;
+  for (int c = threadIdx.x; c < a.K; c += 1024) {
+    int s0, s1, nrows;
+    tiles_of(a, inv_offsets, r, c, s0, s1, nrows);
+    if (nrows == 0) continue;
+    const int n = (s1 - s0 + kSub - 1) / kSub;
+    tiles += n;
+    steps += static_cast<int64_t>(n) * ((nrows + kSub - 1) / kSub);
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    tiles += __shfl_xor_sync(0xFFFFFFFFu, tiles, o);
+    steps += __shfl_xor_sync(0xFFFFFFFFu, steps, o);
+  }
+  if (lane == 0) sums[0][warp] = tiles, sums[1][warp] = steps;
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    int64_t s = 0;
+    for (int w = 0; w < 32; ++w) s += sums[threadIdx.x][w];
+    first[2 * r + threadIdx.x] = s;
+  }
+}
+
+// The key tiles in the order of rows and clusters, and the tile in which each CTA's share of the
+// steps begins: share j of all `total` steps is [j total / ctas, (j + 1) total / ctas).
+__global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* __restrict__ inv_offsets,
+                                                         const int32_t* __restrict__ first_unit,
+                                                         const int64_t* __restrict__ first,
+                                                         KeyTile* __restrict__ tiles,
+                                                         int64_t* __restrict__ total_out,
+                                                         int32_t* __restrict__ start, int ctas, int R,
+                                                         int64_t tiles_max) {
+  __shared__ int64_t sums[3][32];
+  __shared__ int highs[32];
+  pdl_wait();
+  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t tile0 = 0, step0 = 0, total = 0;
+  for (int q = threadIdx.x; q < R; q += 1024) {
+    const int64_t t = first[2 * q], s = first[2 * q + 1];
+    if (q < r) tile0 += t, step0 += s;
+    total += s;
+  }
+  int high = a.q_pos != nullptr ? -1 : a.N;
+  if (a.q_pos != nullptr)
+    for (int i = threadIdx.x; i < a.Nq; i += 1024)
+      high = max(high, min(a.q_pos[static_cast<int64_t>(r / a.Hkv) * a.Nq + i], a.N));
+  high = __reduce_max_sync(0xFFFFFFFFu, high);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    tile0 += __shfl_xor_sync(0xFFFFFFFFu, tile0, o);
+    step0 += __shfl_xor_sync(0xFFFFFFFFu, step0, o);
+    total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+  }
+  if (lane == 0) sums[0][warp] = tile0, sums[1][warp] = step0, sums[2][warp] = total, highs[warp] = high;
+  __syncthreads();
+  tile0 = step0 = total = 0;
+  for (int w = 0; w < 32; ++w) {
+    tile0 += sums[0][w], step0 += sums[1][w], total += sums[2][w];
+    high = max(high, highs[w]);
+  }
+  if (r == 0 && threadIdx.x == 0) *total_out = total;
+  if (r == 0 && total == 0)
+    for (int j = threadIdx.x; j < ctas; j += 1024) start[j] = 0;
+  for (int c0 = 0; c0 < a.K; c0 += 1024) {
+    const int c = c0 + threadIdx.x;
+    int s0, s1, nrows;
+    tiles_of(a, inv_offsets, r, c, s0, s1, nrows);
+    const int n = nrows > 0 ? (s1 - s0 + kSub - 1) / kSub : 0;
+    const int per = (nrows + kSub - 1) / kSub;
+    int64_t ti = n, si = static_cast<int64_t>(n) * per;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t t = __shfl_up_sync(0xFFFFFFFFu, ti, o), s = __shfl_up_sync(0xFFFFFFFFu, si, o);
+      if (lane >= o) ti += t, si += s;
+    }
+    __syncthreads();
+    if (lane == 31) sums[0][warp] = ti, sums[1][warp] = si;
+    __syncthreads();
+    int64_t t_at = tile0 + ti - n, s_at = step0 + si - static_cast<int64_t>(n) * per;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) t_at += sums[0][w], s_at += sums[1][w];
+      tile0 += sums[0][w], step0 += sums[1][w];
+    }
+    for (int k = 0; k < n; ++k, ++t_at, s_at += per) {
+      if (t_at >= tiles_max) break;  // never, with the workspace of grad_layout
+      KeyTile t;
+      t.r = r, t.s0 = s0 + k * kSub, t.keys = min(kSub, s1 - s0 - k * kSub), t.high = high;
+      t.row0 = first_unit[static_cast<int64_t>(r) * a.K + c] * kUnitRows;
+      t.nrows = nrows, t.base = s_at;
+      tiles[t_at] = t;
+      // the shares that begin inside: j total / ctas in [s_at, s_at + per)
+      int64_t j = (s_at * ctas + total - 1) / total;
+      for (; j < ctas && j * total / ctas < s_at + per; ++j)
+        if (j * total / ctas >= s_at) start[j] = static_cast<int32_t>(t_at);
+    }
+  }
+}
+
+// A CTA's share as segments: steps [step, end) of the 128-row steps of a key tile.
+struct SegIter {
+  const KeyTile* tiles;
+  int64_t at, to;  // in the sequence of all steps
+  int n, step, end, seg;
+  KeyTile tile;
+  __device__ __forceinline__ SegIter(const KeyTile* t, const int32_t* start, int64_t total)
+      : tiles(t), at(blockIdx.x * total / gridDim.x), to((blockIdx.x + 1) * total / gridDim.x),
+        n(__ldg(start + blockIdx.x)), seg(0) {
+    if (at < to) open();
+  }
+  __device__ __forceinline__ void open() {
+    tile = load_tile(tiles + n);
+    step = static_cast<int>(at - tile.base);
+    end = static_cast<int>(min(static_cast<int64_t>(tile.steps()), to - tile.base));
+  }
+  __device__ __forceinline__ bool valid() const { return at < to; }
+  __device__ __forceinline__ void advance() {
+    at += end - step;
+    ++n;
+    ++seg;
+    if (at < to) open();
+  }
+};
+
+template <int DP>
+struct DkvSmem {
+  static constexpr uint32_t kTile = tc_tile_bytes<DP>();
+  static constexpr uint32_t kK = 0, kV = kTile;
+  static constexpr uint32_t kQ = 2 * kTile;   // two stages
+  static constexpr uint32_t kDo = 4 * kTile;  // two stages
+  static constexpr uint32_t kMeta = 6 * kTile;
+  struct Meta {
+    float lse[2][kSub], delta[2][kSub];  // of a stage's rows
+    int32_t pos[2][kSub];
+    uint64_t kv_full, kv_free, q_full[2], q_free[2], sp_full[2], ds_full[2], acc_full, acc_free;
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+  };
+  static constexpr uint32_t kBytes = kMeta + sizeof(Meta) + 1024;
+};
+
+// Warps 0-3, 4-7: rows 0-63 and 64-127 of a step (a thread a key); 8: the MMAs; 9, 10: gathers
+// of the tile's keys and values; 11, 12: of Q; 13, 14: of dout. part: two fp32 (dV, dK) tiles per
+// CTA, for a first segment that began in another CTA and a last one that goes on in the next.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do, RowMap rk,
+    RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
+    const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
+    const float* __restrict__ row_delta, const KeyTile* __restrict__ tiles,
+    const int64_t* __restrict__ total_steps, const int32_t* __restrict__ start, T* __restrict__ dk,
+    T* __restrict__ dv, float* __restrict__ part, int* err) {
+  using namespace ptx;
+  using S = DkvSmem<DP>;
+  constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t sb = smem_u32(smem);
+  typename S::Meta& mt = *reinterpret_cast<typename S::Meta*>(smem + S::kMeta);
+  volatile int* abort = &mt.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(smem_u32(&mt.q_full[x]), 66);  // two warps' lanes (their rows' data), two warps' bytes
+      mbar_init(smem_u32(&mt.q_free[x]), 1);
+      mbar_init(smem_u32(&mt.sp_full[x]), 1);
+      mbar_init(smem_u32(&mt.ds_full[x]), 128);
+    }
+    mbar_init(smem_u32(&mt.kv_full), 2);
+    mbar_init(smem_u32(&mt.kv_free), 1);
+    mbar_init(smem_u32(&mt.acc_full), 1);
+    mbar_init(smem_u32(&mt.acc_free), 256);
+    mbar_init(smem_u32(&mt.drain), 1);
+    mt.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&mt.tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = mt.tmem;  // S^T at 0, dP^T at 128, dV at 256, dK at 384
+  pdl_wait();
+  const int64_t total = *total_steps;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ P^T and dS^T, output
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // a key
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + half * 64, t_p = t_s + 128;
+    const uint32_t t_acc = tmem + lanes + 256 + half * 128;  // warps 0-3 write dV, 4-7 dK
+    const float sc = a.scale * kLog2e;
+    uint32_t item = 0, s_uses = 0;
+    bool ok = true;
+    for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
+      int key = INT_MAX;
+      if (row < it.tile.keys) {
+        const int k = __ldg(a.order + static_cast<int64_t>(it.tile.r) * a.N + it.tile.s0 + row);
+        if (k >= 0 && k < a.N) key = k;
+      }
+      for (int step = it.step; step < it.end; ++step, ++item) {
+        const int rows = it.tile.nrows - step * kSub - half * 64;
+        if (rows <= 0) continue;
+        const int st = item & 1;
+        ok = warp_mbar_wait(&mt.q_full[st], (item >> 1) & 1, abort) &&
+             warp_mbar_wait(&mt.sp_full[half], s_uses & 1, abort);
+        if (!ok) break;
+        ++s_uses;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c * 32 >= rows) break;
+          float s[32], dp[32];
+          tmem_ld_f32_x32(t_s + c * 32, s);
+          tmem_ld_f32_x32(t_p + c * 32, dp);
+          tmem_wait_ld();
+          const int j0 = half * 64 + c * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const int4 p4 = *reinterpret_cast<const int4*>(&mt.pos[st][j0 + j]);
+            const float4 l4 = *reinterpret_cast<const float4*>(&mt.lse[st][j0 + j]);
+            const float4 d4 = *reinterpret_cast<const float4*>(&mt.delta[st][j0 + j]);
+            const int pos[4] = {p4.x, p4.y, p4.z, p4.w};
+            const float lse[4] = {l4.x, l4.y, l4.z, l4.w}, delta[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool on = key <= pos[e];
+              const float p = ex2(fmaf(s[j + e], sc, -lse[e]));
+              const float ds = p * (dp[j + e] - delta[e]);
+              s[j + e] = on ? p : 0.f;
+              dp[j + e] = on ? ds : 0.f;
+            }
+          }
+          uint32_t x[16], y[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            x[j] = mma::pack2<T>(s[2 * j], s[2 * j + 1]);
+            y[j] = mma::pack2<T>(dp[2 * j], dp[2 * j + 1]);
+          }
+          tmem_st_32x32b_x16(t_s + c * 16, x);  // over values that are read already
+          tmem_st_32x32b_x16(t_p + c * 16, y);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&mt.ds_full[half]));
+      }
+      if (ok) ok = warp_mbar_wait(&mt.acc_full, it.seg & 1, abort);
+      if (!ok) break;
+      tc_fence_after();
+      const bool whole = it.step == 0 && it.end == it.tile.steps();
+      const float scale = half == 0 ? 1.f : a.scale;
+      const int b = it.tile.r / a.Hkv, hk = it.tile.r - b * a.Hkv;
+      T* out = (half == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + (key == INT_MAX ? 0 : key)) * a.D;
+      // a segment that does not begin its tile is the CTA's first
+      float* sums = part + ((static_cast<int64_t>(blockIdx.x) * 2 + (it.step == 0)) * 2 + half) * (kSub * DP) + row * DP;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        float o[32];
+        tmem_ld_f32_x32(t_acc + c * 32, o);
+        tmem_wait_ld();
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            const uint4 v = make_uint4(mma::pack2<T>(o[j] * scale, o[j + 1] * scale), mma::pack2<T>(o[j + 2] * scale, o[j + 3] * scale),
+                                       mma::pack2<T>(o[j + 4] * scale, o[j + 5] * scale), mma::pack2<T>(o[j + 6] * scale, o[j + 7] * scale));
+            if (key != INT_MAX && c * 32 + j < a.D) *reinterpret_cast<uint4*>(out + c * 32 + j) = v;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(sums + c * 32 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&mt.acc_free));
+    }
+    if (!ok) give_up(abort, err, kErrDkv);
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMAs (one thread)
+    if (lane == 0) {
+      const int dsteps = (a.D + 15) / 16;
+      constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, kSub, DP) | kIdescMnB;
+      uint32_t item = 0, ds_uses[2] = {0, 0};
+      struct Pending {
+        bool has, first, last;
+        int stage, ksteps, seg;
+      } pend[2] = {};
+      int to_free = -1;
+      bool ok = true;
+      auto product = [&](int half) {  // dV (+)= P^T dO, dK (+)= dS^T Q over the half's rows
+        Pending& p = pend[half];
+        if (!p.has) return;
+        p.has = false;
+        ok = ok && mbar_wait(smem_u32(&mt.ds_full[half]), ds_uses[half] & 1, abort);
+        ++ds_uses[half];
+        if (ok && p.first) ok = mbar_wait(smem_u32(&mt.acc_free), (p.seg & 1) ^ 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t o = p.stage * S::kTile + half * 64 * 128;
+        mma_tmem_rows(tmem + 256, tmem + half * 64, sb + S::kDo + o, idesc_o, p.ksteps, p.first);
+        mma_tmem_rows(tmem + 384, tmem + 128 + half * 64, sb + S::kQ + o, idesc_o, p.ksteps, p.first);
+        if (p.last) umma_commit(smem_u32(&mt.acc_full));
+      };
+      for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
+        for (int step = it.step; ok && step < it.end; ++step, ++item) {
+          const int st = item & 1;
+          const int rows = it.tile.nrows - step * kSub;
+          for (int half = 0; half < 2; ++half) {
+            product(half);
+            const int mine = min(64, rows - half * 64);
+            if (!ok || mine <= 0) continue;
+            ok = mbar_wait(smem_u32(&mt.kv_full), it.seg & 1, abort) &&
+                 mbar_wait(smem_u32(&mt.q_full[st]), (item >> 1) & 1, abort);
+            if (!ok) break;
+            const int k16 = (mine + 15) / 16;
+            const uint32_t idesc = umma_idesc_f16(kBf16, kSub, 16 * k16);
+            const uint32_t o = st * S::kTile + half * 64 * 128;
+            mma_kmajor<DP>(tmem + half * 64, sb + S::kK, sb + S::kQ + o, idesc, dsteps);
+            mma_kmajor<DP>(tmem + 128 + half * 64, sb + S::kV, sb + S::kDo + o, idesc, dsteps);
+            umma_commit(smem_u32(&mt.sp_full[half]));
+            const bool last = step == it.end - 1 && (half == 1 || rows <= 64);
+            if (last) umma_commit(smem_u32(&mt.kv_free));
+            pend[half] = {true, step == it.step && half == 0, last, st, k16, it.seg};
+          }
+          if (ok && to_free >= 0) umma_commit(smem_u32(&mt.q_free[to_free]));
+          to_free = st;
+        }
+      }
+      for (int half = 0; half < 2; ++half)
+        if (ok) product(half);
+      if (!ok) give_up(abort, err, kErrDkvMma);
+      umma_commit(smem_u32(&mt.drain));  // nothing is in flight when TMEM is freed
+      const int never = 0;
+      mbar_wait(smem_u32(&mt.drain), 0, &never);
+    }
+  } else {
+    // ------------------------------------------------------------ gathers
+    bool ok = true;
+    SegIter it(tiles, start, total);
+    if (warp <= 10) {
+      const bool values = warp == 10;
+      const CUtensorMap* tm = values ? &tm_v : &tm_k;
+      const RowMap rm = values ? rv : rk;
+      for (; it.valid(); it.advance()) {
+        const int32_t* order = a.order + static_cast<int64_t>(it.tile.r) * a.N + it.tile.s0;
+        const int b = it.tile.r / a.Hkv, hk = it.tile.r - b * a.Hkv;
+        int rows[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // a key that no query sees is not read
+          const int k = lane * 4 + j < it.tile.keys ? __ldg(order + lane * 4 + j) : -1;
+          rows[j] = k >= 0 && k < a.N && k <= it.tile.high ? rm.at(b, hk, k) : rm.rows;
+        }
+        ok = warp_mbar_wait(&mt.kv_free, (it.seg & 1) ^ 1, abort);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&mt.kv_full), S::kTile);
+        gather_rows4<DP>(sb + (values ? S::kV : S::kK), tm, &mt.kv_full, lane * 4, rows[0], rows[1],
+                         rows[2], rows[3]);
+        __syncwarp();
+      }
+    } else {
+      const bool grads = warp >= 13;
+      const CUtensorMap* tm = grads ? &tm_do : &tm_q;
+      const int mine = ((warp - 11) & 1) * 64, row0 = mine + (lane & 15) * 4, blk = lane >> 4;
+      const int32_t* src = (grads ? do_row : q_row) + row0;
+      const uint32_t dst = sb + (grads ? S::kDo : S::kQ) + blk * (128 * kSub) + row0 * 128;
+      uint32_t item = 0;
+      int4 ahead;
+      float lse[2], delta[2];
+      int pos[2];
+      auto fetch = [&](const SegIter& s, int step) {
+        const int64_t first = static_cast<int64_t>(s.tile.row0) + static_cast<int64_t>(step) * kSub;
+        ahead = __ldg(reinterpret_cast<const int4*>(src + first));
+        if (grads) return;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int64_t at = first + mine + x * 32 + lane;
+          lse[x] = __ldg(row_lse + at), delta[x] = __ldg(row_delta + at), pos[x] = __ldg(row_pos + at);
+        }
+      };
+      if (it.valid()) fetch(it, it.step);
+      int step = it.valid() ? it.step : 0;
+      while (it.valid()) {
+        const int4 rows = ahead;
+        const float l[2] = {lse[0], lse[1]}, d[2] = {delta[0], delta[1]};
+        const int p[2] = {pos[0], pos[1]};
+        if (++step == it.end) {
+          it.advance();
+          if (it.valid()) step = it.step;
+        }
+        if (it.valid()) fetch(it, step);
+        const int st = item & 1;
+        ok = warp_mbar_wait(&mt.q_free[st], ((item >> 1) & 1) ^ 1, abort);
+        if (!ok) break;
+        if (!grads) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int at = mine + x * 32 + lane;
+            mt.lse[st][at] = l[x], mt.delta[st][at] = d[x], mt.pos[st][at] = p[x];
+          }
+        }
+        if (lane == 0)
+          mbar_arrive_expect_tx(smem_u32(&mt.q_full[st]), S::kTile / 2);
+        else if (!grads)
+          mbar_arrive(smem_u32(&mt.q_full[st]));
+        if (blk < DP / 64)
+          tma_gather4(dst + st * S::kTile, tm, smem_u32(&mt.q_full[st]), blk * 64, rows.x, rows.y, rows.z,
+                      rows.w);
+        __syncwarp();
+        ++item;
+      }
+    }
+    if (!ok) give_up(abort, err, kErrDkvLoad);
+    if (!ok || *abort) {  // copies in flight end before the CTA does
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The key tiles that shares cut: the CTA whose share holds a tile's first step, but not its
+// last, adds the sums of the CTAs that hold the others, in their order. blockIdx.y: 16 keys.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTile* __restrict__ tiles,
+                                                             const int64_t* __restrict__ total_steps,
+                                                             const int32_t* __restrict__ start, int ctas,
+                                                             const float* __restrict__ part,
+                                                             T* __restrict__ dk, T* __restrict__ dv) {
+  pdl_wait();
+  const int64_t total = *total_steps;
+  const int j = blockIdx.x;
+  const int64_t from = j * total / ctas, to = (j + 1) * total / ctas;
+  if (from >= to) return;
+  // the share's last tile: the one in which the next share that is not empty begins
+  int next = j + 1;
+  while (next < ctas && next * total / ctas >= (next + 1) * total / ctas) ++next;
+  if (next >= ctas) return;
+  const KeyTile t = load_tile(tiles + __ldg(start + next));
+  if (t.base >= to || t.base < from) return;  // it begins with the next share, or began before
+  const int64_t end = t.base + t.steps();
+  for (int e = threadIdx.x; e < 2 * 16 * DP / 4; e += 256) {
+    const int which = e / (16 * DP / 4), key = blockIdx.y * 16 + e / (DP / 4) % 16, d = e % (DP / 4) * 4;
+    if (key >= t.keys || d >= a.D) continue;
+    const int k = a.order[static_cast<int64_t>(t.r) * a.N + t.s0 + key];
+    if (k < 0 || k >= a.N) continue;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = j; q < ctas && q * total / ctas < end; ++q) {
+      if (q * total / ctas >= (q + 1) * total / ctas) continue;
+      const float4 v = *reinterpret_cast<const float4*>(
+          part + ((static_cast<int64_t>(q) * 2 + (q == j)) * 2 + which) * (kSub * DP) + key * DP + d);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float scale = which == 0 ? 1.f : a.scale;
+    const int b = t.r / a.Hkv, hk = t.r - b * a.Hkv;
+    T* out = (which == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + k) * a.D + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(mma::pack2<T>(s.x * scale, s.y * scale), mma::pack2<T>(s.z * scale, s.w * scale));
+  }
+}
+
+struct GradLayout {
+  UnitPlan plan;
+  size_t part, scales, first, tiles, total_steps, start, dkv_part, total;
+  int64_t tiles_max;
+};
+
+GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
+  GradLayout l{};
+  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
+  const int64_t DP = a.D <= 64 ? 64 : 128;
+  size_t at = carve_units(a, a.Nq, true, ws, &l.plan);
+  auto take = [&](int64_t bytes) {
+    const size_t p = at;
+    at += align_up(static_cast<size_t>(bytes), 256);
+    return p;
+  };
+  l.tiles_max = R * (std::min<int64_t>(a.K, a.N) + a.N / kSub);
+  l.part = take(l.plan.units_max * kUnitRows * DP * part_bytes);
+  l.scales = take(l.plan.units_max * kUnitRows * 8);
+  l.first = take(R * 16);
+  l.tiles = take(l.tiles_max * static_cast<int64_t>(sizeof(KeyTile)));
+  l.total_steps = take(8);
+  l.start = take(kMaxCtas * 4);
+  l.dkv_part = take(static_cast<int64_t>(std::min(sm_count(), kMaxCtas)) * 4 * kSub * DP * 4);
+  l.total = at;
+  return l;
+}
+
+template <typename T, int DP>
+int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, const T* dout, T* dq, T* dk,
+               T* dv, uint8_t* ws, cudaStream_t stream) {
+  const GradLayout l = grad_layout(a, Part<T>::kBytes, ws);
+  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
+  CUtensorMap tm_q, tm_k, tm_v, tm_do;
+  RowMap rq, rk, rv, rdo;
+  const Strides flat{static_cast<int64_t>(a.Hq) * a.Nq * a.D, static_cast<int64_t>(a.Nq) * a.D, a.D};
+  FKC_TRY(encode_rows(a.q, a.qs, a.batch, a.Hq, a.Nq, a.D, dtype, &tm_q, &rq));
+  FKC_TRY(encode_rows(a.k, a.ks, a.batch, a.Hkv, a.N, a.D, dtype, &tm_k, &rk));
+  FKC_TRY(encode_rows(a.v, a.vs, a.batch, a.Hkv, a.N, a.D, dtype, &tm_v, &rv));
+  FKC_TRY(encode_rows(dout, flat, a.batch, a.Hq, a.Nq, a.D, dtype, &tm_do, &rdo));
+  const int ctas = static_cast<int>(std::min<int64_t>(std::min(sm_count(), kMaxCtas), l.plan.units_max));
+  FKC_TRY(launch_units(a, 0, a.Nq, rq, l.plan, ctas, lse, delta, stream));
+  const int32_t *q_row = l.plan.q_row, *do_row = l.plan.do_row, *pos = l.plan.row_pos;
+  const float *row_lse = l.plan.row_lse, *row_delta = l.plan.row_delta;
+  if (dq != nullptr) {
+    auto kern = tiles_dq_kernel<T, DP>;
+    const int smem = static_cast<int>(DqSmem<DP>::kBytes);
+    FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    float* scales = reinterpret_cast<float*>(ws + l.scales);
+    FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
+                       q_row, do_row, pos, row_lse, row_delta, static_cast<const Unit*>(l.plan.units),
+                       static_cast<const int32_t*>(l.plan.start), ws + l.part, scales, device_error_word()));
+    const int64_t rows = R * a.Nq * a.G;
+    FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
+                       stream, a, static_cast<const int32_t*>(l.plan.pair_row),
+                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, rows));
+  }
+  if (dk == nullptr) return FKC_OK;
+  const size_t bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);
+  FKC_TRY(launch_zero_fill(dk, bytes, stream));
+  FKC_TRY(launch_zero_fill(dv, bytes, stream));
+  int64_t* first = reinterpret_cast<int64_t*>(ws + l.first);
+  int64_t* steps = reinterpret_cast<int64_t*>(ws + l.total_steps);
+  KeyTile* tiles = reinterpret_cast<KeyTile*>(ws + l.tiles);
+  int32_t* start = reinterpret_cast<int32_t*>(ws + l.start);
+  float* part = reinterpret_cast<float*>(ws + l.dkv_part);
+  const int shares = std::min(sm_count(), kMaxCtas);
+  const int32_t* inv = l.plan.inv_offsets;
+  FKC_TRY(launch_pdl(key_count_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv, first));
+  FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv,
+                     static_cast<const int32_t*>(l.plan.first_unit), static_cast<const int64_t*>(first), tiles,
+                     steps, start, shares, static_cast<int>(R), l.tiles_max));
+  auto kern = tiles_dkv_kernel<T, DP>;
+  const int smem = static_cast<int>(DkvSmem<DP>::kBytes);
+  FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  FKC_TRY(launch_pdl(kern, dim3(shares), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
+                     q_row, do_row, pos, row_lse, row_delta, static_cast<const KeyTile*>(tiles),
+                     static_cast<const int64_t*>(steps), static_cast<const int32_t*>(start), dk, dv, part,
+                     device_error_word()));
+  return launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, 8), dim3(256), 0, stream, a,
+                    static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(steps),
+                    static_cast<const int32_t*>(start), shares, static_cast<const float*>(part), dk, dv);
+}
+
+template <typename T>
+int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, const void* dout, void* dq,
+               void* dk, void* dv, uint8_t* ws, cudaStream_t stream) {
+  const T* d = static_cast<const T*>(dout);
+  T *q = static_cast<T*>(dq), *k = static_cast<T*>(dk), *v = static_cast<T*>(dv);
+  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, delta, d, q, k, v, ws, stream)
+                   : grad_typed<T, 128>(a, dtype, lse, delta, d, q, k, v, ws, stream);
+}
+
+}  // namespace
+
+bool use_tiles_grad(const Args& a) {
+  if (!use_tiles(a)) return false;
+  // all queries at once: 32-bit rows of units, and parts of 2^33 bytes at most
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.Hkv * (static_cast<int64_t>(a.Nq) * a.top * a.G + static_cast<int64_t>(a.K) * kUnitRows);
+  return rows <= (1ll << 30) && rows * (a.D <= 64 ? 64 : 128) * 4 <= (1ll << 33) &&
+         static_cast<int64_t>(a.Nq) * a.top * a.G <= (1ll << 30);
+}
+
+size_t tiles_backward_workspace_bytes(const Args& a, int dtype) {
+  return grad_layout(a, dtype == FKC_DTYPE_F16 ? Part<__half>::kBytes : Part<__nv_bfloat16>::kBytes, nullptr)
+      .total;
+}
+
+int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
+                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  return dtype == FKC_DTYPE_F16
+             ? grad_dtype<__half>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream)
+             : grad_dtype<__nv_bfloat16>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream);
+}
+
+}  // namespace attn
+}  // namespace fkc

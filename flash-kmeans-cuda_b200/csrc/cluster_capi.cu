@@ -217,7 +217,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* 
 FKC_CAPI_EXPORT size_t fkc_cluster_attention_grad_workspace_size(const fkc_attention_desc* desc) {
   attn::Args a;
   if (fill_args(desc, true, &a) != FKC_OK) return 0;
-  return attn::backward_workspace_bytes(a);
+  return attn::backward_workspace_bytes(a, desc->dtype);
 }
 
 FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, const void* out,
@@ -235,7 +235,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, c
     FKC_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15u) == 0,
                 "out, dout and the gradients must be 16-byte aligned");
   FKC_TRY(check_workspace("attention gradient", workspace, workspace_bytes,
-                          attn::backward_workspace_bytes(a)));
+                          attn::backward_workspace_bytes(a, desc->dtype)));
   FKC_TRY(check_device());
   return attn::launch_backward(a, desc->dtype, out, lse, dout, dq, dk, dv, workspace,
                                as_stream(stream));

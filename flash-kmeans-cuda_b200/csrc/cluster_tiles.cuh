@@ -135,6 +135,13 @@ __device__ __forceinline__ bool warp_mbar_wait(const uint64_t* bar, uint32_t par
   return __all_sync(0xFFFFFFFFu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort));
 }
 
+__device__ __forceinline__ void tmem_ld_f32_x32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  ptx::tmem_ld_32x32b_x32(taddr, r);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
 // A bounded wait gave up: every role leaves, the host reads the code (fkc_device_status).
 __device__ __forceinline__ void give_up(volatile int* abort, int* err, int code) {
   *abort = 1;
@@ -179,16 +186,61 @@ struct UnitPlan {
   int32_t* q_row;        // row of Q's map; the one past its last for a row that sees nothing
   int32_t* row_pos;      // last position that the row sees; -1: none, or no row
   int32_t* pair_row;     // (R, nq * top) unit row of a pair's first head; -1: no key
+  int32_t* first_unit;   // (R, K) of clusters that have units
+  // for the gradients: row of dout's map, as q_row; lse to base 2 and delta of the row
+  int32_t* do_row;
+  float *row_lse, *row_delta;
   void* group_ws;
   int64_t units_max;
 };
-size_t carve_units(const Args& a, int64_t nq, uint8_t* ws, UnitPlan* out);
+size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* out);
 // Groups sel of the queries [i0, i0 + nq), lists the units, fills the rows and shares the
-// units among `ctas` CTAs.
+// units among `ctas` CTAs. lse and delta (batch, Hq, Nq) with rows of the gradients only.
 int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
-                 cudaStream_t stream);
+                 const float* lse, const float* delta, cudaStream_t stream);
 constexpr int kMaxCtas = 1024;
 int sm_count();
+
+// A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn, the next one always
+// fetched ahead. Keys and values are loaded into two stages, load number `load` into
+// stage load & 1; a unit of the same cluster as the one before it, whose steps both
+// stages hold, uses them again.
+struct UnitIter {
+  const Unit* units;
+  int n, total;
+  uint32_t load;        // number of the unit's first step among the loads
+  bool again, keep;     // the unit uses the loads of the one before; the next one will use its
+  Unit un, next;
+
+  __device__ __forceinline__ UnitIter(const Unit* u, const int32_t* start)
+      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), load(0), again(false) {
+    if (n < total) un = load_unit(units + n);
+    look();
+  }
+  __device__ __forceinline__ void look() {
+    keep = false;
+    if (n + 1 >= total) return;
+    next = load_unit(units + n + 1);
+    keep = next.c == un.c && next.r == un.r && un.steps() <= 2;
+  }
+  __device__ __forceinline__ bool valid() const { return n < total; }
+  __device__ __forceinline__ void advance() {
+    if (!keep) load += un.steps();
+    again = keep;
+    ++n;
+    un = next;
+    if (n < total) look();
+  }
+};
+
+// A part's output over one cluster as stored: fp32, or for bf16 inputs fp16 values under a
+// power of two of the row's own. Two of its roundings of 2^-11 stay far below the 2^-8
+// of out, and the parts are most of what the two kernels move.
+template <typename T>
+struct Part {
+  static constexpr bool kHalf = !std::is_same<T, __half>::value;
+  static constexpr int kBytes = kHalf ? 2 : 4;
+};
 
 }  // namespace attn
 }  // namespace fkc
