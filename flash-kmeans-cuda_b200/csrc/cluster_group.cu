@@ -27,7 +27,8 @@ constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxBits = 11;
 constexpr int kBatch = 8;        // 32-position steps whose keys are loaded together
-constexpr int kMinChunk = 4096;  // positions per chunk: a multiple of kThreads ...
+constexpr int kOneChunk = 4096;  // rows up to here are one chunk
+constexpr int kMinChunk = 1024;  // positions per chunk of longer rows: a multiple of kThreads ...
 constexpr int kMaxChunk = 16384; // ... and below 65536: ranks fit 16 bits
 
 struct GroupGeom {
@@ -40,10 +41,12 @@ GroupGeom group_geom(int64_t B, int64_t N, int64_t K) {
   GroupGeom g;
   g.passes = (total + kMaxBits - 1) / kMaxBits;
   g.bits = (total + g.passes - 1) / g.passes;
-  // about two chunks per SM where the rows are long enough
+  // about two chunks per SM where the rows are long enough (a chunk's warps walk their
+  // positions one 32-wide step after another: 1024 positions are two steps)
   int64_t r = (B * N + 2 * 148 - 1) / (2 * 148);
   r = (r + kThreads - 1) / kThreads * kThreads;
-  g.R = static_cast<int>(std::min<int64_t>(std::max<int64_t>(r, kMinChunk), kMaxChunk));
+  g.R = N <= kOneChunk ? kOneChunk
+                       : static_cast<int>(std::min<int64_t>(std::max<int64_t>(r, kMinChunk), kMaxChunk));
   g.C = static_cast<int>((N + g.R - 1) / g.R);
   return g;
 }
@@ -108,6 +111,29 @@ __global__ void __launch_bounds__(1024) group_prefix_kernel(int32_t* __restrict_
     }
     if (grp == 31) total[static_cast<int64_t>(b) * bins + d] = run;
   }
+}
+
+// The same for few chunks: a thread per digit.
+__global__ void __launch_bounds__(256) group_prefix_few_kernel(int32_t* __restrict__ hist,
+                                                               int32_t* __restrict__ total, int bins,
+                                                               int C, int64_t digits) {
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= digits) return;
+  const int64_t b = i / bins;
+  int32_t* h = hist + b * C * bins + (i - b * bins);
+  int run = 0;
+  for (int c0 = 0; c0 < C; c0 += 8) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = c0 + u < C ? h[static_cast<int64_t>(c0 + u) * bins] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (c0 + u < C) h[static_cast<int64_t>(c0 + u) * bins] = run;
+      run += v[u];
+    }
+  }
+  total[i] = run;
 }
 
 // Positions (and, before the last pass, their keys) of a chunk to their slots.
@@ -206,26 +232,38 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
   });
 }
 
-// offsets[b, k] = number of sorted keys below k (sorts of several passes).
+// offsets[b, k] = number of sorted keys below k (sorts of several passes): a search among
+// every step-th key in shared memory, then among the keys of one step.
+constexpr int kSamples = 1024;
 __global__ void __launch_bounds__(256) group_offsets_kernel(const int32_t* __restrict__ keys,
                                                             int32_t* __restrict__ offsets, int N,
-                                                            int K, int64_t count) {
+                                                            int K, int per_row) {
+  __shared__ int32_t sample[kSamples];
   pdl_wait();
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
-       i += stride) {
-    const int64_t b = i / (K + 1);
-    const int k = static_cast<int>(i - b * (K + 1));
-    const int32_t* kb = keys + b * N;
-    int lo = 0, hi = N;
+  const int b = blockIdx.x / per_row;
+  const int32_t* kb = keys + static_cast<int64_t>(b) * N;
+  const int step = (N + kSamples - 1) / kSamples, n = (N + step - 1) / step;
+  for (int i = threadIdx.x; i < n; i += 256) sample[i] = kb[static_cast<int64_t>(i) * step];
+  __syncthreads();
+  for (int k = (blockIdx.x - b * per_row) * 256 + threadIdx.x; k <= K; k += per_row * 256) {
+    int lo = 0, hi = n;  // the first sample that is not below k
     while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if (kb[mid] < k)
+      const int mid = (lo + hi) / 2;
+      if (sample[mid] < k)
         lo = mid + 1;
       else
         hi = mid;
     }
-    offsets[i] = lo;
+    int64_t from = lo == 0 ? 0 : static_cast<int64_t>(lo - 1) * step + 1;
+    int64_t to = lo == n ? N : static_cast<int64_t>(lo) * step;
+    while (from < to) {
+      const int64_t mid = (from + to) / 2;
+      if (kb[mid] < k)
+        from = mid + 1;
+      else
+        to = mid;
+    }
+    offsets[static_cast<int64_t>(b) * (K + 1) + k] = static_cast<int32_t>(from);
   }
 }
 
@@ -268,8 +306,12 @@ int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in, int
     FKC_TRY(launch_pdl(group_hist_kernel<Id>, grid, dim3(kThreads), bins * 4, stream, keys_in,
                        stride, n, k, g.R, g.C, shift, g.bits, w.hist));
     const int per_row = (bins + 31) / 32;
-    FKC_TRY(launch_pdl(group_prefix_kernel, dim3(static_cast<unsigned>(B * per_row)), dim3(1024), 0,
-                       stream, w.hist, w.total, bins, g.C, per_row));
+    if (g.C <= 64)  // eight loads in flight a thread; more chunks are split over warps
+      FKC_TRY(launch_pdl(group_prefix_few_kernel, dim3(static_cast<unsigned>((B * bins + 255) / 256)),
+                         dim3(256), 0, stream, w.hist, w.total, bins, g.C, B * bins));
+    else
+      FKC_TRY(launch_pdl(group_prefix_kernel, dim3(static_cast<unsigned>(B * per_row)), dim3(1024), 0,
+                         stream, w.hist, w.total, bins, g.C, per_row));
   }
   const size_t smem = static_cast<size_t>(bins) * (4 + 2 * kWarps);
   if (smem > 48 * 1024)
@@ -297,11 +339,10 @@ int launch_group_typed(const Id* ids, int64_t stride, int32_t* order, int32_t* o
     FKC_TRY(group_pass<int32_t>(g, w, w.keys[cur], N, w.vals[cur], w.keys[cur ^ 1],
                                 last ? order : w.vals[cur ^ 1], nullptr, p, B, N, K, stream));
   }
-  const int64_t count = B * (K + 1);
-  const int64_t blocks = std::min<int64_t>((count + 255) / 256, 148 * 16);
-  return launch_pdl(group_offsets_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+  const int per_row = static_cast<int>(std::min<int64_t>((K + 256) / 256, 148));
+  return launch_pdl(group_offsets_kernel, dim3(static_cast<unsigned>(B * per_row)), dim3(256), 0, stream,
                     static_cast<const int32_t*>(w.keys[cur]), offsets, static_cast<int>(N),
-                    static_cast<int>(K), count);
+                    static_cast<int>(K), per_row);
 }
 
 }  // namespace

@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRows = 4;   // rows in flight per group, lookup
-constexpr int kFlight = 8; // rows in flight per group, gradient
+constexpr int kFlight = 8; // vectors in flight per lane, gradient
 
 // A vector of VEC elements of T: 16 bytes, or one element where rows are not
 // whole 16-byte vectors in 16-byte aligned memory.
@@ -92,128 +92,200 @@ __device__ __forceinline__ void add_vec(float (&acc)[VEC], const Vec<T, VEC>& v)
   for (int e = 0; e < VEC; ++e) acc[e] += to_f32<T>(v.v[e]);
 }
 
-// acc += column c of dy at the sorted positions [p0, p1), in order.
-template <typename T, int VEC>
-__device__ __forceinline__ void sum_rows(float (&acc)[VEC], const Vec<T, VEC>* __restrict__ dy,
-                                         const int32_t* __restrict__ order, int p0, int p1,
-                                         int nvec, int c) {
-  using V = Vec<T, VEC>;
-  int p = p0;
-  for (; p + kFlight <= p1; p += kFlight) {
-    V v[kFlight];
+// The next F rows: acc[w] += vector c + w * L of each, in order.
+template <int F, typename T, int VEC, int WIDE>
+__device__ __forceinline__ void sum_some(float (&acc)[WIDE][VEC], const Vec<T, VEC>* __restrict__ dy,
+                                         const int32_t* __restrict__ order, int nvec, int c, int L) {
+  Vec<T, VEC> v[F][WIDE];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) v[u] = dy[static_cast<int64_t>(order[p + u]) * nvec + c];
+  for (int u = 0; u < F; ++u) {
+    const Vec<T, VEC>* row = dy + static_cast<int64_t>(order[u]) * nvec;
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) add_vec<T, VEC>(acc, v[u]);
+    for (int w = 0; w < WIDE; ++w)
+      if (w == 0 || c + w * L < nvec) v[u][w] = row[c + w * L];
   }
-  for (; p < p1; ++p) add_vec<T, VEC>(acc, dy[static_cast<int64_t>(order[p]) * nvec + c]);
+#pragma unroll
+  for (int u = 0; u < F; ++u)
+#pragma unroll
+    for (int w = 0; w < WIDE; ++w)
+      if (w == 0 || c + w * L < nvec) add_vec<T, VEC>(acc[w], v[u][w]);
 }
 
-// Units 0 .. B*J - 1: blocks of Lb sorted positions (partial rows of large
-// clusters); then B*K units: the clusters that are not large.
-template <typename T, int VEC, typename Id>
+// acc[w] += vector c + w * L of dy at the sorted positions [p0, p1), in order. The next
+// flight's row numbers are fetched with this one's rows.
+template <typename T, int VEC, int WIDE>
+__device__ __forceinline__ void sum_rows(float (&acc)[WIDE][VEC], const Vec<T, VEC>* __restrict__ dy,
+                                         const int32_t* __restrict__ order, int p0, int p1,
+                                         int nvec, int c, int L) {
+  constexpr int F = kFlight / WIDE;
+  int p = p0;
+  if (p + F <= p1) {
+    int idx[F];
+#pragma unroll
+    for (int u = 0; u < F; ++u) idx[u] = order[p + u];
+    while (p + F <= p1) {
+      int now[F];
+#pragma unroll
+      for (int u = 0; u < F; ++u) now[u] = idx[u];
+      p += F;
+      const int q = min(p, p1 - F);  // in range; what is not a whole flight is not used
+#pragma unroll
+      for (int u = 0; u < F; ++u) idx[u] = order[q + u];
+      sum_some<F, T, VEC, WIDE>(acc, dy, now, nvec, c, L);
+    }
+  }
+  if constexpr (F > 4)
+    if (p + 4 <= p1) {
+      sum_some<4, T, VEC, WIDE>(acc, dy, order + p, nvec, c, L);
+      p += 4;
+    }
+  if (p + 2 <= p1) {
+    sum_some<2, T, VEC, WIDE>(acc, dy, order + p, nvec, c, L);
+    p += 2;
+  }
+  if (p < p1) sum_some<1, T, VEC, WIDE>(acc, dy, order + p, nvec, c, L);
+}
+
+template <typename T, int VEC, int WIDE>
+__device__ __forceinline__ void store_scaled(Vec<T, VEC>* dst, const float (&acc)[WIDE][VEC], int nvec,
+                                             int c, int L, float scale) {
+#pragma unroll
+  for (int w = 0; w < WIDE; ++w) {
+    if (c + w * L >= nvec) break;
+    Vec<T, VEC> o;
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) o.v[x] = from_f32<T>(acc[w][x] * scale);
+    dst[c + w * L] = o;
+  }
+}
+
+// CTAs 0 .. block_ctas - 1: blocks of Lb sorted positions, groups of 2^log_b lanes (partial rows
+// of the large clusters). The other CTAs: groups of 2^log_l lanes over the clusters that
+// are not large.
+template <typename T, int VEC, int WIDE, typename Id>
 __global__ void __launch_bounds__(kThreads) lookup_grad_kernel(
     const T* __restrict__ dy, const Id* __restrict__ ids, const int32_t* __restrict__ order,
     const int32_t* __restrict__ offsets, T* __restrict__ dt, float* __restrict__ part, int N, int K,
-    int nvec, int log_l, int Lb, int J, int64_t blocks_total, int64_t units, float scale) {
+    int nvec, int log_l, int log_b, int Lb, int J, int64_t blocks_total, int block_ctas,
+    int64_t clusters, float scale) {
   using V = Vec<T, VEC>;
-  const int L = 1 << log_l;
-  const int lane = threadIdx.x & (L - 1), grp = threadIdx.x >> log_l;
-  const int groups = kThreads >> log_l;
   pdl_wait();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * groups + grp; u < units; u += step) {
-    if (u < blocks_total) {
-      const int64_t b = u / J;
-      const int32_t* of = offsets + b * (K + 1);
-      const int32_t* ord = order + b * N;
-      const V* rows = reinterpret_cast<const V*>(dy) + b * N * nvec;
-      const int used = of[K];
-      const int p0 = static_cast<int>(u - b * J) * Lb;
-      if (p0 >= used) continue;
-      const int p1 = min(p0 + Lb, used);
+  if (static_cast<int>(blockIdx.x) < block_ctas) {
+    const int L = 1 << log_b;
+    const int lane = threadIdx.x & (L - 1);
+    const int64_t u = (static_cast<int64_t>(blockIdx.x) << (8 - log_b)) + (threadIdx.x >> log_b);
+    if (u >= blocks_total) return;
+    const int64_t b = u / J;
+    const int32_t* of = offsets + b * (K + 1);
+    const int32_t* ord = order + b * N;
+    const V* rows = reinterpret_cast<const V*>(dy) + b * N * nvec;
+    const int used = of[K];
+    const int p0 = static_cast<int>(u - b * J) * Lb;
+    if (p0 >= used) return;
+    const int p1 = min(p0 + Lb, used);
 #pragma unroll
-      for (int slot = 0; slot < 2; ++slot) {
-        const int64_t k = row_of<Id>(ids[b * N + ord[slot == 0 ? p0 : p1 - 1]], K);
-        if (k < 0) continue;  // order does not group these ids
-        const int s = of[k], e = of[k + 1];
-        if (e - s <= 2 * Lb || (slot == 1 && s <= p0)) continue;
-        float* dst = part + (u * 2 + slot) * nvec * VEC;
-        for (int c = lane; c < nvec; c += L) {
-          float acc[VEC] = {};
-          sum_rows<T, VEC>(acc, rows, ord, max(s, p0), min(e, p1), nvec, c);
+    for (int slot = 0; slot < 2; ++slot) {
+      const int64_t k = row_of<Id>(ids[b * N + ord[slot == 0 ? p0 : p1 - 1]], K);
+      if (k < 0) continue;  // order does not group these ids
+      const int s = of[k], e = of[k + 1];
+      if (e - s <= 2 * Lb || (slot == 1 && s <= p0)) continue;
+      float* dst = part + (u * 2 + slot) * nvec * VEC;
+      for (int c = lane; c < nvec; c += L) {
+        float acc[1][VEC] = {};
+        sum_rows<T, VEC, 1>(acc, rows, ord, max(s, p0), min(e, p1), nvec, c, L);
 #pragma unroll
-          for (int x = 0; x < VEC; ++x) dst[c * VEC + x] = acc[x];
-        }
+        for (int x = 0; x < VEC; ++x) dst[c * VEC + x] = acc[0][x];
       }
-      continue;
     }
-    const int64_t row = u - blocks_total;  // b * K + k
+    return;
+  }
+  const int L = 1 << log_l;
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t step = static_cast<int64_t>(gridDim.x - block_ctas) << (8 - log_l);
+  for (int64_t row = (static_cast<int64_t>(blockIdx.x - block_ctas) << (8 - log_l)) + (threadIdx.x >> log_l);
+       row < clusters; row += step) {  // b * K + k
     const int64_t b = row / K;
     const int32_t* of = offsets + b * (K + 1) + (row - b * K);
     const int s = of[0], e = of[1];
     if (e - s > 2 * Lb) continue;
     const V* rows = reinterpret_cast<const V*>(dy) + b * N * nvec;
     V* dst = reinterpret_cast<V*>(dt) + row * nvec;
-    for (int c = lane; c < nvec; c += L) {
-      float acc[VEC] = {};
-      sum_rows<T, VEC>(acc, rows, order + b * N, s, e, nvec, c);
-      V o;
-#pragma unroll
-      for (int x = 0; x < VEC; ++x) o.v[x] = from_f32<T>(acc[x] * scale);
-      dst[c] = o;
+    for (int c = lane; c < nvec; c += L * WIDE) {
+      float acc[WIDE][VEC] = {};
+      sum_rows<T, VEC, WIDE>(acc, rows, order + b * N, s, e, nvec, c, L);
+      store_scaled<T, VEC, WIDE>(dst, acc, nvec, c, L, scale);
     }
   }
 }
 
-// The large clusters: their partial rows in block order.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const int32_t* __restrict__ offsets,
-                                                             const float* __restrict__ part,
-                                                             T* __restrict__ dt, int K, int nvec,
-                                                             int log_l, int Lb, int J, int64_t rows,
-                                                             float scale) {
+// The large clusters, by the block in which each begins: their partial rows in block order.
+template <typename T, int VEC, typename Id>
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(
+    const Id* __restrict__ ids, const int32_t* __restrict__ order,
+    const int32_t* __restrict__ offsets, const float* __restrict__ part, T* __restrict__ dt, int N,
+    int K, int nvec, int log_l, int Lb, int J, int64_t blocks_total, float scale) {
   using V = Vec<T, VEC>;
+  constexpr int kAhead = 8;  // partial rows in flight
   const int L = 1 << log_l;
   const int lane = threadIdx.x & (L - 1), grp = threadIdx.x >> log_l;
-  const int groups = kThreads >> log_l;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * (kThreads >> log_l) + grp;
   pdl_wait();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * groups + grp; row < rows; row += step) {
-    const int64_t b = row / K;
-    const int32_t* of = offsets + b * (K + 1) + (row - b * K);
-    const int s = of[0], e = of[1];
-    if (e - s <= 2 * Lb) continue;
-    const int j0 = s / Lb, j1 = (e - 1) / Lb;
-    V* dst = reinterpret_cast<V*>(dt) + row * nvec;
-    for (int c = lane; c < nvec; c += L) {
-      float acc[VEC] = {};
-      for (int j = j0; j <= j1; ++j) {
-        const int slot = j == j0 && s % Lb != 0 ? 1 : 0;
-        const float* src = part + ((b * J + j) * 2 + slot) * nvec * VEC + c * VEC;
+  if (u >= blocks_total) return;
+  const int64_t b = u / J;
+  const int32_t* of = offsets + b * (K + 1);
+  const int p0 = static_cast<int>(u - b * J) * Lb, used = of[K];
+  if (p0 >= used) return;
+  // the last cluster of the block: a large one that begins here reaches over its end
+  const int64_t k = row_of<Id>(ids[b * N + order[b * N + min(p0 + Lb, used) - 1]], K);
+  if (k < 0) return;
+  const int s = of[k], e = of[k + 1];
+  if (e - s <= 2 * Lb || s < p0) return;
+  const int j0 = s / Lb, j1 = (e - 1) / Lb;
+  V* dst = reinterpret_cast<V*>(dt) + (b * K + k) * nvec;
+  for (int c = lane; c < nvec; c += L) {
+    float acc[VEC] = {};
+    int j = j0;
+    auto some = [&](auto count) {
+      constexpr int F = decltype(count)::value;
+      Vec<float, VEC> v[F];
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) acc[x] += src[x];
+      for (int q = 0; q < F; ++q) {
+        const int slot = j + q == j0 && s % Lb != 0 ? 1 : 0;
+        const float* src = part + ((b * J + j + q) * 2 + slot) * nvec * VEC + c * VEC;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) v[q].v[x] = src[x];
       }
-      V o;
 #pragma unroll
-      for (int x = 0; x < VEC; ++x) o.v[x] = from_f32<T>(acc[x] * scale);
-      dst[c] = o;
-    }
+      for (int q = 0; q < F; ++q)
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[x] += v[q].v[x];
+      j += F;
+    };
+    while (j + kAhead - 1 <= j1) some(std::integral_constant<int, kAhead>{});
+    while (j + 1 <= j1) some(std::integral_constant<int, 2>{});
+    if (j <= j1) some(std::integral_constant<int, 1>{});
+    V o;
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) o.v[x] = from_f32<T>(acc[x] * scale);
+    dst[c] = o;
   }
 }
 
-// Lanes per row: the vectors of a row rounded up to a power of two, a CTA at most.
-int lanes_log2(int64_t nvec) {
+// Lanes per row: the vectors of a row rounded up to a power of two, `most` at most.
+int lanes_log2(int64_t nvec, int most) {
   int l = 0;
-  while ((1 << l) < nvec && (1 << l) < kThreads) ++l;
+  while ((1 << l) < nvec && (1 << l) < most) ++l;
   return l;
 }
 
-// Positions per block: longer blocks for longer rows, so that neither a block's
-// sum (Lb rows) nor a cluster's join (N / Lb partial rows) becomes a long chain.
-int block_len(int64_t N) {
-  int lb = 64;
-  while (lb < 512 && static_cast<int64_t>(lb) * lb * 4 < N) lb *= 2;
+// Positions per block: longer blocks for longer rows of ids, so that neither a block's sum (Lb
+// rows) nor a cluster's join (N / Lb partial rows) becomes a long chain; shorter ones where a
+// row of the table is wider than a warp, since a group then passes its rows several times
+// (16384 ids, rows of 1024 bf16: 88 us at 64, a cluster of 128 rows taking 64 flights).
+int block_len(int64_t N, int64_t row_bytes) {
+  const bool wide = row_bytes > 512;
+  int lb = wide ? 16 : 64;
+  while (lb < 512 && static_cast<int64_t>(lb) * lb * (wide ? 64 : 4) < N) lb *= 2;
   return lb;
 }
 
@@ -228,9 +300,9 @@ struct GradLayout {
   int64_t J;
 };
 
-GradLayout grad_layout(int64_t B, int64_t N, int64_t K, int64_t D) {
+GradLayout grad_layout(int64_t B, int64_t N, int64_t K, int64_t D, int64_t elem) {
   GradLayout l{};
-  l.Lb = block_len(N);
+  l.Lb = block_len(N, D * elem);
   l.J = (N + l.Lb - 1) / l.Lb;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -256,7 +328,7 @@ template <typename T, int VEC>
 int lookup_typed(const void* table, const void* ids, bool ids_64, void* y, int64_t B, int64_t N,
                  int64_t K, int64_t D, float scale, cudaStream_t stream) {
   const int nvec = static_cast<int>(D / VEC);
-  const int log_l = lanes_log2(nvec);
+  const int log_l = lanes_log2(nvec, kThreads);
   const int64_t total = B * N;
   const dim3 grid(grid_for((total + kRows - 1) / kRows, log_l));
   const T* t = static_cast<const T*>(table);
@@ -272,34 +344,40 @@ int lookup_typed(const void* table, const void* ids, bool ids_64, void* y, int64
 template <typename T, int VEC>
 int grad_typed(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B, int64_t N,
                int64_t K, int64_t D, float scale, uint8_t* ws, cudaStream_t stream) {
-  const GradLayout l = grad_layout(B, N, K, D);
+  const GradLayout l = grad_layout(B, N, K, D, sizeof(T));
   int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + l.offsets);
   float* part = reinterpret_cast<float*>(ws + l.part);
   FKC_TRY(launch_group(ids, ids_64, N, order, offsets, B, N, K, ws + l.group, stream));
   const int nvec = static_cast<int>(D / VEC);
-  const int log_l = lanes_log2(nvec);
+  // a warp at most: most clusters of a large table have no row or one, and what counts is how
+  // many are in flight
+  const int log_l = lanes_log2(nvec, 32), log_b = lanes_log2(nvec, kThreads);
   const bool large = N > 2 * l.Lb;
   const int64_t blocks = large ? B * l.J : 0;
-  const int64_t units = blocks + B * K;
-  const dim3 grid(grid_for(units, log_l));
+  const int64_t block_ctas = (blocks + (kThreads >> log_b) - 1) / (kThreads >> log_b);
+  const int64_t clusters = B * K;
+  const int64_t ctas = block_ctas + grid_for(clusters, log_l);
+  FKC_REQUIRE(ctas <= 2147483647ll, "lookup gradient: too many clusters");
+  const dim3 grid(static_cast<unsigned>(ctas));
   const int n = static_cast<int>(N), k = static_cast<int>(K), j = static_cast<int>(l.J);
   const T* g = static_cast<const T*>(dy);
   T* o = static_cast<T*>(dt);
-  if (ids_64)
-    FKC_TRY(launch_pdl(lookup_grad_kernel<T, VEC, int64_t>, grid, dim3(kThreads), 0, stream, g,
-                       static_cast<const int64_t*>(ids), static_cast<const int32_t*>(order),
-                       static_cast<const int32_t*>(offsets), o, part, n, k, nvec, log_l, l.Lb, j,
-                       blocks, units, scale));
-  else
-    FKC_TRY(launch_pdl(lookup_grad_kernel<T, VEC, int32_t>, grid, dim3(kThreads), 0, stream, g,
-                       static_cast<const int32_t*>(ids), static_cast<const int32_t*>(order),
-                       static_cast<const int32_t*>(offsets), o, part, n, k, nvec, log_l, l.Lb, j,
-                       blocks, units, scale));
-  if (!large) return FKC_OK;
-  return launch_pdl(grad_join_kernel<T, VEC>, dim3(grid_for(B * K, log_l)), dim3(kThreads), 0,
-                    stream, static_cast<const int32_t*>(offsets), static_cast<const float*>(part), o,
-                    k, nvec, log_l, l.Lb, j, B * K, scale);
+  auto run = [&](auto id) {
+    using Id = decltype(id);
+    const Id* in = static_cast<const Id*>(ids);
+    // rows wider than a warp: two vectors of a row at once
+    auto kern = nvec > 32 ? lookup_grad_kernel<T, VEC, 2, Id> : lookup_grad_kernel<T, VEC, 1, Id>;
+    FKC_TRY(launch_pdl(kern, grid, dim3(kThreads), 0, stream, g, in, static_cast<const int32_t*>(order),
+                       static_cast<const int32_t*>(offsets), o, part, n, k, nvec, log_l, log_b, l.Lb, j,
+                       blocks, static_cast<int>(block_ctas), clusters, scale));
+    if (!large) return static_cast<int>(FKC_OK);
+    return launch_pdl(grad_join_kernel<T, VEC, Id>, dim3(static_cast<unsigned>(block_ctas)),
+                      dim3(kThreads), 0, stream, in, static_cast<const int32_t*>(order),
+                      static_cast<const int32_t*>(offsets), static_cast<const float*>(part), o, n, k,
+                      nvec, log_b, l.Lb, j, blocks, scale);
+  };
+  return ids_64 ? run(int64_t{}) : run(int32_t{});
 }
 
 }  // namespace
@@ -321,7 +399,7 @@ int launch_lookup(const void* table, const void* ids, bool ids_64, void* y, int6
 }
 
 size_t lookup_grad_workspace_bytes(int64_t B, int64_t N, int64_t K, int64_t D) {
-  return grad_layout(B, N, K, D).total;
+  return std::max(grad_layout(B, N, K, D, 2).total, grad_layout(B, N, K, D, 4).total);
 }
 
 int launch_lookup_grad(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B,
