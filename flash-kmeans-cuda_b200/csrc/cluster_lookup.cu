@@ -357,7 +357,9 @@ int grad_typed(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B
   const int64_t blocks = large ? B * l.J : 0;
   const int64_t block_ctas = (blocks + (kThreads >> log_b) - 1) / (kThreads >> log_b);
   const int64_t clusters = B * K;
-  const int64_t ctas = block_ctas + grid_for(clusters, log_l);
+  // CTAs that the GPU holds at once: each warp goes on to its next cluster by itself, while a CTA
+  // of few clusters would keep its place until the largest is done
+  const int64_t ctas = block_ctas + std::min<int64_t>(grid_for(clusters, log_l), 148 * 5);
   FKC_REQUIRE(ctas <= 2147483647ll, "lookup gradient: too many clusters");
   const dim3 grid(static_cast<unsigned>(ctas));
   const int n = static_cast<int>(N), k = static_cast<int>(K), j = static_cast<int>(l.J);

@@ -12,8 +12,8 @@
 //          walked one by one and the running maximum stays in the accumulator layout,
 //          so any group size fills the instruction (m16n8k16, fp32 accumulation). Also
 //          the largest norms of a query's heads and of a tile's centroids.
-//   choose (choose_warp_kernel, one warp per query up to 1024 clusters, and
-//          choose_cta_kernel)  the top-th largest fp32 score t by bisection over its
+//   choose (choose_warp_kernel, one warp per query up to 1024 clusters, and for few queries or
+//          more clusters choose_cta_kernel)  the top-th largest fp32 score t by bisection over its
 //          bits. What lies above t by more than the scores can be off is in, what lies
 //          below by more is out; where that leaves more candidates than places, theirs
 //          are computed again in 64 bits and ranked. So the selection is that of exact
@@ -54,8 +54,10 @@ __device__ __forceinline__ float fold_max(float a, float b) {
   return (isnan(a) || isnan(b)) ? INFINITY : fmaxf(a, b);  // a NaN norm counts as unbounded
 }
 
-// QW warps along the queries, 4 / QW along the clusters.
-template <typename T, int DP, int QW>
+// QW warps along the queries, 4 / QW along the clusters. PACK (QW = 1): at most 16 rows (query,
+// head) in all, side by side in one tile; the maximum over a query's heads is taken in
+// shared memory.
+template <typename T, int DP, int QW, bool PACK>
 __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restrict__ scores,
                                                     float* __restrict__ q_norm,
                                                     float* __restrict__ c_norm, int ctiles,
@@ -67,6 +69,7 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
   __shared__ float s_bias[kClusters];
   __shared__ int s_first[kClusters];  // first position; INT_MAX: never selected
   __shared__ float s_red[4];
+  __shared__ float s_pack[PACK ? 16 * (kClusters + 4) : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t ct = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
@@ -89,9 +92,9 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
     const uint32_t qt = qt0 + buf * (MQ * DP * 2);
     for (int e = tid; e < MQ * CH; e += 128) {
       const int row = e / CH, c = e % CH;
-      const bool ok = i0 + row < a.Nq && c < dchunks;
-      mma::cp_async16(qt + tile_at<DP>(row, c),
-                      q + (ok ? h * a.qs.h + (i0 + row) * a.qs.n + c * 8 : 0), ok);
+      const int i = PACK ? row / a.G : i0 + row, hh = PACK ? row - i * a.G : h;
+      const bool ok = i < a.Nq && c < dchunks;
+      mma::cp_async16(qt + tile_at<DP>(row, c), q + (ok ? hh * a.qs.h + i * a.qs.n + c * 8 : 0), ok);
     }
   };
   load_q(0, 0);
@@ -119,10 +122,12 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
 #pragma unroll
     for (int e = 0; e < 4; ++e) best[n][e] = -INFINITY;
   float qn = 0.f;  // largest norm^2 of the heads, thread tid < MQ: query i0 + tid
-  for (int h = 0; h < a.G; ++h) {
+  const int passes = PACK ? 1 : a.G;
+#pragma unroll 1
+  for (int h = 0; h < passes; ++h) {
     mma::cp_async_wait<0>();
     __syncthreads();
-    if (h + 1 < a.G) load_q(h + 1, (h + 1) & 1);
+    if (h + 1 < passes) load_q(h + 1, (h + 1) & 1);
     mma::cp_async_commit();
     const uint32_t qt = qt0 + (h & 1) * (MQ * DP * 2);
     if (tile == 0 && tid < MQ) {
@@ -161,8 +166,25 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
 #pragma unroll
       for (int e = 0; e < 4; ++e) best[n][e] = fmaxf(best[n][e], acc[n][e]);
   }
-  if (tile == 0 && tid < MQ && i0 + tid < a.Nq)
+  if (!PACK && tile == 0 && tid < MQ && i0 + tid < a.Nq)
     q_norm[static_cast<int64_t>(r) * a.Nq + i0 + tid] = sqrtf(qn);
+  if constexpr (PACK) {
+    __syncthreads();
+    if (tid < 16) s_pack[tid] = qn;
+    __syncthreads();
+    if (tile == 0 && tid < a.Nq) {
+      float m = 0.f;
+      for (int h = 0; h < a.G; ++h) m = fold_max(m, s_pack[tid * a.G + h]);
+      q_norm[static_cast<int64_t>(r) * a.Nq + tid] = sqrtf(m);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s_pack[(g + (e >> 1) * 8) * (kClusters + 4) + (wc * NW + n) * 8 + t4 * 2 + (e & 1)] = best[n][e];
+    __syncthreads();
+  }
   if (qtile == 0) {  // the tile's largest centroid norm, of the clusters that can be selected
     float s = 0.f;
     for (int c = 0; c < CH; ++c) {
@@ -185,6 +207,16 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
           sqrtf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
   }
   const float scale = static_cast<float>(a.scale);
+  if constexpr (PACK) {
+    for (int i = 0; i < a.Nq && c0 + tid < a.K; ++i) {
+      const int pos =
+          a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.Nq + i], a.N) : a.N;
+      float m = -INFINITY;
+      for (int h = 0; h < a.G; ++h) m = fmaxf(m, s_pack[(i * a.G + h) * (kClusters + 4) + tid]);
+      scores[(static_cast<int64_t>(r) * a.Nq + i) * a.K + c0 + tid] =
+          s_first[tid] > pos ? __uint_as_float(kNever) : m * scale + s_bias[tid];
+    }
+  } else {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int i = i0 + wq * 16 + half * 8 + g;
@@ -202,6 +234,7 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
         row[c0 + cl] = s_first[cl] > pos ? __uint_as_float(kNever) : s;
       }
   }
+  }
 }
 
 // fp32 scores as integers that compare the same way; 0: cannot be selected.
@@ -215,28 +248,38 @@ __device__ __forceinline__ float key_score(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-// The score of cluster c for query i in 64 bits, over the warp.
+// The score of cluster c for query i in 64 bits, by eight lanes (the same in each); c < 0: none.
 template <typename T>
 __device__ double exact_score(const SelectArgs& a, int r, int i, int c) {
-  const int lane = threadIdx.x & 31;
+  const int l8 = threadIdx.x & 7;
   const int b = r / a.Hkv, hk = r - b * a.Hkv;
-  const T* cen = static_cast<const T*>(a.centroids) + (static_cast<int64_t>(r) * a.K + c) * a.D;
+  const T* cen = static_cast<const T*>(a.centroids) +
+                 (static_cast<int64_t>(r) * a.K + (c < 0 ? 0 : c)) * a.D;
   const T* q = static_cast<const T*>(a.q) + b * a.qs.b + static_cast<int64_t>(hk) * a.G * a.qs.h +
                i * a.qs.n;
   double best = -INFINITY;
   bool nan = false;
   for (int h = 0; h < a.G; ++h) {
     double s = 0.0;
-    for (int d = lane; d < a.D; d += 32)
-      s += static_cast<double>(to_f32<T>(q[h * a.qs.h + d])) * static_cast<double>(to_f32<T>(cen[d]));
+    for (int d = l8 * 8; d < a.D; d += 64) {
+      const uint4 x = *reinterpret_cast<const uint4*>(q + h * a.qs.h + d);
+      const uint4 y = *reinterpret_cast<const uint4*>(cen + d);
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = mma::unpack2<T>(u[k]), g = mma::unpack2<T>(v[k]);
+        s += static_cast<double>(f.x) * static_cast<double>(g.x);
+        s += static_cast<double>(f.y) * static_cast<double>(g.y);
+      }
+    }
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     nan |= isnan(s);
     best = fmax(best, s);
   }
   double s = best * a.scale;
-  if (a.bias != nullptr) s += static_cast<double>(a.bias[static_cast<int64_t>(r) * a.K + c]);
-  return nan || isnan(s) ? -INFINITY : s;
+  if (a.bias != nullptr && c >= 0) s += static_cast<double>(a.bias[static_cast<int64_t>(r) * a.K + c]);
+  return nan || isnan(s) || c < 0 ? -INFINITY : s;
 }
 
 // The band around the top-th score t in which fp32 cannot tell; infinite where a
@@ -264,6 +307,7 @@ __global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
                                                           int ctiles, int32_t* __restrict__ sel,
                                                           int64_t queries) {
   __shared__ double s_exact[4][KPL * 32];
+  __shared__ uint16_t s_list[4][KPL * 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   const int64_t qi = static_cast<int64_t>(blockIdx.x) * 4 + warp;
@@ -279,15 +323,34 @@ __global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
   }
   have = __reduce_add_sync(0xFFFFFFFFu, have);
   const uint32_t below = (1u << lane) - 1u;
-  uint32_t t = 0;
+  // t: the want-th largest key, bit by bit below the bits that all keys share; where a count
+  // meets it, the smallest key counted
   const int want = min(a.top, have);
+  uint32_t t = 0;
   if (have > 0) {
-    for (int bit = 31; bit >= 0; --bit) {
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+    for (int j = 0; j < KPL; ++j)
+      if (key[j] != 0u) low = min(low, key[j]), high = max(high, key[j]);
+    low = __reduce_min_sync(0xFFFFFFFFu, low);
+    high = __reduce_max_sync(0xFFFFFFFFu, high);
+    const int open_bits = 32 - __clz(low ^ high);
+    t = want == have ? low : open_bits == 32 ? 0u : high >> open_bits << open_bits;
+    for (int bit = want == have ? -1 : open_bits - 1; bit >= 0; --bit) {
       const uint32_t cand = t | (1u << bit);
       int n = 0;
 #pragma unroll
       for (int j = 0; j < KPL; ++j) n += key[j] >= cand;
-      if (__reduce_add_sync(0xFFFFFFFFu, n) >= want) t = cand;
+      n = __reduce_add_sync(0xFFFFFFFFu, n);
+      if (n >= want) t = cand;
+      if (n == want) {
+        uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+        for (int j = 0; j < KPL; ++j)
+          if (key[j] >= cand) least = min(least, key[j]);
+        t = __reduce_min_sync(0xFFFFFFFFu, least);
+        break;
+      }
     }
   }
   const float cn = largest_norm(c_norm, r, ctiles);
@@ -313,15 +376,20 @@ __global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
     in |= mid;  // no choice to make
   } else if (undecided > 0) {
     double* ex = s_exact[warp];
-#pragma unroll 1
+    uint16_t* list = s_list[warp];
+    int listed = 0;
+#pragma unroll
     for (int j = 0; j < KPL; ++j) {
-      uint32_t todo = __ballot_sync(0xFFFFFFFFu, mid >> j & 1u);
-      while (todo != 0) {
-        const int who = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const double s = exact_score<T>(a, r, i, j * 32 + who);
-        if (lane == who) ex[j * 32 + lane] = s;
-      }
+      const uint32_t who = __ballot_sync(0xFFFFFFFFu, mid >> j & 1u);
+      if (mid >> j & 1u) list[listed + __popc(who & below)] = static_cast<uint16_t>(j * 32 + lane);
+      listed += __popc(who);
+    }
+    __syncwarp();
+    for (int k = 0; k < listed; k += 4) {  // four at a time, eight lanes each
+      const int at = k + (lane >> 3);
+      const int c = at < listed ? list[at] : -1;
+      const double s = exact_score<T>(a, r, i, c);
+      if (c >= 0 && (lane & 7) == 0) ex[c] = s;
     }
     __syncwarp();
     // the places best of them: largest score, then lowest index
@@ -362,25 +430,42 @@ __global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
 
 constexpr int kCtaThreads = 512;
 
-// Sum over the CTA (every thread gets it).
-__device__ __forceinline__ int cta_sum(int v, int* red) {
-  v = __reduce_add_sync(0xFFFFFFFFu, v);
+// Sum over the CTA (every thread gets it). red: two rows used in turn, so that one barrier is
+// enough.
+struct CtaSum {
+  int (*red)[kCtaThreads / 32];
+  int turn = 0;
+  __device__ __forceinline__ int operator()(int v) {
+    v = __reduce_add_sync(0xFFFFFFFFu, v);
+    int* r = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < kCtaThreads / 32; ++w) s += r[w];
+    return s;
+  }
+};
+__device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xFFFFFFFFu, v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  int s = 0;
+  uint32_t m = 0;
 #pragma unroll
-  for (int w = 0; w < kCtaThreads / 32; ++w) s += red[w];
-  return s;
+  for (int w = 0; w < kCtaThreads / 32; ++w) m = max(m, red[w]);
+  return m;
 }
 
-// One CTA per query, up to 16384 clusters: keys, states and 64-bit scores in shared memory.
+// One CTA per query, for few queries or many clusters, up to 16384: keys, states and 64-bit scores in shared memory.
 template <typename T>
 __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
     SelectArgs a, const float* __restrict__ scores, const float* __restrict__ q_norm,
     const float* __restrict__ c_norm, int ctiles, int32_t* __restrict__ sel) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int red[kCtaThreads / 32];
+  __shared__ int sums[2][kCtaThreads / 32], red[kCtaThreads / 32];
+  __shared__ uint32_t maxima[kCtaThreads / 32];
   __shared__ double s_best[kCtaThreads / 32];
   __shared__ int s_at[kCtaThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -391,21 +476,39 @@ __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
   const int64_t qi = blockIdx.x;
   const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
   const float* row = scores + qi * a.K;
+  CtaSum cta_sum{sums};
   int have = 0;
+  uint32_t low = 0, high = 0;  // low: the complement of the smallest
   for (int c = tid; c < a.K; c += kCtaThreads) {
-    key[c] = sort_key(row[c]);
-    have += key[c] != 0u;
+    const uint32_t k = sort_key(row[c]);
+    key[c] = k;
+    if (k == 0u) continue;
+    ++have;
+    low = max(low, ~k), high = max(high, k);
   }
-  have = cta_sum(have, red);
+  have = cta_sum(have);
+  low = ~cta_max(low, maxima);
+  high = cta_max(high, maxima);
   const int want = min(a.top, have);
-  uint32_t t = 0;
-  if (have > 0)
-    for (int bit = 31; bit >= 0; --bit) {
+  uint32_t t = 0;  // as in choose_warp_kernel
+  if (have > 0) {
+    const int open_bits = 32 - __clz(low ^ high);
+    t = want == have ? low : open_bits == 32 ? 0u : high >> open_bits << open_bits;
+    for (int bit = want == have ? -1 : open_bits - 1; bit >= 0; --bit) {
       const uint32_t cand = t | (1u << bit);
       int n = 0;
       for (int c = tid; c < a.K; c += kCtaThreads) n += key[c] >= cand;
-      if (cta_sum(n, red) >= want) t = cand;
+      n = cta_sum(n);
+      if (n >= want) t = cand;
+      if (n == want) {
+        uint32_t least = 0;
+        for (int c = tid; c < a.K; c += kCtaThreads)
+          if (key[c] >= cand) least = max(least, ~key[c]);
+        t = ~cta_max(least, maxima);
+        break;
+      }
     }
+  }
   const float cn = largest_norm(c_norm, r, ctiles);
   const float ts = key_score(t);
   const float band = t <= 1u ? INFINITY : band_of(a, ts, q_norm[qi], cn);
@@ -422,17 +525,19 @@ __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
     }
     state[c] = st;
   }
-  sure = cta_sum(sure, red);
-  undecided = cta_sum(undecided, red);
+  sure = cta_sum(sure);
+  undecided = cta_sum(undecided);
   const int places = want - sure;
   const bool all = undecided == places && !open;
   if (!all && undecided > 0) {
     __syncthreads();
-    for (int c = warp; c < a.K; c += kCtaThreads / 32)
-      if (state[c] == 2) {
-        const double s = exact_score<T>(a, r, i, c);
-        if (lane == 0) ex[c] = s;
-      }
+    for (int c0 = warp * 4; c0 < a.K; c0 += kCtaThreads / 8) {  // four at a time, eight lanes each
+      const int c = c0 + (lane >> 3);
+      const bool mine = c < a.K && state[c] == 2;
+      if (!__any_sync(0xFFFFFFFFu, mine)) continue;
+      const double s = exact_score<T>(a, r, i, mine ? c : -1);
+      if (mine && (lane & 7) == 0) ex[c] = s;
+    }
     __syncthreads();
     for (int n = 0; n < places; ++n) {
       double best = -INFINITY;
@@ -495,12 +600,12 @@ SelectLayout select_layout(int64_t R, int64_t Nq, int64_t K) {
   return l;
 }
 
-template <typename T, int DP, int QW>
+template <typename T, int DP, int QW, bool PACK = false>
 int score_typed(const SelectArgs& a, int64_t R, float* scores, float* qn, float* cn, int ctiles,
                 cudaStream_t stream) {
   const int qtiles = (a.Nq + 16 * QW - 1) / (16 * QW);
   const int smem = (kClusters + 2 * 16 * QW) * DP * 2;
-  auto kern = score_kernel<T, DP, QW>;
+  auto kern = score_kernel<T, DP, QW, PACK>;
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int64_t blocks = R * qtiles * ctiles;
   FKC_REQUIRE(blocks <= 2147483647ll, "select: too many tiles");
@@ -514,16 +619,20 @@ int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cuda
   float* scores = reinterpret_cast<float*>(ws + l.scores);
   float* qn = reinterpret_cast<float*>(ws + l.q_norm);
   float* cn = reinterpret_cast<float*>(ws + l.c_norm);
-  // a few queries: one warp's rows, the other warps take clusters
-  const bool few = a.Nq <= 16;
-  if (a.D <= 64)
-    FKC_TRY((few ? score_typed<T, 64, 1> : score_typed<T, 64, 4>)(a, R, scores, qn, cn, l.ctiles,
-                                                                  stream));
-  else
-    FKC_TRY((few ? score_typed<T, 128, 1> : score_typed<T, 128, 4>)(a, R, scores, qn, cn, l.ctiles,
-                                                                    stream));
+  // a few queries: one warp's rows (of all heads at once where they fit), the other warps
+  // take clusters
+  const bool pack = static_cast<int64_t>(a.Nq) * a.G <= 16, few = a.Nq <= 16;
+  auto score = a.D <= 64 ? (pack  ? score_typed<T, 64, 1, true>
+                            : few ? score_typed<T, 64, 1>
+                                  : score_typed<T, 64, 4>)
+                         : (pack  ? score_typed<T, 128, 1, true>
+                            : few ? score_typed<T, 128, 1>
+                                  : score_typed<T, 128, 4>);
+  FKC_TRY(score(a, R, scores, qn, cn, l.ctiles, stream));
   const int64_t queries = R * a.Nq;
-  if (a.K <= 1024) {
+  // a warp's registers hold the scores of 1024 clusters; where there are fewer warps than
+  // schedulers (148 x 4), a CTA per query is faster (128 queries of 1024 clusters: see below)
+  if (a.K <= 1024 && queries > 592) {
     auto kern = a.K <= 128   ? choose_warp_kernel<T, 4>
                 : a.K <= 256 ? choose_warp_kernel<T, 8>
                 : a.K <= 512 ? choose_warp_kernel<T, 16>
