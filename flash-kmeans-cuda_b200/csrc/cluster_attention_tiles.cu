@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         ok = ok && mbar_wait(smem_u32(&mt.v_full[p.stage]), p.parity, abort);
         if (!ok) return;
         tc_fence_after();
-        mma_tmem_rows(tmem + sub * 256 + 128, tmem + sub * 256, sb + S::kV + p.stage * S::kTile,
+        mma_tmem_rows<8>(tmem + sub * 256 + 128, tmem + sub * 256, sb + S::kV + p.stage * S::kTile,
                       idesc_o, p.ksteps, p.first);
         if (p.last) umma_commit(smem_u32(&mt.o_full[sub]));
       };
@@ -554,88 +554,87 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   }
 }
 
-// One warp per (query, head): joins the parts of its clusters, whose log-sum-exps are to base
-// 2. A part's row takes L lanes of 16 bytes.
+// One warp per (query, GP heads): joins the parts of its clusters, whose log-sum-exps are to
+// base 2.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
+__global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq, int gp, int chunks,
                                                          const int32_t* __restrict__ pair_row,
                                                          const uint8_t* __restrict__ part_o,
                                                          const float2* __restrict__ part_lse,
                                                          T* __restrict__ out,
-                                                         float* __restrict__ lse, int64_t rows) {
-  constexpr int E = 16 / Part<T>::kBytes, L = DP / E, P = 32 / L;
-  constexpr int kAhead = 8;  // loads in flight: 8 * P parts
+                                                         float* __restrict__ lse, int64_t warps) {
+  constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
+  constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
-  const int lane = threadIdx.x & 31, grp = lane / L, d = lane % L * E;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i - i0, h)
-  if (row >= rows) return;
-  const int h = static_cast<int>(row % a.G);
-  const int64_t qi = row / a.G;
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i - i0, heads)
+  if (w0 >= warps) return;
+  const JoinLane me(gp);
+  const int h = static_cast<int>(w0 % chunks) * gp + me.head;
+  const int64_t qi = w0 / chunks;
   const int r = static_cast<int>(qi / nq), i = i0 + static_cast<int>(qi % nq);
-  const int b = r / a.Hkv, hq = (r - b * a.Hkv) * a.G + h;
+  const int b = r / a.Hkv, per = 4 / gp;
   const int32_t* pairs = pair_row + qi * a.top;
-  float top = -INFINITY, sum = 0.f, acc[E];
+  float top = -INFINITY, sum = 0.f, acc[SEGS][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < a.top; s0 += kAhead * P) {
-    uint4 v[kAhead];
+  for (int g = 0; g < SEGS; ++g)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
+  for (int s0 = 0; s0 < a.top; s0 += kAhead * per) {
+    uint4 v[kAhead][SEGS];
     float2 w[kAhead];
     float big = top;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int s = s0 + u * P + grp;
-      const int64_t n = s < a.top ? pairs[s] : -1;
+      const int s = s0 + u * per + me.slot;
+      const int64_t n = s < a.top && h < a.G ? pairs[s] : -1;
       w[u] = n >= 0 ? part_lse[n + h] : make_float2(-INFINITY, 0.f);
-      v[u] = make_uint4(0, 0, 0, 0);
-      if (n >= 0)
-        v[u] = __ldcs(reinterpret_cast<const uint4*>(
-            part_o + part_at(n + h, lane % L, DP * Part<T>::kBytes)));
-      big = fmaxf(big, w[u].x);
+#pragma unroll
+      for (int g = 0; g < SEGS; ++g) {
+        v[u][g] = make_uint4(0, 0, 0, 0);
+        if (n >= 0)
+          v[u][g] = __ldcs(reinterpret_cast<const uint4*>(
+              part_o + part_at(n + h, g * 8 + me.piece, DP * kBytes)));
+      }
     }
 #pragma unroll
-    for (int o = 16; o >= L; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+    for (int u = 0; u < kAhead; ++u) big = fmaxf(big, w[u].x);
     const float from = big == -INFINITY ? 0.f : big, alpha = exp2f(top - from);
     top = big;
     sum *= alpha;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= alpha;
+    for (int g = 0; g < SEGS; ++g)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[g][e] *= alpha;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (w[u].x == -INFINITY) continue;  // no part, or it sees nothing of its cluster
-      const float p = exp2f(w[u].x - from), f = p * w[u].y;
+      const float p = exp2f(w[u].x - from);
       sum += p;
-      const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      if constexpr (Part<T>::kHalf) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y = mma::unpack2<__half>(x[e]);
-          acc[2 * e] += f * y.x;
-          acc[2 * e + 1] += f * y.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += f * __uint_as_float(x[e]);
-      }
+      for (int g = 0; g < SEGS; ++g) add_part<T, E>(acc[g], v[u][g], p * w[u].y);
     }
   }
+  for (int o = 8 * gp; o < 32; o <<= 1) {  // the slots' lanes
+    const float other = __shfl_xor_sync(0xFFFFFFFFu, top, o), big = fmaxf(top, other);
+    const float from = big == -INFINITY ? 0.f : big;
+    const float mine = exp2f(top - from), its = exp2f(other - from);
+    sum = sum * mine + __shfl_xor_sync(0xFFFFFFFFu, sum, o) * its;
 #pragma unroll
-  for (int o = 16; o >= L; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    for (int g = 0; g < SEGS; ++g)
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], o);
+      for (int e = 0; e < E; ++e)
+        acc[g][e] = acc[g][e] * mine + __shfl_xor_sync(0xFFFFFFFFu, acc[g][e], o) * its;
+    top = big;
   }
+  if (me.slot != 0 || h >= a.G) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t at = (static_cast<int64_t>(b) * a.Hq + hq) * a.Nq + i;
-  if (grp == 0 && d < a.D) {
-    uint32_t y[E / 2];
+  const int64_t at = (static_cast<int64_t>(b) * a.Hq + (r - b * a.Hkv) * a.G + h) * a.Nq + i;
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    if constexpr (E == 8)
-      *reinterpret_cast<uint4*>(out + at * a.D + d) = make_uint4(y[0], y[1], y[2], y[3]);
-    else
-      *reinterpret_cast<uint2*>(out + at * a.D + d) = make_uint2(y[0], y[1]);
+  for (int g = 0; g < SEGS; ++g) {
+    const int d = (g * 8 + me.piece) * E;
+    if (d < a.D) store_out<T, E>(out + at * a.D + d, acc[g], inv);
   }
-  if (lane == 0) lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (me.piece == 0) lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // Queries that one round takes: rounds of equal size whose parts stay below some 2^31 bytes
@@ -693,12 +692,13 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
                        static_cast<const Unit*>(l.plan.units),
                        static_cast<const int32_t*>(l.plan.start), part_o, part_lse,
                        device_error_word()));
-    const int64_t rows = R * nq * a.G;
-    FKC_TRY(launch_pdl(tiles_join_kernel<T, DP>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256),
-                       0, stream, a, static_cast<int>(i0), nq,
+    const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
+    const int64_t warps = R * nq * chunks;
+    FKC_TRY(launch_pdl(tiles_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
+                       0, stream, a, static_cast<int>(i0), nq, gp, chunks,
                        static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(part_o),
-                       static_cast<const float2*>(part_lse), out, lse, rows));
+                       static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse), out,
+                       lse, warps));
   }
   return FKC_OK;
 }

@@ -12,8 +12,10 @@
 //           border leaves fp32 sums of each side, and tiles_dkv_join_kernel adds them in order.
 //           The sequence is fixed by the inputs, so two runs give the same bits.
 //
-// Both run 128 columns as two halves of 64, a warpgroup each (a thread a row of TMEM): while
-// one turns its scores into dS the other's products run on the tensor cores. P and dS are
+// The 128 columns of a step are two halves of 64, a warpgroup each (a thread a row of TMEM), whose
+// products start as each is done. (S and dP of 64 columns at a time, so that one half's
+// products would run beside the other's scores, took twice as long: an MMA of N = 64 costs
+// about as much as one of 128.) P and dS are
 // rounded to the 16-bit input type, as the operand type demands, dS of dQ into two terms
 // (see cluster_attention_grad.cu).
 #include <algorithm>
@@ -79,7 +81,7 @@ struct DqSmem {
   static constexpr uint32_t kMeta = kOut + 8 * 4096;
   struct Meta {
     int32_t key[2][kKeysStep];
-    uint64_t k_full[2], v_full[2], kv_free[2], q_full, q_free, sp_full[2], ds_full[2], dq_full, dq_free;
+    uint64_t k_full[2], v_full[2], kv_free[2], q_full, q_free, sp_full, ds_full[2], dq_full, dq_free;
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -116,11 +118,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
       mbar_init(smem_u32(&mt.k_full[x]), 32);  // the gathering lanes (their keys), and the bytes
       mbar_init(smem_u32(&mt.v_full[x]), 1);
       mbar_init(smem_u32(&mt.kv_free[x]), 1);
-      mbar_init(smem_u32(&mt.sp_full[x]), 1);
       mbar_init(smem_u32(&mt.ds_full[x]), 128);
     }
     mbar_init(smem_u32(&mt.q_full), 4);
     mbar_init(smem_u32(&mt.q_free), 1);
+    mbar_init(smem_u32(&mt.sp_full), 1);
     mbar_init(smem_u32(&mt.dq_full), 1);
     mbar_init(smem_u32(&mt.dq_free), 256);
     mbar_init(smem_u32(&mt.drain), 1);
@@ -160,15 +162,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
       const float lse = lse_next, delta = delta_next;
       fetch(it.next_row());
       const int steps = it.un.steps();
-      for (int step = 0; step < steps; ++step) {
+      for (int step = 0; step < steps; ++step, ++s_uses) {
         const int keys = it.un.keys(step) - half * 64;
         if (keys <= 0) continue;
         const uint32_t load = it.load + step;
         const int st = load & 1;
         ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
-             warp_mbar_wait(&mt.sp_full[half], s_uses & 1, abort);
+             warp_mbar_wait(&mt.sp_full, s_uses & 1, abort);
         if (!ok) break;
-        ++s_uses;
         tc_fence_after();
         const int32_t* key = mt.key[st] + half * 64;
 #pragma unroll
@@ -279,8 +280,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         if (!ok) return;
         tc_fence_after();
         const uint32_t kt = sb + S::kK + p.stage * S::kTile + half * 64 * 128;
-        mma_tmem_rows(tmem + 256, tmem + half * 64, kt, idesc_o, p.ksteps, p.first);
-        mma_tmem_rows(tmem + 256, tmem + 128 + half * 64, kt, idesc_o, p.ksteps, false);
+        mma_tmem_rows<4>(tmem + 256, tmem + half * 64, kt, idesc_o, p.ksteps, p.first);
+        mma_tmem_rows<4>(tmem + 256, tmem + 128 + half * 64, kt, idesc_o, p.ksteps, false);
         if (p.last) umma_commit(smem_u32(&mt.dq_full));
       };
       for (SubIter it(units, start); ok && it.valid(); it.advance(), ++uses) {
@@ -289,25 +290,20 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
           const uint32_t load = it.load + step;
           const int st = load & 1;
           const int keys = it.un.keys(step);
-          for (int half = 0; half < 2; ++half) {
-            product(half);
-            const int mine = min(64, keys - half * 64);
-            if (!ok || mine <= 0) continue;
-            ok = mbar_wait(smem_u32(&mt.k_full[st]), (load >> 1) & 1, abort) &&
-                 mbar_wait(smem_u32(&mt.v_full[st]), (load >> 1) & 1, abort) &&
-                 mbar_wait(smem_u32(&mt.q_full), uses & 1, abort);
-            if (!ok) break;
-            const int k16 = (mine + 15) / 16;
-            const uint32_t idesc = umma_idesc_f16(kBf16, kSub, 16 * k16);
-            mma_kmajor<DP>(tmem + half * 64, sb + S::kQ, sb + S::kK + st * S::kTile + half * 64 * 128,
-                           idesc, dsteps);
-            mma_kmajor<DP>(tmem + 128 + half * 64, sb + S::kDo,
-                           sb + S::kV + st * S::kTile + half * 64 * 128, idesc, dsteps);
-            umma_commit(smem_u32(&mt.sp_full[half]));
-            const bool last = step == steps - 1 && (half == 1 || keys <= 64);
-            if (last) umma_commit(smem_u32(&mt.q_free));
-            pend[half] = {true, step == 0 && half == 0, last, st, k16, uses};
-          }
+          product(0);
+          product(1);
+          ok = ok && mbar_wait(smem_u32(&mt.k_full[st]), (load >> 1) & 1, abort) &&
+               mbar_wait(smem_u32(&mt.v_full[st]), (load >> 1) & 1, abort) &&
+               mbar_wait(smem_u32(&mt.q_full), uses & 1, abort);
+          if (!ok) break;
+          const uint32_t idesc = umma_idesc_f16(kBf16, kSub, (keys + 15) / 16 * 16);
+          mma_kmajor<DP>(tmem, sb + S::kQ, sb + S::kK + st * S::kTile, idesc, dsteps);
+          mma_kmajor<DP>(tmem + 128, sb + S::kDo, sb + S::kV + st * S::kTile, idesc, dsteps);
+          umma_commit(smem_u32(&mt.sp_full));
+          const bool end = step == steps - 1, two = keys > 64;
+          if (end) umma_commit(smem_u32(&mt.q_free));
+          pend[0] = {true, step == 0, end && !two, st, (min(keys, 64) + 15) / 16, uses};
+          if (two) pend[1] = {true, false, end, st, (keys - 64 + 15) / 16, uses};
           if (ok && to_free >= 0) umma_commit(smem_u32(&mt.kv_free[to_free]));
           to_free = it.keep ? -1 : st;
         }
@@ -405,70 +401,62 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
   }
 }
 
-// One warp per (query, head): dq = the sum of its clusters' parts. A part's row takes L
-// lanes of 16 bytes.
+// One warp per (query, GP heads): dq = the sum of its clusters' parts.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, const int32_t* __restrict__ pair_row,
+__global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int chunks,
+                                                            const int32_t* __restrict__ pair_row,
                                                             const uint8_t* __restrict__ part,
                                                             const float* __restrict__ part_scale,
-                                                            T* __restrict__ dq, int64_t rows) {
-  constexpr int E = 16 / Part<T>::kBytes, L = DP / E, P = 32 / L;
-  constexpr int kAhead = 8;  // loads in flight: 8 * P parts
+                                                            T* __restrict__ dq, int64_t warps) {
+  constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
+  constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
-  const int lane = threadIdx.x & 31, grp = lane / L, d = lane % L * E;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i, h)
-  if (row >= rows) return;
-  const int h = static_cast<int>(row % a.G);
-  const int64_t qi = row / a.G;
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i, heads)
+  if (w0 >= warps) return;
+  const JoinLane me(gp);
+  const int h = static_cast<int>(w0 % chunks) * gp + me.head;
+  const int64_t qi = w0 / chunks;
   const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
-  const int b = r / a.Hkv, hq = (r - b * a.Hkv) * a.G + h;
+  const int b = r / a.Hkv, per = 4 / gp;
   const int32_t* pairs = pair_row + qi * a.top;
-  float acc[E];
+  float acc[SEGS][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < a.top; s0 += kAhead * P) {
-    uint4 v[kAhead];
-    float f[kAhead];
+  for (int g = 0; g < SEGS; ++g)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
+  for (int s0 = 0; s0 < a.top; s0 += kAhead * per) {
+    uint4 v[kAhead][SEGS];
+    float f[kAhead][SEGS];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int s = s0 + u * P + grp;
-      const int64_t n = s < a.top ? pairs[s] : -1;
-      v[u] = make_uint4(0, 0, 0, 0);
-      f[u] = 0.f;
-      if (n >= 0) {
-        v[u] = __ldcs(reinterpret_cast<const uint4*>(part + part_at(n + h, lane % L, DP * Part<T>::kBytes)));
-        f[u] = Part<T>::kHalf ? part_scale[(n + h) * 2 + (lane % L) / 8] : 1.f;
+      const int s = s0 + u * per + me.slot;
+      const int64_t n = s < a.top && h < a.G ? pairs[s] : -1;
+#pragma unroll
+      for (int g = 0; g < SEGS; ++g) {
+        v[u][g] = make_uint4(0, 0, 0, 0);
+        f[u][g] = 0.f;
+        if (n < 0) continue;
+        v[u][g] = __ldcs(reinterpret_cast<const uint4*>(part + part_at(n + h, g * 8 + me.piece, DP * kBytes)));
+        f[u][g] = Part<T>::kHalf ? part_scale[(n + h) * 2 + g] : 1.f;
       }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      if constexpr (Part<T>::kHalf) {
+    for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y = mma::unpack2<__half>(x[e]);
-          acc[2 * e] += f[u] * y.x;
-          acc[2 * e + 1] += f[u] * y.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += __uint_as_float(x[e]);
-      }
-    }
+      for (int g = 0; g < SEGS; ++g) add_part<T, E>(acc[g], v[u][g], f[u][g]);
   }
+  for (int o = 8 * gp; o < 32; o <<= 1)  // the slots' lanes
 #pragma unroll
-  for (int o = 16; o >= L; o >>= 1)
+    for (int g = 0; g < SEGS; ++g)
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], o);
-  if (grp != 0 || d >= a.D) return;
-  T* out = dq + ((static_cast<int64_t>(b) * a.Hq + hq) * a.Nq + i) * a.D + d;
-  uint32_t y[E / 2];
+      for (int e = 0; e < E; ++e) acc[g][e] += __shfl_xor_sync(0xFFFFFFFFu, acc[g][e], o);
+  if (me.slot != 0 || h >= a.G) return;
+  T* out = dq + ((static_cast<int64_t>(b) * a.Hq + (r - b * a.Hkv) * a.G + h) * a.Nq + i) * a.D;
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(acc[2 * e], acc[2 * e + 1]);
-  if constexpr (E == 8)
-    *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
-  else
-    *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[1]);
+  for (int g = 0; g < SEGS; ++g) {
+    const int d = (g * 8 + me.piece) * E;
+    if (d < a.D) store_out<T, E>(out + d, acc[g], 1.f);
+  }
 }
 
 // ---------------------------------------------------------------------------- dK, dV
@@ -638,7 +626,7 @@ struct DkvSmem {
   struct Meta {
     float lse[2][kSub], delta[2][kSub];  // of a stage's rows
     int32_t pos[2][kSub];
-    uint64_t kv_full, kv_free, q_full[2], q_free[2], sp_full[2], ds_full[2], acc_full, acc_free;
+    uint64_t kv_full, kv_free, q_full[2], q_free[2], sp_full, ds_full[2], acc_full, acc_free;
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -671,11 +659,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&mt.q_full[x]), 66);  // two warps' lanes (their rows' data), two warps' bytes
       mbar_init(smem_u32(&mt.q_free[x]), 1);
-      mbar_init(smem_u32(&mt.sp_full[x]), 1);
       mbar_init(smem_u32(&mt.ds_full[x]), 128);
     }
     mbar_init(smem_u32(&mt.kv_full), 2);
     mbar_init(smem_u32(&mt.kv_free), 1);
+    mbar_init(smem_u32(&mt.sp_full), 1);
     mbar_init(smem_u32(&mt.acc_full), 1);
     mbar_init(smem_u32(&mt.acc_free), 256);
     mbar_init(smem_u32(&mt.drain), 1);
@@ -700,7 +688,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     const uint32_t t_s = tmem + lanes + half * 64, t_p = t_s + 128;
     const uint32_t t_acc = tmem + lanes + 256 + half * 128;  // warps 0-3 write dV, 4-7 dK
     const float sc = a.scale * kLog2e;
-    uint32_t item = 0, s_uses = 0;
+    uint32_t item = 0;
     bool ok = true;
     for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
       int key = INT_MAX;
@@ -713,9 +701,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
         if (rows <= 0) continue;
         const int st = item & 1;
         ok = warp_mbar_wait(&mt.q_full[st], (item >> 1) & 1, abort) &&
-             warp_mbar_wait(&mt.sp_full[half], s_uses & 1, abort);
+             warp_mbar_wait(&mt.sp_full, item & 1, abort);
         if (!ok) break;
-        ++s_uses;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -808,31 +795,28 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
         if (!ok) return;
         tc_fence_after();
         const uint32_t o = p.stage * S::kTile + half * 64 * 128;
-        mma_tmem_rows(tmem + 256, tmem + half * 64, sb + S::kDo + o, idesc_o, p.ksteps, p.first);
-        mma_tmem_rows(tmem + 384, tmem + 128 + half * 64, sb + S::kQ + o, idesc_o, p.ksteps, p.first);
+        mma_tmem_rows<4>(tmem + 256, tmem + half * 64, sb + S::kDo + o, idesc_o, p.ksteps, p.first);
+        mma_tmem_rows<4>(tmem + 384, tmem + 128 + half * 64, sb + S::kQ + o, idesc_o, p.ksteps, p.first);
         if (p.last) umma_commit(smem_u32(&mt.acc_full));
       };
       for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
         for (int step = it.step; ok && step < it.end; ++step, ++item) {
           const int st = item & 1;
           const int rows = it.tile.nrows - step * kSub;
-          for (int half = 0; half < 2; ++half) {
-            product(half);
-            const int mine = min(64, rows - half * 64);
-            if (!ok || mine <= 0) continue;
-            ok = mbar_wait(smem_u32(&mt.kv_full), it.seg & 1, abort) &&
-                 mbar_wait(smem_u32(&mt.q_full[st]), (item >> 1) & 1, abort);
-            if (!ok) break;
-            const int k16 = (mine + 15) / 16;
-            const uint32_t idesc = umma_idesc_f16(kBf16, kSub, 16 * k16);
-            const uint32_t o = st * S::kTile + half * 64 * 128;
-            mma_kmajor<DP>(tmem + half * 64, sb + S::kK, sb + S::kQ + o, idesc, dsteps);
-            mma_kmajor<DP>(tmem + 128 + half * 64, sb + S::kV, sb + S::kDo + o, idesc, dsteps);
-            umma_commit(smem_u32(&mt.sp_full[half]));
-            const bool last = step == it.end - 1 && (half == 1 || rows <= 64);
-            if (last) umma_commit(smem_u32(&mt.kv_free));
-            pend[half] = {true, step == it.step && half == 0, last, st, k16, it.seg};
-          }
+          product(0);
+          product(1);
+          ok = ok && mbar_wait(smem_u32(&mt.kv_full), it.seg & 1, abort) &&
+               mbar_wait(smem_u32(&mt.q_full[st]), (item >> 1) & 1, abort);
+          if (!ok) break;
+          const int mine = min(kSub, rows);
+          const uint32_t idesc = umma_idesc_f16(kBf16, kSub, (mine + 15) / 16 * 16);
+          mma_kmajor<DP>(tmem, sb + S::kK, sb + S::kQ + st * S::kTile, idesc, dsteps);
+          mma_kmajor<DP>(tmem + 128, sb + S::kV, sb + S::kDo + st * S::kTile, idesc, dsteps);
+          umma_commit(smem_u32(&mt.sp_full));
+          const bool end = step == it.end - 1, two = mine > 64;
+          if (end) umma_commit(smem_u32(&mt.kv_free));
+          pend[0] = {true, step == it.step, end && !two, st, (min(mine, 64) + 15) / 16, it.seg};
+          if (two) pend[1] = {true, false, end, st, (mine - 64 + 15) / 16, it.seg};
           if (ok && to_free >= 0) umma_commit(smem_u32(&mt.q_free[to_free]));
           to_free = st;
         }
@@ -1027,10 +1011,11 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
     FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                        q_row, do_row, pos, row_lse, row_delta, static_cast<const Unit*>(l.plan.units),
                        static_cast<const int32_t*>(l.plan.start), ws + l.part, scales, device_error_word()));
-    const int64_t rows = R * a.Nq * a.G;
-    FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
-                       stream, a, static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, rows));
+    const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
+    const int64_t warps = R * a.Nq * chunks;
+    FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0,
+                       stream, a, gp, chunks, static_cast<const int32_t*>(l.plan.pair_row),
+                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, warps));
   }
   if (dk == nullptr) return FKC_OK;
   const size_t bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);

@@ -53,26 +53,43 @@ constexpr uint32_t tc_tile_bytes() {
   return kSub * DP * 2;
 }
 
-// D (+)= A B^T over the first `depth` elements (a multiple of 16) of K-major tiles.
+// The issue loops below run in one thread, whose instructions per MMA bound them: descriptors are
+// two halves of which a step adds a constant to one, and the usual depth is unrolled.
+//
+// D = A B^T over 16 * ksteps elements of K-major tiles.
 template <int DP>
 __device__ __forceinline__ void mma_kmajor(uint32_t d, uint32_t a_tile, uint32_t b_tile,
                                            uint32_t idesc, int ksteps) {
   constexpr uint32_t hi = ptx::umma_desc_hi(1024, ptx::kLayoutSwizzle128B);
   const uint32_t a = ptx::umma_desc_lo(a_tile), b = ptx::umma_desc_lo(b_tile);
-#pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    if (k >= ksteps) break;
+  auto step = [&](int k) {
     const uint32_t o = ((k >> 2) * (128 * kSub) + (k & 3) * 32) >> 4;
     ptx::umma_f16(d, ptx::umma_desc(a + o, hi), ptx::umma_desc(b + o, hi), idesc, k > 0);
+  };
+  if (ksteps == DP / 16) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) step(k);
+  } else {
+    for (int k = 0; k < ksteps; ++k) step(k);
   }
 }
 
 // D (+)= A B, A [lanes x 16 * ksteps] in TMEM, B the first 16 * ksteps rows of a tile (MN-major).
+// MOST: the usual number of steps.
+template <int MOST>
 __device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a_tmem, uint32_t b_tile,
                                               uint32_t idesc, int ksteps, bool fresh) {
-  for (int k = 0; k < ksteps; ++k)
-    ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc_mn(b_tile + k * 2048, 128 * kSub), idesc,
-                     !(fresh && k == 0));
+  constexpr uint32_t hi = ptx::umma_desc_hi(1024, ptx::kLayoutSwizzle128B);
+  const uint32_t b = ((b_tile >> 4) & 0x3FFFu) | ((128u * kSub >> 4) << 16);
+  ptx::umma_f16_ta(d, a_tmem, ptx::umma_desc(b, hi), idesc, fresh ? 0u : 1u);
+  if (ksteps == MOST) {
+#pragma unroll
+    for (int k = 1; k < MOST; ++k)
+      ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc(b + k * 128, hi), idesc, 1u);
+  } else {
+    for (int k = 1; k < ksteps; ++k)
+      ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc(b + k * 128, hi), idesc, 1u);
+  }
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -241,6 +258,47 @@ struct Part {
   static constexpr bool kHalf = !std::is_same<T, __half>::value;
   static constexpr int kBytes = kHalf ? 2 : 4;
 };
+
+// How a warp of the joins reads the parts of GP neighbouring heads of a query (the largest power
+// of two up to 4 and G): eight lanes take 128 bytes of a head's row, GP heads side by side, so
+// that a load covers 128 * GP bytes that lie together, and 4 / GP slots of sel at once.
+struct JoinLane {
+  int piece, head, slot;  // of 16 bytes; of the heads; of the slots
+  __device__ __forceinline__ JoinLane(int gp) {
+    const int lane = threadIdx.x & 31;
+    piece = lane & 7;
+    head = (lane >> 3) & (gp - 1);
+    slot = (lane >> 3) / gp;
+  }
+};
+inline int join_heads(int G) { return G >= 4 ? 4 : G >= 2 ? 2 : 1; }
+// The values in 16 bytes of a part, times f, added to acc.
+template <typename T, int E>
+__device__ __forceinline__ void add_part(float (&acc)[E], const uint4& v, float f) {
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (Part<T>::kHalf) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 y = mma::unpack2<__half>(x[e]);
+      acc[2 * e] += f * y.x;
+      acc[2 * e + 1] += f * y.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += f * __uint_as_float(x[e]);
+  }
+}
+// E values rounded to T.
+template <typename T, int E>
+__device__ __forceinline__ void store_out(T* out, const float (&v)[E], float f) {
+  uint32_t y[E / 2];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(v[2 * e] * f, v[2 * e + 1] * f);
+  if constexpr (E == 8)
+    *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
+  else
+    *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[1]);
+}
 
 }  // namespace attn
 }  // namespace fkc

@@ -403,13 +403,9 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t lo, uint32_t hi) {
   return d;
 }
 
-// Descriptor of an MN-major operand with 128-byte swizzle: columns of 64 16-bit elements
-// along M or N (128 bytes), one per k; lbo: byte distance between column blocks of 64, 1024
-// bytes between groups of eight k.
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t start, uint32_t lbo_bytes) {
-  return umma_desc(((start >> 4) & 0x3FFFu) | (((lbo_bytes >> 4) & 0x3FFFu) << 16),
-                   umma_desc_hi(1024, kLayoutSwizzle128B));
-}
+// Descriptors of an MN-major operand with 128-byte swizzle: columns of 64 16-bit elements
+// along M or N (128 bytes), one per k; the LBO field holds the byte distance between column
+// blocks of 64, the SBO 1024 bytes between groups of eight k.
 constexpr uint32_t kIdescMnB = 1u << 16;  // instruction descriptor: B is MN-major
 
 // kind::f16 instruction descriptor: fp32 accumulator, K-major A and B.
