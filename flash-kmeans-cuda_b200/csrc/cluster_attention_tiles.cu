@@ -17,6 +17,7 @@
 // row, with the running maximum and sum in fp32, and write O out. P is rounded to the 16-bit
 // input type for the second product, as its operand type demands.
 #include <algorithm>
+#include <atomic>
 #include <numeric>
 
 #include "cluster_attention.cuh"
@@ -93,7 +94,8 @@ __global__ void __launch_bounds__(1024) tile_units_kernel(Args a,
     for (int t = 0; t < n; ++t) {
       const int64_t u = static_cast<int64_t>(at & 0xFFFFFFFFu) + t;
       un.row0 = t * rows;
-      un.nrows = static_cast<int>(min(static_cast<int64_t>(rows), all - static_cast<int64_t>(t) * rows));
+      un.nrows = static_cast<int>(min(static_cast<int64_t>(rows), all - static_cast<int64_t>(t) * rows)) |
+                 (t + 1 < n ? Unit::kMore : 0);
       if (u < units_max) {  // always, with the workspace of carve_units
         units[u] = un;
         cum[u] = static_cast<int32_t>((at >> 32) + static_cast<unsigned long long>(t) * un.cost());
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, 
     const int rr = j * 32 + lane;
     int pos = -1, row = rq.rows;
     int64_t flat = -1;  // row of (batch, Hq, Nq)
-    if (rr < un.nrows) {
+    if (rr < (un.nrows & (Unit::kMore - 1))) {
       const int at = un.row0 + rr, e = at / a.G, h = at - e * a.G;
       const int p = list[e], i = i0 + p / a.top;
       if (h == 0) pair_row[pairs0 + p] = static_cast<int32_t>(u * kUnitRows + rr);
@@ -183,10 +185,15 @@ struct FwdSmem {
 
 enum : int { kErrLoad = 151, kErrMma = 152, kErrSoftmax = 153 };
 
-// Warps 0-3 and 4-7: softmax and output of rows 0-127 and 128-255 of a unit (a thread a
-// row); warp 8: the MMAs; warps 9, 10: gathers of keys and of values; 11-14: of Q, 64 rows
-// each (a gather takes its warp some 70 cycles to issue, so they are spread over warps).
-constexpr int kFwdThreads = 32 * 15;
+// Warps 0-3 and 4-7: softmax of rows 0-127 and 128-255 of a unit (a thread a row); 8-11 and
+// 12-15: their output, while the softmax goes on to the next unit; warp 16: the MMAs; warps 17,
+// 18: gathers of keys and of values; 19-22: of Q, 64 rows each (a gather takes its warp some 70
+// cycles to issue, so they are spread over warps); 23 has nothing to do.
+constexpr int kFwdThreads = 32 * 24;
+// Registers of the three kinds of warpgroups: as many in all as the launch's 80 a thread.
+constexpr int kLaunchRegs = 80, kSoftmaxRegs = 112, kOutputRegs = 72, kOtherRegs = 56;
+static_assert(256 * (kSoftmaxRegs + kOutputRegs + kOtherRegs) <= kFwdThreads * kLaunchRegs,
+              "setmaxnreg would wait for registers that the block does not have");
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const __grid_constant__ CUtensorMap tm_v, RowMap rk, RowMap rv, Args a,
     const int32_t* __restrict__ q_row, const int32_t* __restrict__ row_pos,
     const Unit* __restrict__ units, const int32_t* __restrict__ start, uint8_t* __restrict__ part_o,
-    float2* __restrict__ part_lse, int* err) {
+    float2* __restrict__ part_lse, float* __restrict__ part_scale, int* err) {
   using namespace ptx;
   using S = FwdSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     mt.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(&mt.tmem), 512);
     tmem_relinquish();
   }
@@ -231,12 +238,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   pdl_wait();
 
   if (warp < 8) {
-    // ------------------------------------------------------------ softmax, output
+    // ------------------------------------------------------------ softmax
+    more_registers<kSoftmaxRegs>();
     const int sub = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + sub * 256, t_o = t_s + 128;
     const float sc = a.scale * kLog2e;
-    uint32_t uses = 0, s_uses = 0;
+    uint32_t s_uses = 0;
     bool ok = true;
     UnitIter it(units, start);
     const int32_t* meta = row_pos + sub * kSub + row;
@@ -262,9 +270,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         tc_fence_after();
         const int keys = un.keys(step);
         const int32_t* key = mt.key[st];
+        // (loops over chunks stay loops: unrolled, the code of the kernel's roles outgrew the
+        // instruction cache)
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         uint32_t open = 0;  // 32-key chunks that every row of the warp sees whole
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kKeysStep / 32; ++c) {
           if (c * 32 >= keys) break;
           uint32_t s[32];
@@ -293,7 +303,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         m = mn;
         if (step > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
           // the product of the step before has ended: its commit came before this S's
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DP / 32; ++c) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(t_o + c * 32, o);
@@ -304,7 +314,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
           }
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kKeysStep / 32; ++c) {
           if (c * 32 >= keys) break;
           uint32_t s[32], p[16];
@@ -340,22 +350,32 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         mbar_arrive(smem_u32(&mt.p_full[sub]));
       }
       if (!ok) break;
+      part_lse[static_cast<int64_t>(it.n) * kUnitRows + sub * kSub + row] =
+          make_float2(l == 0.f ? -INFINITY : m + log2f(l), l == 0.f ? 0.f : 1.f / l);
+    }
+  } else if (warp < 16) {
+    // ------------------------------------------------------------ output
+    fewer_registers<kOutputRegs>();
+    const int sub = (warp >> 2) - 2, row = (warp & 3) * 32 + lane;
+    const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + sub * 256 + 128;
+    uint32_t uses = 0;
+    bool ok = true;
+    for (UnitIter it(units, start); ok && it.valid(); it.advance()) {
+      if (it.un.nrows <= sub * kSub) continue;
       ok = warp_mbar_wait(&mt.o_full[sub], uses & 1, abort);
       if (!ok) {
         give_up(abort, err, kErrSoftmax);
         break;
       }
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t urow = static_cast<int64_t>(it.n) * kUnitRows + sub * kSub + row;
-      const float ls = l == 0.f ? -INFINITY : m + log2f(l);
-      const uint32_t buf = sb + S::kOut + warp * 4096;
+      const uint32_t buf = sb + S::kOut + (warp - 8) * 4096;
       constexpr int kBytes = Part<T>::kBytes, kCols = 128 / kBytes;  // columns in 128 bytes
       uint8_t* dst = part_o + (urow - lane) * (DP * kBytes);
-      float scale = inv, back = 1.f;
+      float scale = 1.f;
       if constexpr (Part<T>::kHalf) {
         float big[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(t_o + c * 32, o);
@@ -364,16 +384,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
           for (int j = 0; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], fabsf(__uint_as_float(o[j])));
         }
         // the row's largest value to [2^14, 2^15); a row that is not finite stays as it is
-        const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * inv;
+        const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
         const int e =
             top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -112) : 0;
-        scale = inv * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        part_scale[urow] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
       }
-      part_lse[urow] = make_float2(ls, back);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < DP / kCols; ++c) {
-        uint4 piece[8];
+        begin_segment();
 #pragma unroll
         for (int x = 0; x < kCols / 32; ++x) {
           uint32_t o[32];
@@ -389,22 +408,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
               for (int e = 0; e < 4; ++e)
                 y[e] = mma::pack2<__half>(__uint_as_float(o[8 * j + 2 * e]),
                                           __uint_as_float(o[8 * j + 2 * e + 1]));
-              piece[x * 4 + j] = make_uint4(y[0], y[1], y[2], y[3]);
+              put_piece(buf, x * 4 + j, make_uint4(y[0], y[1], y[2], y[3]));
             } else {
-              piece[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              put_piece(buf, j, make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
             }
           }
         }
-        store_segment(buf, piece, dst + c * 4096);
+        end_segment(buf, dst + c * 4096);
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.o_free[sub]));
       ++uses;
     }
     if (lane == 0) bulk_wait_all();
-  } else if (warp == 8) {
-    // ------------------------------------------------------------ MMAs (one thread)
-    if (lane == 0) {
+  } else {
+    fewer_registers<kOtherRegs>();
+    if (warp == 16 && lane == 0) {
+      // ---------------------------------------------------------- MMAs (one thread)
       const int dsteps = (a.D + 15) / 16;
       constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, kSub, DP) | kIdescMnB;
       uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
@@ -464,12 +484,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       const int never = 0;
       mbar_wait(smem_u32(&mt.drain), 0, &never);
     }
-  } else {
     // ------------------------------------------------------------ gathers
     // The next step's (or unit's) row numbers are fetched while this one's copies run.
     bool ok = true;
-    if (warp <= 10) {
-      const bool values = warp == 10;
+    if (warp == 17 || warp == 18) {
+      const bool values = warp == 18;
       const CUtensorMap* tm = values ? &tm_v : &tm_k;
       const RowMap rm = values ? rv : rk;
       const uint32_t tiles = sb + (values ? S::kV : S::kK);
@@ -514,8 +533,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
           gather_rows4<DP>(tiles + st * S::kTile, tm, full, lane * 4, rows[0], rows[1], rows[2], rows[3]);
         __syncwarp();
       }
-    } else {
-      const int x = (warp - 11) >> 1, row0 = ((warp - 11) & 1) * 64 + (lane & 15) * 4;
+    } else if (warp >= 19 && warp < 23) {
+      const int x = (warp - 19) >> 1, row0 = ((warp - 19) & 1) * 64 + (lane & 15) * 4;
       const int4* src = reinterpret_cast<const int4*>(q_row) + (x * kSub + row0) / 4;
       UnitIter it(units, start);
       int4 ahead = it.valid() ? __ldg(src + static_cast<int64_t>(it.n) * (kUnitRows / 4)) : make_int4(0, 0, 0, 0);
@@ -539,7 +558,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     if (!ok) give_up(abort, err, kErrLoad);
     // copies in flight end before the CTA does: the MMA warp waits for all of them, and
     // after a wait that gave up they are waited for here
-    if (!ok || *abort) {
+    if (warp > 16 && (!ok || *abort)) {
       const uint64_t t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 1000000ull) {
       }
@@ -548,7 +567,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -561,6 +580,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
                                                          const int32_t* __restrict__ pair_row,
                                                          const uint8_t* __restrict__ part_o,
                                                          const float2* __restrict__ part_lse,
+                                                         const float* __restrict__ part_scale,
                                                          T* __restrict__ out,
                                                          float* __restrict__ lse, int64_t warps) {
   constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
@@ -588,6 +608,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
       const int s = s0 + u * per + me.slot;
       const int64_t n = s < a.top && h < a.G ? pairs[s] : -1;
       w[u] = n >= 0 ? part_lse[n + h] : make_float2(-INFINITY, 0.f);
+      if (Part<T>::kHalf && n >= 0) w[u].y *= part_scale[n + h];
 #pragma unroll
       for (int g = 0; g < SEGS; ++g) {
         v[u][g] = make_uint4(0, 0, 0, 0);
@@ -649,7 +670,7 @@ int64_t queries_per_round(const Args& a) {
 
 struct Layout {
   UnitPlan plan;
-  size_t part_lse, part_o, total;
+  size_t part_lse, part_scale, part_o, total;
   int64_t nq;
 };
 
@@ -663,6 +684,7 @@ Layout fwd_layout(const Args& a, int part_bytes, uint8_t* ws) {
     return p;
   };
   l.part_lse = take(l.plan.units_max * kUnitRows * 8);
+  l.part_scale = take(l.plan.units_max * kUnitRows * 4);
   l.part_o = take(l.plan.units_max * kUnitRows * (a.D <= 64 ? 64 : 128) * part_bytes);
   l.total = at;
   return l;
@@ -673,6 +695,7 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   const Layout l = fwd_layout(a, Part<T>::kBytes, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   float2* part_lse = reinterpret_cast<float2*>(ws + l.part_lse);
+  float* part_scale = reinterpret_cast<float*>(ws + l.part_scale);
   uint8_t* part_o = ws + l.part_o;
   CUtensorMap tm_q, tm_k, tm_v;
   RowMap rq, rk, rv;
@@ -681,6 +704,15 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   FKC_TRY(encode_rows(a.v, a.vs, a.batch, a.Hkv, a.N, a.D, dtype, &tm_v, &rv));
   auto kern = tiles_fwd_kernel<T, DP>;
   const int smem = static_cast<int>(FwdSmem<DP>::kBytes);
+  // the compiler gives the block as many registers as its warpgroups take in all, or they would wait
+  static std::atomic<int> regs{0};  // of this kernel, the same on every device
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes fa{};
+    FKC_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
+    regs.store(fa.numRegs, std::memory_order_relaxed);
+  }
+  FKC_REQUIRE(regs.load(std::memory_order_relaxed) >= kLaunchRegs, "attention: the kernel was built with %d registers",
+              regs.load(std::memory_order_relaxed));
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
@@ -690,15 +722,15 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
                        static_cast<const int32_t*>(l.plan.q_row),
                        static_cast<const int32_t*>(l.plan.row_pos),
                        static_cast<const Unit*>(l.plan.units),
-                       static_cast<const int32_t*>(l.plan.start), part_o, part_lse,
+                       static_cast<const int32_t*>(l.plan.start), part_o, part_lse, part_scale,
                        device_error_word()));
     const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
     const int64_t warps = R * nq * chunks;
     FKC_TRY(launch_pdl(tiles_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
                        0, stream, a, static_cast<int>(i0), nq, gp, chunks,
                        static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse), out,
-                       lse, warps));
+                       static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse),
+                       static_cast<const float*>(part_scale), out, lse, warps));
   }
   return FKC_OK;
 }

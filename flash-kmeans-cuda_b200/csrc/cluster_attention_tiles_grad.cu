@@ -35,19 +35,22 @@ struct SubIter {
   const Unit* units;
   int n, total, x;
   uint32_t load;
-  bool again, keep;
+  bool again, keep, follows;  // follows: another unit of the cluster, in this CTA
   Unit un, next;
 
   __device__ __forceinline__ SubIter(const Unit* u, const int32_t* start)
-      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), x(0), load(0), again(false) {
-    if (n < total) un = load_unit(units + n);
-    if (n + 1 < total) next = load_unit(units + n + 1);
-    look();
+      : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), x(0), load(0),
+        again(false), keep(false), follows(false) {
+    if (n < total) next = load_unit(units + n);
+    open();
   }
-  __device__ __forceinline__ void look() {
-    keep = false;
-    if (n >= total || un.steps() > 2) return;
-    keep = more() || (n + 1 < total && next.c == un.c && next.r == un.r);
+  __device__ __forceinline__ void open() {
+    if (n >= total) return;
+    un = next;
+    if (n + 1 < total) next = load_unit(units + n + 1);
+    follows = (un.nrows & Unit::kMore) != 0 && n + 1 < total;
+    un.nrows &= Unit::kMore - 1;
+    keep = un.steps() <= 2 && (more() || follows);
   }
   __device__ __forceinline__ bool more() const { return x == 0 && un.nrows > kSub; }
   __device__ __forceinline__ bool valid() const { return n < total; }
@@ -61,13 +64,13 @@ struct SubIter {
     again = keep;
     if (more()) {
       x = 1;
+      keep = un.steps() <= 2 && follows;
     } else {
       x = 0;
       ++n;
-      un = next;
-      if (n + 1 < total) next = load_unit(units + n + 1);
+      keep = false;
+      open();
     }
-    look();
   }
 };
 
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         if (!ok) break;
         tc_fence_after();
         const int32_t* key = mt.key[st] + half * 64;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           if (c * 32 >= keys) break;
           float s[32], dp[32];
@@ -212,11 +215,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
 #pragma unroll
       for (int c = 0; c < kSegs; ++c) {  // the segments are shared out
         if ((kSegs == 1 ? 0 : c * 2 / kSegs) != half) continue;
-        uint4 piece[8];
         float scale = a.scale, back = 1.f;
         if constexpr (Part<T>::kHalf) {
           float big[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < kCols / 32; ++x) {
             float o[32];
             tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
@@ -232,7 +234,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
           back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
           part_scale[urow * 2 + c] = back;
         }
-#pragma unroll
+        begin_segment();
+#pragma unroll 1
         for (int x = 0; x < kCols / 32; ++x) {
           float o[32];
           tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
@@ -242,15 +245,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
 #pragma unroll
           for (int j = 0; j < 8 * 32 / kCols; ++j) {
             if constexpr (Part<T>::kHalf)
-              piece[x * 4 + j] =
+              put_piece(buf, x * 4 + j,
                   make_uint4(mma::pack2<__half>(o[8 * j], o[8 * j + 1]), mma::pack2<__half>(o[8 * j + 2], o[8 * j + 3]),
-                             mma::pack2<__half>(o[8 * j + 4], o[8 * j + 5]), mma::pack2<__half>(o[8 * j + 6], o[8 * j + 7]));
+                             mma::pack2<__half>(o[8 * j + 4], o[8 * j + 5]), mma::pack2<__half>(o[8 * j + 6], o[8 * j + 7])));
             else
-              piece[j] = make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
-                                    __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3]));
+              put_piece(buf, j, make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                           __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
           }
         }
-        store_segment(buf, piece, dst + c * 4096);
+        end_segment(buf, dst + c * 4096);
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.dq_free));
@@ -704,7 +707,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
              warp_mbar_wait(&mt.sp_full, item & 1, abort);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           if (c * 32 >= rows) break;
           float s[32], dp[32];
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
       T* out = (half == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + (key == INT_MAX ? 0 : key)) * a.D;
       // a segment that does not begin its tile is the CTA's first
       float* sums = part + ((static_cast<int64_t>(blockIdx.x) * 2 + (it.step == 0)) * 2 + half) * (kSub * DP) + row * DP;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         float o[32];
         tmem_ld_f32_x32(t_acc + c * 32, o);

@@ -24,12 +24,15 @@ struct __align__(16) Unit {
   int c, row0, s0, s1;
   int e0, nrows, r, high;
 
+  // in memory, nrows carries a flag: another unit of the cluster follows
+  static constexpr int kMore = 1 << 16;
+
   __device__ __forceinline__ int steps() const { return (s1 - s0 + kKeysStep - 1) / kKeysStep; }
-  // in about 550 cycles: rows in and out (8), each of the one or two steps whose keys stay in
-  // shared memory from unit to unit (9), or each step of more, which every unit loads
-  // again (18); capped, so that sums stay below 2^31
+  // in about 580 cycles: each of the one or two steps whose keys stay in shared memory from
+  // unit to unit (16), or each step of more, which every unit loads again (18), and what a
+  // unit takes besides; capped, so that sums stay below 2^31
   __device__ __forceinline__ int cost() const {
-    return min(8 + (steps() <= 2 ? 9 : 18) * steps(), 1020);
+    return min(steps() <= 2 ? 1 + 16 * steps() : 8 + 18 * steps(), 1020);
   }
   __device__ __forceinline__ int keys(int step) const {
     return min(kKeysStep, s1 - s0 - step * kKeysStep);
@@ -114,19 +117,33 @@ __device__ __forceinline__ int64_t part_at(int64_t n, int j, int bytes) {
 }
 // One segment: lane l's 128 bytes of row l, to 4 KB at dst, through the warp's buffer; the copy
 // goes on while the warp does other things (the stores themselves, 16 bytes a lane to
-// rows or to whole lines alike, held the warps for some 170 cycles each).
-__device__ __forceinline__ void store_segment(uint32_t buf, const uint4 (&piece)[8], uint8_t* dst) {
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) ptx::bulk_wait_read();  // the buffer's last copy
+// rows or to whole lines alike, held the warps for some 170 cycles each). begin, eight
+// pieces, end.
+__device__ __forceinline__ void begin_segment() {
+  if ((threadIdx.x & 31) == 0) ptx::bulk_wait_read();  // the buffer's last copy
   __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 8; ++j) st_shared_v4(buf + lane * 128 + ((j ^ (lane & 7)) << 4), piece[j]);
+}
+__device__ __forceinline__ void put_piece(uint32_t buf, int j, const uint4& v) {
+  const int lane = threadIdx.x & 31;
+  st_shared_v4(buf + lane * 128 + ((j ^ (lane & 7)) << 4), v);
+}
+__device__ __forceinline__ void end_segment(uint32_t buf, uint8_t* dst) {
   ptx::fence_proxy_async_smem();
   __syncwarp();
-  if (lane == 0) {
+  if ((threadIdx.x & 31) == 0) {
     ptx::bulk_store(dst, buf, 4096);
     ptx::bulk_commit();
   }
+}
+
+// Registers of the warpgroup's threads from here on.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
@@ -218,10 +235,10 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
 constexpr int kMaxCtas = 1024;
 int sm_count();
 
-// A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn, the next one always
-// fetched ahead. Keys and values are loaded into two stages, load number `load` into
-// stage load & 1; a unit of the same cluster as the one before it, whose steps both
-// stages hold, uses them again.
+// A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn. The next one is fetched while
+// one is worked on, and nothing but its turn waits for it. Keys and values are loaded into two
+// stages, load number `load` into stage load & 1; a unit of the same cluster as the one
+// before it, whose steps both stages hold, uses them again.
 struct UnitIter {
   const Unit* units;
   int n, total;
@@ -231,22 +248,24 @@ struct UnitIter {
 
   __device__ __forceinline__ UnitIter(const Unit* u, const int32_t* start)
       : units(u), n(__ldg(start + blockIdx.x)), total(__ldg(start + blockIdx.x + 1)), load(0), again(false) {
-    if (n < total) un = load_unit(units + n);
-    look();
+    if (n < total) next = load_unit(units + n);
+    open();
   }
-  __device__ __forceinline__ void look() {
+  __device__ __forceinline__ void open() {
     keep = false;
-    if (n + 1 >= total) return;
-    next = load_unit(units + n + 1);
-    keep = next.c == un.c && next.r == un.r && un.steps() <= 2;
+    if (n >= total) return;
+    un = next;
+    if (n + 1 < total) next = load_unit(units + n + 1);
+    const bool more = (un.nrows & Unit::kMore) != 0;
+    un.nrows &= Unit::kMore - 1;
+    keep = more && n + 1 < total && un.steps() <= 2;
   }
   __device__ __forceinline__ bool valid() const { return n < total; }
   __device__ __forceinline__ void advance() {
     if (!keep) load += un.steps();
     again = keep;
     ++n;
-    un = next;
-    if (n < total) look();
+    open();
   }
 };
 
