@@ -519,13 +519,13 @@ __global__ void __launch_bounds__(1024) key_count_kernel(Args a, const int32_t* 
   }
 }
 
-// The key tiles in the order of rows and clusters, and the tile in which each CTA's share of the
-// steps begins: share j of all `total` steps is [j total / ctas, (j + 1) total / ctas).
+// The key tiles in the order of rows and clusters, each CTA's share of the steps, [share[j],
+// share[j + 1]) with share[j] = j total / ctas, and the tile in which it begins.
 __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* __restrict__ inv_offsets,
                                                          const int32_t* __restrict__ first_unit,
                                                          const int64_t* __restrict__ first,
                                                          KeyTile* __restrict__ tiles,
-                                                         int64_t* __restrict__ total_out,
+                                                         int64_t* __restrict__ share,
                                                          int32_t* __restrict__ start, int ctas, int R,
                                                          int64_t tiles_max) {
   __shared__ int64_t sums[3][32];
@@ -556,9 +556,11 @@ __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* 
     tile0 += sums[0][w], step0 += sums[1][w], total += sums[2][w];
     high = max(high, highs[w]);
   }
-  if (r == 0 && threadIdx.x == 0) *total_out = total;
-  if (r == 0 && total == 0)
-    for (int j = threadIdx.x; j < ctas; j += 1024) start[j] = 0;
+  if (r == 0)
+    for (int j = threadIdx.x; j <= ctas; j += 1024) {
+      share[j] = j * total / ctas;
+      if (total == 0 && j < ctas) start[j] = 0;
+    }
   for (int c0 = 0; c0 < a.K; c0 += 1024) {
     const int c = c0 + threadIdx.x;
     int s0, s1, nrows;
@@ -587,9 +589,8 @@ __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* 
       t.nrows = nrows, t.base = s_at;
       tiles[t_at] = t;
       // the shares that begin inside: j total / ctas in [s_at, s_at + per)
-      int64_t j = (s_at * ctas + total - 1) / total;
-      for (; j < ctas && j * total / ctas < s_at + per; ++j)
-        if (j * total / ctas >= s_at) start[j] = static_cast<int32_t>(t_at);
+      for (int64_t j = (s_at * ctas + total - 1) / total; j < ctas && j * total < (s_at + per) * ctas; ++j)
+        start[j] = static_cast<int32_t>(t_at);
     }
   }
 }
@@ -600,8 +601,8 @@ struct SegIter {
   int64_t at, to;  // in the sequence of all steps
   int n, step, end, seg;
   KeyTile tile;
-  __device__ __forceinline__ SegIter(const KeyTile* t, const int32_t* start, int64_t total)
-      : tiles(t), at(blockIdx.x * total / gridDim.x), to((blockIdx.x + 1) * total / gridDim.x),
+  __device__ __forceinline__ SegIter(const KeyTile* t, const int32_t* start, const int64_t* share)
+      : tiles(t), at(__ldg(share + blockIdx.x)), to(__ldg(share + blockIdx.x + 1)),
         n(__ldg(start + blockIdx.x)), seg(0) {
     if (at < to) open();
   }
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
     const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
     const float* __restrict__ row_delta, const KeyTile* __restrict__ tiles,
-    const int64_t* __restrict__ total_steps, const int32_t* __restrict__ start, T* __restrict__ dk,
+    const int64_t* __restrict__ share, const int32_t* __restrict__ start, T* __restrict__ dk,
     T* __restrict__ dv, float* __restrict__ part, int* err) {
   using namespace ptx;
   using S = DkvSmem<DP>;
@@ -682,7 +683,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
   tc_fence_after();
   const uint32_t tmem = mt.tmem;  // S^T at 0, dP^T at 128, dV at 256, dK at 384
   pdl_wait();
-  const int64_t total = *total_steps;
 
   if (warp < 8) {
     // ------------------------------------------------------------ P^T and dS^T, output
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     const float sc = a.scale * kLog2e;
     uint32_t item = 0;
     bool ok = true;
-    for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
+    for (SegIter it(tiles, start, share); ok && it.valid(); it.advance()) {
       int key = INT_MAX;
       if (row < it.tile.keys) {
         const int k = __ldg(a.order + static_cast<int64_t>(it.tile.r) * a.N + it.tile.s0 + row);
@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
         mma_tmem_rows<4>(tmem + 384, tmem + 128 + half * 64, sb + S::kQ + o, idesc_o, p.ksteps, p.first);
         if (p.last) umma_commit(smem_u32(&mt.acc_full));
       };
-      for (SegIter it(tiles, start, total); ok && it.valid(); it.advance()) {
+      for (SegIter it(tiles, start, share); ok && it.valid(); it.advance()) {
         for (int step = it.step; ok && step < it.end; ++step, ++item) {
           const int st = item & 1;
           const int rows = it.tile.nrows - step * kSub;
@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
   } else {
     // ------------------------------------------------------------ gathers
     bool ok = true;
-    SegIter it(tiles, start, total);
+    SegIter it(tiles, start, share);
     if (warp <= 10) {
       const bool values = warp == 10;
       const CUtensorMap* tm = values ? &tm_v : &tm_k;
@@ -924,33 +924,32 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
 }
 
 // The key tiles that shares cut: the CTA whose share holds a tile's first step, but not its
-// last, adds the sums of the CTAs that hold the others, in their order. blockIdx.y: 16 keys.
+// last, adds the sums of the CTAs that hold the others, in their order. blockIdx.y: 4 keys.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTile* __restrict__ tiles,
-                                                             const int64_t* __restrict__ total_steps,
+                                                             const int64_t* __restrict__ share,
                                                              const int32_t* __restrict__ start, int ctas,
                                                              const float* __restrict__ part,
                                                              T* __restrict__ dk, T* __restrict__ dv) {
   pdl_wait();
-  const int64_t total = *total_steps;
   const int j = blockIdx.x;
-  const int64_t from = j * total / ctas, to = (j + 1) * total / ctas;
+  const int64_t from = share[j], to = share[j + 1];
   if (from >= to) return;
   // the share's last tile: the one in which the next share that is not empty begins
   int next = j + 1;
-  while (next < ctas && next * total / ctas >= (next + 1) * total / ctas) ++next;
+  while (next < ctas && share[next] >= share[next + 1]) ++next;
   if (next >= ctas) return;
   const KeyTile t = load_tile(tiles + __ldg(start + next));
   if (t.base >= to || t.base < from) return;  // it begins with the next share, or began before
   const int64_t end = t.base + t.steps();
-  for (int e = threadIdx.x; e < 2 * 16 * DP / 4; e += 256) {
-    const int which = e / (16 * DP / 4), key = blockIdx.y * 16 + e / (DP / 4) % 16, d = e % (DP / 4) * 4;
+  for (int e = threadIdx.x; e < 2 * 4 * DP / 4; e += 256) {
+    const int which = e / (4 * DP / 4), key = blockIdx.y * 4 + e / (DP / 4) % 4, d = e % (DP / 4) * 4;
     if (key >= t.keys || d >= a.D) continue;
     const int k = a.order[static_cast<int64_t>(t.r) * a.N + t.s0 + key];
     if (k < 0 || k >= a.N) continue;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = j; q < ctas && q * total / ctas < end; ++q) {
-      if (q * total / ctas >= (q + 1) * total / ctas) continue;
+    for (int q = j; q < ctas && share[q] < end; ++q) {
+      if (share[q] >= share[q + 1]) continue;
       const float4 v = *reinterpret_cast<const float4*>(
           part + ((static_cast<int64_t>(q) * 2 + (q == j)) * 2 + which) * (kSub * DP) + key * DP + d);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
@@ -964,7 +963,7 @@ __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTi
 
 struct GradLayout {
   UnitPlan plan;
-  size_t part, scales, first, tiles, total_steps, start, dkv_part, total;
+  size_t part, scales, first, tiles, share, start, dkv_part, total;
   int64_t tiles_max;
 };
 
@@ -983,7 +982,7 @@ GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
   l.scales = take(l.plan.units_max * kUnitRows * 8);
   l.first = take(R * 16);
   l.tiles = take(l.tiles_max * static_cast<int64_t>(sizeof(KeyTile)));
-  l.total_steps = take(8);
+  l.share = take((kMaxCtas + 1) * 8);
   l.start = take(kMaxCtas * 4);
   l.dkv_part = take(static_cast<int64_t>(std::min(sm_count(), kMaxCtas)) * 4 * kSub * DP * 4);
   l.total = at;
@@ -1025,7 +1024,7 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
   FKC_TRY(launch_zero_fill(dk, bytes, stream));
   FKC_TRY(launch_zero_fill(dv, bytes, stream));
   int64_t* first = reinterpret_cast<int64_t*>(ws + l.first);
-  int64_t* steps = reinterpret_cast<int64_t*>(ws + l.total_steps);
+  int64_t* share = reinterpret_cast<int64_t*>(ws + l.share);
   KeyTile* tiles = reinterpret_cast<KeyTile*>(ws + l.tiles);
   int32_t* start = reinterpret_cast<int32_t*>(ws + l.start);
   float* part = reinterpret_cast<float*>(ws + l.dkv_part);
@@ -1034,16 +1033,16 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
   FKC_TRY(launch_pdl(key_count_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv, first));
   FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv,
                      static_cast<const int32_t*>(l.plan.first_unit), static_cast<const int64_t*>(first), tiles,
-                     steps, start, shares, static_cast<int>(R), l.tiles_max));
+                     share, start, shares, static_cast<int>(R), l.tiles_max));
   auto kern = tiles_dkv_kernel<T, DP>;
   const int smem = static_cast<int>(DkvSmem<DP>::kBytes);
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   FKC_TRY(launch_pdl(kern, dim3(shares), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                      q_row, do_row, pos, row_lse, row_delta, static_cast<const KeyTile*>(tiles),
-                     static_cast<const int64_t*>(steps), static_cast<const int32_t*>(start), dk, dv, part,
+                     static_cast<const int64_t*>(share), static_cast<const int32_t*>(start), dk, dv, part,
                      device_error_word()));
-  return launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, 8), dim3(256), 0, stream, a,
-                    static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(steps),
+  return launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, kSub / 4), dim3(256), 0, stream, a,
+                    static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(share),
                     static_cast<const int32_t*>(start), shares, static_cast<const float*>(part), dk, dv);
 }
 
