@@ -15,8 +15,12 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void need(bool ok, const std::string& msg) {
+void need(bool ok, const char* msg) {
   if (!ok) throw std::runtime_error(msg);
+}
+// The same about a named tensor.
+void need(bool ok, const char* name, const char* msg) {
+  if (!ok) throw std::runtime_error(std::string(name) + msg);
 }
 
 // The error of the package's ops for a tensor elsewhere.
@@ -28,7 +32,8 @@ void need_cuda(const Tensor& t, const char* name) {
 
 void need_on(const Tensor& t, const char* name, const Tensor& first) {
   need_cuda(t, name);
-  need(t.device() == first.device(), std::string(name) + " must be on " + first.device().str());
+  if (t.device() != first.device())
+    throw std::runtime_error(std::string(name) + " must be on " + first.device().str());
 }
 
 Tensor workspace(size_t bytes, const Tensor& like) {
@@ -43,7 +48,7 @@ bool is_64(const Tensor& ids) {
 
 Tensor int32_of(const Tensor& t, const char* name, const Tensor& first) {
   need_on(t, name, first);
-  need(t.scalar_type() == at::kInt, std::string(name) + " must be int32");
+  need(t.scalar_type() == at::kInt, name, " must be int32");
   return t.contiguous();
 }
 
@@ -100,8 +105,8 @@ Tensor lookup_forward(const Tensor& table, const Tensor& ids, double scale) {
 
 // Gradients are given as they are, not as functions of the inputs.
 void need_first_order(const char* what) {
-  need(!at::GradMode::is_enabled(),
-       std::string(what) + " is differentiable once: its gradient has no graph (create_graph)");
+  need(!at::GradMode::is_enabled(), what,
+       " is differentiable once: its gradient has no graph (create_graph)");
 }
 
 class Lookup : public torch::autograd::Function<Lookup> {
@@ -164,20 +169,22 @@ void put_strides(const Tensor& t, int64_t* s) {
 void check_q(const Tensor& q) {
   need_cuda(q, "q");
   need(q.dim() == 4, "q must be (batch, q_heads, n_queries, head_dim)");
-  need(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
-       std::string("q must be float16 or bfloat16 (got ") + c10::toString(q.scalar_type()) + ")");
-  need(q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= 128,
-       "head_dim must be a multiple of 8 between 8 and 128 (got " + std::to_string(q.size(3)) + ")");
+  if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16)
+    throw std::runtime_error(std::string("q must be float16 or bfloat16 (got ") +
+                             c10::toString(q.scalar_type()) + ")");
+  if (q.size(3) % 8 != 0 || q.size(3) < 8 || q.size(3) > 128)
+    throw std::runtime_error("head_dim must be a multiple of 8 between 8 and 128 (got " +
+                             std::to_string(q.size(3)) + ")");
 }
 
 // Sizes that come with q and the clusters: rows = batch * kv_heads.
 fkc_attention_desc describe(const Tensor& q, int64_t rows, int64_t n_keys, int64_t n_clusters,
                             int64_t top_k, double scale) {
   const int64_t batch = q.size(0);
-  need(batch == 0 ? rows == 0 : rows % batch == 0 && rows > 0 && q.size(1) % (rows / batch) == 0,
-       "the clusters have " + std::to_string(rows) + " rows: they must be batch * kv_heads, and "
-       "q_heads a multiple of kv_heads (q is " + std::to_string(batch) + " x " +
-       std::to_string(q.size(1)) + " heads)");
+  if (batch == 0 ? rows != 0 : rows % batch != 0 || rows == 0 || q.size(1) % (rows / batch) != 0)
+    throw std::runtime_error("the clusters have " + std::to_string(rows) + " rows: they must be "
+                             "batch * kv_heads, and q_heads a multiple of kv_heads (q is " +
+                             std::to_string(batch) + " x " + std::to_string(q.size(1)) + " heads)");
   fkc_attention_desc d{};
   d.q = q.data_ptr();
   put_strides(q, d.q_stride);
@@ -274,7 +281,7 @@ Attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
     need_on(*t, name, q);
     need(t->scalar_type() == q.scalar_type(), "q, k and v must share dtype");
     need(t->dim() == 4 && t->size(0) == q.size(0) && t->size(3) == q.size(3),
-         std::string(name) + " must be (batch, kv_heads, n_keys, head_dim)");
+         name, " must be (batch, kv_heads, n_keys, head_dim)");
   }
   need(k.size(1) == v.size(1) && k.size(2) == v.size(2), "k and v must have the same sizes");
   const int64_t rows = k.size(0) * k.size(1), N = k.size(2);

@@ -290,10 +290,125 @@ def test_attention(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("B,Hkv,G,Nq,N,K,D,top", [(1, 2, 4, 700, 1500, 23, 128, 7), (2, 1, 3, 1001, 1300, 17, 72, 5),
                                                   (1, 1, 16, 400, 2500, 30, 64, 9), (2, 2, 1, 3000, 3001, 100, 32, 5),
-                                                  (1, 1, 24, 300, 1500, 9, 128, 9)])
+                                                  (1, 1, 24, 300, 1500, 9, 128, 9), (1, 2, 2, 2000, 2100, 40, 8, 6),
+                                                  (1, 1, 5, 900, 1300, 20, 104, 6), (3, 1, 2, 1700, 1700, 6, 64, 3)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_many_queries(clusters, dtype, B, Hkv, G, Nq, N, K, D, top, causal):
     attention_check(clusters, *attention_case(B, Hkv, G, Nq, N, K, D, top, dtype, seed=Nq + D, causal=causal))
+
+
+def many(seed=5, dtype=BF, **kw):
+    """A case of the form by clusters: 1000 queries, two sequences."""
+    return attention_case(2, 1, 4, 1000, 1500, 15, 64, 5, dtype, seed=seed, **kw)
+
+
+def test_many_queries_same_cluster_twice(clusters):
+    q, k, v, sel, order, offsets, pos = many(drop=0.0)
+    sel[..., 2] = sel[..., 0]
+    attention_check(clusters, q, k, v, sel, order, offsets, pos)
+
+
+def test_many_queries_bad_entries_read_nothing(clusters):
+    q, k, v, sel, order, offsets, pos = many(drop=0.0)
+    sel[0, :, 0] = 15
+    sel[1, :, 0] = -(1 << 31)
+    sel[1, :, 1] = (1 << 31) - 1
+    order[0, 5], order[1, 7], order[1, 9] = 1500, -5, (1 << 31) - 1
+    attention_check(clusters, q, k, v, sel, order, offsets, pos)
+
+
+def test_many_queries_empty_clusters_and_blind_queries(clusters):
+    q, k, v, sel, order, offsets, pos = many()
+    offsets[:, 4:] = offsets[:, 4:5]  # the clusters from the fourth on are empty
+    pos[:, 100:400] = -1
+    sel[:, 500:600] = -1
+    attention_check(clusters, q, k, v, sel, order, offsets, pos)
+    pos[:] = -1
+    attention_check(clusters, q, k, v, sel, order, offsets, pos)
+
+
+def test_many_queries_strided_inputs(clusters):
+    q, k, v, sel, order, offsets, pos = many(drop=0.0)
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    out, _ = attention_check(clusters, *turned, sel, order, offsets, pos)
+    padded = [torch.nn.functional.pad(t, (0, 8))[..., :64] for t in (q, k, v)]
+    assert torch.equal(out, attention_check(clusters, *padded, sel, order, offsets, pos)[0])
+    odd = [torch.nn.functional.pad(t, (0, 3))[..., :64] for t in (q, k, v)]
+    assert torch.equal(out, attention_check(clusters, *odd, sel, order, offsets, pos)[0])
+
+
+def test_many_queries_some_gradients_only(clusters):
+    q, k, v, sel, order, offsets, pos = many()
+    _, full = attention_check(clusters, q, k, v, sel, order, offsets, pos)
+    dout = randn(*q.shape, seed=9).to(BF)
+    for which in ((0,), (1,), (0, 2)):
+        a = [t.detach().requires_grad_(i in which) for i, t in enumerate((q, k, v))]
+        out = clusters.cluster_attention(*a, sel, order, offsets, q_pos=pos)
+        for i, g in zip(which, torch.autograd.grad(out, [a[i] for i in which], dout)):
+            assert torch.equal(g, full[i])
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_many_queries_masked_places_hold_anything(clusters, what):
+    q, k, v, sel, order, offsets, pos = many()
+    pos[1, 500:] = -1
+    pos.clamp_(max=1200)
+    k[:, :, 1201:] = what
+    v[:, :, 1201:] = what
+    q[1, :, 500:] = what
+    sees = (pos >= 0)[:, None, :, None]
+    val, tol = attention_ref(q, k, v, sel, order, offsets, pos, None, torch.ones_like(q))
+    a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = clusters.cluster_attention(*a, sel, order, offsets, q_pos=pos)
+    grads = torch.autograd.grad(out, a, torch.where(sees, 1.0, what).to(BF).expand_as(q).contiguous())
+    close(out.detach(), val["out"], tol["out"], "out")
+    close(grads[1], val["dk"], tol["dk"], "dk")
+    close(grads[2], val["dv"], tol["dv"], "dv")
+    live = sees.expand_as(q)
+    close(grads[0][live], val["dq"][live], tol["dq"][live], "dq")
+    assert grads[0][~live].eq(0).all()
+
+
+def test_many_queries_far_apart_values(clusters):
+    """Rows of out whose magnitudes differ by 2**60 and more: parts keep a power of two each."""
+    q, k, v, sel, order, offsets, pos = many(drop=0.0)
+    v = (v.float() * torch.exp2(torch.randint(-60, 61, (2, 1, 1500, 1), generator=gen(8), device="cuda").float())).to(BF)
+    out, lse = clusters.cluster_attention(q, k, v, sel, order, offsets, q_pos=pos, return_lse=True)
+    val, tol = attention_ref(q, k, v, sel, order, offsets, pos)
+    close(out, val["out"], tol["out"], "out")
+    close(lse, val["lse"], tol["lse"], "lse")
+
+
+def test_many_queries_two_streams_at_once(clusters):
+    """Two calls that run beside each other, and a captured one replayed beside an eager one."""
+    a, b = many(seed=5), many(seed=50)
+
+    def step(c):
+        leaves = [t.detach().requires_grad_(True) for t in c[:3]]
+        out = clusters.cluster_attention(*leaves, *c[3:6], q_pos=c[6])
+        return (out.detach(), *torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+    want = [step(a), step(b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(3):
+        for c, s in zip((a, b), streams):
+            with torch.cuda.stream(s):
+                got.append(step(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for x, y in zip(g, want[i % 2]):
+            assert torch.equal(x, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(a)
+    graph.replay()
+    eager = step(b)
+    torch.cuda.synchronize()
+    for x, y in zip(held + eager, want[0] + want[1]):
+        assert torch.equal(x, y)
 
 
 def test_attention_rounds(clusters):
