@@ -32,7 +32,7 @@ CORE_SOURCES = ["capi.cu", "assign_tc.cu", "norm_ext.cu", "assign_simt.cu", "upd
                 "update_det.cu",
                 "finalize.cu", "lloyd_graph.cu", "assign_noalloc.cu", "selftest.cu",
                 "cluster_group.cu", "cluster_lookup.cu", "cluster_select.cu",
-                "cluster_attention.cu", "cluster_attention_tiles.cu",
+                "cluster_attention.cu", "cluster_attention_tiles.cu", "cluster_masked.cu",
                 "cluster_attention_grad.cu", "cluster_attention_tiles_grad.cu",
                 "cluster_capi.cu"]
 CORE_LIB = OUT_DIR / "libfkc_b200.so"

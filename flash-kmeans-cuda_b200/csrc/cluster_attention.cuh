@@ -121,6 +121,11 @@ __device__ __forceinline__ void load_b_trans(uint32_t (&f)[4], uint32_t tile, in
   mma::ldmatrix_x4_trans(f, tile + tile_at<DP>(row0 + (lane & 7) + (m & 1) * 8, nd * 2 + (m >> 1)));
 }
 
+// 0 while all of x are finite (from a so_far of 0).
+__device__ __forceinline__ float not_finite(float x, float so_far) { return fmaf(x, 0.f, so_far); }
+
+int sm_count();  // of the current device
+
 // Launchers (cluster_select.cu, cluster_attention.cu, cluster_attention_grad.cu); dtype is
 // FKC_DTYPE_F16 or FKC_DTYPE_BF16. out, dout and the gradients are contiguous.
 size_t select_workspace_bytes(int64_t R, int64_t Nq, int64_t K);
@@ -136,7 +141,12 @@ int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* 
 bool use_tiles_grad(const Args& a);
 size_t tiles_backward_workspace_bytes(const Args& a, int dtype);
 int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
-                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
+                          void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream);
+// After the kernels above, where they set *odd: results that are not finite, from what their rows
+// see alone (cluster_masked.cu). Forward: rows is out. Gradients (dout given): rows is dq.
+int launch_again(const Args& a, int dtype, const int32_t* odd, const float* lse, const float* delta,
+                 const void* dout, void* rows, const int32_t* inv_order, const int32_t* inv_offsets,
+                 void* dk, void* dv, cudaStream_t stream);
 size_t backward_workspace_bytes(const Args& a, int dtype);
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);

@@ -49,8 +49,9 @@ template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ out,
                                                          const T* __restrict__ dout,
                                                          float* __restrict__ delta, int D,
-                                                         int64_t rows) {
+                                                         int32_t* odd, int64_t rows) {
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *odd = 0;
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
     Args a, const T* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ delta, const int32_t* __restrict__ inv_order,
     const int32_t* __restrict__ inv_offsets, const int32_t* __restrict__ tile_off,
-    T* __restrict__ dk, T* __restrict__ dv, int tiles_max) {
+    T* __restrict__ dk, T* __restrict__ dv, int32_t* __restrict__ odd, int tiles_max) {
   constexpr int KS = DP / 16, CH = DP / 8;
   using S = DkvSmem<DP>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -477,12 +478,15 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
   }
   mma::cp_async_wait<0>();
   const int64_t kv = (static_cast<int64_t>(b) * a.Hkv + hk) * a.N;
+  float bad = 0.f;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int row = half == 0 ? row0 : row1;
     if (row < 0) continue;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) bad = not_finite(ak[n][half * 2 + e], not_finite(av[n][half * 2 + e], bad));
       const int d = n * 8 + t4 * 2;
       if (d >= a.D) continue;
       const int64_t at = (kv + row) * a.D + d;
@@ -491,10 +495,11 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
       *reinterpret_cast<uint32_t*>(dv + at) = mma::pack2<T>(av[n][half * 2], av[n][half * 2 + 1]);
     }
   }
+  if (bad != 0.f) *odd = 1;
 }
 
 struct GradLayout {
-  size_t delta, inv_order, inv_offsets, tile_off, group, tiles, total;
+  size_t delta, odd, inv_order, inv_offsets, tile_off, group, tiles, total;
 };
 
 GradLayout grad_layout(const Args& a, int dtype) {
@@ -507,6 +512,7 @@ GradLayout grad_layout(const Args& a, int dtype) {
     return p;
   };
   l.delta = take(static_cast<size_t>(a.batch) * a.Hq * a.Nq * 4);
+  l.odd = take(4);
   if (use_tiles_grad(a)) {
     l.tiles = take(tiles_backward_workspace_bytes(a, dtype));
     l.total = at;
@@ -538,15 +544,16 @@ int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T
                uint8_t* ws, cudaStream_t stream) {
   const GradLayout l = grad_layout(a, dtype);
   float* delta = reinterpret_cast<float*>(ws + l.delta);
+  int32_t* odd = reinterpret_cast<int32_t*>(ws + l.odd);
   int32_t* inv_order = reinterpret_cast<int32_t*>(ws + l.inv_order);
   int32_t* inv_offsets = reinterpret_cast<int32_t*>(ws + l.inv_offsets);
   int32_t* tile_off = reinterpret_cast<int32_t*>(ws + l.tile_off);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.Hq * a.Nq;
   FKC_TRY(launch_pdl(attn_delta_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
-                     stream, out, dout, delta, a.D, rows));
+                     stream, out, dout, delta, a.D, odd, rows));
   if (use_tiles_grad(a))
-    return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, ws + l.tiles, stream);
+    return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, odd, ws + l.tiles, stream);
   if (dq != nullptr) {
     if (a.G <= 8)
       FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, stream)));
@@ -566,11 +573,13 @@ int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T
   auto kern = attn_dkv_kernel<T, DP>;
   const int smem = DkvSmem<DP>::kBytes;
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  return launch_pdl(kern, dim3(static_cast<unsigned>(R * tiles_max)), dim3(128), smem, stream, a,
-                    dout, lse, static_cast<const float*>(delta),
-                    static_cast<const int32_t*>(inv_order),
-                    static_cast<const int32_t*>(inv_offsets),
-                    static_cast<const int32_t*>(tile_off), dk, dv, static_cast<int>(tiles_max));
+  FKC_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(R * tiles_max)), dim3(128), smem, stream, a,
+                     dout, lse, static_cast<const float*>(delta),
+                     static_cast<const int32_t*>(inv_order),
+                     static_cast<const int32_t*>(inv_offsets),
+                     static_cast<const int32_t*>(tile_off), dk, dv, odd, static_cast<int>(tiles_max)));
+  // dq's walk takes one query's keys at a time: none that the query does not see
+  return launch_again(a, dtype, odd, lse, delta, dout, nullptr, inv_order, inv_offsets, dk, dv, stream);
 }
 
 template <typename T>

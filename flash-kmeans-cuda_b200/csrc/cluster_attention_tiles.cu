@@ -28,10 +28,11 @@ namespace attn {
 namespace {
 
 __global__ void __launch_bounds__(256) tile_init_kernel(int64_t* count, int32_t* __restrict__ pair_row,
-                                                        int64_t pairs) {
+                                                        int64_t pairs, int32_t* odd) {
   pdl_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i == 0) *count = 0;
+  if (i == 0 && odd != nullptr) *odd = 0;
   for (int64_t p = i; p < pairs; p += static_cast<int64_t>(gridDim.x) * 256) pair_row[p] = -1;
 }
 
@@ -582,7 +583,8 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
                                                          const float2* __restrict__ part_lse,
                                                          const float* __restrict__ part_scale,
                                                          T* __restrict__ out,
-                                                         float* __restrict__ lse, int64_t warps) {
+                                                         float* __restrict__ lse,
+                                                         int32_t* __restrict__ odd, int64_t warps) {
   constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
   constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
@@ -655,6 +657,12 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
     const int d = (g * 8 + me.piece) * E;
     if (d < a.D) store_out<T, E>(out + at * a.D + d, acc[g], inv);
   }
+  float bad = 0.f;
+#pragma unroll
+  for (int g = 0; g < SEGS; ++g)
+#pragma unroll
+    for (int e = 0; e < E; ++e) bad = not_finite(acc[g][e], bad);
+  if (bad != 0.f) *odd = 1;
   if (me.piece == 0) lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
@@ -730,9 +738,9 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
                        0, stream, a, static_cast<int>(i0), nq, gp, chunks,
                        static_cast<const int32_t*>(l.plan.pair_row),
                        static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse),
-                       static_cast<const float*>(part_scale), out, lse, warps));
+                       static_cast<const float*>(part_scale), out, lse, l.plan.odd, warps));
   }
-  return FKC_OK;
+  return launch_again(a, dtype, l.plan.odd, lse, nullptr, nullptr, out, nullptr, nullptr, nullptr, nullptr, stream);
 }
 
 template <typename T>
@@ -793,7 +801,9 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
   p.row_pos = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
   p.pair_row = static_cast<int32_t*>(take(R * pairs * 4));
   p.first_unit = static_cast<int32_t*>(take(R * a.K * 4));
-  if (grad) {
+  if (!grad) {
+    p.odd = static_cast<int32_t*>(take(4));
+  } else {
     p.do_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
     p.row_lse = static_cast<float*>(take(p.units_max * kUnitRows * 4));
     p.row_delta = static_cast<float*>(take(p.units_max * kUnitRows * 4));
@@ -809,7 +819,7 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
   FKC_REQUIRE(p.units_max * kUnitRows <= 2147483647ll, "attention: too many tiles");
   const int64_t blocks = std::min<int64_t>((R * nq * a.top + 255) / 256, sm_count() * 8ll);
   FKC_TRY(launch_pdl(tile_init_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p.count,
-                     p.pair_row, R * nq * a.top));
+                     p.pair_row, R * nq * a.top, i0 == 0 ? p.odd : nullptr));
   FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
                        p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
   FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,

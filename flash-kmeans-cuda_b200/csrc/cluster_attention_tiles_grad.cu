@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int 
                                                             const int32_t* __restrict__ pair_row,
                                                             const uint8_t* __restrict__ part,
                                                             const float* __restrict__ part_scale,
-                                                            T* __restrict__ dq, int64_t warps) {
+                                                            T* __restrict__ dq, int32_t* __restrict__ odd,
+                                                            int64_t warps) {
   constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
   constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
@@ -460,6 +461,12 @@ __global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int 
     const int d = (g * 8 + me.piece) * E;
     if (d < a.D) store_out<T, E>(out + d, acc[g], 1.f);
   }
+  float bad = 0.f;
+#pragma unroll
+  for (int g = 0; g < SEGS; ++g)
+#pragma unroll
+    for (int e = 0; e < E; ++e) bad = not_finite(acc[g][e], bad);
+  if (bad != 0.f) *odd = 1;
 }
 
 // ---------------------------------------------------------------------------- dK, dV
@@ -649,7 +656,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
     const float* __restrict__ row_delta, const KeyTile* __restrict__ tiles,
     const int64_t* __restrict__ share, const int32_t* __restrict__ start, T* __restrict__ dk,
-    T* __restrict__ dv, float* __restrict__ part, int* err) {
+    T* __restrict__ dv, float* __restrict__ part, int32_t* __restrict__ odd, int* err) {
   using namespace ptx;
   using S = DkvSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -753,11 +760,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
       T* out = (half == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + (key == INT_MAX ? 0 : key)) * a.D;
       // a segment that does not begin its tile is the CTA's first
       float* sums = part + ((static_cast<int64_t>(blockIdx.x) * 2 + (it.step == 0)) * 2 + half) * (kSub * DP) + row * DP;
+      float bad = 0.f;
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         float o[32];
         tmem_ld_f32_x32(t_acc + c * 32, o);
         tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) bad = not_finite(o[j], bad);
         if (whole) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
@@ -772,6 +782,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
         }
         __syncwarp();
       }
+      if (bad != 0.f && key != INT_MAX) *odd = 1;
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.acc_free));
     }
@@ -991,7 +1002,7 @@ GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
 
 template <typename T, int DP>
 int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, const T* dout, T* dq, T* dk,
-               T* dv, uint8_t* ws, cudaStream_t stream) {
+               T* dv, int32_t* odd, uint8_t* ws, cudaStream_t stream) {
   const GradLayout l = grad_layout(a, Part<T>::kBytes, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   CUtensorMap tm_q, tm_k, tm_v, tm_do;
@@ -1017,9 +1028,10 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
     const int64_t warps = R * a.Nq * chunks;
     FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0,
                        stream, a, gp, chunks, static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, warps));
+                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, odd, warps));
   }
-  if (dk == nullptr) return FKC_OK;
+  if (dk == nullptr)
+    return launch_again(a, dtype, odd, lse, delta, dout, dq, nullptr, nullptr, nullptr, nullptr, stream);
   const size_t bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);
   FKC_TRY(launch_zero_fill(dk, bytes, stream));
   FKC_TRY(launch_zero_fill(dv, bytes, stream));
@@ -1040,19 +1052,20 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
   FKC_TRY(launch_pdl(kern, dim3(shares), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                      q_row, do_row, pos, row_lse, row_delta, static_cast<const KeyTile*>(tiles),
                      static_cast<const int64_t*>(share), static_cast<const int32_t*>(start), dk, dv, part,
-                     device_error_word()));
-  return launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, kSub / 4), dim3(256), 0, stream, a,
-                    static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(share),
-                    static_cast<const int32_t*>(start), shares, static_cast<const float*>(part), dk, dv);
+                     odd, device_error_word()));
+  FKC_TRY(launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, kSub / 4), dim3(256), 0, stream, a,
+                     static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(share),
+                     static_cast<const int32_t*>(start), shares, static_cast<const float*>(part), dk, dv));
+  return launch_again(a, dtype, odd, lse, delta, dout, dq, l.plan.inv_order, inv, dk, dv, stream);
 }
 
 template <typename T>
 int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, const void* dout, void* dq,
-               void* dk, void* dv, uint8_t* ws, cudaStream_t stream) {
+               void* dk, void* dv, int32_t* odd, uint8_t* ws, cudaStream_t stream) {
   const T* d = static_cast<const T*>(dout);
   T *q = static_cast<T*>(dq), *k = static_cast<T*>(dk), *v = static_cast<T*>(dv);
-  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, delta, d, q, k, v, ws, stream)
-                   : grad_typed<T, 128>(a, dtype, lse, delta, d, q, k, v, ws, stream);
+  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, delta, d, q, k, v, odd, ws, stream)
+                   : grad_typed<T, 128>(a, dtype, lse, delta, d, q, k, v, odd, ws, stream);
 }
 
 }  // namespace
@@ -1071,11 +1084,11 @@ size_t tiles_backward_workspace_bytes(const Args& a, int dtype) {
 }
 
 int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
-                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {
+                          void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream) {
   uint8_t* w = static_cast<uint8_t*>(ws);
   return dtype == FKC_DTYPE_F16
-             ? grad_dtype<__half>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream)
-             : grad_dtype<__nv_bfloat16>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream);
+             ? grad_dtype<__half>(a, dtype, lse, delta, dout, dq, dk, dv, odd, w, stream)
+             : grad_dtype<__nv_bfloat16>(a, dtype, lse, delta, dout, dq, dk, dv, odd, w, stream);
 }
 
 }  // namespace attn

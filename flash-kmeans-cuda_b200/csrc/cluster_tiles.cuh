@@ -146,23 +146,6 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-__device__ __forceinline__ void named_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-// The same; true in all of the threads when `any` is in one.
-__device__ __forceinline__ bool named_barrier_any(int id, int threads, bool any) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %3, 0;\n\t"
-      "bar.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"(any ? 1u : 0u)
-      : "memory");
-  return r != 0;
-}
-
 // Bounded wait of a whole warp; the same answer in every lane.
 __device__ __forceinline__ bool warp_mbar_wait(const uint64_t* bar, uint32_t parity,
                                                const volatile int* abort) {
@@ -221,6 +204,7 @@ struct UnitPlan {
   int32_t* row_pos;      // last position that the row sees; -1: none, or no row
   int32_t* pair_row;     // (R, nq * top) unit row of a pair's first head; -1: no key
   int32_t* first_unit;   // (R, K) of clusters that have units
+  int32_t* odd;          // of the forward: a result is not finite (cluster_masked.cu)
   // for the gradients: row of dout's map, as q_row; lse to base 2 and delta of the row
   int32_t* do_row;
   float *row_lse, *row_delta;
@@ -233,7 +217,6 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
 int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
                  const float* lse, const float* delta, cudaStream_t stream);
 constexpr int kMaxCtas = 1024;
-int sm_count();
 
 // A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn. The next one is fetched while
 // one is worked on, and nothing but its turn waits for it. Keys and values are loaded into two

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from _clusters_ref import attention_ref, order_ref, select_ref
+from _clusters_ref import attention_ref, order_ref, reads, select_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -367,6 +367,34 @@ def test_many_queries_masked_places_hold_anything(clusters, what):
     live = sees.expand_as(q)
     close(grads[0][live], val["dq"][live], tol["dq"][live], "dq")
     assert grads[0][~live].eq(0).all()
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", [(2, 1, 3, 1001, 1300, 17, 72, 5), (1, 2, 4, 700, 1500, 23, 128, 7), (1, 1, 16, 400, 2500, 30, 64, 9),
+                                  (2, 1, 3, 40, 200, 7, 64, 3), (1, 2, 5, 70, 700, 3, 128, 2)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_what_some_do_not_see_holds_anything(clusters, dtype, case, what):
+    """A key, a query and a gradient of out that are not finite show only where they are read."""
+    q, k, v, sel, order, offsets, pos = attention_case(*case, dtype, seed=3)
+    B, Hkv, N, Nq = case[0], case[1], case[4], case[3]
+    dout = randn(*q.shape, seed=8).to(dtype)
+    read = reads(sel, order, offsets, pos, Hkv) > 0                      # (R, Nq, N)
+    odd = torch.zeros_like(read[..., 0])
+    odd[:, [Nq // 3, Nq - 2]] = True                                     # odd queries
+    odd |= read[:, :, [N - 30, N - Nq // 5]].any(-1)                     # and those that read odd keys
+    spoilt = (read & odd[..., None]).any(1).view(B, Hkv, N)              # keys that an odd query reads
+    odd = odd.view(B, Hkv, 1, Nq).expand(B, Hkv, case[2], Nq).reshape(q.shape[:3])
+    assert not odd.all() and not spoilt.all()
+    val, tol = attention_ref(q, k, v, sel, order, offsets, pos, None, dout.masked_fill(odd[..., None], 0.0))
+    for t in (k, v):
+        t[:, :, [N - 30, N - Nq // 5]] = what
+    q[:, :, Nq // 3] = what
+    dout[:, :, Nq - 2] = what
+    a = [t.requires_grad_(True) for t in (q, k, v)]
+    out, lse = clusters.cluster_attention(*a, sel, order, offsets, q_pos=pos, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(out, a, dout)
+    for name, got, keep in (("out", out, ~odd), ("lse", lse, ~odd), ("dq", dq, ~odd), ("dk", dk, ~spoilt), ("dv", dv, ~spoilt)):
+        close(got.detach()[keep], val[name][keep], tol[name][keep], name)
 
 
 def test_many_queries_far_apart_values(clusters):
