@@ -834,19 +834,47 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
                     p.row_lse, p.row_delta);
 }
 
-bool use_tiles(const Args& a) {
+FormWork form_work(const Args& a, int64_t nq) {
+  const double R = static_cast<double>(a.batch) * a.Hkv, pairs = static_cast<double>(nq) * a.top;
+  FormWork w;
+  w.keys = static_cast<double>(a.N) / a.K;
+  w.rows = R * a.Nq * a.top * a.G;
+  w.reads = R * a.Nq * a.top * w.keys * (a.G <= 8 ? 1.0 : 1.2 * ((a.G + 15) / 16));
+  // every cluster with pairs may end in a unit that is not full; fewer units than SMs leave
+  // SMs idle
+  const double rounds = static_cast<double>((a.Nq + nq - 1) / nq);
+  w.units = std::max(rounds * R * std::min<double>(a.K, pairs) + w.rows / kUnitRows, 148.0);
+  return w;
+}
+
+bool tiles_fit(const Args& a, int64_t nq) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t rows = queries_per_round(a) * a.top * a.G;  // of a row's clusters together
+  const int64_t pairs = nq * a.top, DP = a.D <= 64 ? 64 : 128;
   // 32-bit row numbers; a running maximum of unscaled scores; the gathers' maps
-  if (rows > (1ll << 30) || !(a.scale > 0.f) ||
+  if (pairs * a.G > (1ll << 30) || !(a.scale > 0.f) ||
       !row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
       !row_map(a.ks, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr) ||
       !row_map(a.vs, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr))
     return false;
-  // the rows of a cluster fill an MMA, its keys repay its parts, and there are enough tiles
-  // for the GPU
-  return rows >= kSub * static_cast<int64_t>(a.K) && a.N / a.K >= 4 * a.G + 8 &&
-         R * a.Nq * a.top * a.G >= 148ll * kSub;
+  // units that are not full take workspace too: no more than the full ones, or 2^31 bytes
+  return pairs * a.G >= kSub * static_cast<int64_t>(a.K) ||
+         R * std::min<int64_t>(a.K, pairs) * kUnitRows * DP * 4 <= (1ll << 31);
+}
+
+// In us, fitted to calls with D = 128, 8 to 200 keys a cluster, 8 to 2048 rows a cluster and G
+// from 1 to 32: within 8% on average, 25% at worst. The walk, which needs no workspace, keeps what
+// is within a tenth. Measured (walk, by clusters):
+// G 1, 512 queries, 32 clusters of 64 keys: 35, 39; of 128 keys: 53, 41. G 4, 64 queries x 8
+// rows, 8 rows a cluster of 64 keys: 59, 113; 256 queries, 32 rows a cluster: 174, 129. G 16,
+// 2048 queries x 4 rows, 12 keys a cluster: 188, 322; 24 keys: 315, 324; 64 keys: 408, 195 with
+// 1024 queries.
+bool use_tiles(const Args& a) {
+  const int64_t nq = queries_per_round(a);
+  if (!tiles_fit(a, nq)) return false;
+  const FormWork w = form_work(a, nq);
+  const double walk = 18 + 75e-6 * w.reads;
+  const double tiles = 34 + w.units * (0.009 + 0.000136 * w.keys) + 86e-6 * w.rows;
+  return 1.1 * tiles < walk;
 }
 
 size_t tiles_forward_workspace_bytes(const Args& a, int dtype) {

@@ -218,6 +218,15 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
                  const float* lse, const float* delta, cudaStream_t stream);
 constexpr int kMaxCtas = 1024;
 
+// What the choice between the two forms weighs, with nq queries a round: keys of a cluster on
+// average, (query, slot, head) rows, keys that the walk reads (of more than 8 heads, more than
+// once), units.
+struct FormWork {
+  double keys, rows, reads, units;
+};
+FormWork form_work(const Args& a, int64_t nq);
+bool tiles_fit(const Args& a, int64_t nq);  // whether the form by clusters can take the call
+
 // A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn. The next one is fetched while
 // one is worked on, and nothing but its turn waits for it. Keys and values are loaded into two
 // stages, load number `load` into stage load & 1; a unit of the same cluster as the one
