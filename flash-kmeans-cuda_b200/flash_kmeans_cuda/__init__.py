@@ -7,7 +7,8 @@ Same public API as OpsiClear/flash-kmeans-cuda (``flash_kmeans_cuda/__init__.py`
 package fails if that library is missing (there is no CPU or PyTorch fallback).
 Multi-GPU sharding over N or B is in ``flash_kmeans_cuda.distributed``;
 host-resident x streamed through one or more GPUs is
-``flash_kmeans_cuda.largen.kmeans_largeN`` (not a reference export).
+``flash_kmeans_cuda.largen.kmeans_largeN``; lookup by id and attention over
+clustered keys are in ``flash_kmeans_cuda.clusters`` (not reference exports).
 """
 
 from ._version import __version__
