@@ -25,11 +25,14 @@
 // and the rounding of the sum with bias add 2^-22 (scale |q||c| + |score|) at most.
 //
 // The scores go through memory (4 bytes a score, L2 at the usual sizes). 4096 queries x 256
-// clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 70 us (tensor pipe
-// 26% busy: it waits for its tiles of queries, one head after another), choose 59 us (58% of
-// issue slots: 16 leading-bit steps and the border per query). 128 queries of 1024 clusters,
-// 4 heads: 32 us in all, most of it latency (51 us before the heads shared a tile, thresholds
-// started from the scores' common leading bits and borders went four at a time).
+// clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 55 us (three CTAs an SM; it was 70 with
+// two and with norms read again from shared memory by half of the warps), choose 42 us
+// (two thirds of the issue slots, some 890 instructions a query: bisection 6 to 8 steps, a border of
+// 64-bit scores for 6% of them; 59 us with bisection bit by bit and one query a warp, 53 us
+// with as many CTAs as the SMs hold, which the queries with a border leave at different times).
+// 128 queries of 1024 clusters, 4 heads: 31 us in all, most of it latency (51 us before the heads
+// shared a tile, thresholds started from the scores' common leading bits and borders went
+// four at a time).
 #include <algorithm>
 #include <cmath>
 
@@ -62,7 +65,7 @@ __device__ __forceinline__ float fold_max(float a, float b) {
 // head) in all, side by side in one tile; the maximum over a query's heads is taken in
 // shared memory.
 template <typename T, int DP, int QW, bool PACK>
-__global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restrict__ scores,
+__global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __restrict__ scores,
                                                     float* __restrict__ q_norm,
                                                     float* __restrict__ c_norm, int ctiles,
                                                     int qtiles) {
@@ -70,8 +73,8 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
   constexpr int NW = kClusters / CW / 8;  // 8-cluster groups per warp
   constexpr int MQ = 16 * QW;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_bias[kClusters];
-  __shared__ int s_first[kClusters];  // first position; INT_MAX: never selected
+  __shared__ __align__(8) float s_bias[kClusters];
+  __shared__ __align__(8) int s_first[kClusters];  // first position; INT_MAX: never selected
   __shared__ float s_red[4];
   __shared__ float s_pack[PACK ? 16 * (kClusters + 4) : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,7 +128,8 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
   for (int n = 0; n < NW; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) best[n][e] = -INFINITY;
-  float qn = 0.f;  // largest norm^2 of the heads, thread tid < MQ: query i0 + tid
+  float qn[2] = {0.f, 0.f};  // largest norm^2 of the heads: the warp's rows g and g + 8
+  const bool norms = tile == 0 && wc == 0;
   const int passes = PACK ? 1 : a.G;
 #pragma unroll 1
   for (int h = 0; h < passes; ++h) {
@@ -134,21 +138,7 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
     if (h + 1 < passes) load_q(h + 1, (h + 1) & 1);
     mma::cp_async_commit();
     const uint32_t qt = qt0 + (h & 1) * (MQ * DP * 2);
-    if (tile == 0 && tid < MQ) {
-      float s = 0.f;
-      const uint8_t* base = smem + (qt - ct);
-      for (int c = 0; c < CH; ++c) {
-        const uint4 u = *reinterpret_cast<const uint4*>(base + tile_at<DP>(tid, c));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = mma::unpack2<T>(w[k]);
-          s += f.x * f.x + f.y * f.y;
-        }
-      }
-      qn = fold_max(qn, s);
-    }
-    float acc[NW][4];
+    float acc[NW][4], sq[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NW; ++n)
 #pragma unroll
@@ -157,6 +147,13 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
     for (int kk = 0; kk < KS; ++kk) {
       uint32_t fa[4];
       load_a<DP>(fa, qt, wq * 16, kk);
+      if (norms) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = mma::unpack2<T>(fa[e]);
+          sq[e & 1] = fmaf(f.x, f.x, fmaf(f.y, f.y, sq[e & 1]));
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NW; n += 2) {
         uint32_t fb[4];
@@ -169,12 +166,22 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
     for (int n = 0; n < NW; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) best[n][e] = fmaxf(best[n][e], acc[n][e]);
+    if (norms) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        sq[x] += __shfl_xor_sync(0xFFFFFFFFu, sq[x], 1);
+        sq[x] += __shfl_xor_sync(0xFFFFFFFFu, sq[x], 2);
+        qn[x] = fold_max(qn[x], sq[x]);
+      }
+    }
   }
-  if (!PACK && tile == 0 && tid < MQ && i0 + tid < a.Nq)
-    q_norm[static_cast<int64_t>(r) * a.Nq + i0 + tid] = sqrtf(qn);
+  if (!PACK && norms && t4 < 2) {
+    const int i = i0 + wq * 16 + t4 * 8 + g;
+    if (i < a.Nq) q_norm[static_cast<int64_t>(r) * a.Nq + i] = sqrtf(t4 == 0 ? qn[0] : qn[1]);
+  }
   if constexpr (PACK) {
     __syncthreads();
-    if (tid < 16) s_pack[tid] = qn;
+    if (norms && t4 < 2) s_pack[t4 * 8 + g] = t4 == 0 ? qn[0] : qn[1];
     __syncthreads();
     if (tile == 0 && tid < a.Nq) {
       float m = 0.f;
@@ -227,16 +234,21 @@ __global__ void __launch_bounds__(128) score_kernel(SelectArgs a, float* __restr
     if (i >= a.Nq) continue;
     const int pos =
         a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.Nq + i], a.N) : a.N;
-    float* row = scores + (static_cast<int64_t>(r) * a.Nq + i) * a.K;
+    float* row = scores + (static_cast<int64_t>(r) * a.Nq + i) * a.K + c0;
 #pragma unroll
-    for (int n = 0; n < NW; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int cl = (wc * NW + n) * 8 + t4 * 2 + e;
-        if (c0 + cl >= a.K) continue;
-        const float s = best[n][half * 2 + e] * scale + s_bias[cl];
-        row[c0 + cl] = s_first[cl] > pos ? __uint_as_float(kNever) : s;
+    for (int n = 0; n < NW; ++n) {
+      const int cl = (wc * NW + n) * 8 + t4 * 2;
+      const float2 bias = *reinterpret_cast<const float2*>(s_bias + cl);
+      const int2 first = *reinterpret_cast<const int2*>(s_first + cl);
+      const float x = first.x > pos ? __uint_as_float(kNever) : best[n][half * 2] * scale + bias.x;
+      const float y = first.y > pos ? __uint_as_float(kNever) : best[n][half * 2 + 1] * scale + bias.y;
+      if (c0 + cl + 1 < a.K && a.K % 2 == 0) {
+        *reinterpret_cast<float2*>(row + cl) = make_float2(x, y);
+      } else {
+        if (c0 + cl < a.K) row[cl] = x;
+        if (c0 + cl + 1 < a.K) row[cl + 1] = y;
       }
+    }
   }
   }
 }
@@ -302,134 +314,154 @@ __device__ __forceinline__ float largest_norm(const float* c_norm, int64_t r, in
   return m;
 }
 
-// One warp per query; KPL scores a lane, cluster j * 32 + lane.
+// One warp per query at a time, whose next query's scores are on their way meanwhile; KPL scores a
+// lane, cluster j * 32 + lane.
 template <typename T, int KPL>
-__global__ void __launch_bounds__(128) choose_warp_kernel(SelectArgs a,
-                                                          const float* __restrict__ scores,
-                                                          const float* __restrict__ q_norm,
-                                                          const float* __restrict__ c_norm,
-                                                          int ctiles, int32_t* __restrict__ sel,
-                                                          int64_t queries) {
+__global__ void __launch_bounds__(128, KPL <= 8 ? 10 : 4) choose_warp_kernel(
+    SelectArgs a, const float* __restrict__ scores, const float* __restrict__ q_norm,
+    const float* __restrict__ c_norm, int ctiles, int32_t* __restrict__ sel, int64_t queries) {
   __shared__ double s_exact[4][KPL * 32];
   __shared__ uint16_t s_list[4][KPL * 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  const int64_t qi = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (qi >= queries) return;
-  const int r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi % a.Nq);
-  const float* row = scores + qi * a.K;
-  uint32_t key[KPL];
-  int have = 0;
-#pragma unroll
-  for (int j = 0; j < KPL; ++j) {
-    key[j] = j * 32 + lane < a.K ? sort_key(row[j * 32 + lane]) : 0u;
-    have += key[j] != 0u;
-  }
-  have = __reduce_add_sync(0xFFFFFFFFu, have);
   const uint32_t below = (1u << lane) - 1u;
-  // t: the want-th largest key, bit by bit below the bits that all keys share; where a count
-  // meets it, the smallest key counted
-  const int want = min(a.top, have);
-  uint32_t t = 0;
-  if (have > 0) {
-    uint32_t low = 0xFFFFFFFFu, high = 0;
+  pdl_wait();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 4;
+  float ahead[KPL];
+  auto fetch = [&](int64_t qi) {
 #pragma unroll
     for (int j = 0; j < KPL; ++j)
-      if (key[j] != 0u) low = min(low, key[j]), high = max(high, key[j]);
-    low = __reduce_min_sync(0xFFFFFFFFu, low);
-    high = __reduce_max_sync(0xFFFFFFFFu, high);
-    const int open_bits = 32 - __clz(low ^ high);
-    t = want == have ? low : open_bits == 32 ? 0u : high >> open_bits << open_bits;
-    for (int bit = want == have ? -1 : open_bits - 1; bit >= 0; --bit) {
-      const uint32_t cand = t | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < KPL; ++j) n += key[j] >= cand;
-      n = __reduce_add_sync(0xFFFFFFFFu, n);
-      if (n >= want) t = cand;
-      if (n == want) {
-        uint32_t least = 0xFFFFFFFFu;
-#pragma unroll
-        for (int j = 0; j < KPL; ++j)
-          if (key[j] >= cand) least = min(least, key[j]);
-        t = __reduce_min_sync(0xFFFFFFFFu, least);
-        break;
-      }
-    }
-  }
-  const float cn = largest_norm(c_norm, r, ctiles);
-  const float ts = key_score(t);
-  const float band = t <= 1u ? INFINITY : band_of(a, ts, q_norm[qi], cn);
-  const bool open = !(band < INFINITY) || isinf(ts);  // fp32 says nothing: all in 64 bits
-  // in: above the band; undecided: inside
-  uint32_t in = 0, mid = 0;
-  int sure = 0, undecided = 0;
-#pragma unroll
-  for (int j = 0; j < KPL; ++j) {
-    if (key[j] == 0u) continue;
-    const float s = key_score(key[j]);
-    if (!open && s > ts + band)
-      in |= 1u << j, ++sure;
-    else if (open || s >= ts - band)
-      mid |= 1u << j, ++undecided;
-  }
-  sure = __reduce_add_sync(0xFFFFFFFFu, sure);
-  undecided = __reduce_add_sync(0xFFFFFFFFu, undecided);
-  const int places = want - sure;
-  if (undecided == places && !open) {
-    in |= mid;  // no choice to make
-  } else if (undecided > 0) {
-    double* ex = s_exact[warp];
-    uint16_t* list = s_list[warp];
-    int listed = 0;
+      ahead[j] = j * 32 + lane < a.K ? scores[qi * a.K + j * 32 + lane] : __uint_as_float(kNever);
+  };
+  int64_t qi = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (qi < queries) fetch(qi);
+  for (; qi < queries; qi += step) {
+    // (a 64-bit division costs as much as four bisections)
+    const int r = queries <= 0xFFFFFFFFll
+                      ? static_cast<int>(static_cast<uint32_t>(qi) / static_cast<uint32_t>(a.Nq))
+                      : static_cast<int>(qi / a.Nq);
+    const int i = static_cast<int>(qi - static_cast<int64_t>(r) * a.Nq);
+    const float qn = q_norm[qi];
+    uint32_t key[KPL];
+    int have = 0;
 #pragma unroll
     for (int j = 0; j < KPL; ++j) {
-      const uint32_t who = __ballot_sync(0xFFFFFFFFu, mid >> j & 1u);
-      if (mid >> j & 1u) list[listed + __popc(who & below)] = static_cast<uint16_t>(j * 32 + lane);
-      listed += __popc(who);
+      key[j] = sort_key(ahead[j]);
+      have += key[j] != 0u;
     }
-    __syncwarp();
-    for (int k = 0; k < listed; k += 4) {  // four at a time, eight lanes each
-      const int at = k + (lane >> 3);
-      const int c = at < listed ? list[at] : -1;
-      const double s = exact_score<T>(a, r, i, c);
-      if (c >= 0 && (lane & 7) == 0) ex[c] = s;
-    }
-    __syncwarp();
-    // the places best of them: largest score, then lowest index
-    for (int n = 0; n < places; ++n) {
-      double best = -INFINITY;
-      int at = INT_MAX;
-#pragma unroll 1
-      for (int j = 0; j < KPL; ++j)
-        if (mid >> j & 1u) {
-          const double s = ex[j * 32 + lane];
-          if (s > best) best = s, at = j * 32 + lane;
+    if (qi + step < queries) fetch(qi + step);
+    have = __reduce_add_sync(0xFFFFFFFFu, have);
+    // t: the want-th largest key, by bisection between a key that at least `want` reach and one past
+    // the largest; where a count meets it, the smallest key counted
+    const int want = min(a.top, have);
+    uint32_t t = 0;
+    if (have > 0) {
+      uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+      for (int j = 0; j < KPL; ++j) low = min(low, key[j] - 1u), high = max(high, key[j]);
+      // of up to 32 places: each lane's largest key is one of `want` at least
+      const uint32_t tops = __reduce_min_sync(0xFFFFFFFFu, high);
+      low = __reduce_min_sync(0xFFFFFFFFu, low) + 1u;  // keys of 0 were the largest there
+      high = __reduce_max_sync(0xFFFFFFFFu, high) + 1u;  // no key is the largest integer
+      t = want < have && want <= 32 && tops != 0u ? tops : low;
+      while (want < have && high - t > 1u) {
+        // scores on both sides of zero first part there: the keys between are many
+        const uint32_t cand = t < 0x80000000u && high > 0x80000000u ? 0x80000000u : t + (high - t) / 2;
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < KPL; ++j) n += key[j] >= cand;
+        n = __reduce_add_sync(0xFFFFFFFFu, n);
+        if (n < want) {
+          high = cand;
+          continue;
         }
+        t = cand;
+        if (n == want) {
+          uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) {
-        const double s = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-        const int x = __shfl_xor_sync(0xFFFFFFFFu, at, o);
-        if (s > best || (s == best && x < at)) best = s, at = x;
-      }
-      if (at == INT_MAX) break;  // nothing above -inf is left
-      if ((at & 31) == lane) {
-        mid &= ~(1u << (at >> 5));
-        in |= 1u << (at >> 5);
+          for (int j = 0; j < KPL; ++j)
+            if (key[j] >= cand) least = min(least, key[j]);
+          t = __reduce_min_sync(0xFFFFFFFFu, least);
+          break;
+        }
       }
     }
-  }
-  int32_t* out = sel + qi * a.top;
-  int done = 0;
+    const float cn = largest_norm(c_norm, r, ctiles);
+    const float ts = key_score(t);
+    const float band = t <= 1u ? INFINITY : band_of(a, ts, qn, cn);
+    const bool open = !(band < INFINITY) || isinf(ts);  // fp32 says nothing: all in 64 bits
+    // in: above the band; undecided: inside (a step wider, for the two zeros' sake)
+    const uint32_t over = open ? 0xFFFFFFFFu : sort_key(ts + band) + 1u;
+    uint32_t from = open ? 1u : max(sort_key(ts - band), 2u) - 1u;
+    int sure = 0, undecided = 0;
 #pragma unroll
-  for (int j = 0; j < KPL; ++j) {
-    const bool on = in >> j & 1u;
-    const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
-    const int at = done + __popc(who & below);
-    if (on && at < a.top) out[at] = j * 32 + lane;
-    done += __popc(who);
+    for (int j = 0; j < KPL; ++j) {
+      sure += key[j] > over;
+      undecided += key[j] >= from;
+    }
+    sure = __reduce_add_sync(0xFFFFFFFFu, sure);
+    undecided = __reduce_add_sync(0xFFFFFFFFu, undecided) - sure;
+    const int places = want - sure;
+    if ((undecided != places || open) && undecided > 0) {
+      double* ex = s_exact[warp];
+      uint16_t* list = s_list[warp];
+      uint32_t mid = 0;
+      int listed = 0;
+      __syncwarp();  // the last such query's reads
+#pragma unroll
+      for (int j = 0; j < KPL; ++j) {
+        const bool on = key[j] >= from && key[j] <= over;
+        const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
+        if (on) mid |= 1u << j, list[listed + __popc(who & below)] = static_cast<uint16_t>(j * 32 + lane);
+        listed += __popc(who);
+      }
+      __syncwarp();
+      for (int k = 0; k < listed; k += 4) {  // four at a time, eight lanes each
+        const int at = k + (lane >> 3);
+        const int c = at < listed ? list[at] : -1;
+        const double s = exact_score<T>(a, r, i, c);
+        if (c >= 0 && (lane & 7) == 0) ex[c] = s;
+      }
+      __syncwarp();
+      // the places best of them, largest score, then lowest index, get the largest keys
+      uint32_t in = 0;
+      for (int n = 0; n < places; ++n) {
+        double best = -INFINITY;
+        int at = INT_MAX;
+#pragma unroll 1
+        for (int j = 0; j < KPL; ++j)
+          if (mid >> j & 1u) {
+            const double s = ex[j * 32 + lane];
+            if (s > best) best = s, at = j * 32 + lane;
+          }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+          const double s = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+          const int x = __shfl_xor_sync(0xFFFFFFFFu, at, o);
+          if (s > best || (s == best && x < at)) best = s, at = x;
+        }
+        if (at == INT_MAX) break;  // nothing above -inf is left
+        if ((at & 31) == lane) {
+          mid &= ~(1u << (at >> 5));
+          in |= 1u << (at >> 5);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < KPL; ++j)
+        if (in >> j & 1u) key[j] = 0xFFFFFFFFu;
+      from = over == 0xFFFFFFFFu ? over : over + 1u;
+    }
+    int32_t* out = sel + qi * a.top;
+    int done = 0;
+#pragma unroll
+    for (int j = 0; j < KPL; ++j) {
+      const bool on = key[j] >= from;
+      const uint32_t who = __ballot_sync(0xFFFFFFFFu, on);
+      const int at = done + __popc(who & below);
+      if (on && at < a.top) out[at] = j * 32 + lane;
+      done += __popc(who);
+    }
+    for (int j = done + lane; j < a.top; j += 32) out[j] = -1;
   }
-  for (int j = done + lane; j < a.top; j += 32) out[j] = -1;
 }
 
 constexpr int kCtaThreads = 512;
@@ -636,14 +668,17 @@ int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cuda
   const int64_t queries = R * a.Nq;
   // a warp's registers hold the scores of 1024 clusters; where there are fewer warps than
   // schedulers (148 x 4), a CTA per query is faster (128 queries of 1024 clusters: 21 us, a warp
-  // per query 33 us; 32768 queries of 256: a warp 59 us, and a CTA's barriers would come 32768
+  // per query 33 us; 32768 queries of 256: a warp 42 us, and a CTA's barriers would come 32768
   // times)
   if (a.K <= 1024 && queries > 592) {
     auto kern = a.K <= 128   ? choose_warp_kernel<T, 4>
                 : a.K <= 256 ? choose_warp_kernel<T, 8>
                 : a.K <= 512 ? choose_warp_kernel<T, 16>
                              : choose_warp_kernel<T, 32>;
-    return launch_pdl(kern, dim3(static_cast<unsigned>((queries + 3) / 4)), dim3(128), 0, stream, a,
+    // three times what the SMs hold: a warp has a few queries to prefetch over, and their uneven
+    // work evens out
+    const int64_t ctas = std::min<int64_t>((queries + 3) / 4, 148 * (a.K <= 256 ? 30 : 12));
+    return launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, stream, a,
                       static_cast<const float*>(scores), static_cast<const float*>(qn),
                       static_cast<const float*>(cn), l.ctiles, sel, queries);
   }
