@@ -882,8 +882,10 @@ bool tiles_fit(const Args& a, int64_t nq) {
 // 2048 queries x 4 rows, 12 keys a cluster: 188, 322; 24 keys: 315, 324; 64 keys: 408, 195 with
 // 1024 queries.
 bool use_tiles(const Args& a) {
-  const int64_t nq = queries_per_round(a);
+  const int64_t nq = queries_per_round(a), DP = a.D <= 64 ? 64 : 128;
   if (!tiles_fit(a, nq)) return false;
+  // a round of few queries of very many sequences: its parts would be 2^32 bytes and more
+  if (static_cast<int64_t>(a.batch) * a.Hkv * nq * a.top * a.G * DP * 4 > (1ll << 32)) return false;
   const FormWork w = form_work(a, nq);
   const double walk = 18 + 75e-6 * w.reads;
   const double tiles = 34 + w.units * (0.009 + 0.000136 * w.keys) + 86e-6 * w.rows;

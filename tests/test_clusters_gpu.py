@@ -200,6 +200,18 @@ def test_select_ties_and_borders(clusters, K):
     assert torch.equal(got, select_ref(qq, big, offsets, 17))
 
 
+def test_select_many_queries(clusters):
+    """More queries than warps at once, with ties, near ties and masks among them."""
+    q = (randn(1, 4, 7001, 32, seed=1) * 2).round().div(2).to(BF)
+    cen = (randn(4, 90, 32, seed=2) * 2).round().div(2).to(BF)
+    cen[:, 40:50] = cen[:, 10:20]
+    cen[:, 50:60] = cen[:, 20:30] + 2.0 ** -9 * randn(4, 10, 32, seed=3).sign().to(BF)
+    _, order, offsets = key_clusters(4, 2000, 90, 4)
+    pos = torch.randint(-1, 2000, (1, 7001), generator=gen(5), device="cuda", dtype=torch.int32)
+    got = clusters.cluster_select(q, cen, offsets, 13, order=order, q_pos=pos)
+    assert torch.equal(got, select_ref(q, cen, offsets, 13, order, pos))
+
+
 def test_select_infinities(clusters):
     q, cen = randn(1, 2, 4, 16, seed=1).to(BF), randn(1, 6, 16, seed=2).to(BF)
     offsets = torch.arange(7, device="cuda", dtype=torch.int32)[None]
