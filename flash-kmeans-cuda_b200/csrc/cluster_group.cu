@@ -7,7 +7,7 @@
 // at most 11 bits: one pass up to K = 2046, two up to 4 M. Per pass
 //   hist     (group_hist_kernel)    digit counts of chunks of R positions;
 //   prefix   (group_prefix_kernel)  exclusive sums over the chunks per digit, and
-//            the digit totals of the row;
+//            the digit totals of the row (where there are few, the scatter does it);
 //   scatter  (group_scatter_kernel) scan of the totals; every warp ranks its own
 //            positions in order with its own row of 16-bit counters (match_any
 //            ranks the 32 positions of a step), so equal ids keep their order.
@@ -30,6 +30,7 @@ namespace {
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxBits = 11;
+constexpr int kPer = (1 << kMaxBits) / kThreads;  // digits per thread
 constexpr int kBatch = 8;        // 32-position steps whose keys are loaded together
 constexpr int kOneChunk = 4096;  // rows up to here are one chunk
 constexpr int kMinChunk = 1024;  // positions per chunk of longer rows: a multiple of kThreads ...
@@ -141,6 +142,7 @@ __global__ void __launch_bounds__(256) group_prefix_few_kernel(int32_t* __restri
 }
 
 // Positions (and, before the last pass, their keys) of a chunk to their slots.
+// total null: hist holds the chunks' counts, else their prefixes; hist null: one chunk.
 // vals_in null: the value is the position itself. offsets non-null (one-pass
 // sorts): the first slot of every cluster.
 template <typename Id>
@@ -192,10 +194,40 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
       }
     }
   };
+  // each thread takes `per` neighbouring digits: their totals in the row, and before this chunk
+  const int per = (bins + kThreads - 1) / kThreads;
+  const int d0 = min(bins, static_cast<int>(threadIdx.x) * per), d1 = min(bins, d0 + per);
+  int all[kPer], before[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) {
+    all[x] = before[x] = 0;
+    const int d = d0 + x;
+    if (hist == nullptr || d >= d1) continue;
+    if (total != nullptr) {
+      all[x] = total[static_cast<int64_t>(b) * bins + d];
+      before[x] = hist[static_cast<int64_t>(blockIdx.x) * bins + d];
+    } else {
+      const int32_t* h = hist + static_cast<int64_t>(b) * C * bins + d;
+      for (int c1 = 0; c1 < C; c1 += 16) {
+        int v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) v[u] = c1 + u < C ? h[(c1 + u) * bins] : 0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          all[x] += v[u];
+          if (c1 + u < c) before[x] += v[u];
+        }
+      }
+    }
+  }
   walk([](int, int, int, int) {});
   __syncthreads();
-  // counters -> exclusive prefixes over the warps; the chunk's totals
-  for (int d = threadIdx.x; d < bins; d += kThreads) {
+  // counters -> exclusive prefixes over the warps; the chunk's totals where it is the only one
+  int sum = 0;
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) {
+    const int d = d0 + x;
+    if (d >= d1) continue;
     int run = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -203,14 +235,10 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
       cnt[w * bins + d] = static_cast<uint16_t>(run);
       run += v;
     }
-    base[d] = total != nullptr ? total[static_cast<int64_t>(b) * bins + d] : run;
+    if (hist == nullptr) all[x] = run;
+    sum += all[x];
   }
-  __syncthreads();
-  // exclusive scan of the row's digit totals; each thread takes `per` neighbours
-  const int per = (bins + kThreads - 1) / kThreads;
-  const int d0 = min(bins, static_cast<int>(threadIdx.x) * per), d1 = min(bins, d0 + per);
-  int sum = 0;
-  for (int d = d0; d < d1; ++d) sum += base[d];
+  // exclusive scan of the row's digit totals
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -221,11 +249,13 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(
   __syncthreads();
   int run = inc - sum;
   for (int w = 0; w < warp; ++w) run += warp_sum[w];
-  for (int d = d0; d < d1; ++d) {
-    const int v = base[d];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) {
+    const int d = d0 + x;
+    if (d >= d1) continue;
     if (offsets != nullptr && c == 0 && d <= K) offsets[static_cast<int64_t>(b) * (K + 1) + d] = run;
-    base[d] = run + (hist != nullptr ? hist[static_cast<int64_t>(blockIdx.x) * bins + d] : 0);
-    run += v;
+    base[d] = run + before[x];
+    run += all[x];
   }
   __syncthreads();
   walk([&](int r, int key, int d, int slot) {
@@ -306,14 +336,17 @@ int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in, int
   const int bins = 1 << g.bits, shift = pass * g.bits;
   const int n = static_cast<int>(N), k = static_cast<int>(K);
   const dim3 grid(static_cast<unsigned>(B * g.C));
+  // few counts are summed by every CTA of the scatter, which saves a launch: 16 chunks x 256 digits,
+  // two passes, 4 us less; 8 x 2048 7 us more, 32 x 1024 3 us more
+  const bool sums = g.C * bins <= 4096;
   if (g.C > 1) {
     FKC_TRY(launch_pdl(group_hist_kernel<Id>, grid, dim3(kThreads), bins * 4, stream, keys_in,
                        stride, n, k, g.R, g.C, shift, g.bits, w.hist));
     const int per_row = (bins + 31) / 32;
-    if (g.C <= 64)  // eight loads in flight a thread; more chunks are split over warps
+    if (!sums && g.C <= 64)  // eight loads in flight a thread; more chunks are split over warps
       FKC_TRY(launch_pdl(group_prefix_few_kernel, dim3(static_cast<unsigned>((B * bins + 255) / 256)),
                          dim3(256), 0, stream, w.hist, w.total, bins, g.C, B * bins));
-    else
+    else if (!sums)
       FKC_TRY(launch_pdl(group_prefix_kernel, dim3(static_cast<unsigned>(B * per_row)), dim3(1024), 0,
                          stream, w.hist, w.total, bins, g.C, per_row));
   }
@@ -323,7 +356,7 @@ int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in, int
                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       static_cast<int>(smem)));
   return launch_pdl(group_scatter_kernel<Id>, grid, dim3(kThreads), smem, stream, keys_in, stride, vals_in,
-                    static_cast<const int32_t*>(w.hist), static_cast<const int32_t*>(w.total),
+                    static_cast<const int32_t*>(w.hist), static_cast<const int32_t*>(sums ? nullptr : w.total),
                     keys_out, vals_out, offsets, pass == g.passes - 1, n, k, g.R, g.C, shift,
                     g.bits);
 }
