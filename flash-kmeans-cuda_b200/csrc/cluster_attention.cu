@@ -24,10 +24,11 @@
 // several warps (at least four tiles each, about 8 per SM in all), and attn_join_kernel joins the
 // parts by their log-sum-exp.
 //
-// 16 sequences x 8 rows, one query each, 64 of 1024 clusters of 32 keys, D = 128: 54 us for 134 MB
-// of keys and values, 2.5 TB/s of useful bytes; DRAM reads 228 MB, since a key is 256 bytes at an
-// arbitrary place and neighbouring sectors come with it. One query of 512 keys: 12 us, a chain of
-// list, gather, products and join.
+// 16 sequences x 8 rows, one query each, 64 of 1024 clusters, D = 128: on average 3425 keys a query,
+// 224 MB, in 50 us, 4.5 TB/s (the join 5 us, with eight parts' loads in flight; one after another
+// they took 8). While its SMs are busy the walk moves some 6 TB/s; it loses a fifth to the
+// largest queries, whose warps end last (twice as many, shorter parts: 64 us, since each warp
+// builds its list). One query of 512 keys: 10 us, a chain of list, gather, products and join.
 #include <algorithm>
 
 #include "cluster_attention.cuh"
@@ -110,12 +111,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_fwd_kernel(Args a, T* __rest
 
   // keys of the next 32 places (two tiles), fetched one round ahead of their copies
   int cur = 0;
-  int idx = -1, idx_next = list.key(a, order, t_beg * kTile + lane, cur, pos);
+  int idx = -1, idx_next = list.key(a, order, t_beg * kTile + lane, cur);
   auto issue = [&](int t) {  // tiles are issued in order from t_beg
     const int half = (t - t_beg) & 1;
     if (half == 0) {
-      idx = idx_next;
-      idx_next = list.key(a, order, (t + 2) * kTile + lane, cur, pos);
+      idx = KeyList::visible(a, idx_next, pos);
+      idx_next = list.key(a, order, (t + 2) * kTile + lane, cur);
     }
     const int stage = (t - t_beg) % STAGES;
     const uint32_t kt = ring + stage * (2 * kTile * DP * 2), vt = kt + kTile * DP * 2;
@@ -265,31 +266,42 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict_
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const float* pl = part_lse + row * nsplit;
-  float top = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) top = fmaxf(top, pl[s]);
+  // lane l takes columns 4 l ..; of up to 64 parts, it holds the weights of l and l + 32
+  const float* po = part_o + row * nsplit * D + lane * 4;
+  const bool on = lane * 4 < D;
+  float w[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    w[x] = x * 32 + lane < nsplit ? part_lse[row * nsplit + x * 32 + lane] : -INFINITY;
+  float4 v[8];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      v[u] = on && s0 + u < nsplit ? *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s0 + u) * D)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  fetch(0);  // on its way with the weights
+  float top = fmaxf(w[0], w[1]);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float w = exp2f((pl[s] - base) * kLog2e);
-    sum += w;
-    const float* po = part_o + (row * nsplit + s) * D;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (u * 32 + lane < D) acc[u] += w * po[u * 32 + lane];
+  for (int x = 0; x < 2; ++x) w[x] = exp2f((w[x] - base) * kLog2e);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  for (int s0 = 0; s0 < nsplit; s0 += 8) {
+    if (s0 > 0) fetch(s0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u;  // weights behind the last part are 0
+      const float f = __shfl_sync(0xFFFFFFFFu, s < 32 ? w[0] : w[1], s & 31);
+      sum += f;
+      acc[0] += f * v[u].x, acc[1] += f * v[u].y, acc[2] += f * v[u].z, acc[3] += f * v[u].w;
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (u * 32 + lane < D) {
-      const float v = acc[u] * inv;
-      if constexpr (std::is_same<T, __half>::value)
-        out[row * D + u * 32 + lane] = __float2half_rn(v);
-      else
-        out[row * D + u * 32 + lane] = __float2bfloat16_rn(v);
-    }
+  if (on)
+    *reinterpret_cast<uint2*>(out + row * D + lane * 4) =
+        make_uint2(mma::pack2<T>(acc[0] * inv, acc[1] * inv), mma::pack2<T>(acc[2] * inv, acc[3] * inv));
   if (lane == 0) lse[row] = sum == 0.f ? -INFINITY : base + log2f(sum) * kLn2;
 }
 

@@ -75,13 +75,15 @@ struct KeyList {
     __syncwarp();
   }
 
-  // The key at place p (a lane's places ascend; cur is its cursor), or -1: past the
-  // end, or not visible to a query at pos.
-  __device__ __forceinline__ int key(const Args& a, const int32_t* order, int p, int& cur,
-                                     int pos) const {
+  // What order holds for place p (a lane's places ascend; cur is its cursor); -1 past the end.
+  // Nothing here waits for the load: visible() does, at its use.
+  __device__ __forceinline__ int key(const Args& a, const int32_t* order, int p, int& cur) const {
     if (p >= total) return -1;
     while (cur + 1 < a.top && p >= pre[cur + 1]) ++cur;
-    const int row = order[at[cur] + (p - pre[cur])];
+    return order[at[cur] + (p - pre[cur])];
+  }
+  // The key, or -1 where a query at pos does not see it.
+  static __device__ __forceinline__ int visible(const Args& a, int row, int pos) {
     return row >= 0 && row < a.N && row <= pos ? row : -1;
   }
 };

@@ -129,12 +129,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   const int dchunks = a.D / 8;
   int cur = 0;
-  int idx = -1, idx_next = list.key(a, order, lane, cur, pos);
+  int idx = -1, idx_next = list.key(a, order, lane, cur);
   auto issue = [&](int t) {
     const int half = t & 1;
     if (half == 0) {
-      idx = idx_next;
-      idx_next = list.key(a, order, (t + 2) * kTile + lane, cur, pos);
+      idx = KeyList::visible(a, idx_next, pos);
+      idx_next = list.key(a, order, (t + 2) * kTile + lane, cur);
     }
     const int stage = t % STAGES;
     const uint32_t kt = ring + stage * (2 * kTile * DP * 2), vt = kt + kTile * DP * 2;

@@ -19,7 +19,8 @@
 //
 // At 4096 queries x 8 rows of G = 4, 16 of 256 clusters of 64 keys, D = 128 (2.1 M (query, slot,
 // head) rows, 69 GFLOP): the units and rows are listed in 46 us, tiles_fwd_kernel takes 336 us, the
-// join 112 us (the call 484 us: they overlap at their ends). The kernel is bound by its
+// join 112 us (the call 484 us: they overlap at their ends; the larger of the skewed clusters are
+// selected more often, 1779 keys a query instead of 1024, which makes it 119 GFLOP). The kernel is bound by its
 // SMs' instruction issue (48% of all slots, softmax and output) and by the gathers, which it waits
 // for at the start of every unit; its tensor pipe is busy for 22% of the time and DRAM for a
 // third (800 MB: the parts do not fit L2, Q rows come from it). The join moves 564 MB at 5.1 TB/s.

@@ -21,7 +21,7 @@
 //
 // 4096 queries x 4 rows of G = 4, 8 of 64 clusters of 64 keys, D = 128: dQ 140 us and its join 28,
 // dK and dV 129 us and their join 14, rows and tiles listed in 45 (forward and backward together
-// 500 us). The two large kernels are bound by the chain of one 128-row step: gathered rows, two
+// 492 us). The two large kernels are bound by the chain of one 128-row step: gathered rows, two
 // score products, the warpgroups' turn (a thread a row, 64 columns), two or four products; the
 // tensor pipe is busy for 24% and 33%. The walk took 2200 us for the gradients, warp-level matrix
 // instructions as little; scores of 64 columns at a time 630 us, joins of single heads 560.
