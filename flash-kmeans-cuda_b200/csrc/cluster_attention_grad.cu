@@ -6,6 +6,10 @@
 //   delta  (attn_delta_kernel)  one warp per query and head.
 //   dQ     (attn_dq_kernel)     the forward's walk: one warp per query and group, keys and
 //          values gathered in tiles of 16, S^T and dP^T formed transposed, dQ^T += K^T dS^T.
+//          It walks twice, first for delta = sum of P dP: keys of one cluster lie close to one
+//          another, so that what a rounded delta is off by adds up over them (dS no longer sums to
+//          zero). With delta from the 16-bit out, dQ of one cluster of 30 keys was off by
+//          0.0051 of its norm, with four clusters a query by 0.0026; its own rounding is 0.0017.
 //   dK, dV (attn_dkv_kernel)    one CTA per 64 keys of a cluster, whose keys and values stay in
 //          shared memory. The queries that selected the cluster come from the same grouping
 //          that orders the keys (sel as ids: entry e is query e / top), their heads side by
@@ -17,7 +21,7 @@
 // type demands, dS of dQ into two terms: a row of dQ sums few large dS, and with one term its
 // error against 64 bits was 1.7 times that of its own last rounding, with two 1.2 times (the
 // walk waits for its gather, the second product is free). Sums are fp32 and rounded once on the
-// way out. delta comes from the 16-bit out. Keys in no cluster get zeros.
+// way out. delta of dK comes from the 16-bit out (dK sums over queries, which are not alike). Keys in no cluster get zeros.
 //
 // Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
 // of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
@@ -71,7 +75,6 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ o
 template <typename T, int DP, int NT, int STAGES>
 __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* __restrict__ dout,
                                                               const float* __restrict__ lse,
-                                                              const float* __restrict__ delta,
                                                               T* __restrict__ dq, int chunks,
                                                               int64_t units) {
   constexpr int KS = DP / 16;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     for (int e = 0; e < 2; ++e) {
       const int h = n * 8 + t4 * 2 + e;
       ls[n][e] = h < heads ? lse[flat(h)] * kLog2e : 0.f;
-      dl[n][e] = h < heads ? delta[flat(h)] : 0.f;
+      dl[n][e] = 0.f;
     }
   }
   KeyList list;
@@ -128,8 +131,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
   const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   const int dchunks = a.D / 8;
-  int cur = 0;
-  int idx = -1, idx_next = list.key(a, order, lane, cur);
+  int cur = 0, idx = -1, idx_next = -1;
   auto issue = [&](int t) {
     const int half = t & 1;
     if (half == 0) {
@@ -159,12 +161,22 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][kk][e] = 0.f;
+  const float sc = a.scale * kLog2e;
+  // pass 0: delta = sum of P dP; pass 1: dQ
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+  cur = 0;
+  idx_next = list.key(a, order, lane, cur);
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
     if (s < tiles) issue(s);
     mma::cp_async_commit();
   }
-  const float sc = a.scale * kLog2e;
+  float sum[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) sum[n][e] = 0.f;
   for (int t = 0; t < tiles; ++t) {
     mma::cp_async_wait<STAGES - 2>();
     __syncwarp();
@@ -198,7 +210,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
       for (int e = 0; e < 2; ++e) {
         s[n][e] = on0 ? exp2f(s[n][e] * sc - ls[n][e]) * (dp[n][e] - dl[n][e]) : 0.f;
         s[n][2 + e] = on1 ? exp2f(s[n][2 + e] * sc - ls[n][e]) * (dp[n][2 + e] - dl[n][e]) : 0.f;
+        sum[n][e] += s[n][e] + s[n][2 + e];
       }
+    }
+    if (pass == 0) continue;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t h = mma::pack2<T>(s[n][2 * e], s[n][2 * e + 1]);
@@ -219,6 +236,20 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     }
   }
   mma::cp_async_wait<0>();
+  __syncwarp();
+  if (pass == 0) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float d = sum[n][e];
+        d += __shfl_xor_sync(0xFFFFFFFFu, d, 4);
+        d += __shfl_xor_sync(0xFFFFFFFFu, d, 8);
+        d += __shfl_xor_sync(0xFFFFFFFFu, d, 16);
+        dl[n][e] = d;
+      }
+  }
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -528,7 +559,7 @@ GradLayout grad_layout(const Args& a, int dtype) {
 }
 
 template <typename T, int DP, int NT>
-int dq_typed(const Args& a, const T* dout, const float* lse, const float* delta, T* dq,
+int dq_typed(const Args& a, const T* dout, const float* lse, T* dq,
              cudaStream_t stream) {
   constexpr int STAGES = 3;
   const int chunks = (a.G + 8 * NT - 1) / (8 * NT);
@@ -537,7 +568,7 @@ int dq_typed(const Args& a, const T* dout, const float* lse, const float* delta,
   auto kern = attn_dq_kernel<T, DP, NT, STAGES>;
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   return launch_pdl(kern, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
-                    dim3(32 * kWarps), smem, stream, a, dout, lse, delta, dq, chunks, units);
+                    dim3(32 * kWarps), smem, stream, a, dout, lse, dq, chunks, units);
 }
 
 template <typename T, int DP>
@@ -557,9 +588,9 @@ int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T
     return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, odd, ws + l.tiles, stream);
   if (dq != nullptr) {
     if (a.G <= 8)
-      FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, stream)));
+      FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, dq, stream)));
     else
-      FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, delta, dq, stream)));
+      FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, dq, stream)));
   }
   if (dk == nullptr) return FKC_OK;
   FKC_TRY(launch_group(a.sel, false, static_cast<int64_t>(a.Nq) * a.top, inv_order, inv_offsets, R,

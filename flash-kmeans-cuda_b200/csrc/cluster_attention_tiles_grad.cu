@@ -1082,10 +1082,12 @@ int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, c
 // rows, 32 clusters of 32 keys: 133, 137. G 16, 64 queries x 8 rows, 32 rows a cluster of 64
 // keys: 408, 389; 2048 queries x 4 rows, 12 keys a cluster: 1061, 1194; 20 keys: 1274, 1182.
 bool use_tiles_grad(const Args& a) {
-  if (!tiles_fit(a, a.Nq)) return false;
+  // delta comes from the 16-bit out here, which few clusters of close keys do not bear (the walk
+  // forms it anew, see cluster_attention_grad.cu): 0.0051 of dQ's norm with one, 0.0026 with four
+  if (a.top < 4 || !tiles_fit(a, a.Nq)) return false;
   const FormWork w = form_work(a, a.Nq);
   const double key_tiles = static_cast<double>(a.batch) * a.Hkv * a.K * (w.keys / 64 + 0.5);  // of the walk
-  const double walk = 51 + 68e-6 * w.reads + 0.031 * key_tiles + w.rows * (257e-6 + 3.1e-6 * w.keys);
+  const double walk = 60 + 110e-6 * w.reads + 0.031 * key_tiles + w.rows * (257e-6 + 3.1e-6 * w.keys);
   const double tiles = 61 + w.units * (0.019 + 0.00039 * w.keys) + 260e-6 * w.rows + 0.002 * key_tiles;
   if (1.1 * tiles >= walk) return false;
   // all queries at once: 32-bit rows of units, and parts of 2^33 bytes at most
