@@ -25,7 +25,7 @@
 //
 // Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
 // of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
-// 512 clusters of 24 keys: 219 us (by clusters 256); 2048 queries: 678 us (by clusters 274).
+// 512 clusters of 24 keys: 219 us with one pass of dQ (by clusters 256); 2048 queries: 678 us (by clusters 274).
 #include <algorithm>
 
 #include "cluster_attention.cuh"

@@ -1077,7 +1077,8 @@ int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, c
 
 }  // namespace
 
-// In us, as use_tiles. Measured (walk, by clusters, forward included): G 1, 256
+// In us, as use_tiles, fitted when the walk took one pass for dQ; its second pass reads the keys
+// again, 42 of the 110 us per million reads. Measured then (walk, by clusters, forward included): G 1, 256
 // queries x 8 rows, 8 rows a cluster of 24 keys: 297, 358; of 64: 576, 418. G 8, 256 queries x 4
 // rows, 32 clusters of 32 keys: 133, 137. G 16, 64 queries x 8 rows, 32 rows a cluster of 64
 // keys: 408, 389; 2048 queries x 4 rows, 12 keys a cluster: 1061, 1194; 20 keys: 1274, 1182.
