@@ -18,7 +18,7 @@
 //          stay in fp32 registers, in ascending query order, so two runs give the same bits.
 //
 // P and dS are rounded to the 16-bit input type for the second products, as their operand
-// type demands, dS of dQ into two terms: a row of dQ sums few large dS, and with one term its
+// type demands, dS into two terms: a row of dQ sums few large dS, and with one term its
 // error against 64 bits was 1.7 times that of its own last rounding, with two 1.2 times (the
 // walk waits for its gather, the second product is free). Sums are fp32 and rounded once on the
 // way out. delta of dK comes from the 16-bit out (dK sums over queries, which are not alike). Keys in no cluster get zeros.
@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
           mma::m16n8k16<T>(dp[n + 1], fv, f[2], f[3]);
         }
       }
-      uint32_t pp[4][2], ds[4][2];  // rounded, (key g, columns) and (key g + 8, columns)
+      // rounded, (key g, columns) and (key g + 8, columns); lo: what dS's rounding left
+      uint32_t pp[4][2], ds[4][2], lo[4][2];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
 #pragma unroll
@@ -489,11 +490,17 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
         pp[n][1] = mma::pack2<T>(ss[n][2], ss[n][3]);
         ds[n][0] = mma::pack2<T>(dp[n][0], dp[n][1]);
         ds[n][1] = mma::pack2<T>(dp[n][2], dp[n][3]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = mma::unpack2<T>(ds[n][e]);
+          lo[n][e] = mma::pack2<T>(dp[n][2 * e] - f.x, dp[n][2 * e + 1] - f.y);
+        }
       }
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc) {  // 16 columns as depth
         const uint32_t fp[4] = {pp[2 * cc][0], pp[2 * cc][1], pp[2 * cc + 1][0], pp[2 * cc + 1][1]};
         const uint32_t fd[4] = {ds[2 * cc][0], ds[2 * cc][1], ds[2 * cc + 1][0], ds[2 * cc + 1][1]};
+        const uint32_t fl[4] = {lo[2 * cc][0], lo[2 * cc][1], lo[2 * cc + 1][0], lo[2 * cc + 1][1]};
 #pragma unroll
         for (int nd = 0; nd < KS; ++nd) {
           uint32_t f[4];
@@ -503,6 +510,8 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
           load_b_trans<DP>(f, qt, cc * 16, nd);
           mma::m16n8k16<T>(ak[2 * nd], fd, f[0], f[1]);
           mma::m16n8k16<T>(ak[2 * nd + 1], fd, f[2], f[3]);
+          mma::m16n8k16<T>(ak[2 * nd], fl, f[0], f[1]);
+          mma::m16n8k16<T>(ak[2 * nd + 1], fl, f[2], f[3]);
         }
       }
     }
