@@ -494,7 +494,12 @@ __device__ __forceinline__ KeyTile load_tile(const KeyTile* t) {
   return x;
 }
 
-// Key tiles and steps of every row r: first[2 r], first[2 r + 1] before the scan over rows.
+// Key tiles of one row at most: of n keys a cluster has one for every kSub and one for the rest.
+__host__ __device__ __forceinline__ int64_t row_tiles_max(int64_t K, int64_t N) { return (K < N ? K : N) + N / kSub; }
+
+// Key tiles and steps of every row r: first[2 r], first[2 r + 1] before the scan over rows. A row whose
+// offsets no grouping gives (clusters that overlap) may have more tiles than row_tiles_max: it has none
+// at all then, and no gradient of its keys, since the list has no room for them.
 __device__ __forceinline__ void tiles_of(const Args& a, const int32_t* inv_offsets, int r, int c, int& s0,
                                          int& s1, int& nrows) {
   nrows = 0;
@@ -527,9 +532,9 @@ __global__ void __launch_bounds__(1024) key_count_kernel(Args a, const int32_t* 
   if (lane == 0) sums[0][warp] = tiles, sums[1][warp] = steps;
   __syncthreads();
   if (threadIdx.x < 2) {
-    int64_t s = 0;
-    for (int w = 0; w < 32; ++w) s += sums[threadIdx.x][w];
-    first[2 * r + threadIdx.x] = s;
+    int64_t n = 0, s = 0;
+    for (int w = 0; w < 32; ++w) n += sums[0][w], s += sums[threadIdx.x][w];
+    first[2 * r + threadIdx.x] = n <= row_tiles_max(a.K, a.N) ? s : 0;
   }
 }
 
@@ -540,8 +545,7 @@ __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* 
                                                          const int64_t* __restrict__ first,
                                                          KeyTile* __restrict__ tiles,
                                                          int64_t* __restrict__ share,
-                                                         int32_t* __restrict__ start, int ctas, int R,
-                                                         int64_t tiles_max) {
+                                                         int32_t* __restrict__ start, int ctas, int R) {
   __shared__ int64_t sums[3][32];
   __shared__ int highs[32];
   pdl_wait();
@@ -575,6 +579,7 @@ __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* 
       share[j] = j * total / ctas;
       if (total == 0 && j < ctas) start[j] = 0;
     }
+  if (first[2 * r] == 0) return;
   for (int c0 = 0; c0 < a.K; c0 += 1024) {
     const int c = c0 + threadIdx.x;
     int s0, s1, nrows;
@@ -596,7 +601,6 @@ __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, const int32_t* 
       tile0 += sums[0][w], step0 += sums[1][w];
     }
     for (int k = 0; k < n; ++k, ++t_at, s_at += per) {
-      if (t_at >= tiles_max) break;  // never, with the workspace of grad_layout
       KeyTile t;
       t.r = r, t.s0 = s0 + k * kSub, t.keys = min(kSub, s1 - s0 - k * kSub), t.high = high;
       t.row0 = first_unit[static_cast<int64_t>(r) * a.K + c] * kUnitRows;
@@ -982,7 +986,6 @@ __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTi
 struct GradLayout {
   UnitPlan plan;
   size_t part, scales, first, tiles, share, start, dkv_part, total;
-  int64_t tiles_max;
 };
 
 GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
@@ -995,11 +998,10 @@ GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
     at += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  l.tiles_max = R * (std::min<int64_t>(a.K, a.N) + a.N / kSub);
   l.part = take(l.plan.units_max * kUnitRows * DP * part_bytes);
   l.scales = take(l.plan.units_max * kUnitRows * 8);
   l.first = take(R * 16);
-  l.tiles = take(l.tiles_max * static_cast<int64_t>(sizeof(KeyTile)));
+  l.tiles = take(R * row_tiles_max(a.K, a.N) * static_cast<int64_t>(sizeof(KeyTile)));
   l.share = take((kMaxCtas + 1) * 8);
   l.start = take(kMaxCtas * 4);
   l.dkv_part = take(static_cast<int64_t>(std::min(sm_count(), kMaxCtas)) * 4 * kSub * DP * 4);
@@ -1052,7 +1054,7 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
   FKC_TRY(launch_pdl(key_count_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv, first));
   FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a, inv,
                      static_cast<const int32_t*>(l.plan.first_unit), static_cast<const int64_t*>(first), tiles,
-                     share, start, shares, static_cast<int>(R), l.tiles_max));
+                     share, start, shares, static_cast<int>(R)));
   auto kern = tiles_dkv_kernel<T, DP>;
   const int smem = static_cast<int>(DkvSmem<DP>::kBytes);
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));

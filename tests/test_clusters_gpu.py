@@ -701,3 +701,21 @@ def test_other_stream_and_graph_replay(clusters):
     for _, got in graphs:
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+def test_many_queries_offsets_of_no_grouping(clusters):
+    """Offsets whose clusters overlap have more key tiles than a grouping can have: their row's keys get
+    no gradient, the other rows' results stay."""
+    q, k, v, sel, order, offsets, pos = attention_case(1, 3, 4, 1000, 1500, 40, 64, 5, BF, causal=False, drop=0.0)
+    dout = randn(*q.shape, seed=9).to(BF)
+    val, tol = attention_ref(q, k, v, sel, order, offsets, None, None, dout)
+    offsets[1, 0::2], offsets[1, 1::2] = 0, 1500  # every other cluster has all keys: 240 tiles, 51 have room
+    a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = clusters.cluster_attention(*a, sel, order, offsets)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, a, dout))))
+    for name, x in got.items():
+        n = x.shape[1] // 3
+        for rows in (slice(0, n), slice(2 * n, 3 * n)):
+            close(x[:, rows], val[name][:, rows], tol[name][:, rows], name)
+        assert x.isfinite().all()
+    assert got["dk"][:, 1].eq(0).all() and got["dv"][:, 1].eq(0).all()
