@@ -348,8 +348,8 @@ int fwd_dtype(const Args& a, void* out, float* lse, float* ws, cudaStream_t stre
 
 }  // namespace
 
-size_t forward_workspace_bytes(const Args& a, int dtype) {
-  if (use_tiles(a)) return tiles_forward_workspace_bytes(a, dtype);
+size_t forward_workspace_bytes(const Args& a) {
+  if (use_tiles(a)) return tiles_forward_workspace_bytes(a);
   const int nsplit = split_count(a);
   if (nsplit == 1) return 0;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.Hq * a.Nq;

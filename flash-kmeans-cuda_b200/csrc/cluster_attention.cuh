@@ -133,15 +133,15 @@ int sm_count();  // of the current device
 size_t select_workspace_bytes(int64_t R, int64_t Nq, int64_t K);
 int launch_select(const Args& a, const void* centroids, const float* bias, double scale, int dtype,
                   int32_t* sel, void* ws, cudaStream_t stream);
-size_t forward_workspace_bytes(const Args& a, int dtype);
+size_t forward_workspace_bytes(const Args& a);
 int launch_forward(const Args& a, int dtype, void* out, float* lse, void* ws, cudaStream_t stream);
 // The form by clusters (cluster_attention_tiles.cu), taken where use_tiles says so.
 bool use_tiles(const Args& a);
-size_t tiles_forward_workspace_bytes(const Args& a, int dtype);
+size_t tiles_forward_workspace_bytes(const Args& a);
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream);
 bool use_tiles_grad(const Args& a);
-size_t tiles_backward_workspace_bytes(const Args& a, int dtype);
+size_t tiles_backward_workspace_bytes(const Args& a);
 int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
                           void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream);
 // After the kernels above, where they set *odd: results that are not finite, from what their rows
@@ -149,7 +149,7 @@ int launch_tiles_backward(const Args& a, int dtype, const float* lse, const floa
 int launch_again(const Args& a, int dtype, const int32_t* odd, const float* lse, const float* delta,
                  const void* dout, void* rows, const int32_t* inv_order, const int32_t* inv_offsets,
                  void* dk, void* dv, cudaStream_t stream);
-size_t backward_workspace_bytes(const Args& a, int dtype);
+size_t backward_workspace_bytes(const Args& a);
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
 

@@ -543,7 +543,7 @@ struct GradLayout {
   size_t delta, odd, inv_order, inv_offsets, tile_off, group, tiles, total;
 };
 
-GradLayout grad_layout(const Args& a, int dtype) {
+GradLayout grad_layout(const Args& a) {
   GradLayout l{};
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   size_t at = 0;
@@ -555,7 +555,7 @@ GradLayout grad_layout(const Args& a, int dtype) {
   l.delta = take(static_cast<size_t>(a.batch) * a.Hq * a.Nq * 4);
   l.odd = take(4);
   if (use_tiles_grad(a)) {
-    l.tiles = take(tiles_backward_workspace_bytes(a, dtype));
+    l.tiles = take(tiles_backward_workspace_bytes(a));
     l.total = at;
     return l;
   }
@@ -583,7 +583,7 @@ int dq_typed(const Args& a, const T* dout, const float* lse, T* dq,
 template <typename T, int DP>
 int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T* dout, T* dq, T* dk, T* dv,
                uint8_t* ws, cudaStream_t stream) {
-  const GradLayout l = grad_layout(a, dtype);
+  const GradLayout l = grad_layout(a);
   float* delta = reinterpret_cast<float*>(ws + l.delta);
   int32_t* odd = reinterpret_cast<int32_t*>(ws + l.odd);
   int32_t* inv_order = reinterpret_cast<int32_t*>(ws + l.inv_order);
@@ -635,7 +635,7 @@ int grad_dtype(const Args& a, int dtype, const void* out, const float* lse, cons
 
 }  // namespace
 
-size_t backward_workspace_bytes(const Args& a, int dtype) { return grad_layout(a, dtype).total; }
+size_t backward_workspace_bytes(const Args& a) { return grad_layout(a).total; }
 
 int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {

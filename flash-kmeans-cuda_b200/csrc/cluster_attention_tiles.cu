@@ -5,9 +5,9 @@
 // together instead: sel is grouped by cluster (cluster_group.cu: entry e is query
 // e / top), the heads of its queries become the rows of units of 256, and a unit reads the
 // cluster's keys once for all of them. A unit leaves, for every (query, slot of sel, head),
-// the output over that cluster (Part) and its log-sum-exp, and tiles_join_kernel joins a query's
-// top parts. So the traffic is D * (2 + 2 + 2) bytes (bf16; 2 + 4 + 4 for fp16) per (query, slot,
-// head) instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster a tenth.
+// the output over that cluster (a part, three bytes a value) and its log-sum-exp, and tiles_join_kernel
+// joins a query's top parts. So the traffic is D * (2 + 3 + 3) bytes per (query, slot, head)
+// instead of 4 * D per (query, key): at G = 4 and 64 keys a cluster an eighth.
 //
 // tiles_fwd_kernel is persistent, one CTA per SM, over shares of the units of equal estimated cost.
 // TMA row gathers (four rows an instruction) fetch Q, and the cluster's keys and values in steps
@@ -29,7 +29,7 @@
 // 900; rows listed beforehand instead of by the gathering warps 740; shares by cost, kept keys,
 // 16-bit parts and bulk stores 680; joins of four heads side by side 630; warpgroups of
 // their own for the output and loops kept rolled (the roles' unrolled code outgrew the
-// instruction cache) 490.
+// instruction cache) 490; parts of three bytes, whose columns may lie any factor apart, 550.
 #include <algorithm>
 #include <atomic>
 #include <numeric>
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
     const __grid_constant__ CUtensorMap tm_v, RowMap rk, RowMap rv, Args a,
     const int32_t* __restrict__ q_row, const int32_t* __restrict__ row_pos,
     const Unit* __restrict__ units, const int32_t* __restrict__ start, uint8_t* __restrict__ part_o,
-    float2* __restrict__ part_lse, float* __restrict__ part_scale, int* err) {
+    float2* __restrict__ part_lse, int* err) {
   using namespace ptx;
   using S = FwdSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -385,51 +385,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       tc_fence_after();
       const int64_t urow = static_cast<int64_t>(it.n) * kUnitRows + sub * kSub + row;
       const uint32_t buf = sb + S::kOut + (warp - 8) * 4096;
-      constexpr int kBytes = Part<T>::kBytes, kCols = 128 / kBytes;  // columns in 128 bytes
-      uint8_t* dst = part_o + (urow - lane) * (DP * kBytes);
-      float scale = 1.f;
-      if constexpr (Part<T>::kHalf) {
-        float big[4] = {0.f, 0.f, 0.f, 0.f};
+      uint8_t* dst = part_o + (urow - lane) * (DP * kPartBytes);
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(t_o + c * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], fabsf(__uint_as_float(o[j])));
-        }
-        // the row's largest value to [2^14, 2^15); a row that is not finite stays as it is
-        const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-        const int e =
-            top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -112) : 0;
-        scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        part_scale[urow] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      }
-#pragma unroll 1
-      for (int c = 0; c < DP / kCols; ++c) {
-        begin_segment();
-#pragma unroll
-        for (int x = 0; x < kCols / 32; ++x) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(t_o + c * kCols + x * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * scale);
-#pragma unroll
-          for (int j = 0; j < 8 * 32 / kCols; ++j) {
-            if constexpr (Part<T>::kHalf) {
-              uint32_t y[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                y[e] = mma::pack2<__half>(__uint_as_float(o[8 * j + 2 * e]),
-                                          __uint_as_float(o[8 * j + 2 * e + 1]));
-              put_piece(buf, x * 4 + j, make_uint4(y[0], y[1], y[2], y[3]));
-            } else {
-              put_piece(buf, j, make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
-            }
-          }
-        }
-        end_segment(buf, dst + c * 4096);
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_o + c * 32, o);
+        tmem_wait_ld();
+        put_segment(buf, o, dst + c * kSegment);
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.o_free[sub]));
@@ -595,11 +557,10 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
                                                          const int32_t* __restrict__ pair_row,
                                                          const uint8_t* __restrict__ part_o,
                                                          const float2* __restrict__ part_lse,
-                                                         const float* __restrict__ part_scale,
                                                          T* __restrict__ out,
                                                          float* __restrict__ lse,
                                                          int32_t* __restrict__ odd, int64_t warps) {
-  constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
+  constexpr int E = 8, SEGS = DP / 64;
   constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
   const int64_t w0 = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i - i0, heads)
@@ -616,7 +577,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
   for (int s0 = 0; s0 < a.top; s0 += kAhead * per) {
-    uint4 v[kAhead][SEGS];
+    Part8 v[kAhead][SEGS];
     float2 w[kAhead];
     float big = top;
 #pragma unroll
@@ -624,13 +585,10 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
       const int s = s0 + u * per + me.slot;
       const int64_t n = s < a.top && h < a.G ? pairs[s] : -1;
       w[u] = n >= 0 ? part_lse[n + h] : make_float2(-INFINITY, 0.f);
-      if (Part<T>::kHalf && n >= 0) w[u].y *= part_scale[n + h];
 #pragma unroll
       for (int g = 0; g < SEGS; ++g) {
-        v[u][g] = make_uint4(0, 0, 0, 0);
-        if (n >= 0)
-          v[u][g] = __ldcs(reinterpret_cast<const uint4*>(
-              part_o + part_at(n + h, g * 8 + me.piece, DP * kBytes)));
+        v[u][g] = Part8{};
+        if (n >= 0) v[u][g] = load_part<DP>(part_o, n + h, g * 8 + me.piece);
       }
     }
 #pragma unroll
@@ -648,7 +606,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
       const float p = exp2f(w[u].x - from);
       sum += p;
 #pragma unroll
-      for (int g = 0; g < SEGS; ++g) add_part<T, E>(acc[g], v[u][g], p * w[u].y);
+      for (int g = 0; g < SEGS; ++g) add_part(acc[g], v[u][g], p * w[u].y);
     }
   }
   for (int o = 8 * gp; o < 32; o <<= 1) {  // the slots' lanes
@@ -669,7 +627,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
 #pragma unroll
   for (int g = 0; g < SEGS; ++g) {
     const int d = (g * 8 + me.piece) * E;
-    if (d < a.D) store_out<T, E>(out + at * a.D + d, acc[g], inv);
+    if (d < a.D) store_out<T>(out + at * a.D + d, acc[g], inv);
   }
   float bad = 0.f;
 #pragma unroll
@@ -684,7 +642,7 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
 // (a round has its own grouping, so short ones cost launches), 64 queries at least.
 int64_t queries_per_round(const Args& a) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t per = R * a.top * a.G * ((a.D <= 64 ? 64 : 128) * 4 + 8);
+  const int64_t per = R * a.top * a.G * ((a.D <= 64 ? 64 : 128) * kPartBytes + 8);
   const int64_t most = std::max<int64_t>(64, (1ll << 31) / per);
   const int64_t rounds = (a.Nq + most - 1) / most;
   return (a.Nq + rounds - 1) / rounds;
@@ -692,11 +650,11 @@ int64_t queries_per_round(const Args& a) {
 
 struct Layout {
   UnitPlan plan;
-  size_t part_lse, part_scale, part_o, total;
+  size_t part_lse, part_o, total;
   int64_t nq;
 };
 
-Layout fwd_layout(const Args& a, int part_bytes, uint8_t* ws) {
+Layout fwd_layout(const Args& a, uint8_t* ws) {
   Layout l{};
   l.nq = queries_per_round(a);
   size_t at = carve_units(a, l.nq, false, ws, &l.plan);
@@ -706,18 +664,16 @@ Layout fwd_layout(const Args& a, int part_bytes, uint8_t* ws) {
     return p;
   };
   l.part_lse = take(l.plan.units_max * kUnitRows * 8);
-  l.part_scale = take(l.plan.units_max * kUnitRows * 4);
-  l.part_o = take(l.plan.units_max * kUnitRows * (a.D <= 64 ? 64 : 128) * part_bytes);
+  l.part_o = take(l.plan.units_max * kUnitRows * (a.D <= 64 ? 64 : 128) * kPartBytes);
   l.total = at;
   return l;
 }
 
 template <typename T, int DP>
 int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStream_t stream) {
-  const Layout l = fwd_layout(a, Part<T>::kBytes, ws);
+  const Layout l = fwd_layout(a, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   float2* part_lse = reinterpret_cast<float2*>(ws + l.part_lse);
-  float* part_scale = reinterpret_cast<float*>(ws + l.part_scale);
   uint8_t* part_o = ws + l.part_o;
   CUtensorMap tm_q, tm_k, tm_v;
   RowMap rq, rk, rv;
@@ -744,15 +700,15 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
                        static_cast<const int32_t*>(l.plan.q_row),
                        static_cast<const int32_t*>(l.plan.row_pos),
                        static_cast<const Unit*>(l.plan.units),
-                       static_cast<const int32_t*>(l.plan.start), part_o, part_lse, part_scale,
+                       static_cast<const int32_t*>(l.plan.start), part_o, part_lse,
                        device_error_word()));
     const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
     const int64_t warps = R * nq * chunks;
     FKC_TRY(launch_pdl(tiles_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256),
                        0, stream, a, static_cast<int>(i0), nq, gp, chunks,
                        static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse),
-                       static_cast<const float*>(part_scale), out, lse, l.plan.odd, warps));
+                       static_cast<const uint8_t*>(part_o), static_cast<const float2*>(part_lse), out,
+                       lse, l.plan.odd, warps));
   }
   return launch_again(a, dtype, l.plan.odd, lse, nullptr, nullptr, out, nullptr, nullptr, nullptr, nullptr, stream);
 }
@@ -872,7 +828,7 @@ bool tiles_fit(const Args& a, int64_t nq) {
     return false;
   // units that are not full take workspace too: no more than the full ones, or 2^31 bytes
   return pairs * a.G >= kSub * static_cast<int64_t>(a.K) ||
-         R * std::min<int64_t>(a.K, pairs) * kUnitRows * DP * 4 <= (1ll << 31);
+         R * std::min<int64_t>(a.K, pairs) * kUnitRows * DP * kPartBytes <= (1ll << 31);
 }
 
 // In us, fitted to calls with D = 128, 8 to 200 keys a cluster, 8 to 2048 rows a cluster and G
@@ -886,18 +842,14 @@ bool use_tiles(const Args& a) {
   const int64_t nq = queries_per_round(a), DP = a.D <= 64 ? 64 : 128;
   if (!tiles_fit(a, nq)) return false;
   // a round of few queries of very many sequences: its parts would be 2^32 bytes and more
-  if (static_cast<int64_t>(a.batch) * a.Hkv * nq * a.top * a.G * DP * 4 > (1ll << 32)) return false;
+  if (static_cast<int64_t>(a.batch) * a.Hkv * nq * a.top * a.G * DP * kPartBytes > (1ll << 32)) return false;
   const FormWork w = form_work(a, nq);
   const double walk = 18 + 75e-6 * w.reads;
   const double tiles = 34 + w.units * (0.009 + 0.000136 * w.keys) + 86e-6 * w.rows;
   return 1.1 * tiles < walk;
 }
 
-size_t tiles_forward_workspace_bytes(const Args& a, int dtype) {
-  return fwd_layout(a, dtype == FKC_DTYPE_F16 ? Part<__half>::kBytes : Part<__nv_bfloat16>::kBytes,
-                    nullptr)
-      .total;
-}
+size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a, nullptr).total; }
 
 int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* ws,
                          cudaStream_t stream) {

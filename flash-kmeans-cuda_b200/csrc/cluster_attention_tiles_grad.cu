@@ -3,7 +3,7 @@
 //
 //   dQ      (tiles_dq_kernel)   a unit's 128 rows against the cluster's keys in steps of 128:
 //           S = Q K^T and dP = dO V^T into TMEM, dS in place, dQ += dS K. A row leaves its
-//           gradient over that cluster as the forward leaves its output (Part), and
+//           gradient over that cluster as the forward leaves its output, and
 //           tiles_dq_join_kernel adds a query's top parts.
 //   dK, dV  (tiles_dkv_kernel)  128 keys of a cluster against the cluster's rows in steps of
 //           128: S^T = K Q^T and dP^T = V dO^T, P^T and dS^T in place, dV += P^T dO and
@@ -110,13 +110,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
     const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
     const float* __restrict__ row_delta, const Unit* __restrict__ units,
-    const int32_t* __restrict__ start, uint8_t* __restrict__ part, float* __restrict__ part_scale,
-    int* err) {
+    const int32_t* __restrict__ start, uint8_t* __restrict__ part, int* err) {
   using namespace ptx;
   using S = DqSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
-  constexpr int kBytes = Part<T>::kBytes, kCols = 128 / kBytes;  // columns in a segment
-  constexpr int kSegs = DP / kCols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t sb = smem_u32(smem);
@@ -218,49 +215,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
       tc_fence_after();
       const int64_t urow = it.row() + row;
       const uint32_t buf = sb + S::kOut + warp * 4096;
-      uint8_t* dst = part + (urow - lane) * (DP * kBytes);
-#pragma unroll
-      for (int c = 0; c < kSegs; ++c) {  // the segments are shared out
-        if ((kSegs == 1 ? 0 : c * 2 / kSegs) != half) continue;
-        float scale = a.scale, back = 1.f;
-        if constexpr (Part<T>::kHalf) {
-          float big[4] = {0.f, 0.f, 0.f, 0.f};
+      uint8_t* dst = part + (urow - lane) * (DP * kPartBytes);
 #pragma unroll 1
-          for (int x = 0; x < kCols / 32; ++x) {
-            float o[32];
-            tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], fabsf(o[j]));
-          }
-          // the segment's largest value to [2^14, 2^15); one that is not finite stays as it is
-          const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * fabsf(a.scale);
-          const int e =
-              top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -112) : 0;
-          scale *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          part_scale[urow * 2 + c] = back;
-        }
-        begin_segment();
-#pragma unroll 1
-        for (int x = 0; x < kCols / 32; ++x) {
-          float o[32];
-          tmem_ld_f32_x32(t_q + c * kCols + x * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] *= scale;
-#pragma unroll
-          for (int j = 0; j < 8 * 32 / kCols; ++j) {
-            if constexpr (Part<T>::kHalf)
-              put_piece(buf, x * 4 + j,
-                  make_uint4(mma::pack2<__half>(o[8 * j], o[8 * j + 1]), mma::pack2<__half>(o[8 * j + 2], o[8 * j + 3]),
-                             mma::pack2<__half>(o[8 * j + 4], o[8 * j + 5]), mma::pack2<__half>(o[8 * j + 6], o[8 * j + 7])));
-            else
-              put_piece(buf, j, make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
-                                           __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
-          }
-        }
-        end_segment(buf, dst + c * 4096);
+      for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {  // the segments are shared out
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_q + c * 32, o);
+        tmem_wait_ld();
+        put_segment(buf, o, dst + c * kSegment);
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&mt.dq_free));
@@ -411,15 +372,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
   }
 }
 
-// One warp per (query, GP heads): dq = the sum of its clusters' parts.
+// One warp per (query, GP heads): dq = scale * the sum of its clusters' parts.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int chunks,
                                                             const int32_t* __restrict__ pair_row,
                                                             const uint8_t* __restrict__ part,
-                                                            const float* __restrict__ part_scale,
                                                             T* __restrict__ dq, int32_t* __restrict__ odd,
                                                             int64_t warps) {
-  constexpr int kBytes = Part<T>::kBytes, E = 16 / kBytes, SEGS = DP * kBytes / 128;
+  constexpr int E = 8, SEGS = DP / 64;
   constexpr int kAhead = 8 / SEGS;  // slots in flight per lane
   pdl_wait();
   const int64_t w0 = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (r, i, heads)
@@ -436,25 +396,21 @@ __global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int 
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
   for (int s0 = 0; s0 < a.top; s0 += kAhead * per) {
-    uint4 v[kAhead][SEGS];
-    float f[kAhead][SEGS];
+    Part8 v[kAhead][SEGS];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int s = s0 + u * per + me.slot;
       const int64_t n = s < a.top && h < a.G ? pairs[s] : -1;
 #pragma unroll
       for (int g = 0; g < SEGS; ++g) {
-        v[u][g] = make_uint4(0, 0, 0, 0);
-        f[u][g] = 0.f;
-        if (n < 0) continue;
-        v[u][g] = __ldcs(reinterpret_cast<const uint4*>(part + part_at(n + h, g * 8 + me.piece, DP * kBytes)));
-        f[u][g] = Part<T>::kHalf ? part_scale[(n + h) * 2 + g] : 1.f;
+        v[u][g] = Part8{};
+        if (n >= 0) v[u][g] = load_part<DP>(part, n + h, g * 8 + me.piece);
       }
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int g = 0; g < SEGS; ++g) add_part<T, E>(acc[g], v[u][g], f[u][g]);
+      for (int g = 0; g < SEGS; ++g) add_part(acc[g], v[u][g], 1.f);
   }
   for (int o = 8 * gp; o < 32; o <<= 1)  // the slots' lanes
 #pragma unroll
@@ -466,7 +422,7 @@ __global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int 
 #pragma unroll
   for (int g = 0; g < SEGS; ++g) {
     const int d = (g * 8 + me.piece) * E;
-    if (d < a.D) store_out<T, E>(out + d, acc[g], 1.f);
+    if (d < a.D) store_out<T>(out + d, acc[g], a.scale);
   }
   float bad = 0.f;
 #pragma unroll
@@ -985,10 +941,10 @@ __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTi
 
 struct GradLayout {
   UnitPlan plan;
-  size_t part, scales, first, tiles, share, start, dkv_part, total;
+  size_t part, first, tiles, share, start, dkv_part, total;
 };
 
-GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
+GradLayout grad_layout(const Args& a, uint8_t* ws) {
   GradLayout l{};
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t DP = a.D <= 64 ? 64 : 128;
@@ -998,8 +954,7 @@ GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
     at += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  l.part = take(l.plan.units_max * kUnitRows * DP * part_bytes);
-  l.scales = take(l.plan.units_max * kUnitRows * 8);
+  l.part = take(l.plan.units_max * kUnitRows * DP * kPartBytes);
   l.first = take(R * 16);
   l.tiles = take(R * row_tiles_max(a.K, a.N) * static_cast<int64_t>(sizeof(KeyTile)));
   l.share = take((kMaxCtas + 1) * 8);
@@ -1012,7 +967,7 @@ GradLayout grad_layout(const Args& a, int part_bytes, uint8_t* ws) {
 template <typename T, int DP>
 int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, const T* dout, T* dq, T* dk,
                T* dv, int32_t* odd, uint8_t* ws, cudaStream_t stream) {
-  const GradLayout l = grad_layout(a, Part<T>::kBytes, ws);
+  const GradLayout l = grad_layout(a, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   CUtensorMap tm_q, tm_k, tm_v, tm_do;
   RowMap rq, rk, rv, rdo;
@@ -1029,15 +984,14 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
     auto kern = tiles_dq_kernel<T, DP>;
     const int smem = static_cast<int>(DqSmem<DP>::kBytes);
     FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    float* scales = reinterpret_cast<float*>(ws + l.scales);
     FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                        q_row, do_row, pos, row_lse, row_delta, static_cast<const Unit*>(l.plan.units),
-                       static_cast<const int32_t*>(l.plan.start), ws + l.part, scales, device_error_word()));
+                       static_cast<const int32_t*>(l.plan.start), ws + l.part, device_error_word()));
     const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
     const int64_t warps = R * a.Nq * chunks;
     FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0,
                        stream, a, gp, chunks, static_cast<const int32_t*>(l.plan.pair_row),
-                       static_cast<const uint8_t*>(ws + l.part), static_cast<const float*>(scales), dq, odd, warps));
+                       static_cast<const uint8_t*>(ws + l.part), dq, odd, warps));
   }
   if (dk == nullptr)
     return launch_again(a, dtype, odd, lse, delta, dout, dq, nullptr, nullptr, nullptr, nullptr, stream);
@@ -1095,14 +1049,11 @@ bool use_tiles_grad(const Args& a) {
   if (1.1 * tiles >= walk) return false;
   // all queries at once: 32-bit rows of units, and parts of 2^33 bytes at most
   const int64_t rows = static_cast<int64_t>(a.batch) * a.Hkv * (static_cast<int64_t>(a.Nq) * a.top * a.G + static_cast<int64_t>(a.K) * kUnitRows);
-  return rows <= (1ll << 30) && rows * (a.D <= 64 ? 64 : 128) * 4 <= (1ll << 33) &&
+  return rows <= (1ll << 30) && rows * (a.D <= 64 ? 64 : 128) * kPartBytes <= (1ll << 33) &&
          static_cast<int64_t>(a.Nq) * a.top * a.G <= (1ll << 30);
 }
 
-size_t tiles_backward_workspace_bytes(const Args& a, int dtype) {
-  return grad_layout(a, dtype == FKC_DTYPE_F16 ? Part<__half>::kBytes : Part<__nv_bfloat16>::kBytes, nullptr)
-      .total;
-}
+size_t tiles_backward_workspace_bytes(const Args& a) { return grad_layout(a, nullptr).total; }
 
 int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
                           void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream) {

@@ -197,7 +197,7 @@ FKC_CAPI_EXPORT int fkc_cluster_select(const fkc_attention_desc* desc, const voi
 FKC_CAPI_EXPORT size_t fkc_cluster_attention_workspace_size(const fkc_attention_desc* desc) {
   attn::Args a;
   if (fill_args(desc, true, &a) != FKC_OK) return 0;
-  return attn::forward_workspace_bytes(a, desc->dtype);
+  return attn::forward_workspace_bytes(a);
 }
 
 FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* out, float* lse,
@@ -209,7 +209,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* 
   FKC_REQUIRE(out != nullptr && lse != nullptr, "out and lse must be non-null");
   FKC_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15u) == 0, "out must be 16-byte aligned");
   FKC_TRY(check_workspace("attention", workspace, workspace_bytes,
-                          attn::forward_workspace_bytes(a, desc->dtype)));
+                          attn::forward_workspace_bytes(a)));
   FKC_TRY(check_device());
   return attn::launch_forward(a, desc->dtype, out, lse, workspace, as_stream(stream));
 }
@@ -217,7 +217,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* 
 FKC_CAPI_EXPORT size_t fkc_cluster_attention_grad_workspace_size(const fkc_attention_desc* desc) {
   attn::Args a;
   if (fill_args(desc, true, &a) != FKC_OK) return 0;
-  return attn::backward_workspace_bytes(a, desc->dtype);
+  return attn::backward_workspace_bytes(a);
 }
 
 FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, const void* out,
@@ -235,7 +235,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, c
     FKC_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15u) == 0,
                 "out, dout and the gradients must be 16-byte aligned");
   FKC_TRY(check_workspace("attention gradient", workspace, workspace_bytes,
-                          attn::backward_workspace_bytes(a, desc->dtype)));
+                          attn::backward_workspace_bytes(a)));
   FKC_TRY(check_device());
   return attn::launch_backward(a, desc->dtype, out, lse, dout, dq, dk, dv, workspace,
                                as_stream(stream));

@@ -107,32 +107,77 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, const uint4& v) {
                : "memory");
 }
 
-// What the units' rows leave for the join, one row of `bytes` per (unit, row), is stored as the
-// warps write it: per 32 rows, segments of 128 bytes of each row (4 KB), whose 16-byte pieces
-// are xored with the row's low bits as in the operand tiles. Byte offset of piece j (16 bytes)
-// of row n of all units' rows:
-__device__ __forceinline__ int64_t part_at(int64_t n, int j, int bytes) {
-  const int r = static_cast<int>(n & 31);
-  return (n >> 5) * (32 * bytes) + (j >> 3) * 4096 + r * 128 + (((j & 7) ^ (r & 7)) << 4);
+// What the units' rows leave for the join: a row's output over one cluster, in 24 bits a value (the
+// upper three bytes of its fp32). Sign and exponent are whole, so that columns of a row may lie any
+// factor apart, infinities beside them; what is dropped is at most 2^-16 of the value, against the
+// 2^-12 that the last rounding of out may take from it (2^-9 with bf16). In 16 bits (fp16 under a power
+// of two of the row's own) a column 2^-39 of the row's largest was lost; 4 bytes a value cost the prompt
+// of cluster_attention_tiles.cu 90 us more than 2 did.
+//
+// 32 rows are stored as the warps write them, in segments of 32 columns (3 KB): the rows' upper halves,
+// 64 bytes a row, then their third bytes, 32 a row. The 16-byte pieces of a row are permuted by the
+// row's number, so that eight lanes that store a piece each meet different banks.
+constexpr int kPartBytes = 3;
+constexpr int kSegment = 32 * 32 * kPartBytes;
+__device__ __forceinline__ uint32_t part_hi(int r, int j) {  // 16-byte piece j of the upper halves
+  return static_cast<uint32_t>(r * 64 + ((j ^ (r >> 1 & 3)) << 4));
 }
-// One segment: lane l's 128 bytes of row l, to 4 KB at dst, through the warp's buffer; the copy
-// goes on while the warp does other things (the stores themselves, 16 bytes a lane to
-// rows or to whole lines alike, held the warps for some 170 cycles each). begin, eight
-// pieces, end.
-__device__ __forceinline__ void begin_segment() {
-  if ((threadIdx.x & 31) == 0) ptx::bulk_wait_read();  // the buffer's last copy
-  __syncwarp();
+__device__ __forceinline__ uint32_t part_lo(int r, int j) {  // of the third bytes
+  return static_cast<uint32_t>(2048 + r * 32 + ((j ^ (r >> 2 & 1)) << 4));
 }
-__device__ __forceinline__ void put_piece(uint32_t buf, int j, const uint4& v) {
+// One segment: the lane's 32 values of its row, to dst through the warp's buffer; the copy goes on while
+// the warp does other things (the stores themselves, 16 bytes a lane to rows or to whole lines
+// alike, held the warps for some 170 cycles each).
+__device__ __forceinline__ void put_segment(uint32_t buf, const uint32_t (&v)[32], uint8_t* dst) {
   const int lane = threadIdx.x & 31;
-  st_shared_v4(buf + lane * 128 + ((j ^ (lane & 7)) << 4), v);
-}
-__device__ __forceinline__ void end_segment(uint32_t buf, uint8_t* dst) {
+  if (lane == 0) ptx::bulk_wait_read();  // the buffer's last copy
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __byte_perm(v[8 * j + 2 * e], v[8 * j + 2 * e + 1], 0x7632);
+    st_shared_v4(buf + part_hi(lane, j), make_uint4(y[0], y[1], y[2], y[3]));
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 16 * j + 4 * e;
+      y[e] = __byte_perm(__byte_perm(v[c], v[c + 1], 0x51), __byte_perm(v[c + 2], v[c + 3], 0x51), 0x5410);
+    }
+    st_shared_v4(buf + part_lo(lane, j), make_uint4(y[0], y[1], y[2], y[3]));
+  }
   ptx::fence_proxy_async_smem();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) {
-    ptx::bulk_store(dst, buf, 4096);
+  if (lane == 0) {
+    ptx::bulk_store(dst, buf, kSegment);
     ptx::bulk_commit();
+  }
+}
+// Eight columns of a row, from column 8 * j on, as a lane of the joins reads them.
+struct Part8 {
+  uint4 hi;
+  uint2 lo;
+};
+template <int DP>
+__device__ __forceinline__ Part8 load_part(const uint8_t* parts, int64_t n, int j) {
+  const int r = static_cast<int>(n & 31);
+  const uint8_t* seg = parts + (n >> 5) * (32 * DP * kPartBytes) + (j >> 2) * kSegment;
+  Part8 p;
+  p.hi = __ldcs(reinterpret_cast<const uint4*>(seg + part_hi(r, j & 3)));
+  p.lo = __ldcs(reinterpret_cast<const uint2*>(seg + part_lo(r, (j & 3) >> 1) + (j & 1) * 8));
+  return p;
+}
+// acc += f * the values. The byte that was dropped is filled with the one before it, which keeps
+// zeros and infinities what they are and whose mean is that of the byte.
+__device__ __forceinline__ void add_part(float (&acc)[8], const Part8& p, float f) {
+  const uint32_t hi[4] = {p.hi.x, p.hi.y, p.hi.z, p.hi.w}, lo[2] = {p.lo.x, p.lo.y};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = 4 + (e & 3), h = (e & 1) * 2;
+    acc[e] = fmaf(f, __uint_as_float(__byte_perm(hi[e >> 1], lo[e >> 2], (h + 1) << 12 | h << 8 | b << 4 | b)), acc[e]);
   }
 }
 
@@ -261,20 +306,11 @@ struct UnitIter {
   }
 };
 
-// A part's output over one cluster as stored: fp32, or for bf16 inputs fp16 values under a
-// power of two of the row's own. Two of its roundings of 2^-11 stay far below the 2^-8
-// of out, and the parts are most of what the two kernels move.
-template <typename T>
-struct Part {
-  static constexpr bool kHalf = !std::is_same<T, __half>::value;
-  static constexpr int kBytes = kHalf ? 2 : 4;
-};
-
 // How a warp of the joins reads the parts of GP neighbouring heads of a query (the largest power
-// of two up to 4 and G): eight lanes take 128 bytes of a head's row, GP heads side by side, so
-// that a load covers 128 * GP bytes that lie together, and 4 / GP slots of sel at once.
+// of two up to 4 and G): eight lanes take 64 columns of a head's row, GP heads side by side, and 4 / GP
+// slots of sel at once.
 struct JoinLane {
-  int piece, head, slot;  // of 16 bytes; of the heads; of the slots
+  int piece, head, slot;  // of 8 columns; of the heads; of the slots
   __device__ __forceinline__ JoinLane(int gp) {
     const int lane = threadIdx.x & 31;
     piece = lane & 7;
@@ -283,32 +319,13 @@ struct JoinLane {
   }
 };
 inline int join_heads(int G) { return G >= 4 ? 4 : G >= 2 ? 2 : 1; }
-// The values in 16 bytes of a part, times f, added to acc.
-template <typename T, int E>
-__device__ __forceinline__ void add_part(float (&acc)[E], const uint4& v, float f) {
-  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-  if constexpr (Part<T>::kHalf) {
+// Eight values times f, rounded to T.
+template <typename T>
+__device__ __forceinline__ void store_out(T* out, const float (&v)[8], float f) {
+  uint32_t y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 y = mma::unpack2<__half>(x[e]);
-      acc[2 * e] += f * y.x;
-      acc[2 * e + 1] += f * y.y;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += f * __uint_as_float(x[e]);
-  }
-}
-// E values rounded to T.
-template <typename T, int E>
-__device__ __forceinline__ void store_out(T* out, const float (&v)[E], float f) {
-  uint32_t y[E / 2];
-#pragma unroll
-  for (int e = 0; e < E / 2; ++e) y[e] = mma::pack2<T>(v[2 * e] * f, v[2 * e + 1] * f);
-  if constexpr (E == 8)
-    *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
-  else
-    *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[1]);
+  for (int e = 0; e < 4; ++e) y[e] = mma::pack2<T>(v[2 * e] * f, v[2 * e + 1] * f);
+  *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
 }
 
 }  // namespace attn

@@ -719,3 +719,38 @@ def test_many_queries_offsets_of_no_grouping(clusters):
             close(x[:, rows], val[name][:, rows], tol[name][:, rows], name)
         assert x.isfinite().all()
     assert got["dk"][:, 1].eq(0).all() and got["dv"][:, 1].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_queries_columns_stand_alone(clusters, dtype, D, causal):
+    """One column holds infinities and others lie far apart: each keeps the accuracy of its own last
+    rounding, 2**-8 of a bf16 column's norm at most (2**-11 fp16), P and dS rounded as much once more."""
+    q, k, v, sel, order, offsets, pos = attention_case(2, 1, 4, 1000, 1500, 15, D, 5, dtype, seed=5, causal=causal, drop=0.0)
+    u = torch.finfo(dtype).eps / 2
+    wide = 50 if dtype == BF else 10
+    power = torch.exp2(torch.randint(-wide, wide + 1, (D,), generator=gen(8), device="cuda").float())
+    power[:2] = 1.0
+    q[..., 2::2] = 0  # the scores come from the other half: columns of k there may be anything
+    k[..., 2::2] = (k[..., 2::2].float() * power[2::2]).to(dtype)
+    dout = torch.where(power == 1.0, randn(*q.shape, seed=9), torch.zeros((), device="cuda")).to(dtype)
+    v = (v.float() * power).to(dtype)
+    val, _ = attention_ref(q, k, v, sel, order, offsets, pos, None, dout)
+    dout[..., 0] = 0
+    val["dq"] = attention_ref(q, k, v, sel, order, offsets, pos, None, dout)[0]["dq"]
+    holed = v.clone()
+    holed[:, :, 700:1300:3, 0] = math.inf
+    a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    (dq,) = torch.autograd.grad(clusters.cluster_attention(*a, sel, order, offsets, q_pos=pos), a[0], dout)
+    out = clusters.cluster_attention(q, k, holed, sel, order, offsets, q_pos=pos)
+
+    def columns(got, want, what):
+        off, norm = ((x.double() ** 2).sum((0, 1, 2)).sqrt() for x in (got.double() - want, want))
+        step = {BF: 0.0, HF: 2.0 ** -25}[dtype] * math.sqrt(want[..., 0].numel())  # fp16's smallest values
+        assert (off <= 2 * u * norm + step).all(), (what, (off / norm).tolist())
+
+    columns(out[..., 1:], val["out"][..., 1:], "out")
+    columns(dq, val["dq"], "dq")
+    read = reads(sel, order, offsets, pos, 1)[:, :, 700:1300:3].any(-1)[:, None].expand(out.shape[:3])
+    assert out[..., 0][read].eq(math.inf).all() and out[..., 0][~read].isfinite().all()
