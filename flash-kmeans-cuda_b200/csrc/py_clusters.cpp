@@ -109,6 +109,13 @@ void need_first_order(const char* what) {
        " is differentiable once: its gradient has no graph (create_graph)");
 }
 
+// A tangent of torch.autograd.forward_ad would be dropped here without a word, which reads as a
+// derivative of zero.
+void need_no_tangent(const Tensor& t, const char* what) {
+  need(!t._fw_grad(/*level=*/0).defined(), what,
+       " has no forward-mode derivative: an input carries a tangent");
+}
+
 class Lookup : public torch::autograd::Function<Lookup> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids,
@@ -143,6 +150,7 @@ class Lookup : public torch::autograd::Function<Lookup> {
 };
 
 Tensor cluster_lookup(const Tensor& table, const Tensor& ids, double scale) {
+  need_no_tangent(table, "cluster_lookup");
   need_cuda(table, "table");
   need_on(ids, "ids", table);
   dtype_code(table);
@@ -382,6 +390,7 @@ std::tuple<Tensor, Tensor> cluster_attention(const Tensor& q, const Tensor& k, c
                                              const Tensor& sel, const Tensor& order,
                                              const Tensor& offsets, std::optional<Tensor> q_pos,
                                              std::optional<double> scale) {
+  for (const Tensor* t : {&q, &k, &v}) need_no_tangent(*t, "cluster_attention");
   check_q(q);
   const double sc = scale_of(q, scale);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {

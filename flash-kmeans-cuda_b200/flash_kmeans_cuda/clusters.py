@@ -48,8 +48,9 @@ def cluster_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -
     (B, N), giving (B, N, D): float16, bfloat16 or float32. ids are int32 or int64; one outside
     [0, K) gives a row of zeros and no gradient. The product is formed in float32 and rounded
     once; the gradient ``dtable[k] = scale * sum of dy[n] where ids[n] == k`` is summed in float32
-    in ascending n and rounded once. The gradient itself has no graph: a backward pass with
-    ``create_graph=True`` raises ``RuntimeError``.
+    (in ascending n, of large clusters block by block) and rounded once. The gradient itself has no
+    graph: a backward pass with ``create_graph=True`` raises ``RuntimeError``, and so does a table with
+    a forward-mode tangent.
     """
     return _C.cluster_lookup(table, ids, scale)
 
@@ -108,9 +109,9 @@ def cluster_attention(
 
     Returns out like q (contiguous) and, with ``return_lse``, the float32 log of each row's sum of
     exponentials (batch, q_heads, n_queries), which joins attention over several sets of keys. A
-    query that sees no key gets zeros and -inf. Differentiable in q, k and v (not through lse);
-    the gradient itself has no graph: a backward pass with ``create_graph=True`` raises
-    ``RuntimeError``.
+    query that sees no key gets zeros and -inf. Differentiable in q, k and v, but not through lse: such
+    a join has no gradient. The gradient itself has no graph: a backward pass with
+    ``create_graph=True`` raises ``RuntimeError``, and so does an input with a forward-mode tangent.
     """
     out, lse = _C.cluster_attention(q, k, v, sel, order, offsets, q_pos, scale)
     return (out, lse) if return_lse else out

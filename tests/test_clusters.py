@@ -135,3 +135,17 @@ def test_cpu_tensors_are_refused():
         clusters.cluster_select(q, t[None], ids, 2)
     with pytest.raises(ValueError, match="CUDA"):
         clusters.cluster_attention(q, q, q, ids[None], ids, ids)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor that does not require grad too: its tangent would be dropped, a derivative of zero."""
+    t = torch.zeros(4, 8, dtype=torch.float16)
+    q = torch.zeros(1, 1, 1, 8, dtype=torch.float16)
+    ids = torch.zeros(1, 4, dtype=torch.int32)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            clusters.cluster_lookup(torch.autograd.forward_ad.make_dual(t, t), ids)
+        d = torch.autograd.forward_ad.make_dual(q, q)
+        for args in ((d, q, q), (q, d, q), (q, q, d)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                clusters.cluster_attention(*args, ids[None], ids, ids)

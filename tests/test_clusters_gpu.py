@@ -754,3 +754,18 @@ def test_many_queries_columns_stand_alone(clusters, dtype, D, causal):
     columns(dq, val["dq"], "dq")
     read = reads(sel, order, offsets, pos, 1)[:, :, 700:1300:3].any(-1)[:, None].expand(out.shape[:3])
     assert out[..., 0][read].eq(math.inf).all() and out[..., 0][~read].isfinite().all()
+
+
+def test_forward_mode_tangents_are_refused(clusters):
+    q, k, v, sel, order, offsets, pos = attention_case(1, 1, 2, 4, 30, 3, 16, 2, BF)
+    t, ids = randn(5, 8), torch.tensor([1, 4], device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda x: torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for x in (t, t.detach().requires_grad_(True)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                clusters.cluster_lookup(dual(x), ids)
+        for i in range(3):
+            args = [dual(x) if i == j else x for j, x in enumerate((q, k, v))]
+            with pytest.raises(RuntimeError, match="tangent"):
+                clusters.cluster_attention(*args, sel, order, offsets)
+        assert torch.equal(clusters.cluster_lookup(t, ids), t[ids])
