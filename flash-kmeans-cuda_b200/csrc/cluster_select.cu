@@ -22,7 +22,9 @@
 // How far an fp32 score can be off: a product of two 16-bit values is exact in fp32;
 // adding D of them with truncation to 2^-22 of the largest magnitude so far, none of
 // which exceeds |q||c|, is off by at most D * 2^-22 |q||c|; the two roundings of scale
-// and the rounding of the sum with bias add 2^-22 (scale |q||c| + |score|) at most.
+// and the rounding of the sum with bias add 2^-22 (scale |q||c| + |score|) at most. Squares and
+// products that underflow are covered by the least norm that counts, 2^-50: its square is more than
+// 128 squares below 2^-126 can lose, and D * 2^-22 of two such norms more than D products can.
 //
 // The scores go through memory (4 bytes a score, L2 at the usual sizes). 4096 queries x 256
 // clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 55 us (three CTAs an SM; it was 70 with
@@ -55,7 +57,10 @@ struct SelectArgs {
   const float* bias;  // (R, K) or null
   int Hkv, G, Nq, N, K, top, D;
   double scale;
+  double unsure;  // how far a score can be off, of |q||c|
 };
+
+constexpr float kLeastNorm2 = 0x1p-100f;  // squares of smaller values underflow (see the top)
 
 __device__ __forceinline__ float fold_max(float a, float b) {
   return (isnan(a) || isnan(b)) ? INFINITY : fmaxf(a, b);  // a NaN norm counts as unbounded
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
   }
   if (!PACK && norms && t4 < 2) {
     const int i = i0 + wq * 16 + t4 * 8 + g;
-    if (i < a.Nq) q_norm[static_cast<int64_t>(r) * a.Nq + i] = sqrtf(t4 == 0 ? qn[0] : qn[1]);
+    if (i < a.Nq) q_norm[static_cast<int64_t>(r) * a.Nq + i] = sqrtf(fmaxf(t4 == 0 ? qn[0] : qn[1], kLeastNorm2));
   }
   if constexpr (PACK) {
     __syncthreads();
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
     if (tile == 0 && tid < a.Nq) {
       float m = 0.f;
       for (int h = 0; h < a.G; ++h) m = fold_max(m, s_pack[tid * a.G + h]);
-      q_norm[static_cast<int64_t>(r) * a.Nq + tid] = sqrtf(m);
+      q_norm[static_cast<int64_t>(r) * a.Nq + tid] = sqrtf(fmaxf(m, kLeastNorm2));
     }
     __syncthreads();
 #pragma unroll
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
     __syncthreads();
     if (tid == 0)
       c_norm[static_cast<int64_t>(r) * ctiles + tile] =
-          sqrtf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
+          sqrtf(fmaxf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), kLeastNorm2));
   }
   const float scale = static_cast<float>(a.scale);
   if constexpr (PACK) {
@@ -301,9 +306,8 @@ __device__ double exact_score(const SelectArgs& a, int r, int i, int c) {
 // The band around the top-th score t in which fp32 cannot tell; infinite where a
 // norm or the score is not finite.
 __device__ __forceinline__ float band_of(const SelectArgs& a, float t, float qn, float cn) {
-  const float mag = static_cast<float>(fabs(a.scale)) * qn * cn;
-  const float eps = mag * (static_cast<float>(a.D) * 0x1p-22f + 0x1p-21f) + fabsf(t) * 0x1p-22f;
-  return eps < INFINITY ? 2.f * eps : INFINITY;
+  const float eps = static_cast<float>(a.unsure * qn * cn) + fabsf(t) * 0x1p-22f;
+  return eps < INFINITY ? 2.f * (eps + 0x1p-126f) : INFINITY;  // the least: scores that underflow
 }
 
 __device__ __forceinline__ float largest_norm(const float* c_norm, int64_t r, int ctiles) {
@@ -715,6 +719,8 @@ int launch_select(const Args& f, const void* centroids, const float* bias, doubl
   a.top = f.top;
   a.D = f.D;
   a.scale = scale;
+  // (a scale below fp32's least normal number is off by 2^-150 itself)
+  a.unsure = std::max(std::fabs(scale), 0x1p-126) * (f.D * 0x1p-22 + 0x1p-21);
   const int64_t R = static_cast<int64_t>(f.batch) * f.Hkv;
   uint8_t* w = static_cast<uint8_t*>(ws);
   return dtype == FKC_DTYPE_F16 ? select_dtype<__half>(a, R, w, sel, stream)

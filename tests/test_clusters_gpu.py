@@ -200,6 +200,24 @@ def test_select_ties_and_borders(clusters, K):
     assert torch.equal(got, select_ref(qq, big, offsets, 17))
 
 
+@pytest.mark.parametrize("K,Nq", [(90, 5), (90, 700), (700, 700), (3000, 5)])
+@pytest.mark.parametrize("small", ["neither", "queries", "centroids"])
+def test_select_squares_that_underflow(clusters, K, Nq, small):
+    """Queries or centroids whose squares are below fp32's range: a pair of products of 2**-16 cancels and
+    takes the product of 2**-48 that decides with it, and what fp32 keeps is in another order."""
+    q, cen = torch.zeros(1, 1, Nq, 32, device="cuda"), torch.zeros(1, K, 32, device="cuda")
+    first, second = (torch.randperm(K, generator=gen(i), device="cuda") % 64 + 1 for i in (1, 2))
+    a, b = {"neither": (2.0 ** -8, 2.0 ** -8), "queries": (2.0 ** -78, 2.0 ** 62), "centroids": (2.0 ** 62, 2.0 ** -78)}[small]
+    q[..., :2], cen[..., 0], cen[..., 1] = a, b, -b
+    q[..., 2] = q[..., 20] = a if small == "queries" else a * 2.0 ** -32
+    b = b * 2.0 ** -32 if small == "queries" else b
+    cen[..., 2], cen[..., 20] = first * b, second * b * 2.0 ** -8
+    q, cen = q.to(BF), cen.to(BF)
+    _, _, offsets = key_clusters(1, 50 * K, K, 3)
+    got = clusters.cluster_select(q, cen, offsets, K // 4)
+    assert torch.equal(got, select_ref(q, cen, offsets, K // 4))
+
+
 def test_select_many_queries(clusters):
     """More queries than warps at once, with ties, near ties and masks among them."""
     q = (randn(1, 4, 7001, 32, seed=1) * 2).round().div(2).to(BF)
