@@ -142,16 +142,16 @@ int launch_tiles_forward(const Args& a, int dtype, void* out, float* lse, void* 
                          cudaStream_t stream);
 bool use_tiles_grad(const Args& a);
 size_t tiles_backward_workspace_bytes(const Args& a);
-int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
-                          void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream);
+int launch_tiles_backward(const Args& a, int dtype, const float* lse, float* delta, const void* dout,
+                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
 // After the kernels above, where they set *odd: results that are not finite, from what their rows
 // see alone (cluster_masked.cu). Forward: rows is out. Gradients (dout given): rows is dq.
 int launch_again(const Args& a, int dtype, const int32_t* odd, const float* lse, const float* delta,
                  const void* dout, void* rows, const int32_t* inv_order, const int32_t* inv_offsets,
                  void* dk, void* dv, cudaStream_t stream);
 size_t backward_workspace_bytes(const Args& a);
-int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
-                    void* dq, void* dk, void* dv, void* ws, cudaStream_t stream);
+int launch_backward(const Args& a, int dtype, const float* lse, const void* dout, void* dq,
+                    void* dk, void* dv, void* ws, cudaStream_t stream);
 
 }  // namespace attn
 }  // namespace fkc

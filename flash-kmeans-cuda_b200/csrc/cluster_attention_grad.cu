@@ -1,15 +1,16 @@
 // Gradients of attention over selected clusters. With P = exp(scale S - lse) and
-// delta = rowsum(dout * out) per query and head,
+// delta = rowsum(dout * out) = rowsum(P dP) per query and head,
 //
 //   dV = P^T dout,  dP = dout V^T,  dS = scale P (dP - delta),  dQ = dS K,  dK = dS^T Q.
 //
-//   delta  (attn_delta_kernel)  one warp per query and head.
 //   dQ     (attn_dq_kernel)     the forward's walk: one warp per query and group, keys and
 //          values gathered in tiles of 16, S^T and dP^T formed transposed, dQ^T += K^T dS^T.
-//          It walks twice, first for delta = sum of P dP: keys of one cluster lie close to one
-//          another, so that what a rounded delta is off by adds up over them (dS no longer sums to
-//          zero). With delta from the 16-bit out, dQ of one cluster of 30 keys was off by
-//          0.0051 of its norm, with four clusters a query by 0.0026; its own rounding is 0.0017.
+//          It walks twice, first for delta = sum of P dP (all that is done where dQ is not wanted): keys
+//          lie close to one another within a cluster, and a cache's have offsets in common, so that
+//          what a rounded delta is off by adds up over them (dS no longer sums to zero). With delta
+//          from the 16-bit out, dQ of one cluster of 30 keys was off by 0.0051 of its norm, of 8
+//          clusters of 64 keys with a common offset ten times their spread by 0.019; its own rounding
+//          is 0.0017, and that is what is left.
 //   dK, dV (attn_dkv_kernel)    one CTA per 64 keys of a cluster, whose keys and values stay in
 //          shared memory. The queries that selected the cluster come from the same grouping
 //          that orders the keys (sel as ids: entry e is query e / top), their heads side by
@@ -21,7 +22,7 @@
 // type demands, dS into two terms: a row of dQ sums few large dS, and with one term its
 // error against 64 bits was 1.7 times that of its own last rounding, with two 1.2 times (the
 // walk waits for its gather, the second product is free). Sums are fp32 and rounded once on the
-// way out. delta of dK comes from the 16-bit out (dK sums over queries, which are not alike). Keys in no cluster get zeros.
+// way out. Keys in no cluster get zeros.
 //
 // Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
 // of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
@@ -49,32 +50,11 @@ __host__ __device__ constexpr int warp_smem(int top) {
   return ring_bytes<DP, STAGES>() + ((STAGES * 4 + (2 * top + 1) * 4 + 15) / 16) * 16;
 }
 
-// out and dout of one (sequence, head, query), contiguous rows of D.
-template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const T* __restrict__ out,
-                                                         const T* __restrict__ dout,
-                                                         float* __restrict__ delta, int D,
-                                                         int32_t* odd, int64_t rows) {
-  pdl_wait();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *odd = 0;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  float s = 0.f;
-  for (int d = lane * 4; d < D; d += 128) {
-    const uint2 x = *reinterpret_cast<const uint2*>(out + row * D + d);
-    const uint2 y = *reinterpret_cast<const uint2*>(dout + row * D + d);
-    const float2 x0 = mma::unpack2<T>(x.x), x1 = mma::unpack2<T>(x.y);
-    const float2 y0 = mma::unpack2<T>(y.x), y1 = mma::unpack2<T>(y.y);
-    s += x0.x * y0.x + x0.y * y0.y + x1.x * y1.x + x1.y * y1.y;
-  }
-  s = warp_sum(s);
-  if (lane == 0) delta[row] = s;
-}
-
+// dq may be null: delta alone.
 template <typename T, int DP, int NT, int STAGES>
 __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* __restrict__ dout,
                                                               const float* __restrict__ lse,
+                                                              float* __restrict__ delta,
                                                               T* __restrict__ dq, int chunks,
                                                               int64_t units) {
   constexpr int KS = DP / 16;
@@ -247,7 +227,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
         d += __shfl_xor_sync(0xFFFFFFFFu, d, 8);
         d += __shfl_xor_sync(0xFFFFFFFFu, d, 16);
         dl[n][e] = d;
+        const int h = n * 8 + t4 * 2 + e;
+        if (g == 0 && h < heads) delta[flat(h)] = d;
       }
+    if (dq == nullptr) return;
   }
   }
 #pragma unroll
@@ -268,9 +251,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
 }
 
 // tile_off[r, c]: first key tile of cluster c among the row's; tile_off[r, K]: their number.
-__global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, int32_t* __restrict__ tile_off) {
+__global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, int32_t* __restrict__ tile_off,
+                                                         int32_t* odd) {
   __shared__ int warp_total[32];
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *odd = 0;
   const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int32_t* out = tile_off + static_cast<int64_t>(r) * (a.K + 1);
   int carry = 0;
@@ -553,12 +538,12 @@ GradLayout grad_layout(const Args& a) {
     return p;
   };
   l.delta = take(static_cast<size_t>(a.batch) * a.Hq * a.Nq * 4);
-  l.odd = take(4);
   if (use_tiles_grad(a)) {
     l.tiles = take(tiles_backward_workspace_bytes(a));
     l.total = at;
     return l;
   }
+  l.odd = take(4);
   l.inv_order = take(static_cast<size_t>(R) * a.Nq * a.top * 4);
   l.inv_offsets = take(static_cast<size_t>(R) * (a.K + 1) * 4);
   l.tile_off = take(static_cast<size_t>(R) * (a.K + 1) * 4);
@@ -568,7 +553,7 @@ GradLayout grad_layout(const Args& a) {
 }
 
 template <typename T, int DP, int NT>
-int dq_typed(const Args& a, const T* dout, const float* lse, T* dq,
+int dq_typed(const Args& a, const T* dout, const float* lse, float* delta, T* dq,
              cudaStream_t stream) {
   constexpr int STAGES = 3;
   const int chunks = (a.G + 8 * NT - 1) / (8 * NT);
@@ -577,11 +562,11 @@ int dq_typed(const Args& a, const T* dout, const float* lse, T* dq,
   auto kern = attn_dq_kernel<T, DP, NT, STAGES>;
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   return launch_pdl(kern, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
-                    dim3(32 * kWarps), smem, stream, a, dout, lse, dq, chunks, units);
+                    dim3(32 * kWarps), smem, stream, a, dout, lse, delta, dq, chunks, units);
 }
 
 template <typename T, int DP>
-int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T* dout, T* dq, T* dk, T* dv,
+int grad_typed(const Args& a, int dtype, const float* lse, const T* dout, T* dq, T* dk, T* dv,
                uint8_t* ws, cudaStream_t stream) {
   const GradLayout l = grad_layout(a);
   float* delta = reinterpret_cast<float*>(ws + l.delta);
@@ -590,22 +575,17 @@ int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T
   int32_t* inv_offsets = reinterpret_cast<int32_t*>(ws + l.inv_offsets);
   int32_t* tile_off = reinterpret_cast<int32_t*>(ws + l.tile_off);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.Hq * a.Nq;
-  FKC_TRY(launch_pdl(attn_delta_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0,
-                     stream, out, dout, delta, a.D, odd, rows));
   if (use_tiles_grad(a))
-    return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, odd, ws + l.tiles, stream);
-  if (dq != nullptr) {
-    if (a.G <= 8)
-      FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, dq, stream)));
-    else
-      FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, dq, stream)));
-  }
+    return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, ws + l.tiles, stream);
+  if (a.G <= 8)
+    FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, stream)));
+  else
+    FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, delta, dq, stream)));
   if (dk == nullptr) return FKC_OK;
   FKC_TRY(launch_group(a.sel, false, static_cast<int64_t>(a.Nq) * a.top, inv_order, inv_offsets, R,
                        static_cast<int64_t>(a.Nq) * a.top, a.K, ws + l.group, stream));
   FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
-                     tile_off));
+                     tile_off, odd));
   const size_t kv_bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);
   FKC_TRY(launch_zero_fill(dk, kv_bytes, stream));
   FKC_TRY(launch_zero_fill(dv, kv_bytes, stream));
@@ -624,24 +604,24 @@ int grad_typed(const Args& a, int dtype, const T* out, const float* lse, const T
 }
 
 template <typename T>
-int grad_dtype(const Args& a, int dtype, const void* out, const float* lse, const void* dout, void* dq,
-               void* dk, void* dv, void* ws, cudaStream_t stream) {
-  const T *o = static_cast<const T*>(out), *d = static_cast<const T*>(dout);
+int grad_dtype(const Args& a, int dtype, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+               void* ws, cudaStream_t stream) {
+  const T* d = static_cast<const T*>(dout);
   T *q = static_cast<T*>(dq), *k = static_cast<T*>(dk), *v = static_cast<T*>(dv);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, o, lse, d, q, k, v, w, stream)
-                   : grad_typed<T, 128>(a, dtype, o, lse, d, q, k, v, w, stream);
+  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, d, q, k, v, w, stream)
+                   : grad_typed<T, 128>(a, dtype, lse, d, q, k, v, w, stream);
 }
 
 }  // namespace
 
 size_t backward_workspace_bytes(const Args& a) { return grad_layout(a).total; }
 
-int launch_backward(const Args& a, int dtype, const void* out, const float* lse, const void* dout,
-                    void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {
+int launch_backward(const Args& a, int dtype, const float* lse, const void* dout, void* dq, void* dk,
+                    void* dv, void* ws, cudaStream_t stream) {
   return dtype == FKC_DTYPE_F16
-             ? grad_dtype<__half>(a, dtype, out, lse, dout, dq, dk, dv, ws, stream)
-             : grad_dtype<__nv_bfloat16>(a, dtype, out, lse, dout, dq, dk, dv, ws, stream);
+             ? grad_dtype<__half>(a, dtype, lse, dout, dq, dk, dv, ws, stream)
+             : grad_dtype<__nv_bfloat16>(a, dtype, lse, dout, dq, dk, dv, ws, stream);
 }
 
 }  // namespace attn

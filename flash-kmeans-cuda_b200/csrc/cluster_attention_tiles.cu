@@ -130,10 +130,8 @@ __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, 
                                                         int32_t* __restrict__ row_pos,
                                                         int32_t* __restrict__ pair_row,
                                                         const float* __restrict__ lse,
-                                                        const float* __restrict__ delta,
                                                         int32_t* __restrict__ do_row,
-                                                        float* __restrict__ row_lse,
-                                                        float* __restrict__ row_delta) {
+                                                        float* __restrict__ row_lse) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -171,7 +169,6 @@ __global__ void __launch_bounds__(256) tile_rows_kernel(Args a, int i0, int nq, 
     if (lse != nullptr) {
       do_row[u * kUnitRows + rr] = static_cast<int32_t>(flat >= 0 ? flat : static_cast<int64_t>(a.batch) * a.Hq * a.Nq);
       row_lse[u * kUnitRows + rr] = flat >= 0 ? lse[flat] * kLog2e : 0.f;
-      row_delta[u * kUnitRows + rr] = flat >= 0 ? delta[flat] : 0.f;
     }
     q_row[u * kUnitRows + rr] = row;
     row_pos[u * kUnitRows + rr] = pos;
@@ -695,7 +692,7 @@ int fwd_typed(const Args& a, int dtype, T* out, float* lse, uint8_t* ws, cudaStr
   for (int64_t i0 = 0; i0 < a.Nq; i0 += l.nq) {
     const int nq = static_cast<int>(std::min<int64_t>(l.nq, a.Nq - i0));
     const int ctas = static_cast<int>(std::min<int64_t>(std::min(sm_count(), kMaxCtas), l.plan.units_max));
-    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, ctas, nullptr, nullptr, stream));
+    FKC_TRY(launch_units(a, i0, nq, rq, l.plan, ctas, nullptr, stream));
     FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kFwdThreads), smem, stream, tm_q, tm_k, tm_v, rk, rv, a,
                        static_cast<const int32_t*>(l.plan.q_row),
                        static_cast<const int32_t*>(l.plan.row_pos),
@@ -771,9 +768,8 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
   p.row_pos = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
   p.pair_row = static_cast<int32_t*>(take(R * pairs * 4));
   p.first_unit = static_cast<int32_t*>(take(R * a.K * 4));
-  if (!grad) {
-    p.odd = static_cast<int32_t*>(take(4));
-  } else {
+  p.odd = static_cast<int32_t*>(take(4));
+  if (grad) {
     p.do_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
     p.row_lse = static_cast<float*>(take(p.units_max * kUnitRows * 4));
     p.row_delta = static_cast<float*>(take(p.units_max * kUnitRows * 4));
@@ -784,7 +780,7 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
 }
 
 int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
-                 const float* lse, const float* delta, cudaStream_t stream) {
+                 const float* lse, cudaStream_t stream) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   FKC_REQUIRE(p.units_max * kUnitRows <= 2147483647ll, "attention: too many tiles");
   const int64_t blocks = std::min<int64_t>((R * nq * a.top + 255) / 256, sm_count() * 8ll);
@@ -800,8 +796,8 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
                     static_cast<const int32_t*>(p.inv_order),
                     static_cast<const Unit*>(p.units),
                     static_cast<const int64_t*>(p.count), static_cast<const int32_t*>(p.cum),
-                    p.start, ctas, p.q_row, p.row_pos, p.pair_row, lse, delta, p.do_row,
-                    p.row_lse, p.row_delta);
+                    p.start, ctas, p.q_row, p.row_pos, p.pair_row, lse, p.do_row,
+                    p.row_lse);
 }
 
 FormWork form_work(const Args& a, int64_t nq) {

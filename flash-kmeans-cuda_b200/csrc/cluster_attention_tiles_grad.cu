@@ -1,6 +1,8 @@
 // Gradients of attention over selected clusters, cluster by cluster (see
 // cluster_attention_tiles.cu for units and rows, cluster_attention_grad.cu for the formulas).
 //
+//   delta   (tiles_dq_kernel)   the sum of P dP over each row's keys, cluster by cluster, and
+//           tiles_delta_join_kernel adds a query's top sums (why not from out: cluster_attention_grad.cu).
 //   dQ      (tiles_dq_kernel)   a unit's 128 rows against the cluster's keys in steps of 128:
 //           S = Q K^T and dP = dO V^T into TMEM, dS in place, dQ += dS K. A row leaves its
 //           gradient over that cluster as the forward leaves its output, and
@@ -91,7 +93,7 @@ struct DqSmem {
   static constexpr uint32_t kMeta = kOut + 8 * 4096;
   struct Meta {
     int32_t key[2][kKeysStep];
-    uint64_t k_full[2], v_full[2], kv_free[2], q_full, q_free, sp_full, ds_full[2], dq_full, dq_free;
+    uint64_t k_full[2], v_full[2], kv_free[2], q_full, q_free, sp_full[2], sp_free[2], ds_full[2], dq_full, dq_free;
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -103,7 +105,9 @@ struct DqSmem {
 // values; 11, 12: of Q; 13, 14: of dout.
 constexpr int kGradThreads = 32 * 15;
 
-template <typename T, int DP>
+// kDelta: the sums of P dP over each row's keys instead, two floats a row (one per half of a step's
+// keys), with two S and dP in TMEM in turn since nothing follows them.
+template <typename T, int DP, bool kDelta>
 __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do, RowMap rk,
@@ -124,12 +128,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&mt.k_full[x]), 32);  // the gathering lanes (their keys), and the bytes
       mbar_init(smem_u32(&mt.v_full[x]), 1);
-      mbar_init(smem_u32(&mt.kv_free[x]), 1);
+      mbar_init(smem_u32(&mt.kv_free[x]), kDelta ? 9 : 1);  // kDelta: the warps that read the keys, too
       mbar_init(smem_u32(&mt.ds_full[x]), 128);
+      mbar_init(smem_u32(&mt.sp_full[x]), 1);
+      mbar_init(smem_u32(&mt.sp_free[x]), 256);
     }
     mbar_init(smem_u32(&mt.q_full), 4);
     mbar_init(smem_u32(&mt.q_free), 1);
-    mbar_init(smem_u32(&mt.sp_full), 1);
     mbar_init(smem_u32(&mt.dq_full), 1);
     mbar_init(smem_u32(&mt.dq_free), 256);
     mbar_init(smem_u32(&mt.drain), 1);
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = mt.tmem;  // S at 0, dP at 128, dQ at 256
+  const uint32_t tmem = mt.tmem;  // S at 0, dP at 128, dQ at 256 (kDelta: the second S and dP)
   pdl_wait();
 
   if (warp < 8) {
@@ -161,9 +166,52 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
       if (first < 0) return;
       pos_next = __ldg(row_pos + first + row);
       lse_next = __ldg(row_lse + first + row);
-      delta_next = __ldg(row_delta + first + row);
+      if (!kDelta) delta_next = __ldg(row_delta + first + row);
     };
     if (it.valid()) fetch(it.row());
+    if constexpr (kDelta) {
+      for (; ok && it.valid(); it.advance()) {
+        const int pos = pos_next;
+        const float lse = lse_next;
+        fetch(it.next_row());
+        const int steps = it.un.steps();
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int step = 0; step < steps; ++step, ++s_uses) {
+          const int keys = it.un.keys(step) - half * 64;  // may be none, but every phase is waited for
+          const uint32_t load = it.load + step, buf = s_uses & 1;
+          const int st = load & 1;
+          ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
+               warp_mbar_wait(&mt.sp_full[buf], (s_uses >> 1) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const int32_t* key = mt.key[st] + half * 64;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            if (c * 32 >= keys) break;
+            float s[32], dp[32];
+            tmem_ld_f32_x32(t_s + buf * 256 + c * 32, s);
+            tmem_ld_f32_x32(t_p + buf * 256 + c * 32, dp);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
+              const int k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = ex2(fmaf(s[j + e], sc, -lse)) * dp[j + e];
+                sum[e] += k[e] <= pos ? x : 0.f;
+              }
+            }
+          }
+          tc_fence_before();
+          mbar_arrive(smem_u32(&mt.sp_free[buf]));
+          __syncwarp();
+          if (lane == 0 && !it.keep) mbar_arrive(smem_u32(&mt.kv_free[st]));
+        }
+        if (ok) reinterpret_cast<float*>(part)[(it.row() + row) * 2 + half] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      if (!ok) give_up(abort, err, kErrDq);
+    } else {
     for (; ok && it.valid(); it.advance(), ++uses) {
       const int pos = pos_next;
       const float lse = lse_next, delta = delta_next;
@@ -175,7 +223,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         const uint32_t load = it.load + step;
         const int st = load & 1;
         ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
-             warp_mbar_wait(&mt.sp_full, s_uses & 1, abort);
+             warp_mbar_wait(&mt.sp_full[0], s_uses & 1, abort);
         if (!ok) break;
         tc_fence_after();
         const int32_t* key = mt.key[st] + half * 64;
@@ -228,6 +276,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     }
     if (!ok) give_up(abort, err, kErrDq);
     if (lane == 0) bulk_wait_all();
+    }
   } else if (warp == 8) {
     // ------------------------------------------------------------ MMAs (one thread)
     if (lane == 0) {
@@ -255,24 +304,34 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         mma_tmem_rows<4>(tmem + 256, tmem + 128 + half * 64, kt, idesc_o, p.ksteps, false);
         if (p.last) umma_commit(smem_u32(&mt.dq_full));
       };
+      uint32_t n = 0;  // steps
       for (SubIter it(units, start); ok && it.valid(); it.advance(), ++uses) {
         const int steps = it.un.steps();
-        for (int step = 0; ok && step < steps; ++step) {
-          const uint32_t load = it.load + step;
+        for (int step = 0; ok && step < steps; ++step, ++n) {
+          const uint32_t load = it.load + step, buf = kDelta ? n & 1 : 0;
           const int st = load & 1;
           const int keys = it.un.keys(step);
-          product(0);
-          product(1);
+          if constexpr (kDelta) {
+            ok = mbar_wait(smem_u32(&mt.sp_free[buf]), ((n >> 1) & 1) ^ 1, abort);
+          } else {
+            product(0);
+            product(1);
+          }
           ok = ok && mbar_wait(smem_u32(&mt.k_full[st]), (load >> 1) & 1, abort) &&
                mbar_wait(smem_u32(&mt.v_full[st]), (load >> 1) & 1, abort) &&
                mbar_wait(smem_u32(&mt.q_full), uses & 1, abort);
           if (!ok) break;
           const uint32_t idesc = umma_idesc_f16(kBf16, kSub, (keys + 15) / 16 * 16);
-          mma_kmajor<DP>(tmem, sb + S::kQ, sb + S::kK + st * S::kTile, idesc, dsteps);
-          mma_kmajor<DP>(tmem + 128, sb + S::kDo, sb + S::kV + st * S::kTile, idesc, dsteps);
-          umma_commit(smem_u32(&mt.sp_full));
+          tc_fence_after();
+          mma_kmajor<DP>(tmem + buf * 256, sb + S::kQ, sb + S::kK + st * S::kTile, idesc, dsteps);
+          mma_kmajor<DP>(tmem + buf * 256 + 128, sb + S::kDo, sb + S::kV + st * S::kTile, idesc, dsteps);
+          umma_commit(smem_u32(&mt.sp_full[buf]));
           const bool end = step == steps - 1, two = keys > 64;
           if (end) umma_commit(smem_u32(&mt.q_free));
+          if constexpr (kDelta) {
+            if (!it.keep) umma_commit(smem_u32(&mt.kv_free[st]));
+            continue;
+          }
           pend[0] = {true, step == 0, end && !two, st, (min(keys, 64) + 15) / 16, uses};
           if (two) pend[1] = {true, false, end, st, (keys - 64 + 15) / 16, uses};
           if (ok && to_free >= 0) umma_commit(smem_u32(&mt.kv_free[to_free]));
@@ -369,6 +428,37 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// One thread per (query, head): delta, the sum of its clusters' sums, which are those of the kernels that
+// follow, to their units' rows.
+__global__ void __launch_bounds__(256) tiles_delta_join_kernel(Args a, const int32_t* __restrict__ pair_row,
+                                                               const float2* __restrict__ part,
+                                                               float* __restrict__ delta,
+                                                               float* __restrict__ row_delta, int64_t rows) {
+  pdl_wait();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // (r, i, head)
+  if (t >= rows) return;
+  const int64_t qi = t / a.G;
+  const int h = static_cast<int>(t - qi * a.G), r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi - static_cast<int64_t>(r) * a.Nq);
+  const int32_t* pairs = pair_row + qi * a.top;
+  float sum = 0.f;
+  for (int s0 = 0; s0 < a.top; s0 += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int n = s0 + u < a.top ? pairs[s0 + u] : -1;
+      v[u] = n >= 0 ? part[static_cast<int64_t>(n) + h] : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += v[u].x + v[u].y;
+  }
+  const int b = r / a.Hkv;
+  delta[(static_cast<int64_t>(b) * a.Hq + (r - b * a.Hkv) * a.G + h) * a.Nq + i] = sum;
+  for (int s = 0; s < a.top; ++s) {
+    const int n = pairs[s];
+    if (n >= 0) row_delta[static_cast<int64_t>(n) + h] = sum;
   }
 }
 
@@ -965,8 +1055,8 @@ GradLayout grad_layout(const Args& a, uint8_t* ws) {
 }
 
 template <typename T, int DP>
-int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, const T* dout, T* dq, T* dk,
-               T* dv, int32_t* odd, uint8_t* ws, cudaStream_t stream) {
+int grad_typed(const Args& a, int dtype, const float* lse, float* delta, const T* dout, T* dq, T* dk,
+               T* dv, uint8_t* ws, cudaStream_t stream) {
   const GradLayout l = grad_layout(a, ws);
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   CUtensorMap tm_q, tm_k, tm_v, tm_do;
@@ -977,16 +1067,24 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
   FKC_TRY(encode_rows(a.v, a.vs, a.batch, a.Hkv, a.N, a.D, dtype, &tm_v, &rv));
   FKC_TRY(encode_rows(dout, flat, a.batch, a.Hq, a.Nq, a.D, dtype, &tm_do, &rdo));
   const int ctas = static_cast<int>(std::min<int64_t>(std::min(sm_count(), kMaxCtas), l.plan.units_max));
-  FKC_TRY(launch_units(a, 0, a.Nq, rq, l.plan, ctas, lse, delta, stream));
+  FKC_TRY(launch_units(a, 0, a.Nq, rq, l.plan, ctas, lse, stream));
+  int32_t* odd = l.plan.odd;
   const int32_t *q_row = l.plan.q_row, *do_row = l.plan.do_row, *pos = l.plan.row_pos;
   const float *row_lse = l.plan.row_lse, *row_delta = l.plan.row_delta;
-  if (dq != nullptr) {
-    auto kern = tiles_dq_kernel<T, DP>;
+  auto walk = [&](auto kern) -> int {
     const int smem = static_cast<int>(DqSmem<DP>::kBytes);
     FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    FKC_TRY(launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
+    return launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                        q_row, do_row, pos, row_lse, row_delta, static_cast<const Unit*>(l.plan.units),
-                       static_cast<const int32_t*>(l.plan.start), ws + l.part, device_error_word()));
+                      static_cast<const int32_t*>(l.plan.start), ws + l.part, device_error_word());
+  };
+  FKC_TRY(walk(tiles_dq_kernel<T, DP, true>));
+  const int64_t rows = R * a.Nq * a.G;
+  FKC_TRY(launch_pdl(tiles_delta_join_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, stream, a,
+                     static_cast<const int32_t*>(l.plan.pair_row), reinterpret_cast<const float2*>(ws + l.part),
+                     delta, l.plan.row_delta, rows));
+  if (dq != nullptr) {
+    FKC_TRY(walk(tiles_dq_kernel<T, DP, false>));
     const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
     const int64_t warps = R * a.Nq * chunks;
     FKC_TRY(launch_pdl(tiles_dq_join_kernel<T, DP>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0,
@@ -1023,12 +1121,12 @@ int grad_typed(const Args& a, int dtype, const float* lse, const float* delta, c
 }
 
 template <typename T>
-int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, const void* dout, void* dq,
-               void* dk, void* dv, int32_t* odd, uint8_t* ws, cudaStream_t stream) {
+int grad_dtype(const Args& a, int dtype, const float* lse, float* delta, const void* dout, void* dq,
+               void* dk, void* dv, uint8_t* ws, cudaStream_t stream) {
   const T* d = static_cast<const T*>(dout);
   T *q = static_cast<T*>(dq), *k = static_cast<T*>(dk), *v = static_cast<T*>(dv);
-  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, delta, d, q, k, v, odd, ws, stream)
-                   : grad_typed<T, 128>(a, dtype, lse, delta, d, q, k, v, odd, ws, stream);
+  return a.D <= 64 ? grad_typed<T, 64>(a, dtype, lse, delta, d, q, k, v, ws, stream)
+                   : grad_typed<T, 128>(a, dtype, lse, delta, d, q, k, v, ws, stream);
 }
 
 }  // namespace
@@ -1039,9 +1137,7 @@ int grad_dtype(const Args& a, int dtype, const float* lse, const float* delta, c
 // rows, 32 clusters of 32 keys: 133, 137. G 16, 64 queries x 8 rows, 32 rows a cluster of 64
 // keys: 408, 389; 2048 queries x 4 rows, 12 keys a cluster: 1061, 1194; 20 keys: 1274, 1182.
 bool use_tiles_grad(const Args& a) {
-  // delta comes from the 16-bit out here, which few clusters of close keys do not bear (the walk
-  // forms it anew, see cluster_attention_grad.cu): 0.0051 of dQ's norm with one, 0.0026 with four
-  if (a.top < 4 || !tiles_fit(a, a.Nq)) return false;
+  if (!tiles_fit(a, a.Nq)) return false;
   const FormWork w = form_work(a, a.Nq);
   const double key_tiles = static_cast<double>(a.batch) * a.Hkv * a.K * (w.keys / 64 + 0.5);  // of the walk
   const double walk = 60 + 110e-6 * w.reads + 0.031 * key_tiles + w.rows * (257e-6 + 3.1e-6 * w.keys);
@@ -1055,12 +1151,12 @@ bool use_tiles_grad(const Args& a) {
 
 size_t tiles_backward_workspace_bytes(const Args& a) { return grad_layout(a, nullptr).total; }
 
-int launch_tiles_backward(const Args& a, int dtype, const float* lse, const float* delta, const void* dout,
-                          void* dq, void* dk, void* dv, int32_t* odd, void* ws, cudaStream_t stream) {
+int launch_tiles_backward(const Args& a, int dtype, const float* lse, float* delta, const void* dout,
+                          void* dq, void* dk, void* dv, void* ws, cudaStream_t stream) {
   uint8_t* w = static_cast<uint8_t*>(ws);
   return dtype == FKC_DTYPE_F16
-             ? grad_dtype<__half>(a, dtype, lse, delta, dout, dq, dk, dv, odd, w, stream)
-             : grad_dtype<__nv_bfloat16>(a, dtype, lse, delta, dout, dq, dk, dv, odd, w, stream);
+             ? grad_dtype<__half>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream)
+             : grad_dtype<__nv_bfloat16>(a, dtype, lse, delta, dout, dq, dk, dv, w, stream);
 }
 
 }  // namespace attn

@@ -21,7 +21,7 @@ int check_group(int64_t B, int64_t N, int64_t K) {
   FKC_REQUIRE(B >= 1 && N >= 1 && K >= 1, "B, N and K must be >= 1 (got %lld, %lld, %lld)",
               static_cast<long long>(B), static_cast<long long>(N), static_cast<long long>(K));
   FKC_REQUIRE(N <= kMaxRows && K < kMaxRows && B <= kMaxRows, "B, N and K must fit int32");
-  // the grids: chunks of at least 4096 positions, 32 counters a CTA
+  // the grids: a CTA per chunk of at least 1024 positions, or per 32 counters
   FKC_REQUIRE(B <= (1 << 20) && B * N <= (1ll << 40) && B * K <= (1ll << 40),
               "B must be at most 2^20, B * N and B * K at most 2^40");
   return FKC_OK;
@@ -101,7 +101,6 @@ int fill_args(const fkc_attention_desc* d, bool attention, attn::Args* out) {
 
 cudaStream_t as_stream(fkc_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
-// The kernels use instructions of sm_80 and later only, but are built for sm_100a.
 int check_device() {
   const DeviceInfo* di = nullptr;
   FKC_TRY(current_device_info(&di));
@@ -227,8 +226,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, c
   clear_error();
   attn::Args a;
   FKC_TRY(fill_args(desc, true, &a));
-  FKC_REQUIRE(out != nullptr && lse != nullptr && dout != nullptr,
-              "out, lse and dout must be non-null");
+  FKC_REQUIRE(lse != nullptr && dout != nullptr, "lse and dout must be non-null");
   FKC_REQUIRE((dk == nullptr) == (dv == nullptr), "dk and dv go together");
   for (const void* p : {out, dout, static_cast<const void*>(dq), static_cast<const void*>(dk),
                         static_cast<const void*>(dv)})
@@ -237,8 +235,7 @@ FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, c
   FKC_TRY(check_workspace("attention gradient", workspace, workspace_bytes,
                           attn::backward_workspace_bytes(a)));
   FKC_TRY(check_device());
-  return attn::launch_backward(a, desc->dtype, out, lse, dout, dq, dk, dv, workspace,
-                               as_stream(stream));
+  return attn::launch_backward(a, desc->dtype, lse, dout, dq, dk, dv, workspace, as_stream(stream));
 }
 
 }  // extern "C"

@@ -249,8 +249,9 @@ struct UnitPlan {
   int32_t* row_pos;      // last position that the row sees; -1: none, or no row
   int32_t* pair_row;     // (R, nq * top) unit row of a pair's first head; -1: no key
   int32_t* first_unit;   // (R, K) of clusters that have units
-  int32_t* odd;          // of the forward: a result is not finite (cluster_masked.cu)
-  // for the gradients: row of dout's map, as q_row; lse to base 2 and delta of the row
+  int32_t* odd;          // a result is not finite (cluster_masked.cu)
+  // for the gradients: row of dout's map, as q_row; lse to base 2 of the row; its delta, which
+  // cluster_attention_tiles_grad.cu sets
   int32_t* do_row;
   float *row_lse, *row_delta;
   void* group_ws;
@@ -258,9 +259,9 @@ struct UnitPlan {
 };
 size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* out);
 // Groups sel of the queries [i0, i0 + nq), lists the units, fills the rows and shares the
-// units among `ctas` CTAs. lse and delta (batch, Hq, Nq) with rows of the gradients only.
+// units among `ctas` CTAs. lse (batch, Hq, Nq) with rows of the gradients only.
 int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const UnitPlan& p, int ctas,
-                 const float* lse, const float* delta, cudaStream_t stream);
+                 const float* lse, cudaStream_t stream);
 constexpr int kMaxCtas = 1024;
 
 // What the choice between the two forms weighs, with nq queries a round: keys of a cluster on

@@ -347,7 +347,7 @@ class Attend : public torch::autograd::Function<Attend> {
     const Attention a =
         attention_of(q, k, v, sel, order, offsets, q_pos.value_or(Tensor()), scale);
     auto [out, lse] = attention_forward(a);
-    ctx->save_for_backward({q, k, v, a.sel, a.order, a.offsets, a.q_pos, out, lse});
+    ctx->save_for_backward({q, k, v, a.sel, a.order, a.offsets, a.q_pos, lse});
     ctx->saved_data["scale"] = scale;
     ctx->mark_non_differentiable({lse});
     return {out, lse};
@@ -360,7 +360,7 @@ class Attend : public torch::autograd::Function<Attend> {
     const c10::cuda::CUDAGuard guard(s[0].device());
     Attention a = attention_of(s[0], s[1], s[2], s[3], s[4], s[5], s[6],
                                ctx->saved_data["scale"].toDouble());
-    const Tensor &out = s[7], &lse = s[8];
+    const Tensor& lse = s[7];
     const Tensor dout = dense(grads[0]);
     const bool want_q = ctx->needs_input_grad(0);
     const bool want_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -374,7 +374,7 @@ class Attend : public torch::autograd::Function<Attend> {
       const size_t bytes = fkc_cluster_attention_grad_workspace_size(&a.d);
       const Tensor ws = workspace(bytes, dout);
       check_status(fkc_cluster_attention_grad(
-                       &a.d, out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(),
+                       &a.d, nullptr, lse.data_ptr<float>(), dout.data_ptr(),
                        want_q ? dq.data_ptr() : nullptr, want_kv ? dk.data_ptr() : nullptr,
                        want_kv ? dv.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(dout)),
                    "cluster_attention");

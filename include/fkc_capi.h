@@ -387,8 +387,9 @@ FKC_CAPI_EXPORT int fkc_cluster_attention(const fkc_attention_desc* desc, void* 
                                           void* workspace, size_t workspace_bytes,
                                           fkc_stream_t stream);
 
-/* Gradients of out for dout (contiguous like out), from the forward's out and
- * lse. dq like out; dk, dv (batch, kv_heads, n_keys, head_dim), zeros where no
+/* Gradients of out for dout (contiguous like out), from the forward's lse. out
+ * is not read and may be NULL: what the gradients need of it is summed anew,
+ * since its rounding would add up over keys that are alike. dq like out; dk, dv (batch, kv_heads, n_keys, head_dim), zeros where no
  * query reads. dq may be NULL, and so may dk and dv together. Deterministic. */
 FKC_CAPI_EXPORT size_t fkc_cluster_attention_grad_workspace_size(const fkc_attention_desc* desc);
 FKC_CAPI_EXPORT int fkc_cluster_attention_grad(const fkc_attention_desc* desc, const void* out,

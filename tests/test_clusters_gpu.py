@@ -787,3 +787,28 @@ def test_forward_mode_tangents_are_refused(clusters):
             with pytest.raises(RuntimeError, match="tangent"):
                 clusters.cluster_attention(*args, sel, order, offsets)
         assert torch.equal(clusters.cluster_lookup(t, ids), t[ids])
+
+
+@pytest.mark.parametrize("offset", [0.0, 3.0, 30.0])
+@pytest.mark.parametrize("Nq,top,one", [(30, 1, False), (30, 8, False), (700, 1, False), (700, 2, False), (700, 4, False), (700, 8, False), (700, 16, False),
+                                        (700, 8, True)])
+def test_query_gradient_of_keys_with_an_offset(clusters, Nq, top, one, offset):
+    """Close keys within clusters and an offset that all keys share, as channel means of a cache: dQ keeps the
+    accuracy of its last rounding (2**-8 of its norm at most). delta is summed from the same P and dP, so dS
+    sums to zero but for the errors of P's sum, 2**-18 of it, and of dS's 2**-17: 2**-12 of the norm at 30 times
+    the spread and 64 keys, below the 2**-10 that the scores' errors, some 2**-13 a weight, have."""
+    q, k, v, _, order, offsets, _ = attention_case(1, 2, 4, Nq, 2000, 32, 128, top, BF, causal=False, drop=0.0)
+    common = offset * randn(128, seed=50)
+    for r in range(2):
+        for c in range(32):
+            rows = order[r, offsets[r, c]:offsets[r, c + 1]].long()
+            k[0, r, rows] = (randn(1, 128, seed=100 + c) + 0.5 * k[0, r, rows].float() + common).to(BF)
+    sel = torch.randint(0, 33 - top, (2, Nq, 1), generator=gen(1), device="cuda", dtype=torch.int32) + torch.arange(top, device="cuda", dtype=torch.int32)
+    if one:
+        sel[..., 1:] = -1
+    dout = randn(*q.shape, seed=9).to(BF)
+    val, tol = attention_ref(q, k, v, sel, order, offsets, None, None, dout)
+    a = [t.requires_grad_(True) for t in (q, k, v)]
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(clusters.cluster_attention(*a, sel, order, offsets), a, dout)):
+        off = ((g.double() - val[name]).norm() / val[name].norm()).item()
+        assert off <= 2.0 ** -8 + 2.0 ** -10, (name, off)
