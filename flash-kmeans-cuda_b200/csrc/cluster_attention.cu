@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_fwd_kernel(Args a, T* __rest
         const float base = mn == -INFINITY ? 0.f : mn;  // nothing finite so far
         const float alpha = exp2f(m[n][e] - base);
         m[n][e] = mn;
-        s[n][e] = exp2f(s[n][e] - base);
-        s[n][2 + e] = exp2f(s[n][2 + e] - base);
+        s[n][e] = exp2f(s[n][e] - (base - Range<T>::kShift));
+        s[n][2 + e] = exp2f(s[n][2 + e] - (base - Range<T>::kShift));
         l[n][e] = l[n][e] * alpha + (s[n][e] + s[n][2 + e]);
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) o[n][kk][e] *= alpha, o[n][kk][2 + e] *= alpha;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_fwd_kernel(Args a, T* __rest
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
       inv[e] = sum == 0.f ? 0.f : 1.f / sum;
-      const float ls = sum == 0.f ? -INFINITY : (m[n][e] + log2f(sum)) * kLn2;
+      const float ls = sum == 0.f ? -INFINITY : (m[n][e] - Range<T>::kShift + log2f(sum)) * kLn2;
       const int h = n * 8 + t4 * 2 + e;
       if (g == 0 && h < heads) {
         const int64_t at = (static_cast<int64_t>(b) * a.Hq + h0 + h) * a.Nq + i;

@@ -126,6 +126,30 @@ __device__ __forceinline__ void load_b_trans(uint32_t (&f)[4], uint32_t tile, in
 // 0 while all of x are finite (from a so_far of 0).
 __device__ __forceinline__ float not_finite(float x, float so_far) { return fmaf(x, 0.f, so_far); }
 
+// The 16-bit operands P and dS of fp16 inputs, whose normal range ends at 2^-14: P (at most 1) is
+// held as 2^14 P, and dS under a power of two that the sum A of P |dP| over a row's keys gives, since
+// |dS| <= 2 A: power(A) * A lies in [2^13, 2^14), or below where A is less than 2^-47 (a product of
+// two fp16 rows, 2^39 at most, times the power stays finite). dQ has a power per row, dK one per row of
+// clusters, from the largest A of its queries. (With dout near 1e-4 and 512 keys, dS below 2^-24 made
+// dQ off by 0.004 of its norm.) bf16 has fp32's exponents and needs neither.
+template <typename T>
+struct Range {
+  static constexpr bool kNarrow = std::is_same<T, __half>::value;
+  static constexpr int kShift = kNarrow ? 14 : 0;  // of P
+  static __host__ __device__ constexpr float unshift() { return kNarrow ? 0x1p-14f : 1.f; }
+};
+__device__ __forceinline__ float power(float A) {  // 1 where A is not finite
+  const int e = static_cast<int>(__float_as_uint(A) >> 23);
+  return __uint_as_float(static_cast<uint32_t>(e >= 255 ? 127 : min(267 - e, 127 + 60)) << 23);
+}
+__device__ __forceinline__ float inverse_power(float p) {
+  return __uint_as_float((254u << 23) - __float_as_uint(p));
+}
+// The largest A of a row of clusters; A is not negative, so its bits are ordered as it is.
+__device__ __forceinline__ void note_largest(float* word, float A) {
+  if (A > *reinterpret_cast<volatile float*>(word)) atomicMax(reinterpret_cast<int*>(word), __float_as_int(A));
+}
+
 int sm_count();  // of the current device
 
 // Launchers (cluster_select.cu, cluster_attention.cu, cluster_attention_grad.cu); dtype is

@@ -50,12 +50,12 @@ __host__ __device__ constexpr int warp_smem(int top) {
   return ring_bytes<DP, STAGES>() + ((STAGES * 4 + (2 * top + 1) * 4 + 15) / 16) * 16;
 }
 
-// dq may be null: delta alone.
+// dq may be null: delta alone. largest, with dK: the largest A of each row of clusters.
 template <typename T, int DP, int NT, int STAGES>
 __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* __restrict__ dout,
                                                               const float* __restrict__ lse,
                                                               float* __restrict__ delta,
-                                                              T* __restrict__ dq, int chunks,
+                                                              T* __restrict__ dq, float* __restrict__ largest, int chunks,
                                                               int64_t units) {
   constexpr int KS = DP / 16;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
   auto flat = [&](int h) { return (static_cast<int64_t>(b) * a.Hq + h0 + h) * a.Nq + i; };
 
   uint32_t qf[NT][KS][2], df[NT][KS][2];
-  float ls[NT][2], dl[NT][2];
+  float ls[NT][2], dl[NT][2], pw[NT][2];  // pw: the power of two of dS (1 in the first pass)
   const T* qb = static_cast<const T*>(a.q) + b * a.qs.b + i * a.qs.n;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     for (int e = 0; e < 2; ++e) {
       const int h = n * 8 + t4 * 2 + e;
       ls[n][e] = h < heads ? lse[flat(h)] * kLog2e : 0.f;
-      dl[n][e] = 0.f;
+      dl[n][e] = 0.f, pw[n][e] = 1.f;
     }
   }
   KeyList list;
@@ -152,11 +152,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     if (s < tiles) issue(s);
     mma::cp_async_commit();
   }
-  float sum[NT][2];
+  float sum[NT][2], mag[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) sum[n][e] = 0.f;
+    for (int e = 0; e < 2; ++e) sum[n][e] = mag[n][e] = 0.f;
   for (int t = 0; t < tiles; ++t) {
     mma::cp_async_wait<STAGES - 2>();
     __syncwarp();
@@ -188,9 +188,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        s[n][e] = on0 ? exp2f(s[n][e] * sc - ls[n][e]) * (dp[n][e] - dl[n][e]) : 0.f;
-        s[n][2 + e] = on1 ? exp2f(s[n][2 + e] * sc - ls[n][e]) * (dp[n][2 + e] - dl[n][e]) : 0.f;
+        s[n][e] = on0 ? exp2f(s[n][e] * sc - ls[n][e]) * ((dp[n][e] - dl[n][e]) * pw[n][e]) : 0.f;
+        s[n][2 + e] = on1 ? exp2f(s[n][2 + e] * sc - ls[n][e]) * ((dp[n][2 + e] - dl[n][e]) * pw[n][e]) : 0.f;
         sum[n][e] += s[n][e] + s[n][2 + e];
+        if (Range<T>::kNarrow) mag[n][e] += fabsf(s[n][e]) + fabsf(s[n][2 + e]);
       }
     }
     if (pass == 0) continue;
@@ -218,29 +219,46 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
   mma::cp_async_wait<0>();
   __syncwarp();
   if (pass == 0) {
+    float most = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float d = sum[n][e];
-        d += __shfl_xor_sync(0xFFFFFFFFu, d, 4);
-        d += __shfl_xor_sync(0xFFFFFFFFu, d, 8);
-        d += __shfl_xor_sync(0xFFFFFFFFu, d, 16);
+        float d = sum[n][e], A = mag[n][e];
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) {
+          d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
+          if (Range<T>::kNarrow) A += __shfl_xor_sync(0xFFFFFFFFu, A, o);
+        }
         dl[n][e] = d;
+        if (Range<T>::kNarrow) {
+          pw[n][e] = power(A);
+          if (A < INFINITY) most = fmaxf(most, A);
+        }
         const int h = n * 8 + t4 * 2 + e;
         if (g == 0 && h < heads) delta[flat(h)] = d;
       }
+    if (Range<T>::kNarrow && largest != nullptr) {
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+      if (lane == 0) note_largest(largest + r, most);
+    }
     if (dq == nullptr) return;
   }
   }
+  float out[NT][2];  // what the sums are multiplied by
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) out[n][e] = a.scale * inverse_power(pw[n][e]);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int md = 0; md < KS; ++md) {
       const uint32_t lo =
-          mma::movmatrix_trans(mma::pack2<T>(o[n][md][0] * a.scale, o[n][md][1] * a.scale));
+          mma::movmatrix_trans(mma::pack2<T>(o[n][md][0] * out[n][0], o[n][md][1] * out[n][1]));
       const uint32_t hi =
-          mma::movmatrix_trans(mma::pack2<T>(o[n][md][2] * a.scale, o[n][md][3] * a.scale));
+          mma::movmatrix_trans(mma::pack2<T>(o[n][md][2] * out[n][0], o[n][md][3] * out[n][1]));
       const int h = n * 8 + g, d = md * 16 + t4 * 2;
       if (h < heads) {
         T* row = dq + flat(h) * a.D;
@@ -252,10 +270,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
 
 // tile_off[r, c]: first key tile of cluster c among the row's; tile_off[r, K]: their number.
 __global__ void __launch_bounds__(1024) key_tiles_kernel(Args a, int32_t* __restrict__ tile_off,
-                                                         int32_t* odd) {
+                                                         int32_t* odd, float* __restrict__ largest) {
   __shared__ int warp_total[32];
   pdl_wait();
   if (blockIdx.x == 0 && threadIdx.x == 0) *odd = 0;
+  if (threadIdx.x == 0) largest[blockIdx.x] = 0.f;
   const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int32_t* out = tile_off + static_cast<int64_t>(r) * (a.K + 1);
   int carry = 0;
@@ -298,11 +317,12 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
     Args a, const T* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ delta, const int32_t* __restrict__ inv_order,
     const int32_t* __restrict__ inv_offsets, const int32_t* __restrict__ tile_off,
-    T* __restrict__ dk, T* __restrict__ dv, int32_t* __restrict__ odd, int tiles_max) {
+    const float* __restrict__ largest, T* __restrict__ dk, T* __restrict__ dv,
+    int32_t* __restrict__ odd, int tiles_max) {
   constexpr int KS = DP / 16, CH = DP / 8;
   using S = DkvSmem<DP>;
   extern __shared__ __align__(16) uint8_t smem[];
-  // of two column tiles: lse * log2(e), delta, the query's position (-1: reads nothing)
+  // of two column tiles: lse * log2(e) less P's shift, delta, the query's position (-1: reads nothing)
   __shared__ float c_lse[2][kCols], c_delta[2][kCols];
   __shared__ int c_pos[2][kCols];
   __shared__ int64_t c_q[2][kCols], c_do[2][kCols];  // row offsets
@@ -378,7 +398,7 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
     if (p < first) return x;
     const int64_t at = (static_cast<int64_t>(b) * a.Hq + h) * a.Nq + i;
     x.pos = p;
-    x.lse = lse[at] * kLog2e;
+    x.lse = lse[at] * kLog2e - Range<T>::kShift;
     x.delta = delta[at];
     x.q = b * a.qs.b + h * a.qs.h + i * a.qs.n;
     x.d = at * a.D;
@@ -421,6 +441,7 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
   mma::cp_async_commit();
   const int row0 = s_row[warp * 16 + g], row1 = s_row[warp * 16 + 8 + g];
   const float sc = a.scale * kLog2e;
+  const float pw = Range<T>::kNarrow ? power(largest[r]) : 1.f, ds_power = pw * Range<T>::unshift();
   const bool idle = warp * 16 >= keys;  // no key for this warp
   for (int s = 0; s < steps; ++s) {
     // the other buffer was read in step s - 1, which the barrier below ended
@@ -468,8 +489,8 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
           const float p1 = on1 ? exp2f(ss[n][2 + e] * sc - ls) : 0.f;
           ss[n][e] = p0;
           ss[n][2 + e] = p1;
-          dp[n][e] = on0 ? p0 * (dp[n][e] - dl) : 0.f;
-          dp[n][2 + e] = on1 ? p1 * (dp[n][2 + e] - dl) : 0.f;
+          dp[n][e] = on0 ? p0 * ((dp[n][e] - dl) * ds_power) : 0.f;
+          dp[n][2 + e] = on1 ? p1 * ((dp[n][2 + e] - dl) * ds_power) : 0.f;
         }
         pp[n][0] = mma::pack2<T>(ss[n][0], ss[n][1]);
         pp[n][1] = mma::pack2<T>(ss[n][2], ss[n][3]);
@@ -504,6 +525,7 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
   }
   mma::cp_async_wait<0>();
   const int64_t kv = (static_cast<int64_t>(b) * a.Hkv + hk) * a.N;
+  const float k_out = a.scale * inverse_power(pw), v_out = Range<T>::unshift();
   float bad = 0.f;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -517,15 +539,16 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
       if (d >= a.D) continue;
       const int64_t at = (kv + row) * a.D + d;
       *reinterpret_cast<uint32_t*>(dk + at) =
-          mma::pack2<T>(ak[n][half * 2] * a.scale, ak[n][half * 2 + 1] * a.scale);
-      *reinterpret_cast<uint32_t*>(dv + at) = mma::pack2<T>(av[n][half * 2], av[n][half * 2 + 1]);
+          mma::pack2<T>(ak[n][half * 2] * k_out, ak[n][half * 2 + 1] * k_out);
+      *reinterpret_cast<uint32_t*>(dv + at) =
+          mma::pack2<T>(av[n][half * 2] * v_out, av[n][half * 2 + 1] * v_out);
     }
   }
   if (bad != 0.f) *odd = 1;
 }
 
 struct GradLayout {
-  size_t delta, odd, inv_order, inv_offsets, tile_off, group, tiles, total;
+  size_t delta, odd, largest, inv_order, inv_offsets, tile_off, group, tiles, total;
 };
 
 GradLayout grad_layout(const Args& a) {
@@ -544,6 +567,7 @@ GradLayout grad_layout(const Args& a) {
     return l;
   }
   l.odd = take(4);
+  l.largest = take(static_cast<size_t>(R) * 4);
   l.inv_order = take(static_cast<size_t>(R) * a.Nq * a.top * 4);
   l.inv_offsets = take(static_cast<size_t>(R) * (a.K + 1) * 4);
   l.tile_off = take(static_cast<size_t>(R) * (a.K + 1) * 4);
@@ -553,7 +577,7 @@ GradLayout grad_layout(const Args& a) {
 }
 
 template <typename T, int DP, int NT>
-int dq_typed(const Args& a, const T* dout, const float* lse, float* delta, T* dq,
+int dq_typed(const Args& a, const T* dout, const float* lse, float* delta, T* dq, float* largest,
              cudaStream_t stream) {
   constexpr int STAGES = 3;
   const int chunks = (a.G + 8 * NT - 1) / (8 * NT);
@@ -562,7 +586,7 @@ int dq_typed(const Args& a, const T* dout, const float* lse, float* delta, T* dq
   auto kern = attn_dq_kernel<T, DP, NT, STAGES>;
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   return launch_pdl(kern, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
-                    dim3(32 * kWarps), smem, stream, a, dout, lse, delta, dq, chunks, units);
+                    dim3(32 * kWarps), smem, stream, a, dout, lse, delta, dq, largest, chunks, units);
 }
 
 template <typename T, int DP>
@@ -577,15 +601,18 @@ int grad_typed(const Args& a, int dtype, const float* lse, const T* dout, T* dq,
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   if (use_tiles_grad(a))
     return launch_tiles_backward(a, dtype, lse, delta, dout, dq, dk, dv, ws + l.tiles, stream);
+  float* largest = dk != nullptr ? reinterpret_cast<float*>(ws + l.largest) : nullptr;
+  if (dk != nullptr) {
+    FKC_TRY(launch_group(a.sel, false, static_cast<int64_t>(a.Nq) * a.top, inv_order, inv_offsets, R,
+                         static_cast<int64_t>(a.Nq) * a.top, a.K, ws + l.group, stream));
+    FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
+                       tile_off, odd, largest));
+  }
   if (a.G <= 8)
-    FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, stream)));
+    FKC_TRY((dq_typed<T, DP, 1>(a, dout, lse, delta, dq, largest, stream)));
   else
-    FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, delta, dq, stream)));
+    FKC_TRY((dq_typed<T, DP, 2>(a, dout, lse, delta, dq, largest, stream)));
   if (dk == nullptr) return FKC_OK;
-  FKC_TRY(launch_group(a.sel, false, static_cast<int64_t>(a.Nq) * a.top, inv_order, inv_offsets, R,
-                       static_cast<int64_t>(a.Nq) * a.top, a.K, ws + l.group, stream));
-  FKC_TRY(launch_pdl(key_tiles_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,
-                     tile_off, odd));
   const size_t kv_bytes = static_cast<size_t>(R) * a.N * a.D * sizeof(T);
   FKC_TRY(launch_zero_fill(dk, kv_bytes, stream));
   FKC_TRY(launch_zero_fill(dv, kv_bytes, stream));
@@ -598,7 +625,8 @@ int grad_typed(const Args& a, int dtype, const float* lse, const T* dout, T* dq,
                      dout, lse, static_cast<const float*>(delta),
                      static_cast<const int32_t*>(inv_order),
                      static_cast<const int32_t*>(inv_offsets),
-                     static_cast<const int32_t*>(tile_off), dk, dv, odd, static_cast<int>(tiles_max)));
+                     static_cast<const int32_t*>(tile_off), static_cast<const float*>(largest), dk, dv,
+                     odd, static_cast<int>(tiles_max)));
   // dq's walk takes one query's keys at a time: none that the query does not see
   return launch_again(a, dtype, odd, lse, delta, dout, nullptr, inv_order, inv_offsets, dk, dv, stream);
 }

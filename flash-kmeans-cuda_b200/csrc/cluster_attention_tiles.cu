@@ -42,11 +42,13 @@ namespace attn {
 namespace {
 
 __global__ void __launch_bounds__(256) tile_init_kernel(int64_t* count, int32_t* __restrict__ pair_row,
-                                                        int64_t pairs, int32_t* odd) {
+                                                        int64_t pairs, int32_t* odd, float* largest, int R) {
   pdl_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i == 0) *count = 0;
   if (i == 0 && odd != nullptr) *odd = 0;
+  if (largest != nullptr)
+    for (int64_t r = i; r < R; r += static_cast<int64_t>(gridDim.x) * 256) largest[r] = 0.f;
   for (int64_t p = i; p < pairs; p += static_cast<int64_t>(gridDim.x) * 256) pair_row[p] = -1;
 }
 
@@ -310,8 +312,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float mn = fmaxf(m, top * sc);  // the scale is positive
-        const float from = mn == -INFINITY ? 0.f : mn;
-        const float alpha = ex2(m - from);
+        const float base = mn == -INFINITY ? 0.f : mn, from = base - Range<T>::kShift;
+        const float alpha = ex2(m - base);
         m = mn;
         if (step > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
           // the product of the step before has ended: its commit came before this S's
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
       }
       if (!ok) break;
       part_lse[static_cast<int64_t>(it.n) * kUnitRows + sub * kSub + row] =
-          make_float2(l == 0.f ? -INFINITY : m + log2f(l), l == 0.f ? 0.f : 1.f / l);
+          make_float2(l == 0.f ? -INFINITY : m - Range<T>::kShift + log2f(l), l == 0.f ? 0.f : 1.f / l);
     }
   } else if (warp < 16) {
     // ------------------------------------------------------------ output
@@ -773,6 +775,8 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
     p.do_row = static_cast<int32_t*>(take(p.units_max * kUnitRows * 4));
     p.row_lse = static_cast<float*>(take(p.units_max * kUnitRows * 4));
     p.row_delta = static_cast<float*>(take(p.units_max * kUnitRows * 4));
+    p.row_power = static_cast<float*>(take(p.units_max * kUnitRows * 4));
+    p.largest = static_cast<float*>(take(R * 4));
   }
   p.group_ws = take(static_cast<int64_t>(group_workspace_bytes(R, pairs, a.K)));
   if (out != nullptr) *out = p;
@@ -785,7 +789,8 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
   FKC_REQUIRE(p.units_max * kUnitRows <= 2147483647ll, "attention: too many tiles");
   const int64_t blocks = std::min<int64_t>((R * nq * a.top + 255) / 256, sm_count() * 8ll);
   FKC_TRY(launch_pdl(tile_init_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p.count,
-                     p.pair_row, R * nq * a.top, i0 == 0 ? p.odd : nullptr));
+                     p.pair_row, R * nq * a.top, i0 == 0 ? p.odd : nullptr, p.largest,
+                     static_cast<int>(R)));
   FKC_TRY(launch_group(a.sel + i0 * a.top, false, static_cast<int64_t>(a.Nq) * a.top, p.inv_order,
                        p.inv_offsets, R, nq * a.top, a.K, p.group_ws, stream));
   FKC_TRY(launch_pdl(tile_units_kernel, dim3(static_cast<unsigned>(R)), dim3(1024), 0, stream, a,

@@ -106,15 +106,17 @@ struct DqSmem {
 constexpr int kGradThreads = 32 * 15;
 
 // kDelta: the sums of P dP over each row's keys instead, two floats a row (one per half of a step's
-// keys), with two S and dP in TMEM in turn since nothing follows them.
+// keys), and behind those of all units' rows the same of P |dP| for fp16 (see Range); with two S and dP in
+// TMEM in turn, since nothing follows them.
 template <typename T, int DP, bool kDelta>
 __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do, RowMap rk,
     RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
     const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
-    const float* __restrict__ row_delta, const Unit* __restrict__ units,
-    const int32_t* __restrict__ start, uint8_t* __restrict__ part, int* err) {
+    const float* __restrict__ row_delta, const float* __restrict__ row_power,
+    const Unit* __restrict__ units, const int32_t* __restrict__ start, uint8_t* __restrict__ part,
+    int64_t units_max, int* err) {
   using namespace ptx;
   using S = DqSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -161,12 +163,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
     bool ok = true;
     SubIter it(units, start);
     int pos_next = -1;
-    float lse_next = 0.f, delta_next = 0.f;
+    float lse_next = 0.f, delta_next = 0.f, power_next = 1.f;
     auto fetch = [&](int64_t first) {
       if (first < 0) return;
       pos_next = __ldg(row_pos + first + row);
       lse_next = __ldg(row_lse + first + row);
       if (!kDelta) delta_next = __ldg(row_delta + first + row);
+      if (!kDelta && Range<T>::kNarrow) power_next = __ldg(row_power + first + row);
     };
     if (it.valid()) fetch(it.row());
     if constexpr (kDelta) {
@@ -175,7 +178,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         const float lse = lse_next;
         fetch(it.next_row());
         const int steps = it.un.steps();
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float sum[4] = {0.f, 0.f, 0.f, 0.f}, mag[4] = {0.f, 0.f, 0.f, 0.f};
         for (int step = 0; step < steps; ++step, ++s_uses) {
           const int keys = it.un.keys(step) - half * 64;  // may be none, but every phase is waited for
           const uint32_t load = it.load + step, buf = s_uses & 1;
@@ -200,6 +203,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
               for (int e = 0; e < 4; ++e) {
                 const float x = ex2(fmaf(s[j + e], sc, -lse)) * dp[j + e];
                 sum[e] += k[e] <= pos ? x : 0.f;
+                if (Range<T>::kNarrow) mag[e] += k[e] <= pos ? fabsf(x) : 0.f;
               }
             }
           }
@@ -208,13 +212,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
           __syncwarp();
           if (lane == 0 && !it.keep) mbar_arrive(smem_u32(&mt.kv_free[st]));
         }
-        if (ok) reinterpret_cast<float*>(part)[(it.row() + row) * 2 + half] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!ok) break;
+        float* to = reinterpret_cast<float*>(part) + (it.row() + row) * 2 + half;
+        *to = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (Range<T>::kNarrow) to[units_max * kUnitRows * 2] = (mag[0] + mag[1]) + (mag[2] + mag[3]);
       }
       if (!ok) give_up(abort, err, kErrDq);
     } else {
     for (; ok && it.valid(); it.advance(), ++uses) {
       const int pos = pos_next;
-      const float lse = lse_next, delta = delta_next;
+      const float lse = lse_next, pw = power_next, delta = delta_next * pw;
       fetch(it.next_row());
       const int steps = it.un.steps();
       for (int step = 0; step < steps; ++step, ++s_uses) {
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
             const int k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float p = ex2(fmaf(s[j + e], sc, -lse)) * (dp[j + e] - delta);
+              const float p = ex2(fmaf(s[j + e], sc, -lse)) * fmaf(dp[j + e], pw, -delta);
               s[j + e] = k[e] <= pos ? p : 0.f;
             }
           }
@@ -269,6 +276,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         uint32_t o[32];
         tmem_ld_32x32b_x32(t_q + c * 32, o);
         tmem_wait_ld();
+        if (Range<T>::kNarrow) {
+          const float back = inverse_power(pw);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
+        }
         put_segment(buf, o, dst + c * kSegment);
       }
       tc_fence_before();
@@ -431,35 +443,46 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
   }
 }
 
-// One thread per (query, head): delta, the sum of its clusters' sums, which are those of the kernels that
-// follow, to their units' rows.
+// One thread per (query, head): delta and the power of two of dS from its clusters' sums, to their units'
+// rows, and the largest A of each row of clusters.
+template <typename T>
 __global__ void __launch_bounds__(256) tiles_delta_join_kernel(Args a, const int32_t* __restrict__ pair_row,
                                                                const float2* __restrict__ part,
+                                                               int64_t units_max,
                                                                float* __restrict__ delta,
-                                                               float* __restrict__ row_delta, int64_t rows) {
+                                                               float* __restrict__ row_delta,
+                                                               float* __restrict__ row_power,
+                                                               float* __restrict__ largest, int64_t rows) {
   pdl_wait();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // (r, i, head)
   if (t >= rows) return;
   const int64_t qi = t / a.G;
   const int h = static_cast<int>(t - qi * a.G), r = static_cast<int>(qi / a.Nq), i = static_cast<int>(qi - static_cast<int64_t>(r) * a.Nq);
   const int32_t* pairs = pair_row + qi * a.top;
-  float sum = 0.f;
-  for (int s0 = 0; s0 < a.top; s0 += 8) {
-    float2 v[8];
+  auto total = [&](const float2* x) {
+    float sum = 0.f;
+    for (int s0 = 0; s0 < a.top; s0 += 8) {
+      float2 v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int n = s0 + u < a.top ? pairs[s0 + u] : -1;
-      v[u] = n >= 0 ? part[static_cast<int64_t>(n) + h] : make_float2(0.f, 0.f);
+      for (int u = 0; u < 8; ++u) {
+        const int n = s0 + u < a.top ? pairs[s0 + u] : -1;
+        v[u] = n >= 0 ? x[static_cast<int64_t>(n) + h] : make_float2(0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += v[u].x + v[u].y;
     }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) sum += v[u].x + v[u].y;
-  }
+    return sum;
+  };
+  const float sum = total(part), A = Range<T>::kNarrow ? total(part + units_max * kUnitRows) : 0.f;
   const int b = r / a.Hkv;
   delta[(static_cast<int64_t>(b) * a.Hq + (r - b * a.Hkv) * a.G + h) * a.Nq + i] = sum;
   for (int s = 0; s < a.top; ++s) {
     const int n = pairs[s];
-    if (n >= 0) row_delta[static_cast<int64_t>(n) + h] = sum;
+    if (n < 0) continue;
+    row_delta[static_cast<int64_t>(n) + h] = sum;
+    if (Range<T>::kNarrow) row_power[static_cast<int64_t>(n) + h] = power(A);
   }
+  if (Range<T>::kNarrow && A < INFINITY) note_largest(largest + r, A);
 }
 
 // One warp per (query, GP heads): dq = scale * the sum of its clusters' parts.
@@ -692,7 +715,7 @@ struct DkvSmem {
   static constexpr uint32_t kDo = 4 * kTile;  // two stages
   static constexpr uint32_t kMeta = 6 * kTile;
   struct Meta {
-    float lse[2][kSub], delta[2][kSub];  // of a stage's rows
+    float lse[2][kSub], delta[2][kSub];  // of a stage's rows; lse less P's shift
     int32_t pos[2][kSub];
     uint64_t kv_full, kv_free, q_full[2], q_free[2], sp_full, ds_full[2], acc_full, acc_free;
     uint64_t drain;
@@ -712,8 +735,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
     RowMap rv, Args a, const int32_t* __restrict__ q_row, const int32_t* __restrict__ do_row,
     const int32_t* __restrict__ row_pos, const float* __restrict__ row_lse,
     const float* __restrict__ row_delta, const KeyTile* __restrict__ tiles,
-    const int64_t* __restrict__ share, const int32_t* __restrict__ start, T* __restrict__ dk,
-    T* __restrict__ dv, float* __restrict__ part, int32_t* __restrict__ odd, int* err) {
+    const int64_t* __restrict__ share, const int32_t* __restrict__ start,
+    const float* __restrict__ largest, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part,
+    int32_t* __restrict__ odd, int* err) {
   using namespace ptx;
   using S = DkvSmem<DP>;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : 1u;
@@ -763,6 +787,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
         const int k = __ldg(a.order + static_cast<int64_t>(it.tile.r) * a.N + it.tile.s0 + row);
         if (k >= 0 && k < a.N) key = k;
       }
+      const float pw = Range<T>::kNarrow ? power(__ldg(largest + it.tile.r)) : 1.f, ds_power = pw * Range<T>::unshift();
       for (int step = it.step; step < it.end; ++step, ++item) {
         const int rows = it.tile.nrows - step * kSub - half * 64;
         if (rows <= 0) continue;
@@ -790,7 +815,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
             for (int e = 0; e < 4; ++e) {
               const bool on = key <= pos[e];
               const float p = ex2(fmaf(s[j + e], sc, -lse[e]));
-              const float ds = p * (dp[j + e] - delta[e]);
+              const float ds = p * ((dp[j + e] - delta[e]) * ds_power);
               s[j + e] = on ? p : 0.f;
               dp[j + e] = on ? ds : 0.f;
             }
@@ -812,7 +837,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
       if (!ok) break;
       tc_fence_after();
       const bool whole = it.step == 0 && it.end == it.tile.steps();
-      const float scale = half == 0 ? 1.f : a.scale;
+      const float scale = half == 0 ? Range<T>::unshift() : a.scale * inverse_power(pw);
       const int b = it.tile.r / a.Hkv, hk = it.tile.r - b * a.Hkv;
       T* out = (half == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + (key == INT_MAX ? 0 : key)) * a.D;
       // a segment that does not begin its tile is the CTA's first
@@ -940,7 +965,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int64_t at = first + mine + x * 32 + lane;
-          lse[x] = __ldg(row_lse + at), delta[x] = __ldg(row_delta + at), pos[x] = __ldg(row_pos + at);
+          lse[x] = __ldg(row_lse + at) - Range<T>::kShift, delta[x] = __ldg(row_delta + at), pos[x] = __ldg(row_pos + at);
         }
       };
       if (it.valid()) fetch(it, it.step);
@@ -998,6 +1023,7 @@ __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTi
                                                              const int64_t* __restrict__ share,
                                                              const int32_t* __restrict__ start, int ctas,
                                                              const float* __restrict__ part,
+                                                             const float* __restrict__ largest,
                                                              T* __restrict__ dk, T* __restrict__ dv) {
   pdl_wait();
   const int j = blockIdx.x;
@@ -1022,7 +1048,8 @@ __global__ void __launch_bounds__(256) tiles_dkv_join_kernel(Args a, const KeyTi
           part + ((static_cast<int64_t>(q) * 2 + (q == j)) * 2 + which) * (kSub * DP) + key * DP + d);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const float scale = which == 0 ? 1.f : a.scale;
+    const float pw = Range<T>::kNarrow ? power(largest[t.r]) : 1.f;
+    const float scale = which == 0 ? Range<T>::unshift() : a.scale * inverse_power(pw);
     const int b = t.r / a.Hkv, hk = t.r - b * a.Hkv;
     T* out = (which == 0 ? dv : dk) + ((static_cast<int64_t>(b) * a.Hkv + hk) * a.N + k) * a.D + d;
     *reinterpret_cast<uint2*>(out) = make_uint2(mma::pack2<T>(s.x * scale, s.y * scale), mma::pack2<T>(s.z * scale, s.w * scale));
@@ -1075,14 +1102,15 @@ int grad_typed(const Args& a, int dtype, const float* lse, float* delta, const T
     const int smem = static_cast<int>(DqSmem<DP>::kBytes);
     FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     return launch_pdl(kern, dim3(ctas), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
-                       q_row, do_row, pos, row_lse, row_delta, static_cast<const Unit*>(l.plan.units),
-                      static_cast<const int32_t*>(l.plan.start), ws + l.part, device_error_word());
+                       q_row, do_row, pos, row_lse, row_delta, static_cast<const float*>(l.plan.row_power),
+                      static_cast<const Unit*>(l.plan.units), static_cast<const int32_t*>(l.plan.start), ws + l.part, l.plan.units_max,
+                      device_error_word());
   };
   FKC_TRY(walk(tiles_dq_kernel<T, DP, true>));
   const int64_t rows = R * a.Nq * a.G;
-  FKC_TRY(launch_pdl(tiles_delta_join_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, stream, a,
+  FKC_TRY(launch_pdl(tiles_delta_join_kernel<T>, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, stream, a,
                      static_cast<const int32_t*>(l.plan.pair_row), reinterpret_cast<const float2*>(ws + l.part),
-                     delta, l.plan.row_delta, rows));
+                     l.plan.units_max, delta, l.plan.row_delta, l.plan.row_power, l.plan.largest, rows));
   if (dq != nullptr) {
     FKC_TRY(walk(tiles_dq_kernel<T, DP, false>));
     const int gp = join_heads(a.G), chunks = (a.G + gp - 1) / gp;
@@ -1112,11 +1140,12 @@ int grad_typed(const Args& a, int dtype, const float* lse, float* delta, const T
   FKC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   FKC_TRY(launch_pdl(kern, dim3(shares), dim3(kGradThreads), smem, stream, tm_q, tm_k, tm_v, tm_do, rk, rv, a,
                      q_row, do_row, pos, row_lse, row_delta, static_cast<const KeyTile*>(tiles),
-                     static_cast<const int64_t*>(share), static_cast<const int32_t*>(start), dk, dv, part,
-                     odd, device_error_word()));
+                     static_cast<const int64_t*>(share), static_cast<const int32_t*>(start),
+                     static_cast<const float*>(l.plan.largest), dk, dv, part, odd, device_error_word()));
   FKC_TRY(launch_pdl(tiles_dkv_join_kernel<T, DP>, dim3(shares, kSub / 4), dim3(256), 0, stream, a,
                      static_cast<const KeyTile*>(tiles), static_cast<const int64_t*>(share),
-                     static_cast<const int32_t*>(start), shares, static_cast<const float*>(part), dk, dv));
+                     static_cast<const int32_t*>(start), shares, static_cast<const float*>(part),
+                     static_cast<const float*>(l.plan.largest), dk, dv));
   return launch_again(a, dtype, odd, lse, delta, dout, dq, l.plan.inv_order, inv, dk, dv, stream);
 }
 

@@ -250,10 +250,10 @@ struct UnitPlan {
   int32_t* pair_row;     // (R, nq * top) unit row of a pair's first head; -1: no key
   int32_t* first_unit;   // (R, K) of clusters that have units
   int32_t* odd;          // a result is not finite (cluster_masked.cu)
-  // for the gradients: row of dout's map, as q_row; lse to base 2 of the row; its delta, which
-  // cluster_attention_tiles_grad.cu sets
+  // for the gradients: row of dout's map, as q_row; lse to base 2 of the row; its delta and the power of
+  // two of its dS, and per row of clusters the largest A (see Range), which cluster_attention_tiles_grad.cu sets
   int32_t* do_row;
-  float *row_lse, *row_delta;
+  float *row_lse, *row_delta, *row_power, *largest;
   void* group_ws;
   int64_t units_max;
 };

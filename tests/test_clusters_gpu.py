@@ -812,3 +812,51 @@ def test_query_gradient_of_keys_with_an_offset(clusters, Nq, top, one, offset):
     for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(clusters.cluster_attention(*a, sel, order, offsets), a, dout)):
         off = ((g.double() - val[name]).norm() / val[name].norm()).item()
         assert off <= 2.0 ** -8 + 2.0 ** -10, (name, off)
+
+
+@pytest.mark.parametrize("Nq,top", [(40, 2), (1000, 3)])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 4096.0])
+def test_gradients_of_fp16_far_from_one(clusters, Nq, top, size):
+    """dout far from 1, some queries 2**10 times farther: P and dS leave fp16's range, the gradients do not.
+    Each keeps the accuracy of two roundings, 2**-11 of the norm, beside fp16's least step in its values."""
+    q, k, v, sel, order, offsets, _ = attention_case(2, 1, 4, Nq, 1500, 6, 64, top, HF, causal=False, drop=0.0)
+    dout = randn(*q.shape, seed=9) * size
+    if size < 1:
+        k = k * 8  # and large keys, that dQ stays above fp16's least values
+        q = q / 8
+        dout[:, :, ::7] *= 2.0 ** -10
+    else:
+        q, k = q / 64, k / 64
+    dout = dout.to(HF)
+    val, _ = attention_ref(q, k, v, sel, order, offsets, None, None, dout)
+    a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(clusters.cluster_attention(*a, sel, order, offsets), a, dout)):
+        want = val[name]
+        off, room = (g.double() - want).norm(), 2.0 ** -10 * want.norm() + 2.0 ** -25 * math.sqrt(want.numel())
+        assert off <= room, (name, (off / want.norm()).item(), (room / want.norm()).item())
+
+
+def test_fp16_products_past_its_range(clusters):
+    """dP far above 65504, and a query whose other keys' weights are all 0."""
+    for Nq in (40, 1000):
+        q, k, v, sel, order, offsets, _ = attention_case(2, 1, 4, Nq, 1500, 6, 64, 3, HF, causal=False, drop=0.0)
+        k[:, :, ::2] *= 2.0 ** -8
+        k[:, :, 1::2] *= 2.0 ** -7
+        v, dout = v * 64, (randn(*q.shape, seed=9) * 4096).to(HF)
+        val, _ = attention_ref(q, k, v, sel, order, offsets, None, None, dout)
+        a = q.detach().requires_grad_(True)
+        (g,) = torch.autograd.grad(clusters.cluster_attention(a, k, v, sel, order, offsets), a, dout)
+        assert (g.double() - val["dq"]).norm() <= 2.0 ** -10 * val["dq"].norm()
+        # scores of +-2000: one key has all of the weight, and its dP is 0
+        k[:] = k.sign() / 4
+        k[:, :, 0] = 16.0
+        q[:] = 8.0
+        v[:, :, 0] = 0
+        sel[..., 0] = torch.searchsorted(offsets[:, 1:].contiguous(), (order == 0).int().argmax(1, keepdim=True).int(), right=True)[:, :, None].int()[..., 0]
+        val, tol = attention_ref(q, k, v, sel, order, offsets, None, None, dout)
+        a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = clusters.cluster_attention(*a, sel, order, offsets)
+        for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, a, dout)):
+            held = val[name].abs() + tol[name] <= 65504  # what fp16 can hold: dv of the one key is larger in places
+            close(g[held], val[name][held], tol[name][held], name)
+            assert not g.isnan().any()
