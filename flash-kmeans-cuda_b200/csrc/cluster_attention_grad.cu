@@ -18,11 +18,9 @@
 //          The four warps take 16 keys each; the sums over all queries and heads of the group
 //          stay in fp32 registers, in ascending query order, so two runs give the same bits.
 //
-// P and dS are rounded to the 16-bit input type for the second products, as their operand
-// type demands, dS into two terms: a row of dQ sums few large dS, and with one term its
-// error against 64 bits was 1.7 times that of its own last rounding, with two 1.2 times (the
-// walk waits for its gather, the second product is free). Sums are fp32 and rounded once on the
-// way out. Keys in no cluster get zeros.
+// P and dS enter the second products as two terms of the 16-bit input type, which their operands have:
+// the gradients are off by their own last rounding (0.0017 of the norm with bf16; with one term each
+// 0.0024). Sums are fp32 and rounded once on the way out. Keys in no cluster get zeros.
 //
 // Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
 // of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
@@ -199,10 +197,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_dq_kernel(Args a, const T* _
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint32_t h = mma::pack2<T>(s[n][2 * e], s[n][2 * e + 1]);
-        const float2 f = mma::unpack2<T>(h);
-        hi[n][e] = mma::movmatrix_trans(h);
-        lo[n][e] = mma::movmatrix_trans(mma::pack2<T>(s[n][2 * e] - f.x, s[n][2 * e + 1] - f.y));
+        uint32_t first, second;
+        mma::split2<T>(s[n][2 * e], s[n][2 * e + 1], first, second);
+        hi[n][e] = mma::movmatrix_trans(first);
+        lo[n][e] = mma::movmatrix_trans(second);
       }
     }
 #pragma unroll
@@ -475,8 +473,8 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
           mma::m16n8k16<T>(dp[n + 1], fv, f[2], f[3]);
         }
       }
-      // rounded, (key g, columns) and (key g + 8, columns); lo: what dS's rounding left
-      uint32_t pp[4][2], ds[4][2], lo[4][2];
+      // in two terms, (key g, columns) and (key g + 8, columns)
+      uint32_t pp[4][2], pl[4][2], ds[4][2], dl2[4][2];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
 #pragma unroll
@@ -492,27 +490,26 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(
           dp[n][e] = on0 ? p0 * ((dp[n][e] - dl) * ds_power) : 0.f;
           dp[n][2 + e] = on1 ? p1 * ((dp[n][2 + e] - dl) * ds_power) : 0.f;
         }
-        pp[n][0] = mma::pack2<T>(ss[n][0], ss[n][1]);
-        pp[n][1] = mma::pack2<T>(ss[n][2], ss[n][3]);
-        ds[n][0] = mma::pack2<T>(dp[n][0], dp[n][1]);
-        ds[n][1] = mma::pack2<T>(dp[n][2], dp[n][3]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 f = mma::unpack2<T>(ds[n][e]);
-          lo[n][e] = mma::pack2<T>(dp[n][2 * e] - f.x, dp[n][2 * e + 1] - f.y);
+          mma::split2_weights<T>(ss[n][2 * e], ss[n][2 * e + 1], pp[n][e], pl[n][e]);
+          mma::split2<T>(dp[n][2 * e], dp[n][2 * e + 1], ds[n][e], dl2[n][e]);
         }
       }
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc) {  // 16 columns as depth
         const uint32_t fp[4] = {pp[2 * cc][0], pp[2 * cc][1], pp[2 * cc + 1][0], pp[2 * cc + 1][1]};
         const uint32_t fd[4] = {ds[2 * cc][0], ds[2 * cc][1], ds[2 * cc + 1][0], ds[2 * cc + 1][1]};
-        const uint32_t fl[4] = {lo[2 * cc][0], lo[2 * cc][1], lo[2 * cc + 1][0], lo[2 * cc + 1][1]};
+        const uint32_t fq[4] = {pl[2 * cc][0], pl[2 * cc][1], pl[2 * cc + 1][0], pl[2 * cc + 1][1]};
+        const uint32_t fl[4] = {dl2[2 * cc][0], dl2[2 * cc][1], dl2[2 * cc + 1][0], dl2[2 * cc + 1][1]};
 #pragma unroll
         for (int nd = 0; nd < KS; ++nd) {
           uint32_t f[4];
           load_b_trans<DP>(f, dt, cc * 16, nd);
           mma::m16n8k16<T>(av[2 * nd], fp, f[0], f[1]);
           mma::m16n8k16<T>(av[2 * nd + 1], fp, f[2], f[3]);
+          mma::m16n8k16<T>(av[2 * nd], fq, f[0], f[1]);
+          mma::m16n8k16<T>(av[2 * nd + 1], fq, f[2], f[3]);
           load_b_trans<DP>(f, qt, cc * 16, nd);
           mma::m16n8k16<T>(ak[2 * nd], fd, f[0], f[1]);
           mma::m16n8k16<T>(ak[2 * nd + 1], fd, f[2], f[3]);

@@ -17,9 +17,8 @@
 // The 128 columns of a step are two halves of 64, a warpgroup each (a thread a row of TMEM), whose
 // products start as each is done. (S and dP of 64 columns at a time, so that one half's
 // products would run beside the other's scores, took twice as long: an MMA of N = 64 costs
-// about as much as one of 128.) P and dS are
-// rounded to the 16-bit input type, as the operand type demands, dS of dQ into two terms
-// (see cluster_attention_grad.cu).
+// about as much as one of 128.) P and dS enter
+// their products as two terms each (cluster_attention_grad.cu).
 //
 // 4096 queries x 4 rows of G = 4, 8 of 64 clusters of 64 keys, D = 128: dQ 140 us and its join 28,
 // dK and dV 129 us and their join 14, rows and tiles listed in 45 (forward and backward together
@@ -251,15 +250,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
               s[j + e] = k[e] <= pos ? p : 0.f;
             }
           }
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            hi[j] = mma::pack2<T>(s[2 * j], s[2 * j + 1]);
-            const float2 f = mma::unpack2<T>(hi[j]);
-            lo[j] = mma::pack2<T>(s[2 * j] - f.x, s[2 * j + 1] - f.y);
-          }
-          tmem_st_32x32b_x16(t_s + c * 16, hi);  // over values that are read already
-          tmem_st_32x32b_x16(t_p + c * 16, lo);
+          split32<T, false>(t_s + c * 32, s);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -313,7 +304,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
         tc_fence_after();
         const uint32_t kt = sb + S::kK + p.stage * S::kTile + half * 64 * 128;
         mma_tmem_rows<4>(tmem + 256, tmem + half * 64, kt, idesc_o, p.ksteps, p.first);
-        mma_tmem_rows<4>(tmem + 256, tmem + 128 + half * 64, kt, idesc_o, p.ksteps, false);
         if (p.last) umma_commit(smem_u32(&mt.dq_full));
       };
       uint32_t n = 0;  // steps
@@ -820,14 +810,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dkv_kernel(
               dp[j + e] = on ? ds : 0.f;
             }
           }
-          uint32_t x[16], y[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            x[j] = mma::pack2<T>(s[2 * j], s[2 * j + 1]);
-            y[j] = mma::pack2<T>(dp[2 * j], dp[2 * j + 1]);
-          }
-          tmem_st_32x32b_x16(t_s + c * 16, x);  // over values that are read already
-          tmem_st_32x32b_x16(t_p + c * 16, y);
+          split32<T, true>(t_s + c * 32, s);
+          split32<T, false>(t_p + c * 32, dp);
         }
         tmem_wait_st();
         tc_fence_before();

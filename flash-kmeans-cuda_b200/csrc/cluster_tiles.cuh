@@ -77,22 +77,41 @@ __device__ __forceinline__ void mma_kmajor(uint32_t d, uint32_t a_tile, uint32_t
   }
 }
 
-// D (+)= A B, A [lanes x 16 * ksteps] in TMEM, B the first 16 * ksteps rows of a tile (MN-major).
-// MOST: the usual number of steps.
+// D (+)= A B, A [lanes x 16 * ksteps] in TMEM as split32 leaves it, B the first 16 * ksteps rows of a tile
+// (MN-major). MOST: the usual number of steps.
 template <int MOST>
 __device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a_tmem, uint32_t b_tile,
                                               uint32_t idesc, int ksteps, bool fresh) {
   constexpr uint32_t hi = ptx::umma_desc_hi(1024, ptx::kLayoutSwizzle128B);
   const uint32_t b = ((b_tile >> 4) & 0x3FFFu) | ((128u * kSub >> 4) << 16);
-  ptx::umma_f16_ta(d, a_tmem, ptx::umma_desc(b, hi), idesc, fresh ? 0u : 1u);
+  auto step = [&](int k, uint32_t accumulate) {
+    const uint32_t at = a_tmem + (k >> 1) * 32 + (k & 1) * 8;
+    const uint64_t rows = ptx::umma_desc(b + k * 128, hi);
+    ptx::umma_f16_ta(d, at, rows, idesc, accumulate);
+    ptx::umma_f16_ta(d, at + 16, rows, idesc, 1u);
+  };
+  step(0, fresh ? 0u : 1u);
   if (ksteps == MOST) {
 #pragma unroll
-    for (int k = 1; k < MOST; ++k)
-      ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc(b + k * 128, hi), idesc, 1u);
+    for (int k = 1; k < MOST; ++k) step(k, 1u);
   } else {
-    for (int k = 1; k < ksteps; ++k)
-      ptx::umma_f16_ta(d, a_tmem + k * 8, ptx::umma_desc(b + k * 128, hi), idesc, 1u);
+    for (int k = 1; k < ksteps; ++k) step(k, 1u);
   }
+}
+// 32 fp32 values of a row as two 16-bit terms each: the first ones in 16 columns, what their rounding
+// left in the 16 behind them, so that they take the place of the 32 columns that they came from.
+// kWeights: values that are not negative.
+template <typename T, bool kWeights>
+__device__ __forceinline__ void split32(uint32_t taddr, const float (&v)[32]) {
+  uint32_t y[32];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if constexpr (kWeights)
+      mma::split2_weights<T>(v[2 * j], v[2 * j + 1], y[j], y[16 + j]);
+    else
+      mma::split2<T>(v[2 * j], v[2 * j + 1], y[j], y[16 + j]);
+  }
+  ptx::tmem_st_32x32b_x32(taddr, y);
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -88,5 +88,30 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// The same as two terms: rounded, and what that left, rounded (2^-18 of the value with bf16).
+template <typename T>
+__device__ __forceinline__ void split2(float lo, float hi, uint32_t& first, uint32_t& second) {
+  first = pack2<T>(lo, hi);
+  const float2 f = unpack2<T>(first);
+  second = pack2<T>(lo - f.x, hi - f.y);
+}
+
+// The same for values that are not negative, as terms that are not either: the first is cut off below
+// the value (2^-16 of it less, so that a value of 16 bits is too), and the second positive wherever the
+// value is, so that a product with an infinity is that infinity and not a sum of two of either sign.
+template <typename T>
+__device__ __forceinline__ void split2_weights(float lo, float hi, uint32_t& first, uint32_t& second) {
+  constexpr float kBelow = 1.f - 0x1p-16f;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(first) : "f"(hi * kBelow), "f"(lo * kBelow));
+    const float2 f = unpack2<T>(first);
+    second = pack2<T>(lo - f.x, hi - f.y);
+  } else {
+    const uint32_t x = __float_as_uint(lo * kBelow), y = __float_as_uint(hi * kBelow);
+    first = __byte_perm(x, y, 0x7632);
+    second = pack2<T>(lo - __uint_as_float(x & 0xFFFF0000u), hi - __uint_as_float(y & 0xFFFF0000u));
+  }
+}
+
 }  // namespace mma
 }  // namespace fkc

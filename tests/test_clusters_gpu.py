@@ -860,3 +860,19 @@ def test_fp16_products_past_its_range(clusters):
             held = val[name].abs() + tol[name] <= 65504  # what fp16 can hold: dv of the one key is larger in places
             close(g[held], val[name][held], tol[name][held], name)
             assert not g.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", [(1, 2, 4, 30, 700, 9, 128, 3), (2, 1, 3, 900, 1300, 17, 80, 5), (1, 1, 16, 400, 2500, 30, 64, 9)])
+def test_attention_is_off_by_its_last_rounding(clusters, dtype, case):
+    """What comes before it (two terms of P and dS, 2**-16; parts, 2**-16; fp32 sums and scores) stays below
+    a fifth of the last rounding, whose error is 2**-9.2 of the norm with bf16 and 2**-12.2 with fp16: together
+    no more than sqrt(1 + 0.04) of it."""
+    q, k, v, sel, order, offsets, pos = attention_case(*case, dtype, seed=2)
+    dout = randn(*q.shape, seed=9).to(dtype)
+    val, _ = attention_ref(q, k, v, sel, order, offsets, pos, None, dout)
+    a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = clusters.cluster_attention(*a, sel, order, offsets, q_pos=pos)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, a, dout))):
+        off, least = (got.double() - val[name]).norm(), (val[name].to(dtype).double() - val[name]).norm()
+        assert off <= 1.02 * least, (name, (off / least).item())
