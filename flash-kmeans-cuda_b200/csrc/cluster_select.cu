@@ -26,7 +26,7 @@
 // products that underflow are covered by the least norm that counts, 2^-50: its square is more than
 // 128 squares below 2^-126 can lose, and D * 2^-22 of two such norms more than D products can.
 //
-// The scores go through memory (4 bytes a score, L2 at the usual sizes). 4096 queries x 256
+// The scores go through L2, in rounds of 64 MB at most. 4096 queries x 256
 // clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 55 us (three CTAs an SM; it was 70 with
 // two and with norms read again from shared memory by half of the warps), choose 42 us
 // (two thirds of the issue slots, some 890 instructions a query: bisection 6 to 8 steps, a border of
@@ -55,7 +55,9 @@ struct SelectArgs {
   const int32_t* order;  // with q_pos
   const int32_t* q_pos;
   const float* bias;  // (R, K) or null
+  int32_t* sel;
   int Hkv, G, Nq, N, K, top, D;
+  int r0, all;  // the round's first row of clusters; queries of the call, of which a round takes Nq from q on
   double scale;
   double unsure;  // how far a score can be off, of |q||c|
 };
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
   const uint32_t qt0 = ct + kClusters * DP * 2;
   pdl_wait();
   const int tile = blockIdx.x % ctiles, rest = blockIdx.x / ctiles;
-  const int qtile = rest % qtiles, r = rest / qtiles;
+  const int qtile = rest % qtiles, lr = rest / qtiles, r = a.r0 + lr;  // lr: the scratch's row
   const int b = r / a.Hkv, hk = r - b * a.Hkv;
   const int c0 = tile * kClusters, i0 = qtile * MQ;
   const T* cen = static_cast<const T*>(a.centroids) + (static_cast<int64_t>(r) * a.K + c0) * a.D;
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
   }
   if (!PACK && norms && t4 < 2) {
     const int i = i0 + wq * 16 + t4 * 8 + g;
-    if (i < a.Nq) q_norm[static_cast<int64_t>(r) * a.Nq + i] = sqrtf(fmaxf(t4 == 0 ? qn[0] : qn[1], kLeastNorm2));
+    if (i < a.Nq) q_norm[static_cast<int64_t>(lr) * a.Nq + i] = sqrtf(fmaxf(t4 == 0 ? qn[0] : qn[1], kLeastNorm2));
   }
   if constexpr (PACK) {
     __syncthreads();
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
     if (tile == 0 && tid < a.Nq) {
       float m = 0.f;
       for (int h = 0; h < a.G; ++h) m = fold_max(m, s_pack[tid * a.G + h]);
-      q_norm[static_cast<int64_t>(r) * a.Nq + tid] = sqrtf(fmaxf(m, kLeastNorm2));
+      q_norm[static_cast<int64_t>(lr) * a.Nq + tid] = sqrtf(fmaxf(m, kLeastNorm2));
     }
     __syncthreads();
 #pragma unroll
@@ -219,17 +221,17 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
     if (lane == 0) s_red[warp] = s;
     __syncthreads();
     if (tid == 0)
-      c_norm[static_cast<int64_t>(r) * ctiles + tile] =
+      c_norm[static_cast<int64_t>(lr) * ctiles + tile] =
           sqrtf(fmaxf(fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), kLeastNorm2));
   }
   const float scale = static_cast<float>(a.scale);
   if constexpr (PACK) {
     for (int i = 0; i < a.Nq && c0 + tid < a.K; ++i) {
       const int pos =
-          a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.Nq + i], a.N) : a.N;
+          a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.all + i], a.N) : a.N;
       float m = -INFINITY;
       for (int h = 0; h < a.G; ++h) m = fmaxf(m, s_pack[(i * a.G + h) * (kClusters + 4) + tid]);
-      scores[(static_cast<int64_t>(r) * a.Nq + i) * a.K + c0 + tid] =
+      scores[(static_cast<int64_t>(lr) * a.Nq + i) * a.K + c0 + tid] =
           s_first[tid] > pos ? __uint_as_float(kNever) : m * scale + s_bias[tid];
     }
   } else {
@@ -238,8 +240,8 @@ __global__ void __launch_bounds__(128, 3) score_kernel(SelectArgs a, float* __re
     const int i = i0 + wq * 16 + half * 8 + g;
     if (i >= a.Nq) continue;
     const int pos =
-        a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.Nq + i], a.N) : a.N;
-    float* row = scores + (static_cast<int64_t>(r) * a.Nq + i) * a.K + c0;
+        a.q_pos != nullptr ? min(a.q_pos[static_cast<int64_t>(b) * a.all + i], a.N) : a.N;
+    float* row = scores + (static_cast<int64_t>(lr) * a.Nq + i) * a.K + c0;
 #pragma unroll
     for (int n = 0; n < NW; ++n) {
       const int cl = (wc * NW + n) * 8 + t4 * 2;
@@ -323,7 +325,7 @@ __device__ __forceinline__ float largest_norm(const float* c_norm, int64_t r, in
 template <typename T, int KPL>
 __global__ void __launch_bounds__(128, KPL <= 8 ? 10 : 4) choose_warp_kernel(
     SelectArgs a, const float* __restrict__ scores, const float* __restrict__ q_norm,
-    const float* __restrict__ c_norm, int ctiles, int32_t* __restrict__ sel, int64_t queries) {
+    const float* __restrict__ c_norm, int ctiles, int64_t queries) {
   __shared__ double s_exact[4][KPL * 32];
   __shared__ uint16_t s_list[4][KPL * 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(128, KPL <= 8 ? 10 : 4) choose_warp_kernel(
       for (int k = 0; k < listed; k += 4) {  // four at a time, eight lanes each
         const int at = k + (lane >> 3);
         const int c = at < listed ? list[at] : -1;
-        const double s = exact_score<T>(a, r, i, c);
+        const double s = exact_score<T>(a, a.r0 + r, i, c);
         if (c >= 0 && (lane & 7) == 0) ex[c] = s;
       }
       __syncwarp();
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(128, KPL <= 8 ? 10 : 4) choose_warp_kernel(
         if (in >> j & 1u) key[j] = 0xFFFFFFFFu;
       from = over == 0xFFFFFFFFu ? over : over + 1u;
     }
-    int32_t* out = sel + qi * a.top;
+    int32_t* out = a.sel + (static_cast<int64_t>(a.r0 + r) * a.all + i) * a.top;
     int done = 0;
 #pragma unroll
     for (int j = 0; j < KPL; ++j) {
@@ -502,7 +504,7 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
 template <typename T>
 __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
     SelectArgs a, const float* __restrict__ scores, const float* __restrict__ q_norm,
-    const float* __restrict__ c_norm, int ctiles, int32_t* __restrict__ sel) {
+    const float* __restrict__ c_norm, int ctiles) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int sums[2][kCtaThreads / 32], red[kCtaThreads / 32];
   __shared__ uint32_t maxima[kCtaThreads / 32];
@@ -575,7 +577,7 @@ __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
       const int c = c0 + (lane >> 3);
       const bool mine = c < a.K && state[c] == 2;
       if (!__any_sync(0xFFFFFFFFu, mine)) continue;
-      const double s = exact_score<T>(a, r, i, mine ? c : -1);
+      const double s = exact_score<T>(a, a.r0 + r, i, mine ? c : -1);
       if (mine && (lane & 7) == 0) ex[c] = s;
     }
     __syncthreads();
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
     }
   }
   __syncthreads();
-  int32_t* out = sel + qi * a.top;
+  int32_t* out = a.sel + (static_cast<int64_t>(a.r0 + r) * a.all + i) * a.top;
   int done = 0;
   for (int c0 = 0; c0 < a.K; c0 += kCtaThreads) {
     const int c = c0 + tid;
@@ -625,13 +627,24 @@ __global__ void __launch_bounds__(kCtaThreads) choose_cta_kernel(
 
 size_t cta_smem(int K) { return align_up(static_cast<size_t>(K) * 13, 16); }
 
+// Rounds of rows, or of one row's queries, whose scores stay below 2^24 (64 MB): the scratch does not
+// grow with the prompt, and the scores are still in L2 when the choice reads them.
 struct SelectLayout {
   size_t scores, q_norm, c_norm, total;
+  int64_t rows, queries;  // of a round, at most
   int ctiles;
 };
 
 SelectLayout select_layout(int64_t R, int64_t Nq, int64_t K) {
   SelectLayout l{};
+  auto even = [](int64_t all, int64_t most) {  // rounds of equal size
+    const int64_t rounds = (all + most - 1) / most;
+    return (all + rounds - 1) / rounds;
+  };
+  constexpr int64_t kScores = 1 << 24;
+  l.queries = even(Nq, std::max<int64_t>(1, kScores / K));
+  l.rows = l.queries < Nq ? 1 : even(R, std::max<int64_t>(1, kScores / (Nq * K)));
+  R = l.rows, Nq = l.queries;
   l.ctiles = static_cast<int>((K + kClusters - 1) / kClusters);
   l.scores = 0;
   l.q_norm = align_up(static_cast<size_t>(R * Nq * K) * 4, 256);
@@ -654,8 +667,7 @@ int score_typed(const SelectArgs& a, int64_t R, float* scores, float* qn, float*
 }
 
 template <typename T>
-int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cudaStream_t stream) {
-  const SelectLayout l = select_layout(R, a.Nq, a.K);
+int select_round(const SelectArgs& a, int64_t R, const SelectLayout& l, uint8_t* ws, cudaStream_t stream) {
   float* scores = reinterpret_cast<float*>(ws + l.scores);
   float* qn = reinterpret_cast<float*>(ws + l.q_norm);
   float* cn = reinterpret_cast<float*>(ws + l.c_norm);
@@ -684,7 +696,7 @@ int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cuda
     const int64_t ctas = std::min<int64_t>((queries + 3) / 4, 148 * (a.K <= 256 ? 30 : 12));
     return launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, stream, a,
                       static_cast<const float*>(scores), static_cast<const float*>(qn),
-                      static_cast<const float*>(cn), l.ctiles, sel, queries);
+                      static_cast<const float*>(cn), l.ctiles, queries);
   }
   const size_t smem = cta_smem(a.K);
   FKC_CUDA_TRY(cudaFuncSetAttribute(choose_cta_kernel<T>,
@@ -692,7 +704,25 @@ int select_dtype(const SelectArgs& a, int64_t R, uint8_t* ws, int32_t* sel, cuda
                                     static_cast<int>(smem)));
   return launch_pdl(choose_cta_kernel<T>, dim3(static_cast<unsigned>(queries)), dim3(kCtaThreads),
                     smem, stream, a, static_cast<const float*>(scores),
-                    static_cast<const float*>(qn), static_cast<const float*>(cn), l.ctiles, sel);
+                    static_cast<const float*>(qn), static_cast<const float*>(cn), l.ctiles);
+}
+
+template <typename T>
+int select_dtype(SelectArgs a, int64_t R, uint8_t* ws, cudaStream_t stream) {
+  const SelectLayout l = select_layout(R, a.all, a.K);
+  const T* q = static_cast<const T*>(a.q);
+  const int32_t* q_pos = a.q_pos;
+  int32_t* sel = a.sel;
+  for (int64_t r0 = 0; r0 < R; r0 += l.rows)
+    for (int64_t i0 = 0; i0 < a.all; i0 += l.queries) {
+      a.r0 = static_cast<int>(r0);
+      a.Nq = static_cast<int>(std::min(l.queries, a.all - i0));
+      a.q = q + i0 * a.qs.n;
+      a.q_pos = q_pos != nullptr ? q_pos + i0 : nullptr;
+      a.sel = sel + i0 * a.top;
+      FKC_TRY(select_round<T>(a, std::min(l.rows, R - r0), l, ws, stream));
+    }
+  return FKC_OK;
 }
 
 }  // namespace
@@ -713,7 +743,8 @@ int launch_select(const Args& f, const void* centroids, const float* bias, doubl
   a.bias = bias;
   a.Hkv = f.Hkv;
   a.G = f.G;
-  a.Nq = f.Nq;
+  a.all = f.Nq;
+  a.sel = sel;
   a.N = f.N;
   a.K = f.K;
   a.top = f.top;
@@ -723,8 +754,8 @@ int launch_select(const Args& f, const void* centroids, const float* bias, doubl
   a.unsure = std::max(std::fabs(scale), 0x1p-126) * (f.D * 0x1p-22 + 0x1p-21);
   const int64_t R = static_cast<int64_t>(f.batch) * f.Hkv;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  return dtype == FKC_DTYPE_F16 ? select_dtype<__half>(a, R, w, sel, stream)
-                                : select_dtype<__nv_bfloat16>(a, R, w, sel, stream);
+  return dtype == FKC_DTYPE_F16 ? select_dtype<__half>(a, R, w, stream)
+                                : select_dtype<__nv_bfloat16>(a, R, w, stream);
 }
 
 }  // namespace attn

@@ -149,3 +149,10 @@ def test_forward_mode_tangents_are_refused():
         for args in ((d, q, q), (q, d, q), (q, q, d)):
             with pytest.raises(RuntimeError, match="tangent"):
                 clusters.cluster_attention(*args, ids[None], ids, ids)
+
+
+def test_selection_scratch_does_not_grow_with_the_prompt():
+    for kw in (dict(n_queries=1 << 16, n_clusters=4096), dict(n_queries=1 << 16, n_clusters=16384),
+               dict(batch=1 << 16, n_queries=3, n_clusters=16384), dict(n_queries=1 << 20, n_clusters=1)):
+        need = L.fkc_cluster_select_workspace_size(ctypes.byref(desc(**kw)))
+        assert 0 < need <= 160 << 20, (kw, need)

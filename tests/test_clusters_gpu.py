@@ -230,6 +230,22 @@ def test_select_many_queries(clusters):
     assert torch.equal(got, select_ref(q, cen, offsets, 13, order, pos))
 
 
+@pytest.mark.parametrize("B,Hkv,G,Nq,K,top", [(1, 2, 1, 3001, 6001, 9), (10, 4, 1, 999, 1001, 5), (2, 1, 2, 8000, 2200, 3)])
+def test_select_rounds(clusters, B, Hkv, G, Nq, K, top):
+    """More scores than one round takes: rounds of a row's queries, and of rows."""
+    D, R = 8, B * Hkv
+    q, cen = randn(B, Hkv * G, Nq, D, seed=1).to(BF), randn(R, K, D, seed=2).to(BF)
+    _, order, offsets = key_clusters(R, 5 * K, K, 3)
+    pos = torch.randint(-1, 5 * K, (B, Nq), generator=gen(4), device="cuda", dtype=torch.int32)
+    bias = randn(R, K, seed=5)
+    got = clusters.cluster_select(q, cen, offsets, top, order=order, q_pos=pos, bias=bias)
+    for r in range(R):
+        b, h = divmod(r, Hkv)
+        for part in torch.arange(Nq, device="cuda").split(1000):
+            want = select_ref(q[b:b + 1, h * G:h * G + G, part], cen[r:r + 1], offsets[r:r + 1], top, order[r:r + 1], pos[b:b + 1, part], bias[r:r + 1])
+            assert torch.equal(got[r:r + 1, part], want)
+
+
 def test_select_infinities(clusters):
     q, cen = randn(1, 2, 4, 16, seed=1).to(BF), randn(1, 6, 16, seed=2).to(BF)
     offsets = torch.arange(7, device="cuda", dtype=torch.int32)[None]
