@@ -632,12 +632,12 @@ __global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq,
   if (me.piece == 0) lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// Queries that one round takes: rounds of equal size whose parts stay below some 2^31 bytes
-// (a round has its own grouping, so short ones cost launches), 64 queries at least.
+// Queries that one round takes: rounds of equal size whose rows take some 1.5 GB (a round has its own
+// grouping, so short ones cost launches), 64 queries at least.
 int64_t queries_per_round(const Args& a) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t per = R * a.top * a.G * ((a.D <= 64 ? 64 : 128) * kPartBytes + 8);
-  const int64_t most = std::max<int64_t>(64, (1ll << 31) / per);
+  const int64_t per = R * a.top * a.G * unit_row_bytes(a);
+  const int64_t most = std::max<int64_t>(64, (3ll << 29) / per);
   const int64_t rounds = (a.Nq + most - 1) / most;
   return (a.Nq + rounds - 1) / rounds;
 }
@@ -747,8 +747,7 @@ size_t carve_units(const Args& a, int64_t nq, bool grad, uint8_t* ws, UnitPlan* 
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
   const int64_t pairs = nq * a.top;
   UnitPlan p{};
-  // every cluster with pairs may end in a unit that is not full
-  p.units_max = R * (pairs * a.G / kUnitRows + std::min<int64_t>(a.K, pairs));
+  p.units_max = units_most(a, nq);
   size_t at = 0;
   auto take = [&](int64_t bytes) -> void* {
     void* q = ws != nullptr ? ws + at : nullptr;
@@ -813,18 +812,17 @@ FormWork form_work(const Args& a, int64_t nq) {
   return w;
 }
 
-bool tiles_fit(const Args& a, int64_t nq) {
+bool tiles_fit(const Args& a, int64_t nq, int64_t bytes) {
   const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t pairs = nq * a.top, DP = a.D <= 64 ? 64 : 128;
+  const int64_t pairs = nq * a.top;
   // 32-bit row numbers; a running maximum of unscaled scores; the gathers' maps
   if (pairs * a.G > (1ll << 30) || !(a.scale > 0.f) ||
       !row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
       !row_map(a.ks, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr) ||
       !row_map(a.vs, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr))
     return false;
-  // units that are not full take workspace too: no more than the full ones, or 2^31 bytes
-  return pairs * a.G >= kSub * static_cast<int64_t>(a.K) ||
-         R * std::min<int64_t>(a.K, pairs) * kUnitRows * DP * kPartBytes <= (1ll << 31);
+  const int64_t rows = units_most(a, nq) * kUnitRows;
+  return rows <= (1ll << 30) && rows * unit_row_bytes(a) <= bytes;
 }
 
 // In us, fitted to calls with D = 128, 8 to 200 keys a cluster, 8 to 2048 rows a cluster and G
@@ -835,10 +833,8 @@ bool tiles_fit(const Args& a, int64_t nq) {
 // 2048 queries x 4 rows, 12 keys a cluster: 188, 322; 24 keys: 315, 324; 64 keys: 408, 195 with
 // 1024 queries.
 bool use_tiles(const Args& a) {
-  const int64_t nq = queries_per_round(a), DP = a.D <= 64 ? 64 : 128;
-  if (!tiles_fit(a, nq)) return false;
-  // a round of few queries of very many sequences: its parts would be 2^32 bytes and more
-  if (static_cast<int64_t>(a.batch) * a.Hkv * nq * a.top * a.G * DP * kPartBytes > (1ll << 32)) return false;
+  const int64_t nq = queries_per_round(a);
+  if (!tiles_fit(a, nq, 1ll << 32)) return false;
   const FormWork w = form_work(a, nq);
   const double walk = 18 + 75e-6 * w.reads;
   const double tiles = 34 + w.units * (0.009 + 0.000136 * w.keys) + 86e-6 * w.rows;

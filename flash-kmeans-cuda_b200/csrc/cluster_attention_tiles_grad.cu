@@ -1150,16 +1150,12 @@ int grad_dtype(const Args& a, int dtype, const float* lse, float* delta, const v
 // rows, 32 clusters of 32 keys: 133, 137. G 16, 64 queries x 8 rows, 32 rows a cluster of 64
 // keys: 408, 389; 2048 queries x 4 rows, 12 keys a cluster: 1061, 1194; 20 keys: 1274, 1182.
 bool use_tiles_grad(const Args& a) {
-  if (!tiles_fit(a, a.Nq)) return false;
+  if (!tiles_fit(a, a.Nq, 1ll << 33)) return false;  // all queries at once
   const FormWork w = form_work(a, a.Nq);
   const double key_tiles = static_cast<double>(a.batch) * a.Hkv * a.K * (w.keys / 64 + 0.5);  // of the walk
   const double walk = 60 + 110e-6 * w.reads + 0.031 * key_tiles + w.rows * (257e-6 + 3.1e-6 * w.keys);
   const double tiles = 61 + w.units * (0.019 + 0.00039 * w.keys) + 260e-6 * w.rows + 0.002 * key_tiles;
-  if (1.1 * tiles >= walk) return false;
-  // all queries at once: 32-bit rows of units, and parts of 2^33 bytes at most
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.Hkv * (static_cast<int64_t>(a.Nq) * a.top * a.G + static_cast<int64_t>(a.K) * kUnitRows);
-  return rows <= (1ll << 30) && rows * (a.D <= 64 ? 64 : 128) * kPartBytes <= (1ll << 33) &&
-         static_cast<int64_t>(a.Nq) * a.top * a.G <= (1ll << 30);
+  return 1.1 * tiles < walk;
 }
 
 size_t tiles_backward_workspace_bytes(const Args& a) { return grad_layout(a, nullptr).total; }

@@ -290,7 +290,16 @@ struct FormWork {
   double keys, rows, reads, units;
 };
 FormWork form_work(const Args& a, int64_t nq);
-bool tiles_fit(const Args& a, int64_t nq);  // whether the form by clusters can take the call
+// Whether the form by clusters can take nq queries at once, the scratch of their units' rows (nearly
+// all there is) within `bytes`.
+bool tiles_fit(const Args& a, int64_t nq, int64_t bytes);
+inline int64_t unit_row_bytes(const Args& a) {  // the part, and up to eight words beside it
+  return (a.D <= 64 ? 64 : 128) * kPartBytes + 32;
+}
+inline int64_t units_most(const Args& a, int64_t nq) {  // every cluster with pairs may end in one that is not full
+  const int64_t pairs = nq * a.top;
+  return static_cast<int64_t>(a.batch) * a.Hkv * (pairs * a.G / kUnitRows + std::min<int64_t>(a.K, pairs));
+}
 
 // A CTA's units [start[blockIdx.x], start[blockIdx.x + 1]) in turn. The next one is fetched while
 // one is worked on, and nothing but its turn waits for it. Keys and values are loaded into two

@@ -156,3 +156,15 @@ def test_selection_scratch_does_not_grow_with_the_prompt():
                dict(batch=1 << 16, n_queries=3, n_clusters=16384), dict(n_queries=1 << 20, n_clusters=1)):
         need = L.fkc_cluster_select_workspace_size(ctypes.byref(desc(**kw)))
         assert 0 < need <= 160 << 20, (kw, need)
+
+
+def test_attention_scratch_is_bounded():
+    """Whatever the sizes: 4 GB of units' rows for out and 8 GB for the gradients, a quarter more with all."""
+    for batch, kv, group, nq, n, clusters, top in [(1, 8, 4, 1 << 15, 1 << 15, 512, 16), (1, 8, 4, 1 << 17, 1 << 17, 2048, 64), (64, 8, 8, 4096, 8192, 128, 32),
+                                                   (256, 8, 16, 64, 4096, 64, 64), (1024, 8, 4, 64, 2048, 1024, 16), (1, 1, 128, 1 << 15, 1 << 15, 64, 64)]:
+        for head_dim in (64, 128):
+            d = desc(batch=batch, q_heads=kv * group, kv_heads=kv, n_queries=nq, n_keys=n, n_clusters=clusters, top_k=top, head_dim=head_dim,
+                     q_stride=(kv * group * nq * head_dim, nq * head_dim, head_dim), k_stride=(kv * n * head_dim, n * head_dim, head_dim),
+                     v_stride=(kv * n * head_dim, n * head_dim, head_dim))
+            assert L.fkc_cluster_attention_workspace_size(ctypes.byref(d)) <= 5 << 30
+            assert L.fkc_cluster_attention_grad_workspace_size(ctypes.byref(d)) <= 10 << 30
