@@ -813,8 +813,6 @@ FormWork form_work(const Args& a, int64_t nq) {
 }
 
 bool tiles_fit(const Args& a, int64_t nq, int64_t bytes) {
-  const int64_t R = static_cast<int64_t>(a.batch) * a.Hkv;
-  const int64_t pairs = nq * a.top;
   // 32-bit row numbers; a running maximum of unscaled scores; the gathers' maps
   if (pairs * a.G > (1ll << 30) || !(a.scale > 0.f) ||
       !row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||

@@ -84,8 +84,9 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ 
 #pragma unroll
       for (int u = 0; u < kRows; ++u) {
         if (r0 + u >= total) break;
+        const float f = src[u] >= 0 ? scale : 0.f;  // zeros whatever the scale is
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[u].v[e] = from_f32<T>(to_f32<T>(v[u].v[e]) * scale);
+        for (int e = 0; e < VEC; ++e) v[u].v[e] = from_f32<T>(to_f32<T>(v[u].v[e]) * f);
         out[(r0 + u) * nvec + c] = v[u];
       }
     }

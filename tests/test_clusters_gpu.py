@@ -892,3 +892,10 @@ def test_attention_is_off_by_its_last_rounding(clusters, dtype, case):
     for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, a, dout))):
         off, least = (got.double() - val[name]).norm(), (val[name].to(dtype).double() - val[name]).norm()
         assert off <= 1.02 * least, (name, (off / least).item())
+
+
+def test_lookup_of_no_row_is_zero_whatever_the_scale(clusters):
+    t, ids = randn(5, 24).to(BF), torch.tensor([-1, 2, 5], device="cuda")
+    for scale in (math.inf, math.nan):
+        y = clusters.cluster_lookup(t, ids, scale=scale)
+        assert y[0].eq(0).all() and y[2].eq(0).all() and not y[1].isfinite().any()
