@@ -814,7 +814,7 @@ FormWork form_work(const Args& a, int64_t nq) {
 
 bool tiles_fit(const Args& a, int64_t nq, int64_t bytes) {
   // 32-bit row numbers; a running maximum of unscaled scores; the gathers' maps
-  if (pairs * a.G > (1ll << 30) || !(a.scale > 0.f) ||
+  if (!(a.scale > 0.f) ||
       !row_map(a.qs, a.batch, a.Hq, a.Nq, a.D, nullptr, nullptr) ||
       !row_map(a.ks, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr) ||
       !row_map(a.vs, a.batch, a.Hkv, a.N, a.D, nullptr, nullptr))
