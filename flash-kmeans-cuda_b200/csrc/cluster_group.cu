@@ -4,7 +4,7 @@
 // slot comes after offsets[b, K] and holds -1.
 //
 // A stable least-significant-digit radix sort of (id, position), in digits of
-// at most 11 bits: one pass up to K = 2046, two up to 4 M. Per pass
+// at most 11 bits: one pass up to K = 2047, two up to 4 M. Per pass
 //   hist     (group_hist_kernel)    digit counts of chunks of R positions;
 //   prefix   (group_prefix_kernel)  exclusive sums over the chunks per digit, and
 //            the digit totals of the row (where there are few, the scatter does it);
@@ -336,9 +336,10 @@ int group_pass(const GroupGeom& g, const GroupBuffers& w, const Id* keys_in, int
   const int bins = 1 << g.bits, shift = pass * g.bits;
   const int n = static_cast<int>(N), k = static_cast<int>(K);
   const dim3 grid(static_cast<unsigned>(B * g.C));
-  // few counts are summed by every CTA of the scatter, which saves a launch: 16 chunks x 256 digits,
-  // two passes, 4 us less; 8 x 2048 7 us more, 32 x 1024 3 us more
-  const bool sums = g.C * bins <= 4096;
+  // few counts are summed by every CTA of the scatter, which saves a launch. Measured, with the launch
+  // and without: 16 chunks of 512 digits 9.5, 8.7 us; 32 of 512 18.2, 18.5; 64 of 512 11.9, 11.6; 5 of
+  // 2048 11.1, 13.0; 256 of 32 11.5, 19.5
+  const bool sums = bins <= 512 && g.C <= 64;
   if (g.C > 1) {
     FKC_TRY(launch_pdl(group_hist_kernel<Id>, grid, dim3(kThreads), bins * 4, stream, keys_in,
                        stride, n, k, g.R, g.C, shift, g.bits, w.hist));

@@ -285,14 +285,14 @@ int lanes_log2(int64_t nvec, int most) {
   return l;
 }
 
-// Positions per block: longer blocks for longer rows of ids, so that neither a block's sum (Lb
-// rows) nor a cluster's join (N / Lb partial rows) becomes a long chain; shorter ones where a
-// row of the table is wider than a warp, since a group then passes its rows several times
-// (16384 ids, rows of 1024 bf16: 88 us at 64, a cluster of 128 rows taking 64 flights).
-int block_len(int64_t N, int64_t row_bytes) {
-  const bool wide = row_bytes > 512;
-  int lb = wide ? 16 : 64;
-  while (lb < 512 && static_cast<int64_t>(lb) * lb * (wide ? 64 : 4) < N) lb *= 2;
+// Positions per block: longer blocks for longer rows of ids, so that neither a block's sum (Lb rows) nor a
+// cluster's join (N / Lb partial rows) becomes a long chain. Forward and gradient in us with 16, 32, 64 and
+// 128, over tables of 8, 500 and 50000 rows: 4096 ids, rows of 2 KB: 31 31 76, 25 32 83, 23 44 108, -;
+// 8192: 45 35 84, 34 35 79, 29 43 99, -; 16385, 128 bytes: 49 30 42, 33 27 40, 31 30 42, 38 38 49;
+// 32768, 128 bytes: 79 41 48, 50 32 43, 38 32 47, 41 39 52; 65536, 512 bytes: -, 103 55 85, 62 46 93, 51 51 117.
+int block_len(int64_t N) {
+  int lb = 16;
+  while (lb < 512 && static_cast<int64_t>(lb) * lb * 24 < N) lb *= 2;
   return lb;
 }
 
@@ -307,9 +307,9 @@ struct GradLayout {
   int64_t J;
 };
 
-GradLayout grad_layout(int64_t B, int64_t N, int64_t K, int64_t D, int64_t elem) {
+GradLayout grad_layout(int64_t B, int64_t N, int64_t K, int64_t D) {
   GradLayout l{};
-  l.Lb = block_len(N, D * elem);
+  l.Lb = block_len(N);
   l.J = (N + l.Lb - 1) / l.Lb;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -351,7 +351,7 @@ int lookup_typed(const void* table, const void* ids, bool ids_64, void* y, int64
 template <typename T, int VEC>
 int grad_typed(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B, int64_t N,
                int64_t K, int64_t D, float scale, uint8_t* ws, cudaStream_t stream) {
-  const GradLayout l = grad_layout(B, N, K, D, sizeof(T));
+  const GradLayout l = grad_layout(B, N, K, D);
   int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + l.offsets);
   float* part = reinterpret_cast<float*>(ws + l.part);
@@ -408,7 +408,7 @@ int launch_lookup(const void* table, const void* ids, bool ids_64, void* y, int6
 }
 
 size_t lookup_grad_workspace_bytes(int64_t B, int64_t N, int64_t K, int64_t D) {
-  return std::max(grad_layout(B, N, K, D, 2).total, grad_layout(B, N, K, D, 4).total);
+  return grad_layout(B, N, K, D).total;
 }
 
 int launch_lookup_grad(const void* dy, const void* ids, bool ids_64, void* dt, int64_t B,
