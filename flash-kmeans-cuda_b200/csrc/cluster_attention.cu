@@ -314,17 +314,6 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict_
   if (lane == 0) lse[row] = sum == 0.f ? -INFINITY : base + log2f(sum) * kLn2;
 }
 
-// Warps per query row: the keys of one are split while there are fewer warps than
-// the GPU holds at once (148 SMs x 8; one more would start a second wave), a part taking
-// at least 4 tiles of the average selection (top * N / K keys).
-int split_count(const Args& a) {
-  const int64_t chunks = (a.G + 15) / 16;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.Hkv * a.Nq * chunks;
-  const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.top) * ((a.N + a.K - 1) / a.K), a.N);
-  const int64_t most = std::max<int64_t>(1, keys / (4 * kTile));
-  return static_cast<int>(std::min<int64_t>({most, std::max<int64_t>(1, 148 * 8 / rows), 64}));
-}
-
 template <typename T, int DP, int NT>
 int fwd_typed(const Args& a, void* out, float* lse, float* ws, cudaStream_t stream) {
   constexpr int STAGES = 3;
@@ -356,6 +345,17 @@ int fwd_dtype(const Args& a, void* out, float* lse, float* ws, cudaStream_t stre
 }
 
 }  // namespace
+
+// Warps per query row: the keys of one are split while there are fewer warps than
+// the GPU holds at once (148 SMs x 8; one more would start a second wave), a part taking
+// at least 4 tiles of the average selection (top * N / K keys).
+int split_count(const Args& a) {
+  const int64_t chunks = (a.G + 15) / 16;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.Hkv * a.Nq * chunks;
+  const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.top) * ((a.N + a.K - 1) / a.K), a.N);
+  const int64_t most = std::max<int64_t>(1, keys / (4 * kTile));
+  return static_cast<int>(std::min<int64_t>({most, std::max<int64_t>(1, 148 * 8 / rows), 64}));
+}
 
 size_t forward_workspace_bytes(const Args& a) {
   if (use_tiles(a)) return tiles_forward_workspace_bytes(a);

@@ -157,6 +157,7 @@ int sm_count();  // of the current device
 size_t select_workspace_bytes(int64_t R, int64_t Nq, int64_t K);
 int launch_select(const Args& a, const void* centroids, const float* bias, double scale, int dtype,
                   int32_t* sel, void* ws, cudaStream_t stream);
+int split_count(const Args& a);  // warps that share the keys of a query in the walk
 size_t forward_workspace_bytes(const Args& a);
 int launch_forward(const Args& a, int dtype, void* out, float* lse, void* ws, cudaStream_t stream);
 // The form by clusters (cluster_attention_tiles.cu), taken where use_tiles says so.

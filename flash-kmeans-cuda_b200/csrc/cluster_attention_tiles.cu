@@ -802,6 +802,7 @@ int launch_units(const Args& a, int64_t i0, int64_t nq, const RowMap& rq, const 
 FormWork form_work(const Args& a, int64_t nq) {
   const double R = static_cast<double>(a.batch) * a.Hkv, pairs = static_cast<double>(nq) * a.top;
   FormWork w;
+  w.width = a.D <= 64 ? 0.5 : 1.0;
   w.keys = static_cast<double>(a.N) / a.K;
   w.rows = R * a.Nq * a.top * a.G;
   w.reads = R * a.Nq * a.top * w.keys * (a.G <= 8 ? 1.0 : 1.2 * ((a.G + 15) / 16));
@@ -823,20 +824,21 @@ bool tiles_fit(const Args& a, int64_t nq, int64_t bytes) {
   return rows <= (1ll << 30) && rows * unit_row_bytes(a) <= bytes;
 }
 
-// In us, fitted to calls with D = 128, 8 to 200 keys a cluster, 8 to 2048 rows a cluster and G
-// from 1 to 32: within 8% on average, 25% at worst. The walk, which needs no workspace, keeps what
-// is within a tenth. Measured (walk, by clusters):
-// G 1, 512 queries, 32 clusters of 64 keys: 35, 39; of 128 keys: 53, 41. G 4, 64 queries x 8
-// rows, 8 rows a cluster of 64 keys: 59, 113; 256 queries, 32 rows a cluster: 174, 129. G 16,
-// 2048 queries x 4 rows, 12 keys a cluster: 188, 322; 24 keys: 315, 324; 64 keys: 408, 195 with
-// 1024 queries.
+// In us, fitted to 200 calls of 8 to 200 keys a cluster, 32 to 4096 queries, 1 to 32 heads a row and 1 to 32
+// clusters a query, both widths and types (the walk within 16% on average, this form within 9%): the
+// form that it chooses took 0.5% longer on average than the faster one. The walk's last term is the
+// chain of one warp's key tiles. Measured (walk, by clusters), D = 128 but for the last two:
+// G 8, 218 queries x 8 rows, 4 of 64 clusters of 64 keys: 45, 45. G 4, 375 x 1, 16 of 512 of 100: 46, 49;
+// 142 x 4, 8 of 64 of 100: 37, 35; 2191 x 4, 16 of 256 of 100: 930, 171. G 16, 996 x 4, 3 of 16 of 12:
+// 43, 71. G 1, 886 x 8, 2 of 16 of 32: 50, 35. D = 64: G 4, 444 x 4, 3 of 64 of 16: 8, 29. G 1, 2139 x 4,
+// 16 of 16 of 100: 480, 58.
 bool use_tiles(const Args& a) {
   const int64_t nq = queries_per_round(a);
   if (!tiles_fit(a, nq, 1ll << 32)) return false;
   const FormWork w = form_work(a, nq);
-  const double walk = 18 + 75e-6 * w.reads;
-  const double tiles = 34 + w.units * (0.009 + 0.000136 * w.keys) + 86e-6 * w.rows;
-  return 1.1 * tiles < walk;
+  const double walk = 7.9 + 79.7e-6 * w.reads * w.width + 0.0705 * a.top * w.keys / 16 / split_count(a);
+  const double tiles = 27.8 + w.units * (0.0079 + 0.000162 * w.keys * w.width) + w.rows * (38e-6 + 111e-6 * w.width);
+  return tiles < walk;
 }
 
 size_t tiles_forward_workspace_bytes(const Args& a) { return fwd_layout(a, nullptr).total; }

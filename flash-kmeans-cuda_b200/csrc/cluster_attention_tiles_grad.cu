@@ -1144,18 +1144,21 @@ int grad_dtype(const Args& a, int dtype, const float* lse, float* delta, const v
 
 }  // namespace
 
-// In us, as use_tiles, fitted when the walk took one pass for dQ; its second pass reads the keys
-// again, 42 of the 110 us per million reads. Measured then (walk, by clusters, forward included): G 1, 256
-// queries x 8 rows, 8 rows a cluster of 24 keys: 297, 358; of 64: 576, 418. G 8, 256 queries x 4
-// rows, 32 clusters of 32 keys: 133, 137. G 16, 64 queries x 8 rows, 32 rows a cluster of 64
-// keys: 408, 389; 2048 queries x 4 rows, 12 keys a cluster: 1061, 1194; 20 keys: 1274, 1182.
+// In us, as use_tiles, fitted to the gradients of the same calls (the walk within 16% on average, this form
+// within 9%): the form that it chooses took 1.8% longer on average than the faster one. The
+// walk's chains: a warp's key tiles, twice, and a CTA's columns. Measured (walk, by clusters), the
+// gradients alone, D = 128 but for the last two:
+// G 1, 171 queries x 2 rows, 16 of 256 clusters of 24 keys: 95, 98; 348 x 2, 16 of 128 of 24: 94, 80. G 4,
+// 409 x 4, 8 of 256 of 32: 156, 142. G 32, 190 x 2, 16 of 128 of 16: 177, 195; 3296 x 1, 3 of 16 of 8:
+// 1906, 273. D = 64: G 4, 1297 x 8, 2 of 32 of 24: 90, 117; 2356 x 4, 3 of 32 of 24: 153, 134.
 bool use_tiles_grad(const Args& a) {
   if (!tiles_fit(a, a.Nq, 1ll << 33)) return false;  // all queries at once
   const FormWork w = form_work(a, a.Nq);
-  const double key_tiles = static_cast<double>(a.batch) * a.Hkv * a.K * (w.keys / 64 + 0.5);  // of the walk
-  const double walk = 60 + 110e-6 * w.reads + 0.031 * key_tiles + w.rows * (257e-6 + 3.1e-6 * w.keys);
-  const double tiles = 61 + w.units * (0.019 + 0.00039 * w.keys) + 260e-6 * w.rows + 0.002 * key_tiles;
-  return 1.1 * tiles < walk;
+  const double columns = static_cast<double>(a.Nq) * a.top * a.G / a.K;  // of a cluster
+  const double walk = 35.7 + 107.6e-6 * w.reads * w.width + 1.27 * a.top * w.keys / 16 + 1.85 * columns / 32 +
+                      575e-6 * w.rows * (w.keys / 64 + 0.5) * w.width;
+  const double tiles = 63.9 + w.units * (0.0274 + 0.000535 * w.keys * w.width) + w.rows * (165e-6 + 326e-6 * w.width);
+  return tiles < walk;
 }
 
 size_t tiles_backward_workspace_bytes(const Args& a) { return grad_layout(a, nullptr).total; }

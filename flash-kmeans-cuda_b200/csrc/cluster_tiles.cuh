@@ -285,9 +285,9 @@ constexpr int kMaxCtas = 1024;
 
 // What the choice between the two forms weighs, with nq queries a round: keys of a cluster on
 // average, (query, slot, head) rows, keys that the walk reads (of more than 8 heads, more than
-// once), units.
+// once), units, and the width of the tiles' columns, of 128.
 struct FormWork {
-  double keys, rows, reads, units;
+  double keys, rows, reads, units, width;
 };
 FormWork form_work(const Args& a, int64_t nq);
 // Whether the form by clusters can take nq queries at once, the scratch of their units' rows (nearly
