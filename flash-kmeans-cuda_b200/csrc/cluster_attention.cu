@@ -26,10 +26,10 @@
 // parts by their log-sum-exp.
 //
 // 16 sequences x 8 rows, one query each, 64 of 1024 clusters, D = 128: on average 3425 keys a query,
-// 224 MB, in 50 us, 4.5 TB/s (the join 5 us, with eight parts' loads in flight; one after another
+// 224 MB, in 52 us, 4.3 TB/s (the join 5 us, with eight parts' loads in flight; one after another
 // they took 8). While its SMs are busy the walk moves some 6 TB/s; it loses a fifth to the
 // largest queries, whose warps end last (twice as many, shorter parts: 64 us, since each warp
-// builds its list). One query of 512 keys: 10 us, a chain of list, gather, products and join.
+// builds its list). One query of 512 keys: 11 us, a chain of list, gather, products and join.
 #include <algorithm>
 
 #include "cluster_attention.cuh"

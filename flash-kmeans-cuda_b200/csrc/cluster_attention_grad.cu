@@ -22,9 +22,10 @@
 // the gradients are off by their own last rounding (0.0017 of the norm with bf16; with one term each
 // 0.0024). Sums are fp32 and rounded once on the way out. Keys in no cluster get zeros.
 //
-// Bound by the products and the gathers that feed them: 14 * D flops per (query head, key) pair,
-// of which dK, dV do 8 (S and dP are formed in both walks). 256 queries x 8 rows of 1 head, 16 of
-// 512 clusters of 24 keys: 219 us with one pass of dQ (by clusters 256); 2048 queries: 678 us (by clusters 274).
+// Bound by the products and the gathers that feed them: 24 * D flops per (query head, key) pair, of which
+// the formulas need 10: S and dP are formed three times and the other three products have two terms. 256
+// queries x 8 rows of 1 head, 16 of 512 clusters of 24 keys: 296 us (by clusters 330); 2048 queries: 1186 us
+// (by clusters 368).
 #include <algorithm>
 
 #include "cluster_attention.cuh"

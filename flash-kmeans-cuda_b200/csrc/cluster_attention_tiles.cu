@@ -19,12 +19,12 @@
 // call below from 551 to 615 us, out's error against 64 bits from 0.0023 of its norm to 0.0017.
 //
 // At 4096 queries x 8 rows of G = 4, 16 of 256 clusters of 64 keys, D = 128 (2.1 M (query, slot,
-// head) rows, 69 GFLOP): the units and rows are listed in 46 us, tiles_fwd_kernel takes 336 us, the
-// join 112 us (the call 484 us: they overlap at their ends; the larger of the skewed clusters are
+// head) rows, 69 GFLOP): the units and rows are listed in 55 us, tiles_fwd_kernel takes 383 us, the
+// join 174 us (the call 614 us: each from cold caches alone; the larger of the skewed clusters are
 // selected more often, 1779 keys a query instead of 1024, which makes it 119 GFLOP). The kernel is bound by its
-// SMs' instruction issue (48% of all slots, softmax and output) and by the gathers, which it waits
-// for at the start of every unit; its tensor pipe is busy for 22% of the time and DRAM for a
-// third (800 MB: the parts do not fit L2, Q rows come from it). The join moves 564 MB at 5.1 TB/s.
+// SMs' instruction issue (50% of all slots, softmax and output) and by the gathers, which it waits
+// for at the start of every unit; its tensor pipe is busy for 29% of the time and DRAM for near a
+// half (1.1 GB: the parts do not fit L2, Q rows come from it). The join moves 824 MB at 4.7 TB/s.
 // What was measured on the way, the same call: the walk 3860 us; by clusters with warp-level
 // matrix instructions 1250; tcgen05 with operands copied 16 bytes a thread 940, by row gathers
 // 900; rows listed beforehand instead of by the gathering warps 740; shares by cost, kept keys,

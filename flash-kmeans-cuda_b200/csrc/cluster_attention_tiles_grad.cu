@@ -20,12 +20,14 @@
 // about as much as one of 128.) P and dS enter
 // their products as two terms each (cluster_attention_grad.cu).
 //
-// 4096 queries x 4 rows of G = 4, 8 of 64 clusters of 64 keys, D = 128: dQ 140 us and its join 28,
-// dK and dV 129 us and their join 14, rows and tiles listed in 45 (forward and backward together
-// 492 us). The two large kernels are bound by the chain of one 128-row step: gathered rows, two
-// score products, the warpgroups' turn (a thread a row, 64 columns), two or four products; the
-// tensor pipe is busy for 24% and 33%. The walk took 2200 us for the gradients, warp-level matrix
-// instructions as little; scores of 64 columns at a time 630 us, joins of single heads 560.
+// 4096 queries x 4 rows of G = 4, 8 of 64 clusters of 64 keys, D = 128: delta 108 us and its join 6, dQ 155
+// and its join 41, dK and dV 173 and their join 14, rows and tiles listed in 55 (forward and backward
+// together 682 us; with delta from out, one term of P and of dK's dS and parts of two bytes 494). The
+// three large kernels are bound by the chain of one 128-row step: gathered rows (twice the warps
+// gathering them took 4% off delta's), two score products, the warpgroups' turn (a thread a row, 64
+// columns), two or four products; the tensor pipe is busy for 16%, 22% and 37%. The walk took 2200 us for
+// the gradients, warp-level matrix instructions as little; scores of 64 columns at a time 630 us, joins of
+// single heads 560.
 #include <algorithm>
 
 #include "cluster_tiles.cuh"
@@ -218,67 +220,67 @@ __global__ void __launch_bounds__(kGradThreads, 1) tiles_dq_kernel(
       }
       if (!ok) give_up(abort, err, kErrDq);
     } else {
-    for (; ok && it.valid(); it.advance(), ++uses) {
-      const int pos = pos_next;
-      const float lse = lse_next, pw = power_next, delta = delta_next * pw;
-      fetch(it.next_row());
-      const int steps = it.un.steps();
-      for (int step = 0; step < steps; ++step, ++s_uses) {
-        const int keys = it.un.keys(step) - half * 64;
-        if (keys <= 0) continue;
-        const uint32_t load = it.load + step;
-        const int st = load & 1;
-        ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
-             warp_mbar_wait(&mt.sp_full[0], s_uses & 1, abort);
+      for (; ok && it.valid(); it.advance(), ++uses) {
+        const int pos = pos_next;
+        const float lse = lse_next, pw = power_next, delta = delta_next * pw;
+        fetch(it.next_row());
+        const int steps = it.un.steps();
+        for (int step = 0; step < steps; ++step, ++s_uses) {
+          const int keys = it.un.keys(step) - half * 64;
+          if (keys <= 0) continue;
+          const uint32_t load = it.load + step;
+          const int st = load & 1;
+          ok = warp_mbar_wait(&mt.k_full[st], (load >> 1) & 1, abort) &&
+               warp_mbar_wait(&mt.sp_full[0], s_uses & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const int32_t* key = mt.key[st] + half * 64;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            if (c * 32 >= keys) break;
+            float s[32], dp[32];
+            tmem_ld_f32_x32(t_s + c * 32, s);
+            tmem_ld_f32_x32(t_p + c * 32, dp);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
+              const int k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float p = ex2(fmaf(s[j + e], sc, -lse)) * fmaf(dp[j + e], pw, -delta);
+                s[j + e] = k[e] <= pos ? p : 0.f;
+              }
+            }
+            split32<T, false>(t_s + c * 32, s);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(smem_u32(&mt.ds_full[half]));
+        }
+        if (ok) ok = warp_mbar_wait(&mt.dq_full, uses & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const int32_t* key = mt.key[st] + half * 64;
+        const int64_t urow = it.row() + row;
+        const uint32_t buf = sb + S::kOut + warp * 4096;
+        uint8_t* dst = part + (urow - lane) * (DP * kPartBytes);
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          if (c * 32 >= keys) break;
-          float s[32], dp[32];
-          tmem_ld_f32_x32(t_s + c * 32, s);
-          tmem_ld_f32_x32(t_p + c * 32, dp);
+        for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {  // the segments are shared out
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_q + c * 32, o);
           tmem_wait_ld();
+          if (Range<T>::kNarrow) {
+            const float back = inverse_power(pw);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const int4 k4 = *reinterpret_cast<const int4*>(key + c * 32 + j);
-            const int k[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float p = ex2(fmaf(s[j + e], sc, -lse)) * fmaf(dp[j + e], pw, -delta);
-              s[j + e] = k[e] <= pos ? p : 0.f;
-            }
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
           }
-          split32<T, false>(t_s + c * 32, s);
+          put_segment(buf, o, dst + c * kSegment);
         }
-        tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&mt.ds_full[half]));
+        mbar_arrive(smem_u32(&mt.dq_free));
       }
-      if (ok) ok = warp_mbar_wait(&mt.dq_full, uses & 1, abort);
-      if (!ok) break;
-      tc_fence_after();
-      const int64_t urow = it.row() + row;
-      const uint32_t buf = sb + S::kOut + warp * 4096;
-      uint8_t* dst = part + (urow - lane) * (DP * kPartBytes);
-#pragma unroll 1
-      for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {  // the segments are shared out
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(t_q + c * 32, o);
-        tmem_wait_ld();
-        if (Range<T>::kNarrow) {
-          const float back = inverse_power(pw);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
-        }
-        put_segment(buf, o, dst + c * kSegment);
-      }
-      tc_fence_before();
-      mbar_arrive(smem_u32(&mt.dq_free));
-    }
-    if (!ok) give_up(abort, err, kErrDq);
-    if (lane == 0) bulk_wait_all();
+      if (!ok) give_up(abort, err, kErrDq);
+      if (lane == 0) bulk_wait_all();
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------ MMAs (one thread)

@@ -17,11 +17,12 @@
 //     one that reaches over its start (slot 0) and one that begins in it (slot 1);
 //   * grad_join_kernel adds a large cluster's partial rows in block order.
 //
-// 16384 ids of skewed frequency, table 50000 x 1024 bf16, forward and gradient: 101 us (lookup
-// 14 us, gradient 55 us: 34 MB read, 102 MB written, of which 46 MB reach DRAM within the kernel);
-// 32 x 16384 ids, tables 1024 x 64 fp32: 104 us (lookup 36 us: 268 MB through L2; gradient 45 us
+// 16384 ids of skewed frequency, table 50000 x 1024 bf16, forward and gradient: 100 us (lookup
+// 13 us, gradient 60 us: 34 MB read, 102 MB written, of which 42 MB reach DRAM within the kernel);
+// 32 x 16384 ids, tables 1024 x 64 fp32: 104 us (lookup 36 us: 268 MB through L2; gradient 43 us
 // for 134 MB of dy, 3 TB/s: a cluster's 16 rows are two dependent flights of loads after their
-// positions). Between lookup and gradient lies the grouping, some 15 us of launches.
+// positions). Between lookup and gradient lies the grouping, some 15 us of launches. A few hundred ids take
+// 18 us of launches, and 56 to 58 us with the host's side of a backward pass (a copy's takes 44).
 #include <algorithm>
 
 #include "fkc_common.cuh"

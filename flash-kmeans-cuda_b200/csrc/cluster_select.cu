@@ -27,12 +27,12 @@
 // 128 squares below 2^-126 can lose, and D * 2^-22 of two such norms more than D products can.
 //
 // The scores go through L2, in rounds of 64 MB at most. 4096 queries x 256
-// clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 55 us (three CTAs an SM; it was 70 with
-// two and with norms read again from shared memory by half of the warps), choose 42 us
+// clusters x 8 rows of 4 heads, D = 128: 8.6 GFLOP and 34 MB of scores, score 58 us (three CTAs an SM; it was 70 with
+// two and with norms read again from shared memory by half of the warps), choose 43 us
 // (two thirds of the issue slots, some 890 instructions a query: bisection 6 to 8 steps, a border of
 // 64-bit scores for 6% of them; 59 us with bisection bit by bit and one query a warp, 53 us
 // with as many CTAs as the SMs hold, which the queries with a border leave at different times).
-// 128 queries of 1024 clusters, 4 heads: 31 us in all, most of it latency (51 us before the heads
+// 128 queries of 1024 clusters, 4 heads: 32 us in all, most of it latency (51 us before the heads
 // shared a tile, thresholds started from the scores' common leading bits and borders went
 // four at a time).
 #include <algorithm>
