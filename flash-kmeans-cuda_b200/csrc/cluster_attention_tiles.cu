@@ -20,17 +20,17 @@
 //
 // At 4096 queries x 8 rows of G = 4, 16 of 256 clusters of 64 keys, D = 128 (2.1 M (query, slot,
 // head) rows, 69 GFLOP): the units and rows are listed in 55 us, tiles_fwd_kernel takes 383 us, the
-// join 174 us (the call 614 us: each from cold caches alone; the larger of the skewed clusters are
+// join 143 us (the call 600 us: each from cold caches alone; the larger of the skewed clusters are
 // selected more often, 1779 keys a query instead of 1024, which makes it 119 GFLOP). The kernel is bound by its
 // SMs' instruction issue (50% of all slots, softmax and output) and by the gathers, which it waits
 // for at the start of every unit; its tensor pipe is busy for 29% of the time and DRAM for near a
-// half (1.1 GB: the parts do not fit L2, Q rows come from it). The join moves 824 MB at 4.7 TB/s.
+// half (1.1 GB: the parts do not fit L2, Q rows come from it). The join moves 824 MB at 5.8 TB/s.
 // What was measured on the way, the same call: the walk 3860 us; by clusters with warp-level
 // matrix instructions 1250; tcgen05 with operands copied 16 bytes a thread 940, by row gathers
 // 900; rows listed beforehand instead of by the gathering warps 740; shares by cost, kept keys,
 // 16-bit parts and bulk stores 680; joins of four heads side by side 630; warpgroups of
 // their own for the output and loops kept rolled (the roles' unrolled code outgrew the
-// instruction cache) 490; parts of three bytes, whose columns may lie any factor apart, 550.
+// instruction cache) 490; parts of three bytes, whose columns may lie any factor apart, 550; two terms of P 615; three CTAs an SM for the joins again 600.
 #include <algorithm>
 #include <atomic>
 #include <numeric>
@@ -545,9 +545,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) tiles_fwd_kernel(
 }
 
 // One warp per (query, GP heads): joins the parts of its clusters, whose log-sum-exps are to
-// base 2.
+// base 2. Bound by the parts' loads: three CTAs an SM (80 registers) take 143 us for 824 MB, two 174.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) tiles_join_kernel(Args a, int i0, int nq, int gp, int chunks,
+__global__ void __launch_bounds__(256, 3) tiles_join_kernel(Args a, int i0, int nq, int gp, int chunks,
                                                          const int32_t* __restrict__ pair_row,
                                                          const uint8_t* __restrict__ part_o,
                                                          const float2* __restrict__ part_lse,

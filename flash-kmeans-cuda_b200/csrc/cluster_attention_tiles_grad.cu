@@ -21,8 +21,8 @@
 // their products as two terms each (cluster_attention_grad.cu).
 //
 // 4096 queries x 4 rows of G = 4, 8 of 64 clusters of 64 keys, D = 128: delta 108 us and its join 6, dQ 155
-// and its join 41, dK and dV 173 and their join 14, rows and tiles listed in 55 (forward and backward
-// together 682 us; with delta from out, one term of P and of dK's dS and parts of two bytes 494). The
+// and its join 36, dK and dV 173 and their join 14, rows and tiles listed in 55 (forward and backward
+// together 680 us; with delta from out, one term of P and of dK's dS and parts of two bytes 494). The
 // three large kernels are bound by the chain of one 128-row step: gathered rows (twice the warps
 // gathering them took 4% off delta's), two score products, the warpgroups' turn (a thread a row, 64
 // columns), two or four products; the tensor pipe is busy for 16%, 22% and 37%. The walk took 2200 us for
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) tiles_delta_join_kernel(Args a, const int
 
 // One warp per (query, GP heads): dq = scale * the sum of its clusters' parts.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) tiles_dq_join_kernel(Args a, int gp, int chunks,
+__global__ void __launch_bounds__(256, 3) tiles_dq_join_kernel(Args a, int gp, int chunks,
                                                             const int32_t* __restrict__ pair_row,
                                                             const uint8_t* __restrict__ part,
                                                             T* __restrict__ dq, int32_t* __restrict__ odd,
