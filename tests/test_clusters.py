@@ -168,3 +168,14 @@ def test_attention_scratch_is_bounded():
                      v_stride=(kv * n * head_dim, n * head_dim, head_dim))
             assert L.fkc_cluster_attention_workspace_size(ctypes.byref(d)) <= 5 << 30
             assert L.fkc_cluster_attention_grad_workspace_size(ctypes.byref(d)) <= 10 << 30
+
+
+def test_gradients_do_not_need_out():
+    """out may be left out: the gradients sum what they need of it anew."""
+    if torch.cuda.is_available():
+        pytest.skip("host has a GPU")
+    d = desc()
+    need = L.fkc_cluster_attention_grad_workspace_size(ctypes.byref(d))
+    assert L.fkc_cluster_attention_grad(ctypes.byref(d), None, 4096, 4096, 4096, 4096, 4096, 4096, need, None) == -3
+    assert L.fkc_cluster_attention_grad(ctypes.byref(d), None, None, 4096, 4096, 4096, 4096, 4096, need, None) == -1
+    assert "lse" in _lib.last_error()
